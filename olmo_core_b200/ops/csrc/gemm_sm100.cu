@@ -544,21 +544,9 @@ struct TmapKeyHash {
   }
 };
 
-// Builds (or fetches) a tiled tensor map with 128-byte swizzle. rank 2 or 3; inner box must span 128 bytes.
-bool get_tensor_map(CUtensorMap* out, const void* ptr, int rank, const uint64_t* dims, const uint64_t* strides_bytes,
-                    const uint32_t* box, int elem_bytes) {
-  static std::mutex mu;
-  static std::unordered_map<TmapKey, CUtensorMap, TmapKeyHash> cache;
-  TmapKey key{ptr, dims[0], dims[1], rank > 2 ? dims[2] : 1, strides_bytes[0], rank > 2 ? strides_bytes[1] : 0,
-              box[0], box[1], rank > 2 ? box[2] : 1, static_cast<uint32_t>(elem_bytes)};
-  {
-    std::lock_guard<std::mutex> g(mu);
-    auto it = cache.find(key);
-    if (it != cache.end()) {
-      *out = it->second;
-      return true;
-    }
-  }
+// Builds a tiled tensor map with 128-byte swizzle. rank 2 or 3; inner box must span 128 bytes.
+bool encode_tensor_map(CUtensorMap* out, const void* ptr, int rank, const uint64_t* dims, const uint64_t* strides_bytes,
+                       const uint32_t* box, int elem_bytes) {
   EncodeTiledFn enc = get_encode_fn();
   if (enc == nullptr) return false;
   cuuint64_t gdim[3] = {dims[0], dims[1], rank > 2 ? dims[2] : 1};
@@ -576,7 +564,25 @@ bool get_tensor_map(CUtensorMap* out, const void* ptr, int rank, const uint64_t*
             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   }
   g_last_tmap_error = static_cast<int>(r);
-  if (r != CUDA_SUCCESS) return false;
+  return r == CUDA_SUCCESS;
+}
+
+// The same, fetched from a cache when the same map was built before.
+bool get_tensor_map(CUtensorMap* out, const void* ptr, int rank, const uint64_t* dims, const uint64_t* strides_bytes,
+                    const uint32_t* box, int elem_bytes) {
+  static std::mutex mu;
+  static std::unordered_map<TmapKey, CUtensorMap, TmapKeyHash> cache;
+  TmapKey key{ptr, dims[0], dims[1], rank > 2 ? dims[2] : 1, strides_bytes[0], rank > 2 ? strides_bytes[1] : 0,
+              box[0], box[1], rank > 2 ? box[2] : 1, static_cast<uint32_t>(elem_bytes)};
+  {
+    std::lock_guard<std::mutex> g(mu);
+    auto it = cache.find(key);
+    if (it != cache.end()) {
+      *out = it->second;
+      return true;
+    }
+  }
+  if (!encode_tensor_map(out, ptr, rank, dims, strides_bytes, box, elem_bytes)) return false;
   std::lock_guard<std::mutex> g(mu);
   if (cache.size() > 8192) cache.clear();
   cache.emplace(key, *out);

@@ -46,6 +46,22 @@ int ocb_quantize_e4m3_rowwise(const void* x, void* q, float* scale, int rows, in
 int ocb_quantize_e4m3_colwise_t(const void* x, void* q_t, float* scale, float* scratch, int rows, int cols, long long ldx,
                                 long long ldq, int pow2, cudaStream_t stream);
 
+// ---- e4m3 with one fp32 scale per block of 128 (block_quant_sm100.cu, gemm_block_fp8_sm100.cu) ----------
+// Codes and scales of bf16 matrices x [rows, cols] (row pitch ldx): by rows (s_row [ceil(cols/128)][rows]) and / or by columns
+// (s_col [ceil(rows/128)][cols]), or by 128 x 128 tiles (s_tile [groups][ceil(rows/128)][ceil(cols/128)], matrices x_group /
+// q_group elements apart). Pass null for the forms that are not wanted. ldq % 16 == 0.
+int ocb_quantize_block_fp8(const void* x, void* q_row, float* s_row, void* q_col, float* s_col, void* q_tile, float* s_tile,
+                           int groups, int rows, int cols, long long ldx, long long ldq, long long x_group,
+                           long long q_group, cudaStream_t stream);
+// C[M, N] (=|+=) sum over blocks kb of 128: sa * sb * A_kb B_kb^T. A: [M, K], or stored [K, M] (a_mn); B: [N, K], or stored
+// [K, N] (b_mn). Scale of (kb, row i): s[kb * s_k + (i >> shift) * s_i], shift 0 or 7. With `offsets` (int32 [num_groups + 1])
+// the rows of A and C belong to groups, group g uses the B at b_group_bytes * g and the scales at sb + sb_g * g; rows outside
+// every group stay as they are. epilogue: 0 = bf16 store, 1 = fp32 accumulate, 2 = fp32 store.
+int ocb_gemm_block_fp8(const void* A, const void* B, void* C, const float* sa, const float* sb, const int* offsets,
+                       int num_groups, int M, int N, int K, long long lda, long long ldb, long long ldc,
+                       long long b_group_bytes, long long sa_k, long long sa_i, int sa_shift, long long sb_k, long long sb_i,
+                       long long sb_g, int sb_shift, int a_mn, int b_mn, int epilogue, int* status, cudaStream_t stream);
+
 // ---- mixture of experts (moe_sm100.cu) --------------------------------------------------------------
 // scores = softmax (mode 0) or sigmoid (mode 1) of logits [n_tokens, n_experts]; weights / experts: [n_tokens, top_k];
 // counts: int32 [n_experts] tokens per expert (may be null); scores may be null.
