@@ -44,6 +44,10 @@ class MoERouterConfig(ModuleConfig):
     bias_gamma: Optional[float] = None
     gating_function: MoERouterGatingFunction = MoERouterGatingFunction.softmax
     dtype: Optional[DType] = None
+    n_groups: int = 1
+    """Experts form this many equal groups of consecutive ids; with more than one, groups are selected before experts."""
+    top_k_groups: Optional[int] = None
+    """Groups that stay open for a token: those with the largest sum of their two best (biased) scores. Default: all."""
 
     def num_params(self, d_model: int, num_experts: int) -> int:
         if self.name != MoERouterType.default:
@@ -68,40 +72,14 @@ class MoERouterConfig(ModuleConfig):
             raise OLMoConfigurationError(f"invalid options for '{self.name}' {self.__class__.__name__}, {e}") from e
 
 
-class _FusedSoftmaxTopK(torch.autograd.Function):
-    """
-    ``logits [N, E] -> (softmax scores [N, E], top-k weights [N, k], expert ids [N, k], tokens per expert [E])`` in one
-    kernel (one warp per token keeps its row in registers). Backward is the softmax Jacobian applied to the sum of the
-    gradients that arrive through the scores (auxiliary loss) and through the selected weights.
-    """
+class _FusedSoftmaxTopK:
+    """``(softmax scores, top-k weights, expert ids, tokens per expert)`` of ``logits [N, E]``: :func:`moe_ops.route` without
+    options."""
 
     @staticmethod
-    def forward(ctx, logits: torch.Tensor, top_k: int):  # type: ignore[override]
-        from ...ops import _lib
-
-        n, e = logits.shape
-        scores = torch.empty((n, e), dtype=torch.float32, device=logits.device)
-        weights = torch.empty((n, top_k), dtype=torch.float32, device=logits.device)
-        experts = torch.empty((n, top_k), dtype=torch.int32, device=logits.device)
-        counts = torch.empty(e, dtype=torch.int32, device=logits.device)
-        rc = _lib.lib().ocb_moe_router_topk(logits.data_ptr(), scores.data_ptr(), weights.data_ptr(), experts.data_ptr(),
-                                            counts.data_ptr(), n, e, top_k, 0, 0, logits.stride(0), _lib.dt(logits),
-                                            _lib.stream_ptr())
-        _lib.check(rc, "ocb_moe_router_topk")
-        ids = experts.long()
-        ctx.save_for_backward(scores, ids)
-        ctx.mark_non_differentiable(ids, counts)
-        ctx.in_dtype = logits.dtype
+    def apply(logits: torch.Tensor, top_k: int):
+        weights, ids, scores, counts = moe_ops.route(logits, top_k)
         return scores, weights, ids, counts
-
-    @staticmethod
-    def backward(ctx, d_scores, d_weights, _ids, _counts):  # type: ignore[override]
-        scores, ids = ctx.saved_tensors
-        g = torch.zeros_like(scores) if d_scores is None else d_scores.float().clone()
-        if d_weights is not None:
-            g.scatter_add_(1, ids, d_weights.float())
-        d_logits = scores * (g - (g * scores).sum(dim=-1, keepdim=True))
-        return d_logits.to(ctx.in_dtype), None
 
 
 class MoERouter(nn.Module):
@@ -119,9 +97,20 @@ class MoERouter(nn.Module):
         lb_loss_weight: Optional[float] = None,
         lb_loss_granularity: MoELoadBalancingLossGranularity = MoELoadBalancingLossGranularity.local_batch,
         z_loss_weight: Optional[float] = None,
+        n_groups: int = 1,
+        top_k_groups: Optional[int] = None,
         init_device: str = "cpu",
     ):
         super().__init__()
+        top_k_groups = n_groups if top_k_groups is None else top_k_groups
+        if n_groups < 1 or num_experts % n_groups != 0 or not 1 <= top_k_groups <= n_groups:
+            raise OLMoConfigurationError(f"{num_experts} experts do not form {n_groups} equal groups of which {top_k_groups} stay open")
+        if n_groups > 1 and not 1 <= top_k <= top_k_groups * (num_experts // n_groups):
+            raise OLMoConfigurationError(f"'top_k' ({top_k}) is more than the experts of {top_k_groups} groups")
+        if n_groups > 1 and uniform_expert_assignment:
+            raise OLMoConfigurationError("'uniform_expert_assignment' and expert groups exclude each other")
+        self.n_groups = n_groups
+        self.top_k_groups = top_k_groups
         self.d_model = d_model
         self.num_experts = num_experts
         self.top_k = top_k
@@ -261,11 +250,16 @@ class MoERouter(nn.Module):
         """
         x = self.jitter(x)
         logits = self.get_expert_logits(x).float()
-        fused = (logits.is_cuda and self.gating_function == MoERouterGatingFunction.softmax and self.bias_gamma is None
-                 and not self.uniform_expert_assignment and self.num_experts <= 1024 and self.top_k <= 32)
-        if fused:
-            flat = logits.reshape(-1, self.num_experts)
-            scores, weights, indices, kernel_counts = _FusedSoftmaxTopK.apply(flat, self.top_k)
+        fused = (logits.is_cuda and not self.uniform_expert_assignment
+                 and moe_ops.route_supported(self.num_experts, self.top_k, self.n_groups))
+        normalized = False
+        if fused or self.n_groups > 1:
+            normalized = self.normalize_expert_weights in (1, 2)
+            weights, indices, scores, kernel_counts = moe_ops.route(
+                logits.reshape(-1, self.num_experts), self.top_k, gating=str(self.gating_function),
+                score_bias=None if self.bias_gamma is None else get_local_tensor(self.score_bias).float(),
+                n_groups=self.n_groups, top_k_groups=self.top_k_groups,
+                normalize=int(self.normalize_expert_weights) if normalized else None)
             scores = scores.view_as(logits)
             weights = weights.view(*logits.shape[:-1], self.top_k)
             indices = indices.view(*logits.shape[:-1], self.top_k)
@@ -275,7 +269,7 @@ class MoERouter(nn.Module):
         else:
             scores = torch.sigmoid(logits) + 1e-7
             weights, indices = self.get_top_k(scores)
-        if self.normalize_expert_weights is not None:
+        if self.normalize_expert_weights is not None and not normalized:
             weights = weights / torch.norm(weights, p=self.normalize_expert_weights, dim=-1, keepdim=True)
         with torch.no_grad():
             if fused and self.lb_loss_granularity != MoELoadBalancingLossGranularity.instance:

@@ -58,8 +58,8 @@ _SIGS = {
     "ocb_quantize_e4m3_rowwise": [c_void_p, c_void_p, c_void_p, c_int, c_int, c_longlong, c_longlong, c_int, c_void_p],
     "ocb_quantize_e4m3_colwise_t": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_longlong, c_longlong, c_int,
                                     c_void_p],
-    "ocb_moe_router_topk": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int,
-                            c_longlong, c_int, c_void_p],
+    "ocb_moe_route": [c_void_p] * 6 + [c_int] * 7 + [c_longlong, c_int, c_void_p],
+    "ocb_moe_route_grad": [c_void_p] * 6 + [c_int] * 5 + [c_longlong, c_int, c_void_p],
     "ocb_moe_sort": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p],
     "ocb_moe_gather": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_longlong, c_longlong, c_void_p],
     "ocb_moe_scatter": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_longlong, c_longlong, c_void_p],

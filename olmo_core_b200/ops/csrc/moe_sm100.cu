@@ -1,6 +1,5 @@
-// Mixture-of-experts routing and token permutation for sm_100a.
+// Mixture-of-experts token permutation for sm_100a (routing: moe_route_sm100.cu).
 //
-//   router     logits [N, E] -> softmax scores, top-k (weights, expert ids), tokens per expert      (one pass)
 //   sort       expert ids [N*k] -> stable counting sort: row of every routed copy, copy of every row, group offsets
 //   gather     expert-sorted activation matrix  xs[r] = (w[src[r]] *) x[src[r] / k]
 //   scatter    y[t] = sum_j w[t, j] * ys[dest[t*k + j]]      (fp32 accumulation, fixed order: deterministic)
@@ -21,88 +20,6 @@ namespace ocb {
 
 constexpr int SORT_CHUNK = 2048;  // routed copies ranked by one warp
 constexpr int MAX_EXPERTS = 1024;
-
-__device__ __forceinline__ float ld_act(const void* p, long long i, int dtype) {
-  return dtype == OCB_BF16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i])
-                           : reinterpret_cast<const float*>(p)[i];
-}
-
-// ------------------------------------------------------------------------------------------------ router
-// One warp per token. Each lane keeps E/32 logits in registers (E <= 1024); the top-k are extracted by k rounds of a
-// warp arg-max (ties go to the lower expert id, like torch.topk on a stable sort). mode: 0 = softmax then top-k,
-// 1 = sigmoid scores then top-k. normalize: weights / sum(weights). counts: int32 [E], must be zero on entry.
-template <int PER_LANE>
-__global__ void router_topk_kernel(const void* __restrict__ logits, float* __restrict__ scores, float* __restrict__ weights,
-                                   int* __restrict__ experts, int* __restrict__ counts, int n_tokens, int n_experts,
-                                   int top_k, int mode, int normalize, long long ld, int dtype) {
-  const int warp = (blockIdx.x * blockDim.x + threadIdx.x) >> 5;
-  const int lane = threadIdx.x & 31;
-  if (warp >= n_tokens) return;
-  float v[PER_LANE];
-  float mx = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < PER_LANE; ++i) {
-    const int e = i * 32 + lane;
-    v[i] = e < n_experts ? ld_act(logits, warp * ld + e, dtype) : -INFINITY;
-    mx = fmaxf(mx, v[i]);
-  }
-  if (mode == 0) {
-#pragma unroll
-    for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    float sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < PER_LANE; ++i) {
-      v[i] = (i * 32 + lane) < n_experts ? __expf(v[i] - mx) : 0.f;
-      sum += v[i];
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    const float inv = 1.f / sum;
-#pragma unroll
-    for (int i = 0; i < PER_LANE; ++i) v[i] *= inv;
-  } else {
-#pragma unroll
-    for (int i = 0; i < PER_LANE; ++i) v[i] = (i * 32 + lane) < n_experts ? 1.f / (1.f + __expf(-v[i])) : 0.f;
-  }
-  if (scores != nullptr) {
-#pragma unroll
-    for (int i = 0; i < PER_LANE; ++i) {
-      const int e = i * 32 + lane;
-      if (e < n_experts) scores[static_cast<long long>(warp) * n_experts + e] = v[i];
-    }
-  }
-  float total = 0.f;
-  float picked_w = 0.f;  // lane j keeps the j-th pick (top_k <= 32)
-  int picked_e = 0;
-  for (int j = 0; j < top_k; ++j) {
-    float best = -1.f;
-    int best_e = 0x7fffffff;
-#pragma unroll
-    for (int i = 0; i < PER_LANE; ++i) {
-      const int e = i * 32 + lane;
-      if (e < n_experts && v[i] > best) { best = v[i]; best_e = e; }
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      const float ob = __shfl_xor_sync(0xffffffffu, best, o);
-      const int oe = __shfl_xor_sync(0xffffffffu, best_e, o);
-      if (ob > best || (ob == best && oe < best_e)) { best = ob; best_e = oe; }
-    }
-    if ((best_e & 31) == lane) {  // remove the winner (scores are >= 0); static indexing keeps v[] in registers
-#pragma unroll
-      for (int i = 0; i < PER_LANE; ++i)
-        if (i == (best_e >> 5)) v[i] = -2.f;
-    }
-    if (lane == j) { picked_w = best; picked_e = best_e; }
-    total += best;
-  }
-  if (lane < top_k) {
-    if (normalize) picked_w /= fmaxf(total, 1e-20f);
-    weights[static_cast<long long>(warp) * top_k + lane] = picked_w;
-    experts[static_cast<long long>(warp) * top_k + lane] = picked_e;
-    if (counts != nullptr) atomicAdd(&counts[picked_e], 1);
-  }
-}
 
 // -------------------------------------------------------------------------------------------------- sort
 // Pass 1: one warp per chunk of SORT_CHUNK routed copies. rank[j] = how many earlier copies of the chunk go to the same
@@ -264,28 +181,6 @@ using namespace ocb;
 
 static inline int launch_ok() { return cudaGetLastError() == cudaSuccess ? 0 : -4; }
 
-extern "C" int ocb_moe_router_topk(const void* logits, float* scores, float* weights, int* experts, int* counts,
-                                   int n_tokens, int n_experts, int top_k, int mode, int normalize, long long ld,
-                                   int act_dtype, cudaStream_t stream) {
-  if (n_tokens <= 0) return 0;
-  if (n_experts <= 0 || n_experts > MAX_EXPERTS || top_k <= 0 || top_k > 32 || top_k > n_experts) return -1;
-  if (counts != nullptr && cudaMemsetAsync(counts, 0, sizeof(int) * n_experts, stream) != cudaSuccess) return -4;
-  const int threads = 256;
-  const int blocks = (n_tokens * 32 + threads - 1) / threads;
-#define OCB_ROUTER(PL)                                                                                              \
-  router_topk_kernel<PL><<<blocks, threads, 0, stream>>>(logits, scores, weights, experts, counts, n_tokens, n_experts, \
-                                                         top_k, mode, normalize, ld, act_dtype)
-  if (n_experts <= 32) OCB_ROUTER(1);
-  else if (n_experts <= 64) OCB_ROUTER(2);
-  else if (n_experts <= 128) OCB_ROUTER(4);
-  else if (n_experts <= 256) OCB_ROUTER(8);
-  else if (n_experts <= 512) OCB_ROUTER(16);
-  else OCB_ROUTER(32);
-#undef OCB_ROUTER
-  return launch_ok();
-}
-
-// Scratch: int32 [ocb_moe_sort_scratch_ints(n, n_experts)].
 extern "C" long long ocb_moe_sort_scratch_ints(int n, int n_experts) {
   const long long chunks = (n + SORT_CHUNK - 1) / SORT_CHUNK;
   return static_cast<long long>(n) + chunks * n_experts;

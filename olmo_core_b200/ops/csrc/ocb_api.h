@@ -63,11 +63,18 @@ int ocb_gemm_block_fp8(const void* A, const void* B, void* C, const float* sa, c
                        long long sb_g, int sb_shift, int a_mn, int b_mn, int epilogue, int* status, cudaStream_t stream);
 
 // ---- mixture of experts (moe_sm100.cu) --------------------------------------------------------------
-// scores = softmax (mode 0) or sigmoid (mode 1) of logits [n_tokens, n_experts]; weights / experts: [n_tokens, top_k];
-// counts: int32 [n_experts] tokens per expert (may be null); scores may be null.
-int ocb_moe_router_topk(const void* logits, float* scores, float* weights, int* experts, int* counts, int n_tokens,
-                        int n_experts, int top_k, int mode, int normalize, long long ld, int act_dtype,
-                        cudaStream_t stream);
+// Routing (moe_route_sm100.cu). scores [n_tokens, n_experts] = softmax, or sigmoid + 1e-7, of logits (row pitch ld); experts /
+// weights [n_tokens, top_k]: the experts with the largest score (+ bias [n_experts], may be null) among those of the top_groups
+// best of n_groups equal groups, and their scores, divided by their sum (normalize 1) or 2-norm (normalize 2); counts: int32
+// [n_experts] tokens per expert. scores may be null.
+int ocb_moe_route(const void* logits, float* scores, float* weights, long long* experts, int* counts, const float* bias,
+                  int n_tokens, int n_experts, int top_k, int sigmoid, int normalize, int n_groups, int top_groups,
+                  long long ld, int act_dtype, cudaStream_t stream);
+// d_logits [n_tokens, n_experts] from the gradients of weights and scores (either may be null). Softmax reads the scores,
+// sigmoid the logits.
+int ocb_moe_route_grad(const float* scores, const void* logits, const long long* experts, const float* d_weights,
+                       const float* d_scores, void* d_logits, int n_tokens, int n_experts, int top_k, int sigmoid,
+                       int normalize, long long ld, int act_dtype, cudaStream_t stream);
 // Stable counting sort of n routed copies by expert id. dest[j]: row of copy j in the sorted layout; src: its inverse;
 // sorted_experts (may be null): expert of every row; offsets: int32 [n_experts + 1] prefix sums.
 long long ocb_moe_sort_scratch_ints(int n, int n_experts);

@@ -1,5 +1,5 @@
 """
-Token permutation ops for mixture-of-experts layers (function names of src/olmo_core/ops/moe.py:52-304,
+Routing and token permutation ops for mixture-of-experts layers (function names of src/olmo_core/ops/moe.py:52-304,
 whose reference implementation is a set of Triton copy kernels, src/olmo_core/kernels/moe.py:31-536).
 
 Layout conventions: ``top_experts`` is ``[N, k]``; flattening it gives ``N*k`` routed copies. Sorting the
@@ -17,6 +17,7 @@ import torch
 import torch.distributed as dist
 
 __all__ = [
+    "route",
     "indices_and_bins",
     "gather",
     "scatter",
@@ -33,6 +34,161 @@ __all__ = [
     "BinnedScatterOp",
     "AllToAllOp",
 ]
+
+
+# ------------------------------------------------------------------------------------------------------
+# Routing
+# ------------------------------------------------------------------------------------------------------
+
+SIGMOID_FLOOR = 1e-7
+"""Added to every sigmoid score, so that weights can be normalised when all chosen scores vanish."""
+
+
+def route_supported(num_experts: int, top_k: int, n_groups: int = 1) -> bool:
+    """Whether the CUDA kernels of :func:`route` cover these sizes."""
+    return num_experts <= 1024 and top_k <= 32 and n_groups <= 32
+
+
+def _route_reference(logits, top_k, gating, score_bias, n_groups, top_k_groups, normalize):
+    """PyTorch form of :func:`route` (CPU tensors); autograd differentiates it."""
+    x = logits.float()
+    n, e = x.shape
+    if gating == "softmax":
+        dead = (x == float("-inf")).all(-1, keepdim=True)
+        scores = torch.where(dead, 0.0, torch.where(dead, 0.0, x).softmax(-1))
+    else:
+        scores = torch.sigmoid(x) + SIGMOID_FLOOR
+    with torch.no_grad():  # the ranking is exact arithmetic's, see the kernel
+        xd = x.double()
+        if score_bias is None and n_groups == 1:
+            rank = xd
+        else:
+            rank = xd.softmax(-1).masked_fill(dead, 0.0) if gating == "softmax" else torch.sigmoid(xd) + SIGMOID_FLOOR
+            if score_bias is not None:
+                rank = rank + score_bias.double()
+        if n_groups > 1:
+            best = rank.view(n, n_groups, -1).sort(dim=-1, descending=True)[0][..., :2].sum(-1)
+            kept = best.sort(dim=-1, descending=True, stable=True)[1][:, :top_k_groups]
+            shut = torch.ones(n, n_groups, dtype=torch.bool, device=x.device).scatter_(1, kept, False)
+            shut = shut.repeat_interleave(e // n_groups, 1)
+            # closed experts sort behind every open one, -inf among them
+            order = torch.where(shut, float("-inf"), xd if score_bias is None else rank).sort(dim=-1, descending=True, stable=True)[1]
+            order = order.gather(1, shut.gather(1, order).sort(dim=-1, stable=True)[1])
+        else:
+            order = rank.sort(dim=-1, descending=True, stable=True)[1]
+        experts = order[:, :top_k].contiguous()
+        counts = torch.bincount(experts.reshape(-1), minlength=e).to(torch.int32)
+    weights = scores.gather(1, experts)
+    if normalize:
+        norm = weights.sum(-1, keepdim=True) if normalize == 1 else weights.square().sum(-1, keepdim=True).sqrt()
+        weights = torch.where(norm == 0, 0.0, weights / torch.where(norm == 0, 1.0, norm))
+    return weights, experts, scores, counts
+
+
+def _route_kernel(logits, top_k, gating, score_bias, n_groups, top_k_groups, normalize):
+    from . import _lib
+
+    n, e = logits.shape
+    device = logits.device
+    scores = torch.empty((n, e), dtype=torch.float32, device=device)
+    weights = torch.empty((n, top_k), dtype=torch.float32, device=device)
+    experts = torch.empty((n, top_k), dtype=torch.int64, device=device)
+    counts = torch.empty(e, dtype=torch.int32, device=device)
+    with torch.cuda.device(device):
+        rc = _lib.lib().ocb_moe_route(
+            logits.data_ptr(), scores.data_ptr(), weights.data_ptr(), experts.data_ptr(), counts.data_ptr(),
+            _lib.ptr(score_bias), n, e, top_k, int(gating == "sigmoid"), normalize, n_groups, top_k_groups,
+            logits.stride(0), _lib.dt(logits), _lib.stream_ptr())
+    _lib.check(rc, "ocb_moe_route")
+    return weights, experts, scores, counts
+
+
+class _Route(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, *options):  # type: ignore[override]
+        weights, experts, scores, counts = _route_kernel(logits, *options)
+        _, gating, _, _, _, normalize = options
+        ctx.sigmoid, ctx.normalize = gating == "sigmoid", normalize
+        ctx.save_for_backward(logits if ctx.sigmoid else scores, experts)
+        ctx.logits_dtype = logits.dtype
+        ctx.mark_non_differentiable(experts, counts)
+        ctx.set_materialize_grads(False)
+        return weights, experts, scores, counts
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_weights, _experts, d_scores, _counts):  # type: ignore[override]
+        from . import _lib
+
+        if d_weights is None and d_scores is None:
+            return (None,) * 7
+        kept, experts = ctx.saved_tensors
+        n, e = kept.shape
+        d_weights = None if d_weights is None else d_weights.float().contiguous()
+        d_scores = None if d_scores is None else d_scores.float().contiguous()
+        d_logits = torch.empty((n, e), dtype=ctx.logits_dtype, device=kept.device)
+        with torch.cuda.device(kept.device):
+            rc = _lib.lib().ocb_moe_route_grad(
+                None if ctx.sigmoid else kept.data_ptr(), kept.data_ptr() if ctx.sigmoid else None, experts.data_ptr(),
+                _lib.ptr(d_weights), _lib.ptr(d_scores), d_logits.data_ptr(), n, e, experts.shape[1], int(ctx.sigmoid),
+                ctx.normalize, kept.stride(0), _lib.dt(d_logits), _lib.stream_ptr())
+        _lib.check(rc, "ocb_moe_route_grad")
+        return (d_logits,) + (None,) * 6
+
+
+def route(
+    logits: torch.Tensor,
+    top_k: int,
+    *,
+    gating: str = "softmax",
+    score_bias: Optional[torch.Tensor] = None,
+    n_groups: int = 1,
+    top_k_groups: Optional[int] = None,
+    normalize: Optional[int] = None,
+) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """
+    Choose ``top_k`` experts for every token. ``logits [N, E]`` fp32 or bf16. Returns
+
+    * ``weights [N, top_k]`` fp32: the chosen experts' scores, divided by their sum (``normalize=1``) or 2-norm (``2``),
+    * ``experts [N, top_k]`` int64, best first, the lower id first where two rank the same,
+    * ``scores [N, E]`` fp32: softmax, or sigmoid + 1e-7, of the logits,
+    * ``counts [E]`` int32: tokens per expert.
+
+    Experts are ranked by score plus ``score_bias`` (fp32 ``[E]``; it enters no weight). With ``n_groups > 1`` the experts form
+    that many equal groups of consecutive ids, of which the ``top_k_groups`` with the largest sum of their two best ranked
+    experts stay open. The ranking is that of exact arithmetic. A token without any logit above ``-inf`` gets softmax scores
+    and weights of zero.
+
+    Gradients flow from ``weights`` and ``scores`` to ``logits``. One kernel each way on CUDA (at most 1024 experts, 32 chosen,
+    32 groups).
+    """
+    if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError(f"logits must be float32 or bfloat16 [N, E], got {logits.dtype} {tuple(logits.shape)}")
+    e = logits.shape[1]
+    if gating not in ("softmax", "sigmoid"):
+        raise ValueError(f"gating must be 'softmax' or 'sigmoid', got '{gating}'")
+    top_k_groups = n_groups if top_k_groups is None else top_k_groups
+    if n_groups < 1 or e % n_groups or not 1 <= top_k_groups <= n_groups:
+        raise ValueError(f"{e} experts do not form {n_groups} equal groups of which {top_k_groups} stay open")
+    if not 1 <= top_k <= top_k_groups * (e // n_groups):
+        raise ValueError(f"cannot choose {top_k} of {top_k_groups * (e // n_groups)} experts")
+    if normalize not in (None, 1, 2):
+        raise ValueError(f"normalize must be None, 1 or 2, got {normalize}")
+    if score_bias is not None:
+        if score_bias.dtype != torch.float32 or tuple(score_bias.shape) != (e,) or score_bias.device != logits.device:
+            raise ValueError(f"score_bias must be float32 [{e}] on {logits.device}, got {score_bias.dtype} "
+                             f"{tuple(score_bias.shape)} on {score_bias.device}")
+        score_bias = score_bias.detach().contiguous()
+    options = (top_k, gating, score_bias, n_groups, top_k_groups, int(normalize or 0))
+    if not logits.is_cuda:
+        return _route_reference(logits, *options)
+    if not route_supported(e, top_k, n_groups):
+        raise ValueError(f"the routing kernels take at most 1024 experts, 32 chosen and 32 groups, got {e}, {top_k} and {n_groups}")
+    if logits.stride(1) != 1 and e > 1:
+        logits = logits.contiguous()
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _Route.apply(logits, *options)
+    return _route_kernel(logits, *options)
 
 
 def histc(x: torch.Tensor, num_classes: int) -> torch.Tensor:
