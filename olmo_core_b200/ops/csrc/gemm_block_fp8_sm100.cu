@@ -12,7 +12,8 @@
 // Scales are read through strides: per row of an operand (index shift 0) or per 128 rows (shift 7).
 //
 // CTA layout (384 threads, three warpgroups): warp 0 = TMA producer, warp 1 = MMA issuer and tensor-memory owner, warps 2 and 3
-// only keep the group whole; warps 4..11 = promotion and epilogue: four lane quadrants x two column halves, every thread owns
+// = scales: they run ahead of the promotion by up to eight blocks and leave each block's factors in a shared-memory ring, so
+// that no promotion ever waits for a scale to come from L2; warps 4..11 = promotion and epilogue: four lane quadrants x two column halves, every thread owns
 // one row and BN / 2 columns of the tile, held in registers. The first warpgroup hands registers to the other two (72 against
 // 2 x 216 of the 3 x 168 at launch). All waits are bounded (common.cuh).
 
@@ -29,6 +30,7 @@ constexpr int A_BYTES = BM * BKE;
 constexpr int THREADS = 384;
 constexpr int REGS_FEED = 72, REGS_SUM = 216;  // registers a thread after the hand-over: 72 + 2 * 216 = 3 * 168
 constexpr int EPI_WARPS = 8;
+constexpr int SCALE_SLOTS = 8, SCALE_BATCH = 4;  // ring of factors; blocks whose scales are fetched together
 constexpr uint32_t TMEM_COLS = 512;
 
 enum : int { EPI_BF16 = 0, EPI_F32_ACC = 1, EPI_F32 = 2 };
@@ -39,7 +41,9 @@ struct Tile {
   static constexpr int STAGES = BN == 256 ? 4 : 6;
   static constexpr int ACCS = static_cast<int>(TMEM_COLS) / BN;  // partial tiles in flight between the issuer and the epilogue
   static constexpr int COLS = BN / 2;                            // columns per epilogue thread
-  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 2 * BN * 4 + 1024 /*alignment slack*/ + 256 /*barriers*/;
+  // a block's factors: per row and column half (sa * sb), or sa per row and sb per column
+  static constexpr int FACTORS = BM + BN;
+  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + SCALE_SLOTS * FACTORS * 4 + 1024 /*alignment slack*/ + 512 /*barriers*/;
 };
 
 struct Scales {
@@ -107,30 +111,12 @@ struct Walker {
 
 // Waits for the tensor-memory loads issued so far. The registers pass through, so that nothing that reads them can be
 // scheduled ahead of the wait.
-__device__ __forceinline__ void tmem_ld_wait_for(uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_ld_wait_for(uint32_t (&r)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
-                 "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]),
-                 "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
-                 "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
                :
                : "memory");
-}
-
-// A barrier of the 128 threads of one column half that also says whether all of them are still fine: they leave together.
-__device__ __forceinline__ bool half_barrier_all(int half, bool ok) {
-  uint32_t all;
-  asm volatile(
-      "{\n\t"
-      ".reg .pred p, q;\n\t"
-      "setp.ne.u32 p, %2, 0;\n\t"
-      "barrier.cta.red.and.pred q, %1, 128, p;\n\t"
-      "selp.u32 %0, 1, 0, q;\n\t"
-      "}\n"
-      : "=r"(all)
-      : "r"(1 + half), "r"(static_cast<uint32_t>(ok))
-      : "memory");
-  return all != 0;
 }
 
 // 32 consecutive columns of one row; v holds 16 packed pairs.
@@ -176,8 +162,8 @@ __device__ __forceinline__ void store_chunk(const Params& p, long long row, int 
   }
 }
 
-// BCOL: the scales of B differ from row to row of B (= output column) and travel through shared memory; otherwise B has one
-// scale per 128 of its rows, which is one number for everything a thread owns.
+// BCOL: the scales of B differ from row to row of B (= output column); otherwise B has one scale per 128 of its rows, which
+// is one number for everything a thread owns.
 template <int BN, bool BCOL, int EPI>
 __global__ void __launch_bounds__(THREADS, 1)
 gemm_block_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b, const Params p) {
@@ -185,12 +171,14 @@ gemm_block_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
   constexpr int STAGES = T::STAGES, ACCS = T::ACCS, COLS = T::COLS, STAGE_BYTES = T::STAGE_BYTES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* sb_smem = reinterpret_cast<float*>(smem + STAGES * STAGE_BYTES);  // [2][BN]
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(sb_smem + 2 * BN);
+  float* factors = reinterpret_cast<float*>(smem + STAGES * STAGE_BYTES);  // [SCALE_SLOTS][FACTORS]
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(factors + SCALE_SLOTS * T::FACTORS);
   uint64_t* empty_bar = full_bar + STAGES;
   uint64_t* tfull_bar = empty_bar + STAGES;
   uint64_t* tempty_bar = tfull_bar + ACCS;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty_bar + ACCS);
+  uint64_t* sfull_bar = tempty_bar + ACCS;
+  uint64_t* sempty_bar = sfull_bar + SCALE_SLOTS;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sempty_bar + SCALE_SLOTS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5;
@@ -205,6 +193,10 @@ gemm_block_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
     for (int a = 0; a < ACCS; ++a) {
       mbar_init(&tfull_bar[a], 1);
       mbar_init(&tempty_bar[a], EPI_WARPS);
+    }
+    for (int i = 0; i < SCALE_SLOTS; ++i) {
+      mbar_init(&sfull_bar[i], 2);
+      mbar_init(&sempty_bar[i], EPI_WARPS);
     }
     *abort_flag = 0;
     fence_mbar_init();
@@ -290,69 +282,124 @@ gemm_block_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
         }
       }
     }
-  } else if (warp >= 4) {
+  } else if (warp < 4) {
+    // ------------------------------------------------------------------ scales (warps 2 and 3)
+    const int t64 = threadIdx.x - 64;
+    int slot = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    Walker walker(p, BN);
+    TileInfo t;
+    constexpr int PER = BCOL ? T::FACTORS / 64 : BM / 64;  // scales a thread fetches per block (and, without BCOL, two of B)
+    while (ok && walker.next(t)) {
+      const float* src[PER];
+      long long step[PER];
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {  // factor t64 + 64 i: a row of A, or a column
+        const int f = t64 + 64 * i;
+        const bool is_a = i < BM / 64;
+        const int at = is_a ? t.m0 + f : t.n0 + f - BM;
+        const Scales& sc = is_a ? p.sa : p.sb;
+        step[i] = sc.k_stride;
+        src[i] = at < (is_a ? t.m_end : p.N) ? sc.p + (is_a ? 0 : t.g * sc.group_stride) + static_cast<long long>(at >> sc.shift) * sc.i_stride
+                                             : nullptr;
+      }
+      const float* tile[2] = {nullptr, nullptr};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int col = t.n0 + h * COLS;
+        if (!BCOL && col < p.N) tile[h] = p.sb.p + t.g * p.sb.group_stride + static_cast<long long>(col >> p.sb.shift) * p.sb.i_stride;
+      }
+      for (int kb0 = 0; ok && kb0 < num_kb; kb0 += SCALE_BATCH) {
+        float v[SCALE_BATCH][PER], w[SCALE_BATCH][2];
+#pragma unroll
+        for (int b = 0; b < SCALE_BATCH; ++b) {
+          const bool live = kb0 + b < num_kb;
+#pragma unroll
+          for (int i = 0; i < PER; ++i) v[b][i] = live && src[i] != nullptr ? __ldg(src[i] + (kb0 + b) * step[i]) : 0.f;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) w[b][h] = live && tile[h] != nullptr ? __ldg(tile[h] + (kb0 + b) * p.sb.k_stride) : 0.f;
+        }
+#pragma unroll
+        for (int b = 0; b < SCALE_BATCH; ++b) {
+          if (kb0 + b >= num_kb) break;
+          ok = mbar_wait_bounded(&sempty_bar[slot], phase ^ 1u, abort_flag, p.status, kStatusTimeoutProducer);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          float* dst = factors + slot * T::FACTORS;
+          if (BCOL) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) dst[t64 + 64 * i] = v[b][i];
+          } else {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int i = 0; i < PER; ++i) dst[h * BM + t64 + 64 * i] = v[b][i] * w[b][h];
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sfull_bar[slot]);
+          if (++slot == SCALE_SLOTS) { slot = 0; phase ^= 1u; }
+        }
+      }
+    }
+  } else {
     // ------------------------------------------------------------------ promotion and epilogue
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SUM));
     const int quad = warp & 3, half = (warp - 4) >> 2;
-    const int half_thread = threadIdx.x - 128 - half * 128;
     const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + half * COLS;
-    int acc = 0;
-    uint32_t acc_phase = 0;
-    bool ok = true, given_up = false;
+    // where this thread's factor sits in a slot, and where the column factors of its half start
+    const float* my_factor = factors + (BCOL ? 0 : half * BM) + quad * 32 + lane;
+    const float* col_factors = factors + BM + half * COLS;
+    int acc = 0, slot = 0;
+    uint32_t acc_phase = 0, slot_phase = 0;
+    bool ok = true;
     Walker walker(p, BN);
     TileInfo t;
-    while ((ok || BCOL) && walker.next(t)) {
-      const int row = t.m0 + quad * 32 + lane, col0 = t.n0 + half * COLS;
-      const bool row_ok = row < t.m_end;
-      const float* sa = p.sa.p + static_cast<long long>(row_ok ? row >> p.sa.shift : 0) * p.sa.i_stride;
-      const int sb_col = BCOL ? col0 + (half_thread & (COLS - 1)) : col0;
-      const bool sb_ok = sb_col < p.N && (!BCOL || half_thread < COLS);
-      const float* sb = p.sb.p + t.g * p.sb.group_stride + static_cast<long long>(sb_ok ? sb_col >> p.sb.shift : 0) * p.sb.i_stride;
-      float sa_next = row_ok ? sa[0] : 0.f, sb_next = sb_ok ? sb[0] : 0.f;
+    while (ok && walker.next(t)) {
       uint64_t sum[COLS / 2];
 #pragma unroll
       for (int j = 0; j < COLS / 2; ++j) sum[j] = 0ull;
       for (int kb = 0; kb < num_kb; ++kb) {
-        const float sa_now = sa_next, sb_now = sb_next;
-        if (kb + 1 < num_kb) {  // the next block's scales are on their way while this one is promoted
-          sa_next = row_ok ? sa[(kb + 1) * p.sa.k_stride] : 0.f;
-          sb_next = sb_ok ? sb[(kb + 1) * p.sb.k_stride] : 0.f;
-        }
-        const float* sb_row = sb_smem + (kb & 1) * BN + half * COLS;
-        if (BCOL) {
-          if (half_thread < COLS) sb_smem[(kb & 1) * BN + half * COLS + half_thread] = sb_now;
-          // the 128 threads of a column half share its scales; two buffers, so one barrier per block
-          if (!half_barrier_all(half, ok)) { ok = false; given_up = true; break; }
-        }
-        const float s = BCOL ? sa_now : sa_now * sb_now;
-        const uint64_t s2 = pack_f32x2(s, s);
-        ok = ok && mbar_wait_bounded(&tfull_bar[acc], acc_phase, abort_flag, p.status, kStatusTimeoutEpilogue);
+        ok = mbar_wait_bounded(&sfull_bar[slot], slot_phase, abort_flag, p.status, kStatusTimeoutEpilogue) &&
+             mbar_wait_bounded(&tfull_bar[acc], acc_phase, abort_flag, p.status, kStatusTimeoutEpilogue);
         ok = __all_sync(0xffffffffu, ok);
-        if (!ok && !BCOL) break;  // with BCOL the warps of a half leave together, at their next barrier
+        if (!ok) break;
         tc_fence_after();
-        uint32_t r[2][32];
-        tmem_ld_32x32(t_row + acc * BN, r[0]);
+        const uint32_t t_acc = t_row + acc * BN;
+        uint32_t r[2][16];
+        tmem_ld_32x16(t_acc, r[0]);
+        const float s = my_factor[slot * T::FACTORS];
+        const uint64_t s2 = pack_f32x2(s, s);
+        const float* cf = col_factors + slot * T::FACTORS;
         tmem_ld_wait_for(r[0]);
 #pragma unroll
-        for (int c = 0; c < COLS / 32; ++c) {
-          if (c + 1 < COLS / 32) {
-            tmem_ld_32x32(t_row + acc * BN + (c + 1) * 32, r[(c + 1) & 1]);
+        for (int c = 0; c < COLS / 16; ++c) {
+          if (c + 1 < COLS / 16) {
+            tmem_ld_32x16(t_acc + (c + 1) * 16, r[(c + 1) & 1]);
           } else {
             tc_fence_before();
             if (lane == 0) mbar_arrive(&tempty_bar[acc]);
           }
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            uint64_t f = s2;
-            if (BCOL) f = mul_f32x2(s2, *reinterpret_cast<const uint64_t*>(sb_row + c * 32 + 2 * j));
-            sum[c * 16 + j] = fma_f32x2(pack_u32x2(r[c & 1][2 * j], r[c & 1][2 * j + 1]), f, sum[c * 16 + j]);
+          for (int j = 0; j < 8; j += 2) {
+            uint64_t f0 = s2, f1 = s2;
+            if (BCOL) {
+              const float4 col = *reinterpret_cast<const float4*>(cf + c * 16 + 2 * j);
+              f0 = mul_f32x2(s2, pack_f32x2(col.x, col.y));
+              f1 = mul_f32x2(s2, pack_f32x2(col.z, col.w));
+            }
+            sum[c * 8 + j] = fma_f32x2(pack_u32x2(r[c & 1][2 * j], r[c & 1][2 * j + 1]), f0, sum[c * 8 + j]);
+            sum[c * 8 + j + 1] = fma_f32x2(pack_u32x2(r[c & 1][2 * j + 2], r[c & 1][2 * j + 3]), f1, sum[c * 8 + j + 1]);
           }
-          if (c + 1 < COLS / 32) tmem_ld_wait_for(r[(c + 1) & 1]);
+          if (c + 1 < COLS / 16) tmem_ld_wait_for(r[(c + 1) & 1]);
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sempty_bar[slot]);
         if (++acc == ACCS) { acc = 0; acc_phase ^= 1u; }
+        if (++slot == SCALE_SLOTS) { slot = 0; slot_phase ^= 1u; }
       }
-      if (given_up) break;
-      if (ok && row_ok) {
+      const int row = t.m0 + quad * 32 + lane, col0 = t.n0 + half * COLS;
+      if (ok && row < t.m_end) {
 #pragma unroll
         for (int c = 0; c < COLS / 32; ++c)
           if (col0 + c * 32 < p.N) store_chunk<EPI>(p, row, col0 + c * 32, sum + c * 16);
