@@ -1,21 +1,23 @@
-// e4m3 GEMM for sm_100a whose operands carry one fp32 scale per block of 128 reduction elements:
+// e4m3 GEMM for sm_100a whose operands carry one power-of-two scale per block of 128 reduction elements:
 //
 //   C[m, n] (=|+=) sum_kb  sa(kb, m) * sb(kb, n) * sum_{k in block kb}  A[m, k] * B[n, k]
 //
-// The scales change along the reduction, so the tensor core only ever accumulates ONE block (128 elements, four K = 32
-// instructions) into tensor memory; the epilogue warps read that partial tile back and add it, multiplied by its scales,
-// to fp32 accumulators in registers ("promotion"). The sums over the blocks are therefore plain fp32 additions.
+// The scales are applied by the tensor core (tcgen05.mma.kind::mxf8f6f4.block_scale): it takes one E8M0 exponent per 32
+// reduction elements, so a block's exponent is handed to it four times, and the accumulator in tensor memory runs through the
+// whole reduction in fp32. Adding scaled partial sums in registers instead, which would allow scales of any value, was measured
+// first: every block has to be read back from tensor memory, and 8192 x 11008 x 4096 took 403 us (and 625 us with a scale per
+// column of B) against 2 x 8192 x 11008 x 4096 operations in the tensor pipe.
 //
 // Both operands are addressed in place, whatever their orientation: a K-major operand (reduction contiguous) arrives as
-// [128 rows x 128 bytes] boxes, an MN-major one (rows of the product contiguous) as [128 k x 128 bytes] boxes, so the input
+// [rows x 128 bytes] boxes, an MN-major one (rows of the product contiguous) as [128 k x 128 bytes] boxes, so the input
 // gradient reads the forward weight's codes and the weight gradient reads row-major activations without transposed copies.
-// Scales are read through strides: per row of an operand (index shift 0) or per 128 rows (shift 7).
+// Scales are fp32 and read through strides, per row of an operand (index shift 0) or per 128 rows (shift 7); one that is no
+// positive power of two becomes NaN.
 //
-// CTA layout (384 threads, three warpgroups): warp 0 = TMA producer, warp 1 = MMA issuer and tensor-memory owner, warps 2 and 3
-// = scales: they run ahead of the promotion by up to eight blocks and leave each block's factors in a shared-memory ring, so
-// that no promotion ever waits for a scale to come from L2; warps 4..11 = promotion and epilogue: four lane quadrants x two column halves, every thread owns
-// one row and BN / 2 columns of the tile, held in registers. The first warpgroup hands registers to the other two (72 against
-// 2 x 216 of the 3 x 168 at launch). All waits are bounded (common.cuh).
+// CTA layout (384 threads): warp 0 = TMA producer, warp 1 = MMA issuer and tensor-memory owner, warps 2 and 3 = scales (they
+// fetch a few blocks ahead, turn them into exponents and lay those out beside the operands of a stage as the tensor core wants
+// them), warps 4..11 = epilogue (four lane quadrants x two column halves; through shared memory, so that global accesses are
+// whole 128-byte lines). All waits are bounded (common.cuh).
 
 #include "common.cuh"
 #include "ocb_api.h"
@@ -28,22 +30,26 @@ constexpr int BM = 128;
 constexpr int BKE = 128;  // reduction elements (= bytes) per stage = one scale block
 constexpr int A_BYTES = BM * BKE;
 constexpr int THREADS = 384;
-constexpr int REGS_FEED = 72, REGS_SUM = 216;  // registers a thread after the hand-over: 72 + 2 * 216 = 3 * 168
 constexpr int EPI_WARPS = 8;
-constexpr int SCALE_SLOTS = 8, SCALE_BATCH = 4;  // ring of factors; blocks whose scales are fetched together
+constexpr int SCALE_BATCH = 4;  // blocks whose scales are fetched together
 constexpr uint32_t TMEM_COLS = 512;
+constexpr int SF_BLOCK = 512;  // scales of 128 rows for one stage
 
 enum : int { EPI_BF16 = 0, EPI_F32_ACC = 1, EPI_F32 = 2 };
 
-template <int BN>
+// CTAS = 2: a pair of CTAs (cta_group::2) computes 2 x 128 rows together; each stages its own rows of A and half of B.
+template <int BN, int CTAS>
 struct Tile {
-  static constexpr int STAGE_BYTES = A_BYTES + BN * BKE;
-  static constexpr int STAGES = BN == 256 ? 4 : 6;
-  static constexpr int ACCS = static_cast<int>(TMEM_COLS) / BN;  // partial tiles in flight between the issuer and the epilogue
-  static constexpr int COLS = BN / 2;                            // columns per epilogue thread
-  // a block's factors: per row and column half (sa * sb), or sa per row and sb per column
-  static constexpr int FACTORS = BM + BN;
-  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + SCALE_SLOTS * FACTORS * 4 + 1024 /*alignment slack*/ + 512 /*barriers*/;
+  static constexpr int B_ROWS = BN / CTAS;  // rows of B that one CTA stages
+  static constexpr int STAGE_BYTES = A_BYTES + B_ROWS * BKE;
+  static constexpr int STAGES = 5;
+  static constexpr int SF_BYTES = SF_BLOCK * (1 + (BN + 127) / 128);
+  static constexpr int ACCS = BN == 256 ? 1 : 2;     // accumulators in tensor memory
+  static constexpr uint32_t SF_COL = ACCS * BN;      // two alternating sets of scale columns: 4 of A, 4 per 128 columns of B
+  static constexpr uint32_t SF_COLS = SF_BYTES / SF_BLOCK * 4;
+  static constexpr int COLS = BN / 2;                // columns per epilogue thread
+  static constexpr int STG_BYTES = 32 * 128;         // staging of one epilogue warp: 32 rows x 128 bytes
+  static constexpr int SMEM_BYTES = STAGES * (STAGE_BYTES + SF_BYTES) + EPI_WARPS * STG_BYTES + 1024 /*alignment slack*/ + 256;
 };
 
 struct Scales {
@@ -58,23 +64,32 @@ struct Params {
   int M, N, K;
   int group_m;  // rasterisation: row tiles that share a column tile while it is in L2
   int a_mn, b_mn;
+  int aligned;  // C rows start on 16-byte boundaries
   Scales sa, sb;
   const int* offsets;  // [num_groups + 1] row boundaries of the groups, or null: one product
   int num_groups;
   int* status;
 };
 
+// The exponent byte of a scale, four times: what the tensor core wants for the four K = 32 steps of a block.
+__device__ __forceinline__ uint32_t exponent4(float scale) {
+  const uint32_t bits = __float_as_uint(scale);
+  return ((bits & 0x807fffffu) != 0u || bits == 0u ? 0xffu : bits >> 23) * 0x01010101u;
+}
+
 struct TileInfo {
   int m0, m_end, n0, g;
 };
 
+// Walks the tiles (bm x bn) of one CTA or one pair.
+template <int bm, int bn, int CTAS>
 struct Walker {
   const Params& p;
-  int bn, tiles_m, tiles_n, tile, g, base;
-  __device__ Walker(const Params& params, int bn_) : p(params), bn(bn_), g(0), base(0) {
-    tiles_m = (p.M + BM - 1) / BM;
+  int tiles_m, tiles_n, tile, g, base;
+  __device__ Walker(const Params& params) : p(params), g(0), base(0) {
+    tiles_m = (p.M + bm - 1) / bm;
     tiles_n = (p.N + bn - 1) / bn;
-    tile = blockIdx.x;
+    tile = blockIdx.x / CTAS;
   }
   __device__ bool next(TileInfo& t) {
     if (p.offsets == nullptr) {
@@ -83,7 +98,7 @@ struct Walker {
       const int grp = tile / per_group, first_m = grp * p.group_m;
       const int gm = min(tiles_m - first_m, p.group_m);
       const int r = tile - grp * per_group;
-      t.m0 = (first_m + r % gm) * BM;
+      t.m0 = (first_m + r % gm) * bm;
       t.m_end = p.M;
       t.n0 = (r / gm) * bn;
       t.g = 0;
@@ -93,110 +108,227 @@ struct Walker {
         if (g >= p.num_groups) return false;
         lo = min(max(p.offsets[g], 0), p.M);  // whatever the boundaries hold, no row outside the matrix is touched
         rows = max(min(p.offsets[g + 1], p.M) - lo, 0);
-        tm_g = (rows + BM - 1) / BM;
+        tm_g = (rows + bm - 1) / bm;
         if (tile < base + tm_g * tiles_n) break;
         base += tm_g * tiles_n;
         ++g;
       }
       const int local = tile - base;
-      t.m0 = lo + (local % tm_g) * BM;
+      t.m0 = lo + (local % tm_g) * bm;
       t.m_end = lo + rows;
       t.n0 = (local / tm_g) * bn;
       t.g = g;
     }
-    tile += gridDim.x;
+    tile += gridDim.x / CTAS;
     return true;
   }
 };
 
+// A waiting thread asks to be suspended (for up to 20 us) before it starts to look at the clock.
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.b32 %0, 1, 0, p;\n\t"
+      "}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity), "r"(20000u)
+      : "memory");
+  if (ok) return true;
+  return mbar_wait_bounded(bar, parity, abort_flag, status, code);
+}
+
+// ---- CTA pairs ---------------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t cluster_ctarank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t map_to_cta(uint32_t smem_addr, uint32_t cta_rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr), "r"(cta_rank));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Arrive on an mbarrier of any CTA of the cluster (address from map_to_cta).
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// Tiled loads of a CTA: into its own shared memory; of a pair, the bytes count on a barrier that may be the other CTA's.
+template <int CTAS>
+__device__ __forceinline__ void load_2d(void* smem_dst, const CUtensorMap* desc, uint64_t* bar, uint32_t pair_bar, int32_t c0,
+                                        int32_t c1) {
+  if (CTAS == 1) {
+    tma_load_2d(smem_dst, desc, bar, c0, c1);
+  } else {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+        ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(desc)), "r"(pair_bar), "r"(c0), "r"(c1)
+        : "memory");
+  }
+}
+template <int CTAS>
+__device__ __forceinline__ void load_3d(void* smem_dst, const CUtensorMap* desc, uint64_t* bar, uint32_t pair_bar, int32_t c0,
+                                        int32_t c1, int32_t c2) {
+  if (CTAS == 1) {
+    tma_load_3d(smem_dst, desc, bar, c0, c1, c2);
+  } else {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+        ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(desc)), "r"(pair_bar), "r"(c0), "r"(c1), "r"(c2)
+        : "memory");
+  }
+}
+// D (+)= (A * SFA) (B * SFB)^T for K = 32 with E8M0 scales in tensor memory; issued by one thread (of a pair: the leader's).
+template <int CTAS>
+__device__ __forceinline__ void umma(uint32_t tmem_d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t tsfa,
+                                     uint32_t tsfb, uint32_t accumulate) {
+  if (CTAS == 1) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        ".reg .b64 da, db;\n\t"
+        "mov.b64 da, {%1, %3};\n\t"
+        "mov.b64 db, {%2, %3};\n\t"
+        "setp.ne.b32 p, %7, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale [%0], da, db, %4, [%5], [%6], p;\n\t"
+        "}\n" ::"r"(tmem_d),
+        "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(tsfa), "r"(tsfb), "r"(accumulate)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        ".reg .b64 da, db;\n\t"
+        "mov.b64 da, {%1, %3};\n\t"
+        "mov.b64 db, {%2, %3};\n\t"
+        "setp.ne.b32 p, %7, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale [%0], da, db, %4, [%5], [%6], p;\n\t"
+        "}\n" ::"r"(tmem_d),
+        "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(tsfa), "r"(tsfb), "r"(accumulate)
+        : "memory");
+  }
+}
+// 32 rows x 16 bytes of scales from shared memory into 4 columns, replicated to the four lane quadrants; of a pair, each CTA
+// copies from its own shared memory into its own tensor memory.
+template <int CTAS>
+__device__ __forceinline__ void sf_copy(uint32_t tmem_dst, uint32_t smem_src) {
+  // no swizzle, 8-row x 16-byte core matrices every 128 bytes
+  const uint64_t desc = static_cast<uint64_t>((smem_src >> 4) & 0x3FFFu) | (static_cast<uint64_t>(128u >> 4) << 32) | (1ull << 46);
+  if (CTAS == 1) asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem_dst), "l"(desc) : "memory");
+  else asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem_dst), "l"(desc) : "memory");
+}
+// `bar` (and the other CTA's at the same offset) observes the completion of the MMAs issued so far.
+template <int CTAS>
+__device__ __forceinline__ void commit(uint64_t* bar, uint32_t peer_bar) {
+  if (CTAS == 1) {
+    umma_commit(bar);
+  } else {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(peer_bar) : "memory");
+  }
+}
+
 // Waits for the tensor-memory loads issued so far. The registers pass through, so that nothing that reads them can be
 // scheduled ahead of the wait.
-__device__ __forceinline__ void tmem_ld_wait_for(uint32_t (&r)[16]) {
+__device__ __forceinline__ void tmem_ld_wait_for(uint32_t (&r)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
-                 "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]),
+                 "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
+                 "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
                :
                : "memory");
 }
 
-// 32 consecutive columns of one row; v holds 16 packed pairs.
+// 32 consecutive columns of one row, for outputs whose rows are not 16-byte aligned.
 template <int EPI>
-__device__ __forceinline__ void store_chunk(const Params& p, long long row, int col, const uint64_t* v) {
-  float f[32];
+__device__ __forceinline__ void store_chunk(const Params& p, long long row, int col, const uint32_t* v) {
 #pragma unroll
-  for (int j = 0; j < 16; ++j) unpack_f32x2(v[j], f[2 * j], f[2 * j + 1]);
-  if (EPI == EPI_BF16) {
-    __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(p.C) + row * p.ldc + col;
-    if (col + 32 <= p.N && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        uint4 o;
-        o.x = pack_bf16x2(f[8 * q + 0], f[8 * q + 1]);
-        o.y = pack_bf16x2(f[8 * q + 2], f[8 * q + 3]);
-        o.z = pack_bf16x2(f[8 * q + 4], f[8 * q + 5]);
-        o.w = pack_bf16x2(f[8 * q + 6], f[8 * q + 7]);
-        reinterpret_cast<uint4*>(dst)[q] = o;
-      }
+  for (int j = 0; j < 32; ++j) {
+    if (col + j >= p.N) continue;
+    const float f = __uint_as_float(v[j]);
+    if (EPI == EPI_BF16) {
+      reinterpret_cast<__nv_bfloat16*>(p.C)[row * p.ldc + col + j] = __float2bfloat16_rn(f);
     } else {
-#pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (col + j < p.N) dst[j] = __float2bfloat16_rn(f[j]);
-    }
-  } else {
-    float* dst = reinterpret_cast<float*>(p.C) + row * p.ldc + col;
-    if (col + 32 <= p.N && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
-#pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        float4 o = make_float4(f[4 * q], f[4 * q + 1], f[4 * q + 2], f[4 * q + 3]);
-        if (EPI == EPI_F32_ACC) {
-          const float4 old = reinterpret_cast<const float4*>(dst)[q];
-          o.x += old.x; o.y += old.y; o.z += old.z; o.w += old.w;
-        }
-        reinterpret_cast<float4*>(dst)[q] = o;
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (col + j < p.N) dst[j] = EPI == EPI_F32_ACC ? dst[j] + f[j] : f[j];
+      float* dst = reinterpret_cast<float*>(p.C) + row * p.ldc + col + j;
+      *dst = EPI == EPI_F32_ACC ? *dst + f : f;
     }
   }
 }
 
-// BCOL: the scales of B differ from row to row of B (= output column); otherwise B has one scale per 128 of its rows, which
-// is one number for everything a thread owns.
-template <int BN, bool BCOL, int EPI>
+// ---- epilogue staging ------------------------------------------------------------------------------------------------
+// 16-byte slot `chunk` (0..7) of staged row `row` (0..31); the XOR keeps both the row-per-thread and the 8-lanes-per-row
+// access patterns free of bank conflicts.
+__device__ __forceinline__ uint4* stg_slot(uint8_t* stg, int row, int chunk) {
+  return reinterpret_cast<uint4*>(stg + row * 128 + ((chunk ^ (row & 7)) << 4));
+}
+// Moves a staged block to global memory, 8 lanes per 128-byte row; `bytes` of every row are inside the matrix.
+template <int EPI>
+__device__ __forceinline__ void stg_store(uint8_t* stg, uint8_t* dst0, long long ld_bytes, int rows, int bytes, int lane) {
+  const int cc = (lane & 7) * 16;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int rr = i * 4 + (lane >> 3);
+    if (rr >= rows || cc >= bytes) continue;
+    const uint4 v = *stg_slot(stg, rr, lane & 7);
+    uint8_t* dst = dst0 + rr * ld_bytes + cc;
+    if (EPI == EPI_F32_ACC) {
+      const float f[4] = {__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w)};
+      if (cc + 16 <= bytes) {  // one addition per element, performed in L2
+        asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(dst), "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3])
+                     : "memory");
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (cc + 4 * j < bytes) atomicAdd(reinterpret_cast<float*>(dst) + j, f[j]);
+      }
+    } else if (cc + 16 <= bytes) {
+      *reinterpret_cast<uint4*>(dst) = v;
+    } else {
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int j = 0; j < 8; ++j)  // 2-byte pieces serve both element sizes
+        if (cc + 2 * j < bytes) reinterpret_cast<uint16_t*>(dst)[j] = static_cast<uint16_t>(w[j >> 1] >> (16 * (j & 1)));
+    }
+  }
+}
+
+template <int BN, int CTAS, int EPI>
 __global__ void __launch_bounds__(THREADS, 1)
 gemm_block_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b, const Params p) {
-  using T = Tile<BN>;
+  using T = Tile<BN, CTAS>;
+  using Walk = Walker<BM * CTAS, BN, CTAS>;
   constexpr int STAGES = T::STAGES, ACCS = T::ACCS, COLS = T::COLS, STAGE_BYTES = T::STAGE_BYTES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* factors = reinterpret_cast<float*>(smem + STAGES * STAGE_BYTES);  // [SCALE_SLOTS][FACTORS]
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(factors + SCALE_SLOTS * T::FACTORS);
+  uint8_t* sf_smem = smem + STAGES * STAGE_BYTES;
+  uint8_t* stg_smem = sf_smem + STAGES * T::SF_BYTES;
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(stg_smem + EPI_WARPS * T::STG_BYTES);
   uint64_t* empty_bar = full_bar + STAGES;
   uint64_t* tfull_bar = empty_bar + STAGES;
   uint64_t* tempty_bar = tfull_bar + ACCS;
-  uint64_t* sfull_bar = tempty_bar + ACCS;
-  uint64_t* sempty_bar = sfull_bar + SCALE_SLOTS;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sempty_bar + SCALE_SLOTS);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty_bar + ACCS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const int num_kb = (p.K + BKE - 1) / BKE;
+  const uint32_t cta = CTAS == 2 ? cluster_ctarank() : 0u;  // 0 = leader of the pair
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&full_bar[s], 1);
+      mbar_init(&full_bar[s], 1 + 2 * CTAS);  // the producer's byte count and the scale warps (of both CTAs)
       mbar_init(&empty_bar[s], 1);
     }
     for (int a = 0; a < ACCS; ++a) {
       mbar_init(&tfull_bar[a], 1);
-      mbar_init(&tempty_bar[a], EPI_WARPS);
-    }
-    for (int i = 0; i < SCALE_SLOTS; ++i) {
-      mbar_init(&sfull_bar[i], 2);
-      mbar_init(&sempty_bar[i], EPI_WARPS);
+      mbar_init(&tempty_bar[a], EPI_WARPS * CTAS);
     }
     *abort_flag = 0;
     fence_mbar_init();
@@ -206,42 +338,44 @@ gemm_block_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
     tma_prefetch_desc(&tma_b);
   }
   if (warp == 1) {
-    tmem_alloc(tmem_slot, TMEM_COLS);
-    tmem_relinquish();
+    if (CTAS == 1) {
+      tmem_alloc(tmem_slot, TMEM_COLS);
+      tmem_relinquish();
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(TMEM_COLS) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
   }
   tc_fence_before();
   __syncthreads();
+  if (CTAS == 2) cluster_sync_all();  // the other CTA's barriers are initialised before anything is signalled across
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
-  if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_FEED));
   if (warp == 0) {
     // ------------------------------------------------------------------ producer
     if (lane == 0) {
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
-      Walker walker(p, BN);
+      Walk walker(p);
       TileInfo t;
       while (ok && walker.next(t)) {
+        const int m0 = t.m0 + static_cast<int>(cta) * BM, n0 = t.n0 + static_cast<int>(cta) * T::B_ROWS;
         for (int kb = 0; kb < num_kb; ++kb) {
-          ok = mbar_wait_bounded(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, kStatusTimeoutProducer);
+          ok = wait_for(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, kStatusTimeoutProducer);
           if (!ok) break;
           uint8_t* sa = smem + stage * STAGE_BYTES;
           uint8_t* sb = sa + A_BYTES;
           const int k0 = kb * BKE;
-          mbar_arrive_expect_tx(&full_bar[stage], STAGE_BYTES);
+          if (cta == 0) mbar_arrive_expect_tx(&full_bar[stage], CTAS * STAGE_BYTES);
+          const uint32_t pair_bar = CTAS == 2 ? map_to_cta(smem_u32(&full_bar[stage]), 0) : 0u;
           // innermost coordinates are k0 (K-major) or tile origins (MN-major): multiples of 128 bytes either way; group
           // boundaries only enter the outer coordinate of a K-major A
-          if (p.a_mn) tma_load_2d(sa, &tma_a, &full_bar[stage], t.m0, k0);
-          else tma_load_2d(sa, &tma_a, &full_bar[stage], k0, t.m0);
-          if (p.b_mn) {
-#pragma unroll
-            for (int j = 0; j < BN / 128; ++j)
-              tma_load_3d(sb + j * (128 * BKE), &tma_b, &full_bar[stage], t.n0 + j * 128, k0, t.g);
-          } else {
-            tma_load_3d(sb, &tma_b, &full_bar[stage], k0, t.n0, t.g);
-          }
+          if (p.a_mn) load_2d<CTAS>(sa, &tma_a, &full_bar[stage], pair_bar, m0, k0);
+          else load_2d<CTAS>(sa, &tma_a, &full_bar[stage], pair_bar, k0, m0);
+          if (p.b_mn) load_3d<CTAS>(sb, &tma_b, &full_bar[stage], pair_bar, n0, k0, t.g);
+          else load_3d<CTAS>(sb, &tma_b, &full_bar[stage], pair_bar, k0, n0, t.g);
           if (++stage == STAGES) { stage = 0; phase ^= 1u; }
         }
       }
@@ -250,168 +384,178 @@ gemm_block_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
       }
     }
   } else if (warp == 1) {
-    // ------------------------------------------------------------------ issuer
-    if (lane == 0) {
-      // K-major: 8-row swizzle atoms 1024 bytes apart, K = 32 advances 32 bytes along the line. MN-major: 128-column boxes
-      // 16 KB apart (leading offset), 8 k-rows per 1024 bytes, K = 32 advances 32 lines.
+    // ------------------------------------------------------------------ issuer (of a pair: the leader's)
+    if (lane == 0 && cta == 0) {
+      // K-major: 8-row swizzle atoms 1024 bytes apart, K = 32 advances 32 bytes along the line. MN-major: one 128-column box,
+      // 8 k-rows per 1024 bytes, K = 32 advances 32 lines.
       constexpr uint32_t kDescHi = desc_hi_sw128(1024);
-      const uint32_t idesc = make_idesc_e4m3(BM, BN) | (static_cast<uint32_t>(p.a_mn) << 15) | (static_cast<uint32_t>(p.b_mn) << 16);
+      // kind::mxf8f6f4: e4m3 A and B, majors at bits 15 and 16, N >> 3 at 17, E8M0 scales (23), M >> 4 at 24; the scale byte of a
+      // K = 32 step at 29 (A) and 4 (B)
+      const uint32_t idesc = (static_cast<uint32_t>(p.a_mn) << 15) | (static_cast<uint32_t>(p.b_mn) << 16) |
+                             (static_cast<uint32_t>(BN >> 3) << 17) | (1u << 23) | (static_cast<uint32_t>(BM * CTAS >> 4) << 24);
       const uint32_t a_step = p.a_mn ? 256u : 2u, b_step = p.b_mn ? 256u : 2u;
       const uint32_t a_lo0 = desc_lo_sw128(smem_u32(smem), 16);
-      const uint32_t b_lo0 = desc_lo_sw128(smem_u32(smem) + A_BYTES, p.b_mn ? 128 * BKE : 16);
+      const uint32_t b_lo0 = desc_lo_sw128(smem_u32(smem) + A_BYTES, 16);
+      const uint32_t sf0 = smem_u32(sf_smem);
+      const uint32_t empty_peer = CTAS == 2 ? map_to_cta(smem_u32(empty_bar), 1) : 0u;
+      const uint32_t tfull_peer = CTAS == 2 ? map_to_cta(smem_u32(tfull_bar), 1) : 0u;
       int stage = 0, acc = 0;
-      uint32_t phase = 0, acc_phase = 0;
+      uint32_t phase = 0, acc_phase = 0, sf_set = 0;
       bool ok = true;
-      Walker walker(p, BN);
+      Walk walker(p);
       TileInfo t;
       while (ok && walker.next(t)) {
+        ok = wait_for(&tempty_bar[acc], acc_phase ^ 1u, abort_flag, p.status, kStatusTimeoutMma);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + acc * BN;
         for (int kb = 0; kb < num_kb; ++kb) {
-          ok = mbar_wait_bounded(&tempty_bar[acc], acc_phase ^ 1u, abort_flag, p.status, kStatusTimeoutMma) &&
-               mbar_wait_bounded(&full_bar[stage], phase, abort_flag, p.status, kStatusTimeoutMma);
+          ok = wait_for(&full_bar[stage], phase, abort_flag, p.status, kStatusTimeoutMma);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t d_tmem = tmem_base + acc * BN;
+          // copies and MMAs of one thread execute in issue order
+          const uint32_t tsfa = tmem_base + T::SF_COL + sf_set * T::SF_COLS, tsfb = tsfa + 4;
+          const uint32_t ss = sf0 + stage * T::SF_BYTES;
+          sf_copy<CTAS>(tsfa, ss);
+#pragma unroll
+          for (uint32_t b = 0; b < (BN + 127) / 128; ++b) sf_copy<CTAS>(tsfb + 4 * b, ss + SF_BLOCK * (1 + b));
           const uint32_t a_lo = a_lo0 + stage * (STAGE_BYTES >> 4), b_lo = b_lo0 + stage * (STAGE_BYTES >> 4);
 #pragma unroll
           for (uint32_t k = 0; k < BKE / 32; ++k)
-            umma_ss_lean<1>(d_tmem, a_lo + k * a_step, b_lo + k * b_step, kDescHi, idesc, k != 0);
-          umma_commit(&empty_bar[stage]);
-          umma_commit(&tfull_bar[acc]);
+            umma<CTAS>(d_tmem, a_lo + k * a_step, b_lo + k * b_step, kDescHi, idesc | (k << 29) | (k << 4), tsfa | (k << 30),
+                       tsfb | (k << 30), (kb | static_cast<int>(k)) != 0);
+          commit<CTAS>(&empty_bar[stage], empty_peer + stage * 8);
+          sf_set ^= 1u;
           if (++stage == STAGES) { stage = 0; phase ^= 1u; }
-          if (++acc == ACCS) { acc = 0; acc_phase ^= 1u; }
         }
+        if (ok) commit<CTAS>(&tfull_bar[acc], tfull_peer + acc * 8);
+        if (++acc == ACCS) { acc = 0; acc_phase ^= 1u; }
       }
     }
   } else if (warp < 4) {
     // ------------------------------------------------------------------ scales (warps 2 and 3)
     const int t64 = threadIdx.x - 64;
-    int slot = 0;
+    constexpr int PER = (BM + BN) / 64;  // rows whose scales a thread carries: t64 + 64 i of A, then of B
+    const uint32_t full_leader = CTAS == 2 ? map_to_cta(smem_u32(full_bar), 0) : 0u;
+    int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
-    Walker walker(p, BN);
+    Walk walker(p);
     TileInfo t;
-    constexpr int PER = BCOL ? T::FACTORS / 64 : BM / 64;  // scales a thread fetches per block (and, without BCOL, two of B)
     while (ok && walker.next(t)) {
       const float* src[PER];
       long long step[PER];
 #pragma unroll
-      for (int i = 0; i < PER; ++i) {  // factor t64 + 64 i: a row of A, or a column
+      for (int i = 0; i < PER; ++i) {
         const int f = t64 + 64 * i;
         const bool is_a = i < BM / 64;
-        const int at = is_a ? t.m0 + f : t.n0 + f - BM;
+        const int at = is_a ? t.m0 + static_cast<int>(cta) * BM + f : t.n0 + f - BM;
         const Scales& sc = is_a ? p.sa : p.sb;
         step[i] = sc.k_stride;
-        src[i] = at < (is_a ? t.m_end : p.N) ? sc.p + (is_a ? 0 : t.g * sc.group_stride) + static_cast<long long>(at >> sc.shift) * sc.i_stride
-                                             : nullptr;
-      }
-      const float* tile[2] = {nullptr, nullptr};
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int col = t.n0 + h * COLS;
-        if (!BCOL && col < p.N) tile[h] = p.sb.p + t.g * p.sb.group_stride + static_cast<long long>(col >> p.sb.shift) * p.sb.i_stride;
+        src[i] = at < (is_a ? t.m_end : p.N)
+                     ? sc.p + (is_a ? 0 : t.g * sc.group_stride) + static_cast<long long>(at >> sc.shift) * sc.i_stride
+                     : nullptr;
       }
       for (int kb0 = 0; ok && kb0 < num_kb; kb0 += SCALE_BATCH) {
-        float v[SCALE_BATCH][PER], w[SCALE_BATCH][2];
+        float v[SCALE_BATCH][PER];
 #pragma unroll
-        for (int b = 0; b < SCALE_BATCH; ++b) {
-          const bool live = kb0 + b < num_kb;
+        for (int b = 0; b < SCALE_BATCH; ++b)
 #pragma unroll
-          for (int i = 0; i < PER; ++i) v[b][i] = live && src[i] != nullptr ? __ldg(src[i] + (kb0 + b) * step[i]) : 0.f;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) w[b][h] = live && tile[h] != nullptr ? __ldg(tile[h] + (kb0 + b) * p.sb.k_stride) : 0.f;
-        }
+          for (int i = 0; i < PER; ++i)  // rows outside the matrix: any valid scale, their products are not stored
+            v[b][i] = kb0 + b < num_kb && src[i] != nullptr ? __ldg(src[i] + (kb0 + b) * step[i]) : 1.f;
 #pragma unroll
         for (int b = 0; b < SCALE_BATCH; ++b) {
           if (kb0 + b >= num_kb) break;
-          ok = mbar_wait_bounded(&sempty_bar[slot], phase ^ 1u, abort_flag, p.status, kStatusTimeoutProducer);
+          ok = wait_for(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, kStatusTimeoutProducer);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
-          float* dst = factors + slot * T::FACTORS;
-          if (BCOL) {
+          uint32_t* dst = reinterpret_cast<uint32_t*>(sf_smem + stage * T::SF_BYTES);
 #pragma unroll
-            for (int i = 0; i < PER; ++i) dst[t64 + 64 * i] = v[b][i];
-          } else {
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-              for (int i = 0; i < PER; ++i) dst[h * BM + t64 + 64 * i] = v[b][i] * w[b][h];
+          for (int i = 0; i < PER; ++i) {  // row r of a 128-row block: 32-bit word 4 (r % 32) + r / 32 of its 512 bytes
+            const int f = t64 + 64 * i;
+            dst[(f >> 7) * (SF_BLOCK / 4) + (f & 31) * 4 + ((f >> 5) & 3)] = exponent4(v[b][i]);
           }
+          fence_proxy_async_smem();  // the tensor core's copy reads what the threads wrote
           __syncwarp();
-          if (lane == 0) mbar_arrive(&sfull_bar[slot]);
-          if (++slot == SCALE_SLOTS) { slot = 0; phase ^= 1u; }
+          if (lane == 0) {
+            if (CTAS == 1) mbar_arrive(&full_bar[stage]);
+            else mbar_arrive_cluster(full_leader + stage * 8);
+          }
+          if (++stage == STAGES) { stage = 0; phase ^= 1u; }
         }
       }
     }
   } else {
-    // ------------------------------------------------------------------ promotion and epilogue
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SUM));
+    // ------------------------------------------------------------------ epilogue
     const int quad = warp & 3, half = (warp - 4) >> 2;
+    uint8_t* stg = stg_smem + (warp - 4) * T::STG_BYTES;
     const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + half * COLS;
-    // where this thread's factor sits in a slot, and where the column factors of its half start
-    const float* my_factor = factors + (BCOL ? 0 : half * BM) + quad * 32 + lane;
-    const float* col_factors = factors + BM + half * COLS;
-    int acc = 0, slot = 0;
-    uint32_t acc_phase = 0, slot_phase = 0;
+    const uint32_t tempty_leader = CTAS == 2 ? map_to_cta(smem_u32(tempty_bar), 0) : 0u;
+    int acc = 0;
+    uint32_t acc_phase = 0;
     bool ok = true;
-    Walker walker(p, BN);
+    Walk walker(p);
     TileInfo t;
     while (ok && walker.next(t)) {
-      uint64_t sum[COLS / 2];
+      ok = wait_for(&tfull_bar[acc], acc_phase, abort_flag, p.status, kStatusTimeoutEpilogue);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t r[COLS / 32][32];
 #pragma unroll
-      for (int j = 0; j < COLS / 2; ++j) sum[j] = 0ull;
-      for (int kb = 0; kb < num_kb; ++kb) {
-        ok = mbar_wait_bounded(&sfull_bar[slot], slot_phase, abort_flag, p.status, kStatusTimeoutEpilogue) &&
-             mbar_wait_bounded(&tfull_bar[acc], acc_phase, abort_flag, p.status, kStatusTimeoutEpilogue);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t t_acc = t_row + acc * BN;
-        uint32_t r[2][16];
-        tmem_ld_32x16(t_acc, r[0]);
-        const float s = my_factor[slot * T::FACTORS];
-        const uint64_t s2 = pack_f32x2(s, s);
-        const float* cf = col_factors + slot * T::FACTORS;
-        tmem_ld_wait_for(r[0]);
+      for (int c = 0; c < COLS / 32; ++c) tmem_ld_32x32(t_row + acc * BN + c * 32, r[c]);
 #pragma unroll
-        for (int c = 0; c < COLS / 16; ++c) {
-          if (c + 1 < COLS / 16) {
-            tmem_ld_32x16(t_acc + (c + 1) * 16, r[(c + 1) & 1]);
-          } else {
-            tc_fence_before();
-            if (lane == 0) mbar_arrive(&tempty_bar[acc]);
-          }
-#pragma unroll
-          for (int j = 0; j < 8; j += 2) {
-            uint64_t f0 = s2, f1 = s2;
-            if (BCOL) {
-              const float4 col = *reinterpret_cast<const float4*>(cf + c * 16 + 2 * j);
-              f0 = mul_f32x2(s2, pack_f32x2(col.x, col.y));
-              f1 = mul_f32x2(s2, pack_f32x2(col.z, col.w));
-            }
-            sum[c * 8 + j] = fma_f32x2(pack_u32x2(r[c & 1][2 * j], r[c & 1][2 * j + 1]), f0, sum[c * 8 + j]);
-            sum[c * 8 + j + 1] = fma_f32x2(pack_u32x2(r[c & 1][2 * j + 2], r[c & 1][2 * j + 3]), f1, sum[c * 8 + j + 1]);
-          }
-          if (c + 1 < COLS / 16) tmem_ld_wait_for(r[(c + 1) & 1]);
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sempty_bar[slot]);
-        if (++acc == ACCS) { acc = 0; acc_phase ^= 1u; }
-        if (++slot == SCALE_SLOTS) { slot = 0; slot_phase ^= 1u; }
+      for (int c = 0; c < COLS / 32; ++c) tmem_ld_wait_for(r[c]);
+      tc_fence_before();  // the accumulator is in registers: the issuer may start the next tile
+      if (lane == 0) {
+        if (CTAS == 1) mbar_arrive(&tempty_bar[acc]);
+        else mbar_arrive_cluster(tempty_leader + acc * 8);
       }
-      const int row = t.m0 + quad * 32 + lane, col0 = t.n0 + half * COLS;
-      if (ok && row < t.m_end) {
+      if (++acc == ACCS) { acc = 0; acc_phase ^= 1u; }
+      const int row0 = t.m0 + static_cast<int>(cta) * BM + quad * 32, col0 = t.n0 + half * COLS;
+      const int rows = min(32, t.m_end - row0);
+      if (rows <= 0) continue;
+      if (!p.aligned) {
 #pragma unroll
         for (int c = 0; c < COLS / 32; ++c)
-          if (col0 + c * 32 < p.N) store_chunk<EPI>(p, row, col0 + c * 32, sum + c * 16);
+          if (lane < rows) store_chunk<EPI>(p, row0 + lane, col0 + c * 32, r[c]);
+        continue;
+      }
+      constexpr int ES = EPI == EPI_BF16 ? 2 : 4, CHUNK = 128 / ES;  // columns of a staged block
+#pragma unroll
+      for (int c = 0; c < COLS / CHUNK; ++c) {
+        const int bytes = min(128, (p.N - (col0 + c * CHUNK)) * ES);
+        if (bytes <= 0) break;
+        __syncwarp();
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          uint4 o;
+          if (EPI == EPI_BF16) {
+            const uint32_t* s = &r[2 * c + (q >> 2)][(q & 3) * 8];
+            o.x = pack_bf16x2(__uint_as_float(s[0]), __uint_as_float(s[1]));
+            o.y = pack_bf16x2(__uint_as_float(s[2]), __uint_as_float(s[3]));
+            o.z = pack_bf16x2(__uint_as_float(s[4]), __uint_as_float(s[5]));
+            o.w = pack_bf16x2(__uint_as_float(s[6]), __uint_as_float(s[7]));
+          } else {
+            const uint32_t* s = &r[c][q * 4];
+            o = make_uint4(s[0], s[1], s[2], s[3]);
+          }
+          *stg_slot(stg, lane, q) = o;
+        }
+        __syncwarp();
+        stg_store<EPI>(stg, reinterpret_cast<uint8_t*>(p.C) + (static_cast<long long>(row0) * p.ldc + col0 + c * CHUNK) * ES,
+                       p.ldc * ES, rows, bytes, lane);
       }
     }
   }
 
   tc_fence_before();
   __syncthreads();
+  if (CTAS == 2) cluster_sync_all();  // nothing of the other CTA signals into this one's shared memory any more
   if (warp == 1) {
     __syncwarp();
-    tmem_dealloc(tmem_base, TMEM_COLS);
+    if (CTAS == 1) tmem_dealloc(tmem_base, TMEM_COLS);
+    else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
   }
 }
 
@@ -421,24 +565,33 @@ static int num_sms() {
   return n;
 }
 
-template <int BN, bool BCOL, int EPI>
+template <int BN, int CTAS, int EPI>
 static int launch(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, long long max_tiles, cudaStream_t stream) {
-  constexpr int bytes = Tile<BN>::SMEM_BYTES;
-  if (cudaFuncSetAttribute(gemm_block_fp8_kernel<BN, BCOL, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
-    return -3;
-  const int sms = num_sms();
-  if (sms <= 0) return -3;
-  const int grid = max_tiles < sms ? static_cast<int>(max_tiles) : sms;
-  gemm_block_fp8_kernel<BN, BCOL, EPI><<<grid, THREADS, bytes, stream>>>(ta, tb, p);
-  return cudaGetLastError() == cudaSuccess ? 0 : -4;
+  constexpr int bytes = Tile<BN, CTAS>::SMEM_BYTES;
+  auto kernel = gemm_block_fp8_kernel<BN, CTAS, EPI>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return -3;
+  const int units = num_sms() / CTAS;
+  if (units <= 0) return -3;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(static_cast<unsigned>(max_tiles < units ? max_tiles : units) * CTAS);
+  config.blockDim = dim3(THREADS);
+  config.dynamicSmemBytes = bytes;
+  config.stream = stream;
+  cudaLaunchAttribute cluster;
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = CTAS;
+  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+  config.attrs = &cluster;
+  config.numAttrs = CTAS == 2 ? 1 : 0;
+  return cudaLaunchKernelEx(&config, kernel, ta, tb, p) == cudaSuccess ? 0 : -4;
 }
 
-template <int BN, bool BCOL>
+template <int BN, int CTAS>
 static int launch_epi(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, long long max_tiles, int epi, cudaStream_t s) {
   switch (epi) {
-    case EPI_BF16: return launch<BN, BCOL, EPI_BF16>(ta, tb, p, max_tiles, s);
-    case EPI_F32_ACC: return launch<BN, BCOL, EPI_F32_ACC>(ta, tb, p, max_tiles, s);
-    case EPI_F32: return launch<BN, BCOL, EPI_F32>(ta, tb, p, max_tiles, s);
+    case EPI_BF16: return launch<BN, CTAS, EPI_BF16>(ta, tb, p, max_tiles, s);
+    case EPI_F32_ACC: return launch<BN, CTAS, EPI_F32_ACC>(ta, tb, p, max_tiles, s);
+    case EPI_F32: return launch<BN, CTAS, EPI_F32>(ta, tb, p, max_tiles, s);
     default: return -1;
   }
 }
@@ -481,13 +634,14 @@ extern "C" int ocb_gemm_block_fp8(const void* A, const void* B, void* C, const f
   p.offsets = offsets;
   p.num_groups = num_groups;
   p.status = status;
+  p.aligned = (reinterpret_cast<uintptr_t>(C) & 15) == 0 && (ldc * (epilogue == blk::EPI_BF16 ? 2 : 4)) % 16 == 0;
   const int bn = 256;
+  const int ctas = 2;
   CUtensorMap ta, tb;
   if (!blk::make_map(&ta, A, a_mn != 0, M, K, 1, lda, 0, blk::BM, 2)) return -1001;
-  if (!blk::make_map(&tb, B, b_mn != 0, N, K, num_groups, ldb, num_groups > 1 ? b_group_bytes : ldb, bn, 3)) return -2001;
+  if (!blk::make_map(&tb, B, b_mn != 0, N, K, num_groups, ldb, num_groups > 1 ? b_group_bytes : ldb, bn / ctas, 3)) return -2001;
   const long long tiles_n = (N + bn - 1) / bn;
-  const long long tiles_m = (M + blk::BM - 1) / blk::BM + (offsets != nullptr ? num_groups : 0);
+  const long long tiles_m = (M + blk::BM * ctas - 1) / (blk::BM * ctas) + (offsets != nullptr ? num_groups : 0);
   const long long tiles = tiles_m * tiles_n;
-  return sb_shift == 0 ? blk::launch_epi<256, true>(ta, tb, p, tiles, epilogue, stream)
-                       : blk::launch_epi<256, false>(ta, tb, p, tiles, epilogue, stream);
+  return blk::launch_epi<256, 2>(ta, tb, p, tiles, epilogue, stream);
 }

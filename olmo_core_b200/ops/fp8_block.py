@@ -1,9 +1,9 @@
 """
-e4m3 products whose operands carry one fp32 scale per block of 128 along the reduction (``csrc/gemm_block_fp8_sm100.cu``),
+e4m3 products whose operands carry one power-of-two scale per block of 128 along the reduction (``csrc/gemm_block_fp8_sm100.cu``),
 and the quantisers that produce such operands (``csrc/block_quant_sm100.cu``).
 
-Three block forms, all with a power-of-two scale (the smallest one, not below ``2^-126``, that brings the block's largest
-magnitude to 448 or below; 1 for a block of zeros), so that the only rounding is the one to e4m3:
+Three block forms. A block's scale is the smallest power of two, not below ``2^-126``, that brings its largest magnitude to
+448 or below, and 1 for a block of zeros, so that the only rounding is the one to e4m3:
 
 * rows: 128 consecutive elements of a row. Activations and output gradients.
 * columns: 128 consecutive elements of a column. Both operands of the weight gradient, whose reduction runs over the rows.
@@ -16,8 +16,10 @@ Operands keep the orientation of the tensor they come from; no product needs a t
     wgrad     dW = q_columns(dy)^T q_columns(x)    fp32, optionally accumulated into ``main_grad``
 
 Codes are e4m3 bytes (``uint8``, ``float8_e4m3fn`` is accepted too) whose rows start on 16-byte boundaries; the quantisers
-return them that way for any width. The products accept any finite scales, not only powers of two. The scales of an operand
-with one scale per row of the product are stored with the reduction block first: ``[ceil(reduction / 128), rows]``.
+return them that way for any width. The scales of an operand with one scale per row of the product are stored with the
+reduction block first: ``[ceil(reduction / 128), rows]``. The tensor core applies the scales as exponents: they must be positive
+normal powers of two, any other scale makes the results that depend on it NaN (a weight that comes with other scales is
+brought into this form by quantising its values: ``quantize_block_tiles(dequantize_block_tiles(codes, scales))``).
 
 On CPU the functions emulate the same arithmetic in PyTorch: the numerical oracle.
 """
@@ -167,6 +169,12 @@ def _values(q: torch.Tensor) -> torch.Tensor:
     return (q if q.dtype == torch.float8_e4m3fn else q.view(torch.float8_e4m3fn)).float()
 
 
+def _exponent_scales(s: torch.Tensor) -> torch.Tensor:
+    """``s`` as the products see it: NaN where it is no positive normal power of two."""
+    bits = s.contiguous().view(torch.int32)
+    return torch.where(((bits & -0x7F800001) == 0) & (bits > 0) & (bits < 0x7F800000), s, float("nan"))
+
+
 def _spread(s: torch.Tensor, dim: int, n: int) -> torch.Tensor:
     return s.repeat_interleave(BLOCK, dim).narrow(dim, 0, n)
 
@@ -274,6 +282,7 @@ def gemm_fp8_block(
     if K == 0:
         return out if accumulate else out.zero_()
     if not a_q.is_cuda:
+        a_s, b_s = _exponent_scales(a_s), _exponent_scales(b_s)
         a = dequantize_block_columns(a_q, a_s).t() if trans_a else dequantize_block_rows(a_q, a_s)
         if b_tiles:
             b = dequantize_block_tiles(b_q, b_s)
@@ -335,7 +344,8 @@ def grouped_gemm_fp8_block(
     if K == 0:
         return out.zero_()
     if not a_q.is_cuda:
-        a, b, bounds = dequantize_block_rows(a_q, a_s), dequantize_block_tiles(b_q, b_s), offsets.tolist()
+        a, b = dequantize_block_rows(a_q, _exponent_scales(a_s)), dequantize_block_tiles(b_q, _exponent_scales(b_s))
+        bounds = offsets.tolist()
         for g, (lo, hi) in enumerate(zip(bounds[:-1], bounds[1:])):
             out[lo:hi] = (a[lo:hi] @ (b[g].t() if trans_b else b[g])).to(out.dtype)
         return out

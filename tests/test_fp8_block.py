@@ -97,14 +97,14 @@ def test_quantisers_take_strided_input_and_stacks(device):
 
 
 def _operand(shape, seed, form, device):
-    """(codes, scales, fp64 values); scales that are no powers of two."""
+    """(codes, scales, fp64 values); scales other than the ones that fit the codes."""
     x = _rand(shape, seed, device)
     fn, deq = {"rows": (fb.quantize_block_rows, fb.dequantize_block_rows),
                "columns": (fb.quantize_block_columns, fb.dequantize_block_columns),
                "tiles": (fb.quantize_block_tiles, fb.dequantize_block_tiles)}[form]
     q, s = fn(x)
     g = torch.Generator().manual_seed(seed + 1)
-    s = s * (0.5 + torch.rand(s.shape, generator=g)).to(device)
+    s = s * torch.exp2(torch.randint(-6, 7, s.shape, generator=g).float()).to(device)
     expand = {"rows": lambda: s.t().repeat_interleave(128, 1)[:, : shape[1]],
               "columns": lambda: s.repeat_interleave(128, 0)[: shape[0]],
               "tiles": lambda: s.repeat_interleave(128, 0)[: shape[0]].repeat_interleave(128, 1)[:, : shape[1]]}[form]()
@@ -173,6 +173,18 @@ def test_product_repeats_bit_for_bit_and_replays(M, N, K):
     side.synchronize()
     for _, out in graphs:
         assert torch.equal(first, out)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("bad", [3.0, 0.0, -2.0, float("inf"), float("nan"), 1e-40])
+def test_scales_that_are_no_powers_of_two_show_as_nan(bad, device):
+    aq, sa, a = _operand((140, 300), 27, "rows", device)
+    bq, sb, b = _operand((200, 300), 28, "tiles", device)
+    sa[1, 7], sb[1, 2] = bad, bad
+    out = fb.gemm_fp8_block(aq, sa, bq, sb)
+    assert out[7].isnan().all() and out[:, 128:].isnan().all()
+    keep = [i for i in range(140) if i != 7]
+    _assert_product(out[keep, :128], a[keep], b[:128])
 
 
 GROUPS = [[128, 256, 128], [100, 0, 333, 7, 1], [0, 0, 5], [1, 1, 2, 0, 1, 3, 1, 1], [1000, 37, 0, 0, 513, 64, 65, 2]]
