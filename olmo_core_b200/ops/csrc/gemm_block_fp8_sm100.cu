@@ -2,9 +2,10 @@
 //
 //   C[m, n] (=|+=) sum_kb  sa(kb, m) * sb(kb, n) * sum_{k in block kb}  A[m, k] * B[n, k]
 //
-// The scales are applied by the tensor core (tcgen05.mma.kind::mxf8f6f4.block_scale): it takes one E8M0 exponent per 32
-// reduction elements, so a block's exponent is handed to it four times, and the accumulator in tensor memory runs through the
-// whole reduction in fp32. Adding scaled partial sums in registers instead, which would allow scales of any value, was measured
+// The scales are applied by the tensor core (tcgen05.mma.kind::mxf8f6f4.block_scale), and the accumulator in tensor memory runs
+// through the whole reduction in fp32. The instruction takes one E8M0 exponent per row and K = 32 step, a byte of a 32-bit word
+// per row in tensor memory that it selects; all four steps of a block select the same byte here, so one word, and one set of
+// copies into tensor memory, serves four blocks. Adding scaled partial sums in registers instead, which would allow scales of any value, was measured
 // first: every block has to be read back from tensor memory, and 8192 x 11008 x 4096 took 403 us (and 625 us with a scale per
 // column of B) against 2 x 8192 x 11008 x 4096 operations in the tensor pipe.
 //
@@ -15,8 +16,7 @@
 // positive power of two becomes NaN.
 //
 // CTA layout (384 threads): warp 0 = TMA producer, warp 1 = MMA issuer and tensor-memory owner, warps 2 and 3 = scales (they
-// fetch a few blocks ahead, turn them into exponents and lay those out beside the operands of a stage as the tensor core wants
-// them), warps 4..11 = epilogue (four lane quadrants x two column halves; through shared memory, so that global accesses are
+// fetch those of four blocks at a time, run up to twelve blocks ahead, and lay the exponents out as the tensor core wants them), warps 4..11 = epilogue (four lane quadrants x two column halves; through shared memory, so that global accesses are
 // whole 128-byte lines). All waits are bounded (common.cuh).
 
 #include "common.cuh"
@@ -31,9 +31,10 @@ constexpr int BKE = 128;  // reduction elements (= bytes) per stage = one scale 
 constexpr int A_BYTES = BM * BKE;
 constexpr int THREADS = 384;
 constexpr int EPI_WARPS = 8;
-constexpr int SCALE_BATCH = 4;  // blocks whose scales are fetched together
+constexpr int SCALE_BATCH = 4;  // blocks whose exponents share a word
+constexpr int SCALE_SLOTS = 3;  // batches in shared memory
 constexpr uint32_t TMEM_COLS = 512;
-constexpr int SF_BLOCK = 512;  // scales of 128 rows for one stage
+constexpr int SF_BLOCK = 512;  // exponents of 128 rows for one batch
 
 enum : int { EPI_BF16 = 0, EPI_F32_ACC = 1, EPI_F32 = 2 };
 
@@ -49,7 +50,7 @@ struct Tile {
   static constexpr uint32_t SF_COLS = SF_BYTES / SF_BLOCK * 4;
   static constexpr int COLS = BN / 2;                // columns per epilogue thread
   static constexpr int STG_BYTES = 32 * 128;         // staging of one epilogue warp: 32 rows x 128 bytes
-  static constexpr int SMEM_BYTES = STAGES * (STAGE_BYTES + SF_BYTES) + EPI_WARPS * STG_BYTES + 1024 /*alignment slack*/ + 256;
+  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + SCALE_SLOTS * SF_BYTES + EPI_WARPS * STG_BYTES + 1024 /*alignment slack*/ + 256;
 };
 
 struct Scales {
@@ -71,10 +72,10 @@ struct Params {
   int* status;
 };
 
-// The exponent byte of a scale, four times: what the tensor core wants for the four K = 32 steps of a block.
-__device__ __forceinline__ uint32_t exponent4(float scale) {
+// Biased exponent of a scale; NaN's where it is no positive normal power of two.
+__device__ __forceinline__ uint32_t exponent_of(float scale) {
   const uint32_t bits = __float_as_uint(scale);
-  return ((bits & 0x807fffffu) != 0u || bits == 0u ? 0xffu : bits >> 23) * 0x01010101u;
+  return (bits & 0x807fffffu) != 0u || bits == 0u ? 0xffu : bits >> 23;
 }
 
 struct TileInfo {
@@ -225,12 +226,13 @@ __device__ __forceinline__ void sf_copy(uint32_t tmem_dst, uint32_t smem_src) {
 }
 // `bar` (and the other CTA's at the same offset) observes the completion of the MMAs issued so far.
 template <int CTAS>
-__device__ __forceinline__ void commit(uint64_t* bar, uint32_t peer_bar) {
+__device__ __forceinline__ void commit(uint64_t* bar) {
   if (CTAS == 1) {
     umma_commit(bar);
   } else {
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(peer_bar) : "memory");
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+                 "h"(static_cast<uint16_t>(3))
+                 : "memory");
   }
 }
 
@@ -308,12 +310,14 @@ gemm_block_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sf_smem = smem + STAGES * STAGE_BYTES;
-  uint8_t* stg_smem = sf_smem + STAGES * T::SF_BYTES;
+  uint8_t* stg_smem = sf_smem + SCALE_SLOTS * T::SF_BYTES;
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(stg_smem + EPI_WARPS * T::STG_BYTES);
   uint64_t* empty_bar = full_bar + STAGES;
   uint64_t* tfull_bar = empty_bar + STAGES;
   uint64_t* tempty_bar = tfull_bar + ACCS;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty_bar + ACCS);
+  uint64_t* sfull_bar = tempty_bar + ACCS;
+  uint64_t* sempty_bar = sfull_bar + SCALE_SLOTS;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sempty_bar + SCALE_SLOTS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5;
@@ -323,8 +327,12 @@ gemm_block_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&full_bar[s], 1 + 2 * CTAS);  // the producer's byte count and the scale warps (of both CTAs)
+      mbar_init(&full_bar[s], 1);
       mbar_init(&empty_bar[s], 1);
+    }
+    for (int i = 0; i < SCALE_SLOTS; ++i) {
+      mbar_init(&sfull_bar[i], 2 * CTAS);  // the scale warps (of both CTAs)
+      mbar_init(&sempty_bar[i], 1);
     }
     for (int a = 0; a < ACCS; ++a) {
       mbar_init(&tfull_bar[a], 1);
@@ -389,18 +397,16 @@ gemm_block_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
       // K-major: 8-row swizzle atoms 1024 bytes apart, K = 32 advances 32 bytes along the line. MN-major: one 128-column box,
       // 8 k-rows per 1024 bytes, K = 32 advances 32 lines.
       constexpr uint32_t kDescHi = desc_hi_sw128(1024);
-      // kind::mxf8f6f4: e4m3 A and B, majors at bits 15 and 16, N >> 3 at 17, E8M0 scales (23), M >> 4 at 24; the scale byte of a
-      // K = 32 step at 29 (A) and 4 (B)
+      // kind::mxf8f6f4: e4m3 A and B, majors at bits 15 and 16, N >> 3 at 17, E8M0 scales (23), M >> 4 at 24; the byte that
+      // holds the exponents at 29 (A) and 4 (B)
       const uint32_t idesc = (static_cast<uint32_t>(p.a_mn) << 15) | (static_cast<uint32_t>(p.b_mn) << 16) |
                              (static_cast<uint32_t>(BN >> 3) << 17) | (1u << 23) | (static_cast<uint32_t>(BM * CTAS >> 4) << 24);
       const uint32_t a_step = p.a_mn ? 256u : 2u, b_step = p.b_mn ? 256u : 2u;
       const uint32_t a_lo0 = desc_lo_sw128(smem_u32(smem), 16);
       const uint32_t b_lo0 = desc_lo_sw128(smem_u32(smem) + A_BYTES, 16);
       const uint32_t sf0 = smem_u32(sf_smem);
-      const uint32_t empty_peer = CTAS == 2 ? map_to_cta(smem_u32(empty_bar), 1) : 0u;
-      const uint32_t tfull_peer = CTAS == 2 ? map_to_cta(smem_u32(tfull_bar), 1) : 0u;
-      int stage = 0, acc = 0;
-      uint32_t phase = 0, acc_phase = 0, sf_set = 0;
+      int stage = 0, acc = 0, slot = 0;
+      uint32_t phase = 0, acc_phase = 0, slot_phase = 0, sf_set = 0;
       bool ok = true;
       Walk walker(p);
       TileInfo t;
@@ -410,25 +416,34 @@ gemm_block_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * BN;
         for (int kb = 0; kb < num_kb; ++kb) {
+          const uint32_t in_batch = static_cast<uint32_t>(kb) & (SCALE_BATCH - 1);
+          const uint32_t tsfa = tmem_base + T::SF_COL + sf_set * T::SF_COLS, tsfb = tsfa + 4;
+          if (in_batch == 0) {  // copies and MMAs of one thread execute in issue order
+            ok = wait_for(&sfull_bar[slot], slot_phase, abort_flag, p.status, kStatusTimeoutMma);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t ss = sf0 + slot * T::SF_BYTES;
+            sf_copy<CTAS>(tsfa, ss);
+#pragma unroll
+            for (uint32_t b = 0; b < (BN + 127) / 128; ++b) sf_copy<CTAS>(tsfb + 4 * b, ss + SF_BLOCK * (1 + b));
+          }
           ok = wait_for(&full_bar[stage], phase, abort_flag, p.status, kStatusTimeoutMma);
           if (!ok) break;
           tc_fence_after();
-          // copies and MMAs of one thread execute in issue order
-          const uint32_t tsfa = tmem_base + T::SF_COL + sf_set * T::SF_COLS, tsfb = tsfa + 4;
-          const uint32_t ss = sf0 + stage * T::SF_BYTES;
-          sf_copy<CTAS>(tsfa, ss);
-#pragma unroll
-          for (uint32_t b = 0; b < (BN + 127) / 128; ++b) sf_copy<CTAS>(tsfb + 4 * b, ss + SF_BLOCK * (1 + b));
           const uint32_t a_lo = a_lo0 + stage * (STAGE_BYTES >> 4), b_lo = b_lo0 + stage * (STAGE_BYTES >> 4);
+          const uint32_t id = idesc | (in_batch << 29) | (in_batch << 4), ta = tsfa | (in_batch << 30), tb = tsfb | (in_batch << 30);
 #pragma unroll
           for (uint32_t k = 0; k < BKE / 32; ++k)
-            umma<CTAS>(d_tmem, a_lo + k * a_step, b_lo + k * b_step, kDescHi, idesc | (k << 29) | (k << 4), tsfa | (k << 30),
-                       tsfb | (k << 30), (kb | static_cast<int>(k)) != 0);
-          commit<CTAS>(&empty_bar[stage], empty_peer + stage * 8);
-          sf_set ^= 1u;
+            umma<CTAS>(d_tmem, a_lo + k * a_step, b_lo + k * b_step, kDescHi, id, ta, tb, (kb | static_cast<int>(k)) != 0);
+          commit<CTAS>(&empty_bar[stage]);
           if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+          if (in_batch == SCALE_BATCH - 1 || kb + 1 == num_kb) {
+            commit<CTAS>(&sempty_bar[slot]);
+            sf_set ^= 1u;
+            if (++slot == SCALE_SLOTS) { slot = 0; slot_phase ^= 1u; }
+          }
         }
-        if (ok) commit<CTAS>(&tfull_bar[acc], tfull_peer + acc * 8);
+        if (ok) commit<CTAS>(&tfull_bar[acc]);
         if (++acc == ACCS) { acc = 0; acc_phase ^= 1u; }
       }
     }
@@ -436,8 +451,8 @@ gemm_block_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
     // ------------------------------------------------------------------ scales (warps 2 and 3)
     const int t64 = threadIdx.x - 64;
     constexpr int PER = (BM + BN) / 64;  // rows whose scales a thread carries: t64 + 64 i of A, then of B
-    const uint32_t full_leader = CTAS == 2 ? map_to_cta(smem_u32(full_bar), 0) : 0u;
-    int stage = 0;
+    const uint32_t sfull_leader = CTAS == 2 ? map_to_cta(smem_u32(sfull_bar), 0) : 0u;
+    int slot = 0;
     uint32_t phase = 0;
     bool ok = true;
     Walk walker(p);
@@ -456,33 +471,40 @@ gemm_block_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
                      ? sc.p + (is_a ? 0 : t.g * sc.group_stride) + static_cast<long long>(at >> sc.shift) * sc.i_stride
                      : nullptr;
       }
-      for (int kb0 = 0; ok && kb0 < num_kb; kb0 += SCALE_BATCH) {
-        float v[SCALE_BATCH][PER];
+      float next[SCALE_BATCH][PER];
+      auto fetch = [&](int kb0) {
 #pragma unroll
         for (int b = 0; b < SCALE_BATCH; ++b)
 #pragma unroll
           for (int i = 0; i < PER; ++i)  // rows outside the matrix: any valid scale, their products are not stored
-            v[b][i] = kb0 + b < num_kb && src[i] != nullptr ? __ldg(src[i] + (kb0 + b) * step[i]) : 1.f;
+            next[b][i] = kb0 + b < num_kb && src[i] != nullptr ? __ldg(src[i] + (kb0 + b) * step[i]) : 1.f;
+      };
+      fetch(0);
+      for (int kb0 = 0; kb0 < num_kb; kb0 += SCALE_BATCH) {
+        uint32_t words[PER];
 #pragma unroll
-        for (int b = 0; b < SCALE_BATCH; ++b) {
-          if (kb0 + b >= num_kb) break;
-          ok = wait_for(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, kStatusTimeoutProducer);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          uint32_t* dst = reinterpret_cast<uint32_t*>(sf_smem + stage * T::SF_BYTES);
+        for (int i = 0; i < PER; ++i) {
+          words[i] = 0u;
 #pragma unroll
-          for (int i = 0; i < PER; ++i) {  // row r of a 128-row block: 32-bit word 4 (r % 32) + r / 32 of its 512 bytes
-            const int f = t64 + 64 * i;
-            dst[(f >> 7) * (SF_BLOCK / 4) + (f & 31) * 4 + ((f >> 5) & 3)] = exponent4(v[b][i]);
-          }
-          fence_proxy_async_smem();  // the tensor core's copy reads what the threads wrote
-          __syncwarp();
-          if (lane == 0) {
-            if (CTAS == 1) mbar_arrive(&full_bar[stage]);
-            else mbar_arrive_cluster(full_leader + stage * 8);
-          }
-          if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+          for (int b = 0; b < SCALE_BATCH; ++b) words[i] |= exponent_of(next[b][i]) << (8 * b);
         }
+        fetch(kb0 + SCALE_BATCH);  // on its way while this batch waits for its slot
+        ok = wait_for(&sempty_bar[slot], phase ^ 1u, abort_flag, p.status, kStatusTimeoutProducer);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        uint32_t* dst = reinterpret_cast<uint32_t*>(sf_smem + slot * T::SF_BYTES);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {  // row r of a 128-row block: 32-bit word 4 (r % 32) + r / 32 of its 512 bytes
+          const int f = t64 + 64 * i;
+          dst[(f >> 7) * (SF_BLOCK / 4) + (f & 31) * 4 + ((f >> 5) & 3)] = words[i];
+        }
+        fence_proxy_async_smem();  // the tensor core's copy reads what the threads wrote
+        __syncwarp();
+        if (lane == 0) {
+          if (CTAS == 1) mbar_arrive(&sfull_bar[slot]);
+          else mbar_arrive_cluster(sfull_leader + slot * 8);
+        }
+        if (++slot == SCALE_SLOTS) { slot = 0; phase ^= 1u; }
       }
     }
   } else {
