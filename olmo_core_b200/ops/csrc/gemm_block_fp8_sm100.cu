@@ -27,7 +27,8 @@ namespace ocb {
 namespace blk {
 
 constexpr int BM = 128;
-constexpr int BKE = 128;  // reduction elements (= bytes) per stage = one scale block
+constexpr int BKE = 128;  // reduction elements (= bytes) of one scale block
+constexpr int KBS = 2;    // blocks per stage: the issuing thread's waits and commits are shared by eight MMAs
 constexpr int A_BYTES = BM * BKE;
 constexpr int THREADS = 384;
 constexpr int EPI_WARPS = 8;
@@ -42,14 +43,15 @@ enum : int { EPI_BF16 = 0, EPI_F32_ACC = 1, EPI_F32 = 2 };
 template <int BN, int CTAS>
 struct Tile {
   static constexpr int B_ROWS = BN / CTAS;  // rows of B that one CTA stages
-  static constexpr int STAGE_BYTES = A_BYTES + B_ROWS * BKE;
-  static constexpr int STAGES = 5;
+  static constexpr int KB_BYTES = A_BYTES + B_ROWS * BKE;
+  static constexpr int STAGE_BYTES = KBS * KB_BYTES;  // [block][A rows, B rows]
+  static constexpr int STAGES = 3;
   static constexpr int SF_BYTES = SF_BLOCK * (1 + (BN + 127) / 128);
   static constexpr int ACCS = BN == 256 ? 1 : 2;     // accumulators in tensor memory
   static constexpr uint32_t SF_COL = ACCS * BN;      // two alternating sets of scale columns: 4 of A, 4 per 128 columns of B
   static constexpr uint32_t SF_COLS = SF_BYTES / SF_BLOCK * 4;
   static constexpr int COLS = BN / 2;                // columns per epilogue thread
-  static constexpr int STG_BYTES = 32 * 128;         // staging of one epilogue warp: 32 rows x 128 bytes
+  static constexpr int STG_BYTES = 16 * 128;         // staging of one epilogue warp: 16 rows x 128 bytes
   static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + SCALE_SLOTS * SF_BYTES + EPI_WARPS * STG_BYTES + 1024 /*alignment slack*/ + 256;
 };
 
@@ -265,7 +267,7 @@ __device__ __forceinline__ void store_chunk(const Params& p, long long row, int 
 }
 
 // ---- epilogue staging ------------------------------------------------------------------------------------------------
-// 16-byte slot `chunk` (0..7) of staged row `row` (0..31); the XOR keeps both the row-per-thread and the 8-lanes-per-row
+// 16-byte slot `chunk` (0..7) of staged row `row` (0..15); the XOR keeps both the row-per-thread and the 8-lanes-per-row
 // access patterns free of bank conflicts.
 __device__ __forceinline__ uint4* stg_slot(uint8_t* stg, int row, int chunk) {
   return reinterpret_cast<uint4*>(stg + row * 128 + ((chunk ^ (row & 7)) << 4));
@@ -275,7 +277,7 @@ template <int EPI>
 __device__ __forceinline__ void stg_store(uint8_t* stg, uint8_t* dst0, long long ld_bytes, int rows, int bytes, int lane) {
   const int cc = (lane & 7) * 16;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < 4; ++i) {
     const int rr = i * 4 + (lane >> 3);
     if (rr >= rows || cc >= bytes) continue;
     const uint4 v = *stg_slot(stg, rr, lane & 7);
@@ -370,20 +372,23 @@ gemm_block_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
       TileInfo t;
       while (ok && walker.next(t)) {
         const int m0 = t.m0 + static_cast<int>(cta) * BM, n0 = t.n0 + static_cast<int>(cta) * T::B_ROWS;
-        for (int kb = 0; kb < num_kb; ++kb) {
+        for (int kb = 0; kb < num_kb; kb += KBS) {
           ok = wait_for(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, kStatusTimeoutProducer);
           if (!ok) break;
-          uint8_t* sa = smem + stage * STAGE_BYTES;
-          uint8_t* sb = sa + A_BYTES;
-          const int k0 = kb * BKE;
-          if (cta == 0) mbar_arrive_expect_tx(&full_bar[stage], CTAS * STAGE_BYTES);
+          const int blocks = min(KBS, num_kb - kb);
+          if (cta == 0) mbar_arrive_expect_tx(&full_bar[stage], CTAS * T::KB_BYTES * blocks);
           const uint32_t pair_bar = CTAS == 2 ? map_to_cta(smem_u32(&full_bar[stage]), 0) : 0u;
-          // innermost coordinates are k0 (K-major) or tile origins (MN-major): multiples of 128 bytes either way; group
-          // boundaries only enter the outer coordinate of a K-major A
-          if (p.a_mn) load_2d<CTAS>(sa, &tma_a, &full_bar[stage], pair_bar, m0, k0);
-          else load_2d<CTAS>(sa, &tma_a, &full_bar[stage], pair_bar, k0, m0);
-          if (p.b_mn) load_3d<CTAS>(sb, &tma_b, &full_bar[stage], pair_bar, n0, k0, t.g);
-          else load_3d<CTAS>(sb, &tma_b, &full_bar[stage], pair_bar, k0, n0, t.g);
+          for (int j = 0; j < blocks; ++j) {
+            uint8_t* sa = smem + stage * STAGE_BYTES + j * T::KB_BYTES;
+            uint8_t* sb = sa + A_BYTES;
+            const int k0 = (kb + j) * BKE;
+            // innermost coordinates are k0 (K-major) or tile origins (MN-major): multiples of 128 bytes either way; group
+            // boundaries only enter the outer coordinate of a K-major A
+            if (p.a_mn) load_2d<CTAS>(sa, &tma_a, &full_bar[stage], pair_bar, m0, k0);
+            else load_2d<CTAS>(sa, &tma_a, &full_bar[stage], pair_bar, k0, m0);
+            if (p.b_mn) load_3d<CTAS>(sb, &tma_b, &full_bar[stage], pair_bar, n0, k0, t.g);
+            else load_3d<CTAS>(sb, &tma_b, &full_bar[stage], pair_bar, k0, n0, t.g);
+          }
           if (++stage == STAGES) { stage = 0; phase ^= 1u; }
         }
       }
@@ -406,7 +411,10 @@ gemm_block_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
       const uint32_t b_lo0 = desc_lo_sw128(smem_u32(smem) + A_BYTES, 16);
       const uint32_t sf0 = smem_u32(sf_smem);
       int stage = 0, acc = 0, slot = 0;
-      uint32_t phase = 0, acc_phase = 0, slot_phase = 0, sf_set = 0;
+      uint32_t phase = 0, acc_phase = 0, slot_phase = 0;
+      // the two sets of scale columns take turns
+      uint32_t tsfa = tmem_base + T::SF_COL;
+      const uint32_t sf_flip = tsfa ^ (tsfa + T::SF_COLS);
       bool ok = true;
       Walk walker(p);
       TileInfo t;
@@ -415,31 +423,39 @@ gemm_block_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
         if (!ok) break;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * BN;
-        for (int kb = 0; kb < num_kb; ++kb) {
-          const uint32_t in_batch = static_cast<uint32_t>(kb) & (SCALE_BATCH - 1);
-          const uint32_t tsfa = tmem_base + T::SF_COL + sf_set * T::SF_COLS, tsfb = tsfa + 4;
-          if (in_batch == 0) {  // copies and MMAs of one thread execute in issue order
+        for (int kb = 0; kb < num_kb; kb += KBS) {
+          const bool first_of_batch = (kb & (SCALE_BATCH - 1)) == 0;
+          if (first_of_batch) {  // copies and MMAs of one thread execute in issue order
             ok = wait_for(&sfull_bar[slot], slot_phase, abort_flag, p.status, kStatusTimeoutMma);
             if (!ok) break;
             tc_fence_after();
             const uint32_t ss = sf0 + slot * T::SF_BYTES;
             sf_copy<CTAS>(tsfa, ss);
 #pragma unroll
-            for (uint32_t b = 0; b < (BN + 127) / 128; ++b) sf_copy<CTAS>(tsfb + 4 * b, ss + SF_BLOCK * (1 + b));
+            for (uint32_t b = 0; b < (BN + 127) / 128; ++b) sf_copy<CTAS>(tsfa + 4 + 4 * b, ss + SF_BLOCK * (1 + b));
           }
           ok = wait_for(&full_bar[stage], phase, abort_flag, p.status, kStatusTimeoutMma);
           if (!ok) break;
           tc_fence_after();
           const uint32_t a_lo = a_lo0 + stage * (STAGE_BYTES >> 4), b_lo = b_lo0 + stage * (STAGE_BYTES >> 4);
-          const uint32_t id = idesc | (in_batch << 29) | (in_batch << 4), ta = tsfa | (in_batch << 30), tb = tsfb | (in_batch << 30);
+          const uint32_t byte0 = first_of_batch ? 0u : 2u;
+          uint32_t id = idesc + byte0 * ((1u << 29) | (1u << 4)), ta = tsfa + (byte0 << 30), tb = ta + 4;
 #pragma unroll
           for (uint32_t k = 0; k < BKE / 32; ++k)
             umma<CTAS>(d_tmem, a_lo + k * a_step, b_lo + k * b_step, kDescHi, id, ta, tb, (kb | static_cast<int>(k)) != 0);
+          if (kb + 1 < num_kb) {
+            id += (1u << 29) | (1u << 4);
+            ta += 1u << 30;
+            tb += 1u << 30;
+#pragma unroll
+            for (uint32_t k = 0; k < BKE / 32; ++k)
+              umma<CTAS>(d_tmem, a_lo + (T::KB_BYTES >> 4) + k * a_step, b_lo + (T::KB_BYTES >> 4) + k * b_step, kDescHi, id, ta, tb, 1u);
+          }
           commit<CTAS>(&empty_bar[stage]);
           if (++stage == STAGES) { stage = 0; phase ^= 1u; }
-          if (in_batch == SCALE_BATCH - 1 || kb + 1 == num_kb) {
+          if (!first_of_batch || kb + KBS >= num_kb) {
             commit<CTAS>(&sempty_bar[slot]);
-            sf_set ^= 1u;
+            tsfa ^= sf_flip;
             if (++slot == SCALE_SLOTS) { slot = 0; slot_phase ^= 1u; }
           }
         }
@@ -548,25 +564,31 @@ gemm_block_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
       for (int c = 0; c < COLS / CHUNK; ++c) {
         const int bytes = min(128, (p.N - (col0 + c * CHUNK)) * ES);
         if (bytes <= 0) break;
-        __syncwarp();
+        uint4 o[8];
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
-          uint4 o;
           if (EPI == EPI_BF16) {
             const uint32_t* s = &r[2 * c + (q >> 2)][(q & 3) * 8];
-            o.x = pack_bf16x2(__uint_as_float(s[0]), __uint_as_float(s[1]));
-            o.y = pack_bf16x2(__uint_as_float(s[2]), __uint_as_float(s[3]));
-            o.z = pack_bf16x2(__uint_as_float(s[4]), __uint_as_float(s[5]));
-            o.w = pack_bf16x2(__uint_as_float(s[6]), __uint_as_float(s[7]));
+            o[q].x = pack_bf16x2(__uint_as_float(s[0]), __uint_as_float(s[1]));
+            o[q].y = pack_bf16x2(__uint_as_float(s[2]), __uint_as_float(s[3]));
+            o[q].z = pack_bf16x2(__uint_as_float(s[4]), __uint_as_float(s[5]));
+            o[q].w = pack_bf16x2(__uint_as_float(s[6]), __uint_as_float(s[7]));
           } else {
             const uint32_t* s = &r[c][q * 4];
-            o = make_uint4(s[0], s[1], s[2], s[3]);
+            o[q] = make_uint4(s[0], s[1], s[2], s[3]);
           }
-          *stg_slot(stg, lane, q) = o;
         }
-        __syncwarp();
-        stg_store<EPI>(stg, reinterpret_cast<uint8_t*>(p.C) + (static_cast<long long>(row0) * p.ldc + col0 + c * CHUNK) * ES,
-                       p.ldc * ES, rows, bytes, lane);
+        uint8_t* dst = reinterpret_cast<uint8_t*>(p.C) + (static_cast<long long>(row0) * p.ldc + col0 + c * CHUNK) * ES;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {  // sixteen rows at a time
+          __syncwarp();
+          if ((lane >> 4) == h) {
+#pragma unroll
+            for (int q = 0; q < 8; ++q) *stg_slot(stg, lane & 15, q) = o[q];
+          }
+          __syncwarp();
+          stg_store<EPI>(stg, dst + h * 16 * p.ldc * ES, p.ldc * ES, rows - 16 * h, bytes, lane);
+        }
       }
     }
   }
