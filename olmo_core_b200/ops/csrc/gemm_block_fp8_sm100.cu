@@ -187,33 +187,36 @@ __device__ __forceinline__ void load_3d(void* smem_dst, const CUtensorMap* desc,
         : "memory");
   }
 }
-// D (+)= (A * SFA) (B * SFB)^T for K = 32 with E8M0 scales in tensor memory; issued by one thread (of a pair: the leader's).
+// D (+)= (A * SFA) (B * SFB)^T for K = 32 with E8M0 scales in tensor memory; issued by the one thread (of a pair: of the leader)
+// whose `issue` is set.
 template <int CTAS>
 __device__ __forceinline__ void umma(uint32_t tmem_d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t tsfa,
-                                     uint32_t tsfb, uint32_t accumulate) {
+                                     uint32_t tsfb, uint32_t accumulate, uint32_t issue) {
   if (CTAS == 1) {
     asm volatile(
         "{\n\t"
-        ".reg .pred p;\n\t"
+        ".reg .pred p, q;\n\t"
+        "setp.ne.b32 q, %8, 0;\n\t"
         ".reg .b64 da, db;\n\t"
         "mov.b64 da, {%1, %3};\n\t"
         "mov.b64 db, {%2, %3};\n\t"
         "setp.ne.b32 p, %7, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale [%0], da, db, %4, [%5], [%6], p;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale [%0], da, db, %4, [%5], [%6], p;\n\t"
         "}\n" ::"r"(tmem_d),
-        "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(tsfa), "r"(tsfb), "r"(accumulate)
+        "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(tsfa), "r"(tsfb), "r"(accumulate), "r"(issue)
         : "memory");
   } else {
     asm volatile(
         "{\n\t"
-        ".reg .pred p;\n\t"
+        ".reg .pred p, q;\n\t"
+        "setp.ne.b32 q, %8, 0;\n\t"
         ".reg .b64 da, db;\n\t"
         "mov.b64 da, {%1, %3};\n\t"
         "mov.b64 db, {%2, %3};\n\t"
         "setp.ne.b32 p, %7, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale [%0], da, db, %4, [%5], [%6], p;\n\t"
+        "@q tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale [%0], da, db, %4, [%5], [%6], p;\n\t"
         "}\n" ::"r"(tmem_d),
-        "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(tsfa), "r"(tsfb), "r"(accumulate)
+        "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(tsfa), "r"(tsfb), "r"(accumulate), "r"(issue)
         : "memory");
   }
 }
@@ -398,7 +401,9 @@ gemm_block_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------------ issuer (of a pair: the leader's)
-    if (lane == 0 && cta == 0) {
+    // The whole warp walks the loop, so that descriptors can live in uniform registers; one lane issues.
+    if (cta == 0) {
+      const uint32_t issue = lane == 0;
       // K-major: 8-row swizzle atoms 1024 bytes apart, K = 32 advances 32 bytes along the line. MN-major: one 128-column box,
       // 8 k-rows per 1024 bytes, K = 32 advances 32 lines.
       constexpr uint32_t kDescHi = desc_hi_sw128(1024);
@@ -430,9 +435,11 @@ gemm_block_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
             if (!ok) break;
             tc_fence_after();
             const uint32_t ss = sf0 + slot * T::SF_BYTES;
-            sf_copy<CTAS>(tsfa, ss);
+            if (issue) {
+              sf_copy<CTAS>(tsfa, ss);
 #pragma unroll
-            for (uint32_t b = 0; b < (BN + 127) / 128; ++b) sf_copy<CTAS>(tsfa + 4 + 4 * b, ss + SF_BLOCK * (1 + b));
+              for (uint32_t b = 0; b < (BN + 127) / 128; ++b) sf_copy<CTAS>(tsfa + 4 + 4 * b, ss + SF_BLOCK * (1 + b));
+            }
           }
           ok = wait_for(&full_bar[stage], phase, abort_flag, p.status, kStatusTimeoutMma);
           if (!ok) break;
@@ -442,24 +449,24 @@ gemm_block_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
           uint32_t id = idesc + byte0 * ((1u << 29) | (1u << 4)), ta = tsfa + (byte0 << 30), tb = ta + 4;
 #pragma unroll
           for (uint32_t k = 0; k < BKE / 32; ++k)
-            umma<CTAS>(d_tmem, a_lo + k * a_step, b_lo + k * b_step, kDescHi, id, ta, tb, (kb | static_cast<int>(k)) != 0);
+            umma<CTAS>(d_tmem, a_lo + k * a_step, b_lo + k * b_step, kDescHi, id, ta, tb, (kb | static_cast<int>(k)) != 0, issue);
           if (kb + 1 < num_kb) {
             id += (1u << 29) | (1u << 4);
             ta += 1u << 30;
             tb += 1u << 30;
 #pragma unroll
             for (uint32_t k = 0; k < BKE / 32; ++k)
-              umma<CTAS>(d_tmem, a_lo + (T::KB_BYTES >> 4) + k * a_step, b_lo + (T::KB_BYTES >> 4) + k * b_step, kDescHi, id, ta, tb, 1u);
+              umma<CTAS>(d_tmem, a_lo + (T::KB_BYTES >> 4) + k * a_step, b_lo + (T::KB_BYTES >> 4) + k * b_step, kDescHi, id, ta, tb, 1u, issue);
           }
-          commit<CTAS>(&empty_bar[stage]);
+          if (issue) commit<CTAS>(&empty_bar[stage]);
           if (++stage == STAGES) { stage = 0; phase ^= 1u; }
           if (!first_of_batch || kb + KBS >= num_kb) {
-            commit<CTAS>(&sempty_bar[slot]);
+            if (issue) commit<CTAS>(&sempty_bar[slot]);
             tsfa ^= sf_flip;
             if (++slot == SCALE_SLOTS) { slot = 0; slot_phase ^= 1u; }
           }
         }
-        if (ok) commit<CTAS>(&tfull_bar[acc]);
+        if (ok && issue) commit<CTAS>(&tfull_bar[acc]);
         if (++acc == ACCS) { acc = 0; acc_phase ^= 1u; }
       }
     }
