@@ -253,6 +253,14 @@ __device__ __forceinline__ void tmem_ld_wait_for(uint32_t (&r)[32]) {
                : "memory");
 }
 
+__device__ __forceinline__ void tmem_ld_wait_for(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                 "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+}
+
 // 32 consecutive columns of one row, for outputs whose rows are not 16-byte aligned.
 template <int EPI>
 __device__ __forceinline__ void store_chunk(const Params& p, long long row, int col, const uint32_t* v) {
@@ -610,6 +618,332 @@ gemm_block_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
   }
 }
 
+// ---- small products --------------------------------------------------------------------------------------------------
+// One CTA per 128 x BN tile and reduction part. Few tokens against a weight: the weight's rows take the 128-row side and the
+// tokens the BN side (SWAP: D is C transposed), so a tile is no larger than it has to be and every SM streams weights. The
+// reduction is split over the CTAs of a cluster; each leaves its fp32 part in its own shared memory, and the CTAs then add the
+// parts in rank order, each for its share of the rows of C (distributed shared memory: no workspace, no atomics, the same bits
+// every time). Groups (SWAP only): a CTA finds its group and its tokens from the device-side boundaries.
+constexpr int SMALL_THREADS = 256;  // warps as above, with one epilogue warpgroup
+
+template <int BN>
+struct SmallTile {
+  static constexpr int KB_BYTES = A_BYTES + BN * BKE;
+  static constexpr int STAGES = BN >= 128 ? 5 : 6;
+  static constexpr uint32_t TMEM = BN >= 128 ? 256 : BN >= 64 ? 128 : BN >= 32 ? 64 : 32;  // BN + 16 scale columns
+  static constexpr int SF_BYTES = 2 * SF_BLOCK;
+  static constexpr int SMEM_BYTES = STAGES * KB_BYTES + SCALE_SLOTS * SF_BYTES + 1024 + 256;
+  // the fp32 part reuses the stages: [BN][128] (SWAP) or [128][BN + 4]
+  static_assert(STAGES * KB_BYTES >= 128 * (BN + 4) * 4, "the parts do not fit");
+};
+
+struct SmallParams {
+  void* C;
+  long long ldc;
+  int M, N, K;   // rows of the 128-row side (of one group), rows of the BN side (all groups), reduction
+  int a_mn, b_mn, epi, vector;  // vector: C rows start on 16-byte boundaries and have a multiple of 4 columns
+  int parts, kb_per_part;
+  Scales sa, sb;
+  const int* offsets;
+  int num_groups;
+  int* status;
+};
+
+__device__ __forceinline__ float4 load_cluster_f4(uint32_t cluster_addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(cluster_addr) : "memory");
+  return v;
+}
+
+template <int BN, bool SWAP>
+__global__ void __launch_bounds__(SMALL_THREADS)
+gemm_block_fp8_small_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b, const SmallParams p) {
+  using T = SmallTile<BN>;
+  constexpr int STAGES = T::STAGES;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sf_smem = smem + STAGES * T::KB_BYTES;
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(sf_smem + SCALE_SLOTS * T::SF_BYTES);
+  uint64_t* empty_bar = full_bar + STAGES;
+  uint64_t* sfull_bar = empty_bar + STAGES;
+  uint64_t* sempty_bar = sfull_bar + SCALE_SLOTS;
+  uint64_t* done_bar = sempty_bar + SCALE_SLOTS;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done_bar + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* tile_info = reinterpret_cast<int*>(tmem_slot + 2);  // group, first row and end of the BN side
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int part = blockIdx.x % p.parts, tile = blockIdx.x / p.parts;
+  const int tiles_a = (p.M + BM - 1) / BM;
+  const int a_tile = tile % tiles_a, b_tile = tile / tiles_a;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int i = 0; i < SCALE_SLOTS; ++i) {
+      mbar_init(&sfull_bar[i], 2);
+      mbar_init(&sempty_bar[i], 1);
+    }
+    mbar_init(done_bar, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tma_a);
+    tma_prefetch_desc(&tma_b);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, T::TMEM);
+    tmem_relinquish();
+  }
+  if (warp == 2) {
+    int g = 0, b0 = b_tile * BN, b_end = p.N;
+    if (p.offsets != nullptr) {  // which group does the b_tile-th tile of the BN side belong to?
+      int before = 0;
+      g = -1;
+      for (int base = 0; base < p.num_groups && g < 0; base += 32) {
+        int lo = 0, rows = 0;
+        if (base + lane < p.num_groups) {
+          lo = min(max(p.offsets[base + lane], 0), p.N);
+          rows = max(min(p.offsets[base + lane + 1], p.N) - lo, 0);
+        }
+        const int tiles = (rows + BN - 1) / BN;
+        int upto = tiles;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int v = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += v;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, b_tile < before + upto);
+        if (hit != 0u) {
+          const int l = __ffs(hit) - 1;
+          g = base + l;
+          const int first = before + __shfl_sync(0xffffffffu, upto - tiles, l);
+          b0 = __shfl_sync(0xffffffffu, lo, l) + (b_tile - first) * BN;
+          b_end = __shfl_sync(0xffffffffu, lo + rows, l);
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
+      }
+    }
+    if (lane == 0) {
+      tile_info[0] = g;
+      tile_info[1] = b0;
+      tile_info[2] = b_end;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  const int g = tile_info[0], b0 = tile_info[1], b_end = tile_info[2];
+  const int a0 = a_tile * BM;
+  const int num_kb = (p.K + BKE - 1) / BKE;
+  const int kb_first = part * p.kb_per_part;
+  const int kbs = g < 0 ? 0 : max(min(p.kb_per_part, num_kb - kb_first), 0);  // a tile nobody needs: no blocks, nothing stored
+  bool ok = true;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ producer
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int kb = 0; kb < kbs; ++kb) {
+        ok = wait_for(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, kStatusTimeoutProducer);
+        if (!ok) break;
+        uint8_t* sa = smem + stage * T::KB_BYTES;
+        uint8_t* sb = sa + A_BYTES;
+        const int k0 = (kb_first + kb) * BKE;
+        const int ga = SWAP ? g : 0, gb = SWAP ? 0 : g;
+        mbar_arrive_expect_tx(&full_bar[stage], T::KB_BYTES);
+        // innermost coordinates: k0 (K-major) or a0 / b0 of an ungrouped operand (MN-major), multiples of 128 bytes
+        if (p.a_mn) tma_load_3d(sa, &tma_a, &full_bar[stage], a0, k0, ga);
+        else tma_load_3d(sa, &tma_a, &full_bar[stage], k0, a0, ga);
+        if (p.b_mn) tma_load_3d(sb, &tma_b, &full_bar[stage], b0, k0, gb);
+        else tma_load_3d(sb, &tma_b, &full_bar[stage], k0, b0, gb);
+        if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+      }
+      if (!ok) {
+        for (int i = 0; i < 64; ++i) __nanosleep(1000);  // let copies in flight land before shared memory is used again
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ issuer
+    const uint32_t issue = lane == 0;
+    constexpr uint32_t kDescHi = desc_hi_sw128(1024);
+    const uint32_t idesc = (static_cast<uint32_t>(p.a_mn) << 15) | (static_cast<uint32_t>(p.b_mn) << 16) |
+                           (static_cast<uint32_t>(BN >> 3) << 17) | (1u << 23) | (static_cast<uint32_t>(BM >> 4) << 24);
+    const uint32_t a_step = p.a_mn ? 256u : 2u, b_step = p.b_mn ? 256u : 2u;
+    const uint32_t a_lo0 = desc_lo_sw128(smem_u32(smem), 16);
+    const uint32_t b_lo0 = desc_lo_sw128(smem_u32(smem) + A_BYTES, 16);
+    const uint32_t sf0 = smem_u32(sf_smem);
+    int stage = 0, slot = 0;
+    uint32_t phase = 0, slot_phase = 0;
+    uint32_t tsfa = tmem_base + BN;
+    const uint32_t sf_flip = tsfa ^ (tsfa + 8);
+    for (int kb = 0; kb < kbs; ++kb) {
+      const uint32_t in_batch = static_cast<uint32_t>(kb) & (SCALE_BATCH - 1);
+      if (in_batch == 0) {
+        ok = wait_for(&sfull_bar[slot], slot_phase, abort_flag, p.status, kStatusTimeoutMma);
+        if (!ok) break;
+        tc_fence_after();
+        if (issue) {
+          sf_copy<1>(tsfa, sf0 + slot * T::SF_BYTES);
+          sf_copy<1>(tsfa + 4, sf0 + slot * T::SF_BYTES + SF_BLOCK);
+        }
+      }
+      ok = wait_for(&full_bar[stage], phase, abort_flag, p.status, kStatusTimeoutMma);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t a_lo = a_lo0 + stage * (T::KB_BYTES >> 4), b_lo = b_lo0 + stage * (T::KB_BYTES >> 4);
+      const uint32_t id = idesc + in_batch * ((1u << 29) | (1u << 4)), ta = tsfa + (in_batch << 30), tb = ta + 4;
+#pragma unroll
+      for (uint32_t k = 0; k < BKE / 32; ++k)
+        umma<1>(tmem_base, a_lo + k * a_step, b_lo + k * b_step, kDescHi, id, ta, tb, (kb | static_cast<int>(k)) != 0, issue);
+      if (issue) commit<1>(&empty_bar[stage]);
+      if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+      if (in_batch == SCALE_BATCH - 1 || kb + 1 == kbs) {
+        if (issue) commit<1>(&sempty_bar[slot]);
+        tsfa ^= sf_flip;
+        if (++slot == SCALE_SLOTS) { slot = 0; slot_phase ^= 1u; }
+      }
+    }
+    if (ok && issue && kbs > 0) commit<1>(done_bar);
+  } else if (warp < 4) {
+    // ------------------------------------------------------------------ scales
+    const int t64 = threadIdx.x - 64;
+    constexpr int PER = 2 + (BN + 63) / 64;
+    const float* src[PER];
+    long long step[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const bool is_a = i < 2;
+      const int f = is_a ? t64 + 64 * i : t64 + 64 * (i - 2);
+      const int at = (is_a ? a0 : b0) + f;
+      const Scales& sc = is_a ? p.sa : p.sb;
+      step[i] = sc.k_stride;
+      const bool in = is_a ? at < p.M : f < BN && at < b_end;
+      src[i] = in ? sc.p + g * sc.group_stride + static_cast<long long>(at >> sc.shift) * sc.i_stride + kb_first * sc.k_stride : nullptr;
+    }
+    int slot = 0;
+    uint32_t phase = 0;
+    float next[SCALE_BATCH][PER];
+    auto fetch = [&](int kb0) {
+#pragma unroll
+      for (int b = 0; b < SCALE_BATCH; ++b)
+#pragma unroll
+        for (int i = 0; i < PER; ++i) next[b][i] = kb0 + b < kbs && src[i] != nullptr ? __ldg(src[i] + (kb0 + b) * step[i]) : 1.f;
+    };
+    fetch(0);
+    for (int kb0 = 0; kb0 < kbs; kb0 += SCALE_BATCH) {
+      uint32_t words[PER];
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        words[i] = 0u;
+#pragma unroll
+        for (int b = 0; b < SCALE_BATCH; ++b) words[i] |= exponent_of(next[b][i]) << (8 * b);
+      }
+      fetch(kb0 + SCALE_BATCH);
+      ok = wait_for(&sempty_bar[slot], phase ^ 1u, abort_flag, p.status, kStatusTimeoutProducer);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      uint32_t* dst = reinterpret_cast<uint32_t*>(sf_smem + slot * T::SF_BYTES);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int f = i < 2 ? t64 + 64 * i : t64 + 64 * (i - 2);
+        dst[(i < 2 ? 0 : SF_BLOCK / 4) + (f & 31) * 4 + ((f >> 5) & 3)] = words[i];
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sfull_bar[slot]);
+      if (++slot == SCALE_SLOTS) { slot = 0; phase ^= 1u; }
+    }
+  } else {
+    // ------------------------------------------------------------------ this CTA's part into shared memory
+    const int quad = warp & 3;
+    if (kbs > 0) {
+      ok = wait_for(done_bar, 0, abort_flag, p.status, kStatusTimeoutEpilogue);
+      ok = __all_sync(0xffffffffu, ok);
+      tc_fence_after();
+    }
+    // every load into the stages has been consumed by an MMA that is complete: their memory is free
+    float* out = reinterpret_cast<float*>(smem);
+    const int row = quad * 32 + lane;
+#pragma unroll
+    for (int c = 0; c < BN / 16; ++c) {
+      uint32_t r[16];
+      if (kbs > 0 && ok) {
+        tmem_ld_32x16(tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + c * 16, r);
+        tmem_ld_wait_for(r);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) r[j] = 0u;
+      }
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        if (SWAP) {
+          out[(c * 16 + j) * 128 + row] = __uint_as_float(r[j]);
+        } else if ((j & 3) == 0) {
+          *reinterpret_cast<uint4*>(out + row * (BN + 4) + c * 16 + j) = make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]);
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (p.parts > 1) cluster_sync_all();  // all parts are in place
+  if (warp == 1) {
+    __syncwarp();
+    tmem_dealloc(tmem_base, T::TMEM);
+  }
+
+  // Sum of the parts, in rank order. A row of C has `inner` columns here; rank `part` takes rows part, part + parts, ...
+  constexpr int INNER = SWAP ? 128 : BN, PITCH = SWAP ? 128 : BN + 4;
+  const int c_row0 = SWAP ? b0 : a0, c_col0 = SWAP ? a0 : b0;
+  const int rows = SWAP ? min(BN, b_end - b0) : min(128, p.M - a0);
+  const int cols = SWAP ? min(128, p.M - a0) : min(BN, b_end - b0);
+  if (g >= 0 && *abort_flag == 0) {
+    const uint32_t mine = smem_u32(smem);
+    constexpr int PER_ROW = INNER / 4, ROWS_AT_ONCE = SMALL_THREADS / PER_ROW;
+    const int q = threadIdx.x % PER_ROW;
+    for (int i = part + (threadIdx.x / PER_ROW) * p.parts; i < rows; i += ROWS_AT_ONCE * p.parts) {
+      const uint32_t at = mine + static_cast<uint32_t>(i * PITCH + 4 * q) * 4;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int r = 0; r < p.parts; ++r) {
+        const float4 x = p.parts > 1 ? load_cluster_f4(map_to_cta(at, r)) : *reinterpret_cast<const float4*>(smem + (i * PITCH + 4 * q) * 4);
+        v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+      }
+      const float f[4] = {v.x, v.y, v.z, v.w};
+      const long long first = static_cast<long long>(c_row0 + i) * p.ldc + c_col0 + 4 * q;
+      const int n = cols - 4 * q;
+      if (n <= 0) continue;
+      if (p.epi == EPI_BF16) {
+        __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(p.C) + first;
+        if (p.vector && n >= 4) {
+          *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]));
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (j < n) dst[j] = __float2bfloat16_rn(f[j]);
+        }
+      } else {
+        float* dst = reinterpret_cast<float*>(p.C) + first;
+        const bool add = p.epi == EPI_F32_ACC;
+        if (p.vector && n >= 4) {
+          float4 old = add ? *reinterpret_cast<const float4*>(dst) : make_float4(0.f, 0.f, 0.f, 0.f);
+          if (add) { v.x += old.x; v.y += old.y; v.z += old.z; v.w += old.w; }
+          *reinterpret_cast<float4*>(dst) = v;
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (j < n) dst[j] = add ? dst[j] + f[j] : f[j];
+        }
+      }
+    }
+  }
+  if (p.parts > 1) cluster_sync_all();  // the other CTAs have read this one's part
+}
+
 static int num_sms() {
   int dev = 0, n = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
@@ -660,6 +994,136 @@ static bool make_map(CUtensorMap* out, const void* ptr, bool mn, uint64_t rows, 
 
 using namespace ocb;
 
+namespace ocb {
+namespace blk {
+
+template <int BN, bool SWAP>
+static int launch_small(const CUtensorMap& ta, const CUtensorMap& tb, const SmallParams& p, long long tiles, cudaStream_t stream) {
+  constexpr int bytes = SmallTile<BN>::SMEM_BYTES;
+  auto kernel = gemm_block_fp8_small_kernel<BN, SWAP>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return -3;
+  if (tiles * p.parts > 0x7fffffffll) return -1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(static_cast<unsigned>(tiles * p.parts));
+  config.blockDim = dim3(SMALL_THREADS);
+  config.dynamicSmemBytes = bytes;
+  config.stream = stream;
+  cudaLaunchAttribute cluster;
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = p.parts;
+  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+  config.attrs = &cluster;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, kernel, ta, tb, p) == cudaSuccess ? 0 : -4;
+}
+
+struct Product {
+  const void *A, *B;
+  void* C;
+  int M, N, K, groups;
+  long long lda, ldb, ldc, b_group_bytes;
+  Scales sa, sb;
+  int a_mn, b_mn, epi;
+  const int* offsets;
+  int* status;
+};
+
+static int run_pair(const Product& x, cudaStream_t stream) {
+  Params p;
+  p.C = x.C;
+  p.ldc = x.ldc;
+  p.M = x.M;
+  p.N = x.N;
+  p.K = x.K;
+  p.group_m = 8;
+  p.a_mn = x.a_mn;
+  p.b_mn = x.b_mn;
+  p.aligned = (reinterpret_cast<uintptr_t>(x.C) & 15) == 0 && (x.ldc * (x.epi == EPI_BF16 ? 2 : 4)) % 16 == 0;
+  p.sa = x.sa;
+  p.sb = x.sb;
+  p.offsets = x.offsets;
+  p.num_groups = x.groups;
+  p.status = x.status;
+  constexpr int BN = 256, CTAS = 2;
+  CUtensorMap ta, tb;
+  if (!make_map(&ta, x.A, x.a_mn != 0, x.M, x.K, 1, x.lda, 0, BM, 2)) return -1001;
+  if (!make_map(&tb, x.B, x.b_mn != 0, x.N, x.K, x.groups, x.ldb, x.groups > 1 ? x.b_group_bytes : x.ldb, BN / CTAS, 3)) return -2001;
+  const long long tiles_m = (x.M + BM * CTAS - 1) / (BM * CTAS) + (x.offsets != nullptr ? x.groups : 0);
+  return launch_epi<BN, CTAS>(ta, tb, p, tiles_m * ((x.N + BN - 1) / BN), x.epi, stream);
+}
+
+// swap: the rows of B take the 128-row side and the rows of A the side of bn.
+static int run_small(const Product& x, bool swap, int bn, int parts, cudaStream_t stream) {
+  SmallParams p;
+  p.C = x.C;
+  p.ldc = x.ldc;
+  p.M = swap ? x.N : x.M;
+  p.N = swap ? x.M : x.N;
+  p.K = x.K;
+  p.a_mn = swap ? x.b_mn : x.a_mn;
+  p.b_mn = swap ? x.a_mn : x.b_mn;
+  p.epi = x.epi;
+  p.vector = (reinterpret_cast<uintptr_t>(x.C) & 15) == 0 && (x.ldc * (x.epi == EPI_BF16 ? 2 : 4)) % 16 == 0;
+  p.parts = parts;
+  p.kb_per_part = ((x.K + BKE - 1) / BKE + parts - 1) / parts;
+  p.sa = swap ? x.sb : x.sa;
+  p.sb = swap ? x.sa : x.sb;
+  p.offsets = x.offsets;
+  p.num_groups = x.groups;
+  p.status = x.status;
+  const long long group_bytes = x.groups > 1 ? x.b_group_bytes : x.ldb;
+  const int rows_a = swap ? bn : BM, rows_b = swap ? BM : bn;
+  CUtensorMap ma, mb;
+  if (!make_map(&ma, x.A, x.a_mn != 0, x.M, x.K, 1, x.lda, x.lda, rows_a, 3)) return -1001;
+  if (!make_map(&mb, x.B, x.b_mn != 0, x.N, x.K, x.groups, x.ldb, group_bytes, rows_b, 3)) return -2001;
+  const CUtensorMap &ta = swap ? mb : ma, &tb = swap ? ma : mb;
+  long long b_tiles = (p.N + bn - 1) / bn;
+  // every group can end inside a tile; a group without rows has none
+  if (x.offsets != nullptr) b_tiles = p.N / bn + (x.groups < p.N ? x.groups : p.N);
+  const long long tiles = b_tiles * ((p.M + BM - 1) / BM);
+  if (swap) {
+    switch (bn) {
+      case 16: return launch_small<16, true>(ta, tb, p, tiles, stream);
+      case 32: return launch_small<32, true>(ta, tb, p, tiles, stream);
+      case 64: return launch_small<64, true>(ta, tb, p, tiles, stream);
+      default: return launch_small<128, true>(ta, tb, p, tiles, stream);
+    }
+  }
+  return launch_small<128, false>(ta, tb, p, tiles, stream);
+}
+
+// Which kernel. The pair kernel moves the fewest bytes per operation but works in 256 x 256 tiles on 74 pairs; with few tiles
+// the 128-row kernel fills the SMs, if need be by splitting the reduction.
+static int run(const Product& x, cudaStream_t stream) {
+  const int sms = num_sms();
+  if (sms <= 0) return -3;
+  const long long kb = (x.K + BKE - 1) / BKE;
+  const long long tiles_n = (x.N + 127) / 128;
+  auto split = [&](long long tiles) {  // parts that bring the CTAs to about two per SM, with two blocks each at least
+    int parts = 1;
+    while (parts < 8 && tiles * parts * 2 <= 2 * sms && kb >= 4 * parts) parts *= 2;
+    return parts;
+  };
+  if (x.offsets != nullptr) {
+    const long long mean = x.M / x.groups;  // rows of a group
+    if (mean > 128) return run_pair(x, stream);
+    const int bn = mean <= 8 ? 16 : mean <= 16 ? 32 : mean <= 48 ? 64 : 128;
+    const long long used = x.groups < x.M ? x.groups : x.M;
+    return run_small(x, true, bn, split(used * tiles_n), stream);
+  }
+  if (x.M <= 128 && !x.a_mn) {
+    const int bn = x.M <= 16 ? 16 : x.M <= 32 ? 32 : x.M <= 64 ? 64 : 128;
+    return run_small(x, true, bn, split(tiles_n), stream);
+  }
+  const long long pair_tiles = static_cast<long long>((x.M + 255) / 256) * ((x.N + 255) / 256);
+  const long long small_tiles = static_cast<long long>((x.M + 127) / 128) * tiles_n;
+  if (pair_tiles * 2 >= sms) return run_pair(x, stream);
+  return run_small(x, false, 128, split(small_tiles), stream);
+}
+
+}  // namespace blk
+}  // namespace ocb
+
 // See ocb_api.h.
 extern "C" int ocb_gemm_block_fp8(const void* A, const void* B, void* C, const float* sa, const float* sb, const int* offsets,
                                   int num_groups, int M, int N, int K, long long lda, long long ldb, long long ldc,
@@ -671,28 +1135,25 @@ extern "C" int ocb_gemm_block_fp8(const void* A, const void* B, void* C, const f
       (reinterpret_cast<uintptr_t>(B) & 15) || sa == nullptr || sb == nullptr)
     return -1;
   if ((sa_shift != 0 && sa_shift != 7) || (sb_shift != 0 && sb_shift != 7) || (offsets != nullptr && a_mn)) return -1;
-  blk::Params p;
-  p.C = C;
-  p.ldc = ldc;
-  p.M = M;
-  p.N = N;
-  p.K = K;
-  p.group_m = 8;
-  p.a_mn = a_mn;
-  p.b_mn = b_mn;
-  p.sa = {sa, sa_k, sa_i, 0, sa_shift};
-  p.sb = {sb, sb_k, sb_i, sb_g, sb_shift};
-  p.offsets = offsets;
-  p.num_groups = num_groups;
-  p.status = status;
-  p.aligned = (reinterpret_cast<uintptr_t>(C) & 15) == 0 && (ldc * (epilogue == blk::EPI_BF16 ? 2 : 4)) % 16 == 0;
-  const int bn = 256;
-  const int ctas = 2;
-  CUtensorMap ta, tb;
-  if (!blk::make_map(&ta, A, a_mn != 0, M, K, 1, lda, 0, blk::BM, 2)) return -1001;
-  if (!blk::make_map(&tb, B, b_mn != 0, N, K, num_groups, ldb, num_groups > 1 ? b_group_bytes : ldb, bn / ctas, 3)) return -2001;
-  const long long tiles_n = (N + bn - 1) / bn;
-  const long long tiles_m = (M + blk::BM * ctas - 1) / (blk::BM * ctas) + (offsets != nullptr ? num_groups : 0);
-  const long long tiles = tiles_m * tiles_n;
-  return blk::launch_epi<256, 2>(ta, tb, p, tiles, epilogue, stream);
+  blk::Product x;
+  x.A = A;
+  x.B = B;
+  x.C = C;
+  x.M = M;
+  x.N = N;
+  x.K = K;
+  x.groups = num_groups;
+  x.lda = lda;
+  x.ldb = ldb;
+  x.ldc = ldc;
+  x.b_group_bytes = b_group_bytes;
+  x.sa = {sa, sa_k, sa_i, 0, sa_shift};
+  x.sb = {sb, sb_k, sb_i, sb_g, sb_shift};
+  x.a_mn = a_mn;
+  x.b_mn = b_mn;
+  x.epi = epilogue;
+  x.offsets = offsets;
+  x.status = status;
+  if (epilogue < blk::EPI_BF16 || epilogue > blk::EPI_F32) return -1;
+  return blk::run(x, stream);
 }

@@ -124,7 +124,7 @@ def _assert_product(out, a, b, base=None):
 
 
 SHAPES = [(1, 1, 1), (1, 300, 520), (7, 128, 128), (100, 257, 129), (128, 256, 256), (129, 1001, 2050), (300, 40, 1000),
-          (520, 513, 384)]
+          (520, 513, 384), (16, 640, 1500), (33, 200, 260), (64, 130, 2000), (2560, 2050, 300)]
 
 
 @pytest.mark.parametrize("device", DEVICES)
@@ -151,7 +151,7 @@ def test_product(M, N, K, trans_a, trans_b, b_tiles, device):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("M,N,K", [(1, 1024, 4096), (640, 768, 512), (2048, 1000, 1160)])
+@pytest.mark.parametrize("M,N,K", [(1, 1024, 4096), (640, 768, 512), (2048, 1000, 1160), (4096, 2304, 512)])
 def test_product_repeats_bit_for_bit_and_replays(M, N, K):
     aq, sa, a = _operand((M, K), 7, "rows", "cuda")
     bq, sb, b = _operand((N, K), 8, "tiles", "cuda")
@@ -187,7 +187,7 @@ def test_scales_that_are_no_powers_of_two_show_as_nan(bad, device):
     _assert_product(out[keep, :128], a[keep], b[:128])
 
 
-GROUPS = [[128, 256, 128], [100, 0, 333, 7, 1], [0, 0, 5], [1, 1, 2, 0, 1, 3, 1, 1], [1000, 37, 0, 0, 513, 64, 65, 2]]
+GROUPS = [[128, 256, 128], [100, 0, 333, 7, 1], [0, 0, 5], [1, 1, 2, 0, 1, 3, 1, 1], [20, 0, 17, 3] * 10, [0] * 40 + [50, 33] + [0] * 3, [1000, 37, 0, 0, 513, 64, 65, 2]]
 
 
 @pytest.mark.parametrize("device", DEVICES)
