@@ -44,14 +44,36 @@ __device__ __forceinline__ int scale_exponent(float amax) {
 }
 __device__ __forceinline__ float pow2_biased(int e) { return __uint_as_float(static_cast<uint32_t>(e) << 23); }
 
-__device__ __forceinline__ uint32_t e4m3x2(float a, float b) {
-  return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+// Packed magnitudes: the larger of two pairs, NaN ignored.
+__device__ __forceinline__ uint32_t max_abs2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("{\n\t.reg .b32 t;\n\tabs.bf16x2 t, %2;\n\tmax.bf16x2 %0, %1, t;\n\t}" : "=r"(r) : "r"(a), "r"(b));
+  return r;
 }
-// x * inv; the product with zero turns an infinity into NaN, which the saturating cast would hide, and adds nothing otherwise.
-__device__ __forceinline__ float scaled(float x, float inv) { return __fmaf_rn(x, 0.f, x * inv); }
-
 __device__ __forceinline__ float lo(uint32_t u) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ float hi(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
+
+// Two elements (bf16 pair) times two powers of two, as e4m3. HAS_INF: the block holds an infinity, whose product with zero
+// makes the NaN that the saturating cast would hide.
+template <bool HAS_INF>
+__device__ __forceinline__ uint32_t e4m3x2(uint32_t pair, float inv0, float inv1) {
+  float a = lo(pair) * inv0, b = hi(pair) * inv1;
+  if (HAS_INF) {
+    a = __fmaf_rn(lo(pair), 0.f, a);
+    b = __fmaf_rn(hi(pair), 0.f, b);
+  }
+  return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+}
+template <bool HAS_INF>
+__device__ __forceinline__ uint2 e4m3x8(const uint4& v, const float (&inv)[8]) {
+  return make_uint2(e4m3x2<HAS_INF>(v.x, inv[0], inv[1]) | (e4m3x2<HAS_INF>(v.y, inv[2], inv[3]) << 16),
+                    e4m3x2<HAS_INF>(v.z, inv[4], inv[5]) | (e4m3x2<HAS_INF>(v.w, inv[6], inv[7]) << 16));
+}
+template <bool HAS_INF>
+__device__ __forceinline__ uint2 e4m3x8(const uint4& v, float inv) {
+  return make_uint2(e4m3x2<HAS_INF>(v.x, inv, inv) | (e4m3x2<HAS_INF>(v.y, inv, inv) << 16),
+                    e4m3x2<HAS_INF>(v.z, inv, inv) | (e4m3x2<HAS_INF>(v.w, inv, inv) << 16));
+}
 
 __device__ __forceinline__ void store8(uint8_t* dst, uint2 v, int n) {
   if (n >= 8) {
@@ -62,8 +84,9 @@ __device__ __forceinline__ void store8(uint8_t* dst, uint2 v, int n) {
 }
 
 template <int MODE>
-__global__ void __launch_bounds__(THREADS) quantize_block_kernel(const Params p, int vec) {
-  __shared__ float red[8][B];  // column maxima of each warp; the tile form uses red[0][0..7]
+__global__ void __launch_bounds__(THREADS, MODE == (ROWS | COLUMNS) ? 3 : 4) quantize_block_kernel(const Params p, int vec) {
+  __shared__ uint32_t red[8][B / 2];  // column maxima (pairs) of each warp; the tile form uses red[0][0..7]
+  __shared__ float factor[B], row_scale[B];
   const int across = threadIdx.x & 15, down = threadIdx.x >> 4;
   const int warp = threadIdx.x >> 5;
   const int col = blockIdx.x * B + across * 8;
@@ -92,75 +115,76 @@ __global__ void __launch_bounds__(THREADS) quantize_block_kernel(const Params p,
 
   if (MODE & ROWS) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-      float amax = 0.f;
+    for (int i = 0; i < 8; i += 2) {  // two rows share a register on their way through the half-warp
+      const uint32_t a = max_abs2(max_abs2(max_abs2(max_abs2(0u, v[i].x), v[i].y), v[i].z), v[i].w);
+      const uint32_t b = max_abs2(max_abs2(max_abs2(max_abs2(0u, v[i + 1].x), v[i + 1].y), v[i + 1].z), v[i + 1].w);
+      uint32_t m2 = max_abs2(__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632));
 #pragma unroll
-      for (int j = 0; j < 4; ++j) amax = fmaxf(amax, fmaxf(fabsf(lo(w[j])), fabsf(hi(w[j]))));
+      for (int o = 8; o; o >>= 1) m2 = max_abs2(m2, __shfl_xor_sync(0xffffffffu, m2, o));
 #pragma unroll
-      for (int o = 8; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-      const int e = scale_exponent(amax);
-      const float inv = pow2_biased(254 - e);
-      const long long row = row0 + down + 16 * i;
-      if (row < p.rows) {
-        uint2 o;
-        o.x = e4m3x2(scaled(lo(w[0]), inv), scaled(hi(w[0]), inv)) | (e4m3x2(scaled(lo(w[1]), inv), scaled(hi(w[1]), inv)) << 16);
-        o.y = e4m3x2(scaled(lo(w[2]), inv), scaled(hi(w[2]), inv)) | (e4m3x2(scaled(lo(w[3]), inv), scaled(hi(w[3]), inv)) << 16);
-        if (n_col > 0) store8(p.q_row + row * p.ldq + col, o, n_col);
-        if (across == 0) p.s_row[static_cast<long long>(blockIdx.x) * p.rows + row] = pow2_biased(e);
+      for (int h = 0; h < 2; ++h) {
+        const float amax = h ? hi(m2) : lo(m2);
+        const int e = scale_exponent(amax);
+        const float inv = pow2_biased(254 - e);
+        const int local = down + 16 * (i + h);
+        const long long row = row0 + local;
+        if (across == 0) row_scale[local] = pow2_biased(e);
+        if (row < p.rows && n_col > 0)
+          store8(p.q_row + row * p.ldq + col, amax == INFINITY ? e4m3x8<true>(v[i + h], inv) : e4m3x8<false>(v[i + h], inv), n_col);
       }
     }
   }
 
   if (MODE & (COLUMNS | TILES)) {
-    float m[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) m[j] = 0.f;
+    uint32_t m2[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        m[2 * j] = fmaxf(m[2 * j], fabsf(lo(w[j])));
-        m[2 * j + 1] = fmaxf(m[2 * j + 1], fabsf(hi(w[j])));
-      }
+      m2[0] = max_abs2(m2[0], v[i].x);
+      m2[1] = max_abs2(m2[1], v[i].y);
+      m2[2] = max_abs2(m2[2], v[i].z);
+      m2[3] = max_abs2(m2[3], v[i].w);
     }
     float inv[8];
+    bool has_inf = false;
     if (MODE & COLUMNS) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) m[j] = fmaxf(m[j], __shfl_xor_sync(0xffffffffu, m[j], 16));
-      if ((threadIdx.x & 16) == 0) {
+      for (int j = 0; j < 4; ++j) m2[j] = max_abs2(m2[j], __shfl_xor_sync(0xffffffffu, m2[j], 16));
+      if ((threadIdx.x & 16) == 0) *reinterpret_cast<uint4*>(&red[warp][across * 4]) = make_uint4(m2[0], m2[1], m2[2], m2[3]);
+      __syncthreads();
+      if (threadIdx.x < B / 2) {
+        uint32_t top = red[0][threadIdx.x];
 #pragma unroll
-        for (int j = 0; j < 8; j += 4)
-          *reinterpret_cast<float4*>(&red[warp][across * 8 + j]) = make_float4(m[j], m[j + 1], m[j + 2], m[j + 3]);
+        for (int w = 1; w < 8; ++w) top = max_abs2(top, red[w][threadIdx.x]);
+        const float amax[2] = {lo(top), hi(top)};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int e = scale_exponent(amax[h]);
+          // the reciprocal; its sign says that the column holds an infinity
+          factor[2 * threadIdx.x + h] = amax[h] == INFINITY ? -pow2_biased(254 - e) : pow2_biased(254 - e);
+          const int c = blockIdx.x * B + 2 * threadIdx.x + h;
+          if (c < p.cols) p.s_col[static_cast<long long>(blockIdx.y) * p.cols + c] = pow2_biased(e);
+        }
       }
       __syncthreads();
-      if (threadIdx.x < B) {
-        float top = red[0][threadIdx.x];
 #pragma unroll
-        for (int w = 1; w < 8; ++w) top = fmaxf(top, red[w][threadIdx.x]);
-        const int e = scale_exponent(top);
-        red[0][threadIdx.x] = pow2_biased(254 - e);
-        const int c = blockIdx.x * B + threadIdx.x;
-        if (c < p.cols) p.s_col[static_cast<long long>(blockIdx.y) * p.cols + c] = pow2_biased(e);
+      for (int j = 0; j < 8; j += 4) {
+        const float4 f = *reinterpret_cast<const float4*>(&factor[across * 8 + j]);
+        inv[j] = fabsf(f.x); inv[j + 1] = fabsf(f.y); inv[j + 2] = fabsf(f.z); inv[j + 3] = fabsf(f.w);
+        has_inf |= fminf(fminf(f.x, f.y), fminf(f.z, f.w)) < 0.f;
       }
-      __syncthreads();
-#pragma unroll
-      for (int j = 0; j < 8; ++j) inv[j] = red[0][across * 8 + j];
     } else {
-      float top = 0.f;
+      uint32_t top2 = max_abs2(max_abs2(m2[0], m2[1]), max_abs2(m2[2], m2[3]));
 #pragma unroll
-      for (int j = 0; j < 8; ++j) top = fmaxf(top, m[j]);
-#pragma unroll
-      for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      if ((threadIdx.x & 31) == 0) red[0][warp] = top;
+      for (int o = 16; o; o >>= 1) top2 = max_abs2(top2, __shfl_xor_sync(0xffffffffu, top2, o));
+      if ((threadIdx.x & 31) == 0) red[0][warp] = top2;
       __syncthreads();
 #pragma unroll
-      for (int w = 0; w < 8; ++w) top = fmaxf(top, red[0][w]);
+      for (int w = 0; w < 8; ++w) top2 = max_abs2(top2, red[0][w]);
+      const float top = fmaxf(lo(top2), hi(top2));
+      has_inf = top == INFINITY;
       const int e = scale_exponent(top);
-      const float f = pow2_biased(254 - e);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) inv[j] = f;
+      for (int j = 0; j < 8; ++j) inv[j] = pow2_biased(254 - e);
       if (threadIdx.x == 0)
         p.s_tile[(static_cast<long long>(blockIdx.z) * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x] = pow2_biased(e);
     }
@@ -169,16 +193,14 @@ __global__ void __launch_bounds__(THREADS) quantize_block_kernel(const Params p,
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const long long row = row0 + down + 16 * i;
-        if (row >= p.rows) continue;
-        const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-        uint2 o;
-        o.x = e4m3x2(scaled(lo(w[0]), inv[0]), scaled(hi(w[0]), inv[1])) |
-              (e4m3x2(scaled(lo(w[1]), inv[2]), scaled(hi(w[1]), inv[3])) << 16);
-        o.y = e4m3x2(scaled(lo(w[2]), inv[4]), scaled(hi(w[2]), inv[5])) |
-              (e4m3x2(scaled(lo(w[3]), inv[6]), scaled(hi(w[3]), inv[7])) << 16);
-        store8(q + row * p.ldq + col, o, n_col);
+        if (row < p.rows) store8(q + row * p.ldq + col, has_inf ? e4m3x8<true>(v[i], inv) : e4m3x8<false>(v[i], inv), n_col);
       }
     }
+  }
+  if (MODE & ROWS) {
+    __syncthreads();
+    if (threadIdx.x < B && row0 + threadIdx.x < p.rows)
+      p.s_row[static_cast<long long>(blockIdx.x) * p.rows + row0 + threadIdx.x] = row_scale[threadIdx.x];
   }
 }
 
