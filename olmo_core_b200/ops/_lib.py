@@ -179,6 +179,15 @@ def stream_ptr() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
+def on_device(device: torch.device, launcher, *args) -> int:
+    """``launcher(*args, stream)`` with ``device`` current and its current stream; costs nothing where it already is."""
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        return launcher(*args, torch._C._cuda_getCurrentRawStream(index))
+    with torch.cuda.device(device):
+        return launcher(*args, torch._C._cuda_getCurrentRawStream(index))
+
+
 def ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 

@@ -1157,3 +1157,14 @@ extern "C" int ocb_gemm_block_fp8(const void* A, const void* B, void* C, const f
   if (epilogue < blk::EPI_BF16 || epilogue > blk::EPI_F32) return -1;
   return blk::run(x, stream);
 }
+
+// See ocb_api.h.
+extern "C" int ocb_linear_block_fp8(const void* x, long long ldx, void* q_row, float* s_row, void* q_col, float* s_col,
+                                    long long ldq, const void* W, const float* sw, const int* offsets, int num_groups, void* C,
+                                    int M, int N, int K, long long ldw, long long w_group_bytes, long long sw_k, long long sw_i,
+                                    long long sw_g, int w_mn, long long ldc, int epilogue, int* status, cudaStream_t stream) {
+  const int rc = ocb_quantize_block_fp8(x, q_row, s_row, q_col, s_col, nullptr, nullptr, 1, M, K, ldx, ldq, 0, 0, stream);
+  if (rc != 0) return rc;
+  return ocb_gemm_block_fp8(q_row, W, C, s_row, sw, offsets, num_groups, M, N, K, ldq, ldw, ldc, w_group_bytes, M, 1, 0, sw_k,
+                            sw_i, sw_g, 7, 0, w_mn, epilogue, status, stream);
+}

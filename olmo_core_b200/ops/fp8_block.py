@@ -53,6 +53,8 @@ def _lib_block():
         _lib.register_signature("ocb_quantize_block_fp8", [c_void_p] * 7 + [c_int] * 3 + [c_longlong] * 4 + [c_void_p])
         _lib.register_signature("ocb_gemm_block_fp8", [c_void_p] * 6 + [c_int] * 4 + [c_longlong] * 6 + [c_int]
                                 + [c_longlong] * 3 + [c_int] * 4 + [c_void_p] * 2)
+        _lib.register_signature("ocb_linear_block_fp8", [c_void_p, c_longlong] + [c_void_p] * 4 + [c_longlong] + [c_void_p] * 3
+                                + [c_int, c_void_p] + [c_int] * 3 + [c_longlong] * 5 + [c_int, c_longlong, c_int] + [c_void_p] * 2)
         _lib_sigs_done = True
     return lib
 
@@ -92,6 +94,11 @@ def _codes(lead, rows: int, cols: int, device) -> torch.Tensor:
     return torch.empty((*lead, rows, (cols + 15) // 16 * 16), dtype=torch.uint8, device=device)[..., :cols]
 
 
+def _pitch(q: torch.Tensor) -> int:
+    """Bytes between the rows of a code matrix (a single row may carry any stride)."""
+    return q.stride(-2) if q.shape[-2] > 1 else (q.shape[-1] + 15) // 16 * 16
+
+
 def _check_matrix(x: torch.Tensor, what: str, dims: Tuple[int, ...] = (2,)) -> torch.Tensor:
     if x.dim() not in dims:
         raise ValueError(f"{what} must have {' or '.join(map(str, dims))} dimensions, got shape {tuple(x.shape)}")
@@ -104,11 +111,10 @@ def _launch_quantize(x: torch.Tensor, q_row, s_row, q_col, s_col, q_tile=None, s
     R, C = x.shape[-2:]
     groups = x.shape[0] if x.dim() == 3 else 1
     q = next(t for t in (q_row, q_col, q_tile) if t is not None)
-    with torch.cuda.device(x.device):
-        rc = _lib_block().ocb_quantize_block_fp8(
-            x.data_ptr(), _lib.ptr(q_row), _lib.ptr(s_row), _lib.ptr(q_col), _lib.ptr(s_col), _lib.ptr(q_tile),
-            _lib.ptr(s_tile), groups, R, C, x.stride(-2), q.stride(-2), x.stride(0) if x.dim() == 3 else 0,
-            q.stride(0) if x.dim() == 3 else 0, _lib.stream_ptr())
+    rc = _lib.on_device(
+        x.device, _lib_block().ocb_quantize_block_fp8, x.data_ptr(), _lib.ptr(q_row), _lib.ptr(s_row), _lib.ptr(q_col),
+        _lib.ptr(s_col), _lib.ptr(q_tile), _lib.ptr(s_tile), groups, R, C, x.stride(-2), _pitch(q),
+        x.stride(0) if x.dim() == 3 else 0, q.stride(0) if x.dim() == 3 else 0)
     _lib.check(rc, "ocb_quantize_block_fp8")
 
 
@@ -293,19 +299,13 @@ def gemm_fp8_block(
         sb_k, sb_i = (b_s.stride(1), b_s.stride(0)) if trans_b else (b_s.stride(0), b_s.stride(1))
     else:
         sb_k, sb_i = b_s.stride()
-    with torch.cuda.device(a_q.device):
-        rc = _lib_block().ocb_gemm_block_fp8(
-            a_q.data_ptr(), b_q.data_ptr(), out.data_ptr(), a_s.data_ptr(), b_s.data_ptr(), None, 1, M, N, K, _pitch(a_q),
-            _pitch(b_q), out.stride(0), 0, a_s.stride(0), a_s.stride(1), 0, sb_k, sb_i, 0, 7 if b_tiles else 0,
-            int(trans_a), int(not trans_b), _epilogue(out, accumulate), _lib.status_buffer(a_q.device).data_ptr(),
-            _lib.stream_ptr())
+    rc = _lib.on_device(
+        a_q.device, _lib_block().ocb_gemm_block_fp8, a_q.data_ptr(), b_q.data_ptr(), out.data_ptr(), a_s.data_ptr(),
+        b_s.data_ptr(), None, 1, M, N, K, _pitch(a_q), _pitch(b_q), out.stride(0), 0, a_s.stride(0), a_s.stride(1), 0, sb_k,
+        sb_i, 0, 7 if b_tiles else 0, int(trans_a), int(not trans_b), _epilogue(out, accumulate),
+        _lib.status_buffer(a_q.device).data_ptr())
     _lib.check(rc, "ocb_gemm_block_fp8")
     return out
-
-
-def _pitch(q: torch.Tensor) -> int:
-    """Bytes between the rows of a code matrix (a single row may carry any stride)."""
-    return q.stride(-2) if q.shape[-2] > 1 else (q.shape[-1] + 15) // 16 * 16
 
 
 def grouped_gemm_fp8_block(
@@ -350,12 +350,11 @@ def grouped_gemm_fp8_block(
             out[lo:hi] = (a[lo:hi] @ (b[g].t() if trans_b else b[g])).to(out.dtype)
         return out
     sb_k, sb_i = (b_s.stride(2), b_s.stride(1)) if trans_b else (b_s.stride(1), b_s.stride(2))
-    with torch.cuda.device(a_q.device):
-        rc = _lib_block().ocb_gemm_block_fp8(
-            a_q.data_ptr(), b_q.data_ptr(), out.data_ptr(), a_s.data_ptr(), b_s.data_ptr(), offsets.data_ptr(), G, R, N, K,
-            _pitch(a_q), _pitch(b_q), out.stride(0), b_q.stride(0) if G > 1 else b_q.shape[1] * _pitch(b_q), a_s.stride(0),
-            a_s.stride(1), 0, sb_k, sb_i, b_s.stride(0), 7, 0, int(not trans_b), _lib.EPI_BF16,
-            _lib.status_buffer(a_q.device).data_ptr(), _lib.stream_ptr())
+    rc = _lib.on_device(
+        a_q.device, _lib_block().ocb_gemm_block_fp8, a_q.data_ptr(), b_q.data_ptr(), out.data_ptr(), a_s.data_ptr(),
+        b_s.data_ptr(), offsets.data_ptr(), G, R, N, K, _pitch(a_q), _pitch(b_q), out.stride(0),
+        b_q.stride(0) if G > 1 else b_q.shape[1] * _pitch(b_q), a_s.stride(0), a_s.stride(1), 0, sb_k, sb_i, b_s.stride(0), 7,
+        0, int(not trans_b), _lib.EPI_BF16, _lib.status_buffer(a_q.device).data_ptr())
     _lib.check(rc, "ocb_gemm_block_fp8")
     return out
 
@@ -374,81 +373,157 @@ def _check_offsets(offsets: torch.Tensor, groups: int, device: torch.device) -> 
 # ------------------------------------------------------------------------------------------------------
 
 
+def _quantized_product(x: torch.Tensor, w_q: torch.Tensor, w_s: torch.Tensor, trans_b: bool,
+                       offsets: Optional[torch.Tensor] = None, keep_columns: bool = False):
+    """
+    ``q_rows(x) @ op(W)`` (bf16) for checked operands on a GPU, quantiser and product in one call. With ``keep_columns`` also
+    the column-scaled form of ``x``, as ``(buffer of codes and scales,)``.
+    """
+    M, K = x.shape
+    N = w_q.shape[-2] if trans_b else w_q.shape[-1]
+    out = torch.empty((M, N), dtype=torch.bfloat16, device=x.device)
+    if M == 0 or N == 0 or K == 0:
+        return (out.zero_() if M and N else out), (_column_buffer(M, K, x.device) if keep_columns else None)
+    pitch = (K + 15) & -16
+    codes = M * pitch
+    rows = torch.empty(codes + 4 * _blocks(K) * M, dtype=torch.uint8, device=x.device)
+    columns = _column_buffer(M, K, x.device) if keep_columns else None
+    sw_k, sw_i = (w_s.stride(-1), w_s.stride(-2)) if trans_b else (w_s.stride(-2), w_s.stride(-1))
+    grouped = w_q.dim() == 3
+    groups = w_q.shape[0] if grouped else 1
+    at, at_c = rows.data_ptr(), None if columns is None else columns.data_ptr()
+    rc = _lib.on_device(
+        x.device, _lib_block().ocb_linear_block_fp8, x.data_ptr(), x.stride(0), at, at + codes, at_c,
+        None if at_c is None else at_c + codes, pitch, w_q.data_ptr(), w_s.data_ptr(), _lib.ptr(offsets), groups,
+        out.data_ptr(), M, N, K, _pitch(w_q), w_q.stride(0) if groups > 1 else w_q.shape[-2] * _pitch(w_q), sw_k, sw_i,
+        w_s.stride(0) if grouped else 0, int(not trans_b), N, _lib.EPI_BF16, _lib.status_buffer(x.device).data_ptr())
+    _lib.check(rc, "ocb_linear_block_fp8")
+    return out, columns
+
+
+def _column_buffer(M: int, K: int, device) -> torch.Tensor:
+    """Codes ``[M, K rounded up to 16]`` and behind them scales ``[ceil(M / 128), K]`` of a column-scaled matrix, in one buffer."""
+    return torch.empty(M * ((K + 15) & -16) + 4 * _blocks(M) * K, dtype=torch.uint8, device=device)
+
+
+def _column_views(buffer: torch.Tensor, M: int, K: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    pitch = (K + 15) & -16
+    return (buffer[: M * pitch].view(M, pitch)[:, :K],
+            buffer[M * pitch:].view(torch.float32).view(_blocks(M), K))
+
+
+def _wgrad(dy_columns: torch.Tensor, x_columns: torch.Tensor, M: int, N: int, K: int, out: torch.Tensor, accumulate: bool) -> None:
+    """``out [N, K] (=|+=) q_columns(dy)^T q_columns(x)`` from two column buffers."""
+    a, b = dy_columns.data_ptr(), x_columns.data_ptr()
+    pitch_a, pitch_b = (N + 15) & -16, (K + 15) & -16
+    rc = _lib.on_device(
+        out.device, _lib_block().ocb_gemm_block_fp8, a, b, out.data_ptr(), a + M * pitch_a, b + M * pitch_b, None, 1, N, K, M,
+        pitch_a, pitch_b, out.stride(0), 0, N, 1, 0, K, 1, 0, 0, 1, 1, _epilogue(out, accumulate),
+        _lib.status_buffer(out.device).data_ptr())
+    _lib.check(rc, "ocb_gemm_block_fp8")
+
+
 def fp8_block_matmul(x: torch.Tensor, w_q: torch.Tensor, w_s: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """
     ``x @ W^T (+ bias)`` for a weight that is kept in 8 bits: codes ``w_q [N, K]`` with tile scales ``w_s`` (from
     :func:`quantize_block_tiles` or a checkpoint). ``x [..., K]`` is quantised by rows; the result is bf16. No gradient.
     """
+    _check_codes(w_q, "w_q", 2)
+    N, K = w_q.shape
+    if x.shape[-1] != K:
+        raise ValueError(f"x has {x.shape[-1]} features, the weight takes {K}")
+    if x.device != w_q.device:
+        raise ValueError(f"x is on {x.device}, the weight on {w_q.device}")
+    _check_scales(w_s, "w_s", (_blocks(N), _blocks(K)), w_q.device)
     with torch.no_grad():
-        x2 = x.reshape(-1, x.shape[-1])
-        q, s = quantize_block_rows(x2)
-        y = gemm_fp8_block(q, s, w_q, w_s)
-    y = y.view(*x.shape[:-1], w_q.shape[0])
-    return y if bias is None else y + bias.to(y.dtype)
+        x2 = _check_matrix(x if x.dim() == 2 else x.reshape(-1, K), "x")
+        if x2.is_cuda:
+            y, _ = _quantized_product(x2, w_q, w_s, True)
+        else:
+            y = gemm_fp8_block(*quantize_block_rows(x2), w_q, w_s)
+        y = y if x.dim() == 2 else y.view(*x.shape[:-1], N)
+        return y if bias is None else y + bias.to(y.dtype)
 
 
 def fp8_block_grouped_matmul(x: torch.Tensor, w_q: torch.Tensor, w_s: torch.Tensor, offsets: torch.Tensor, *,
                              trans_b: bool = True) -> torch.Tensor:
     """
     The experts' product for weights that are kept in 8 bits: ``y[rows of g] = x[rows of g] @ op(W_g)``; ``x [R, K]`` sorted
-    by group, ``w_q [G, N, K]`` (``trans_b``) or ``[G, K, N]`` with tile scales, ``offsets`` int32 ``[G + 1]``. No gradient.
+    by group, ``w_q [G, N, K]`` (``trans_b``) or ``[G, K, N]`` with tile scales, ``offsets`` int32 ``[G + 1]`` (row boundaries,
+    see :func:`grouped_gemm_fp8_block`). Rows outside every group are undefined. No gradient.
     """
+    _check_codes(w_q, "w_q", 3)
+    G, n, k = w_q.shape
+    if x.dim() != 2 or x.shape[1] != (k if trans_b else n):
+        raise ValueError(f"x of shape {tuple(x.shape)} does not fit experts that take {k if trans_b else n} features")
+    if x.device != w_q.device:
+        raise ValueError(f"x is on {x.device}, the weights on {w_q.device}")
+    _check_offsets(offsets, G, w_q.device)
+    _check_scales(w_s, "w_s", (G, _blocks(n), _blocks(k)), w_q.device)
     with torch.no_grad():
-        q, s = quantize_block_rows(x)
-        return grouped_gemm_fp8_block(q, s, w_q, w_s, offsets, trans_b=trans_b)
+        x2 = _check_matrix(x, "x")
+        if x2.is_cuda and G:
+            return _quantized_product(x2, w_q, w_s, trans_b, offsets)[0]
+        return grouped_gemm_fp8_block(*quantize_block_rows(x2), w_q, w_s, offsets, trans_b=trans_b)
 
 
 class BlockFloat8LinearFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, wgrad_high_precision: bool, cache: Optional[dict] = None):  # type: ignore[override]
         w = compute_weight(weight, torch.bfloat16)
-        x2 = _check_matrix(x.reshape(-1, x.shape[-1]), "x")
+        x2 = _check_matrix(x if x.dim() == 2 else x.reshape(-1, x.shape[-1]), "x")
         wq, sw = cached_weight_cast(cache, "block_tiles", lambda: quantize_block_tiles(w), weight._version)
         needs_dw = ctx.needs_input_grad[1] or getattr(weight, "main_grad", None) is not None
-        if needs_dw and not wgrad_high_precision:
-            # what the backward pass keeps of x is its column-scaled form: one byte per element
-            xq, sx, xc, sxc = quantize_block_rows_columns(x2)
-            kept = (xc, sxc)
+        in_fp8 = needs_dw and not wgrad_high_precision
+        # what the backward pass keeps of x is its column-scaled form: one byte per element
+        if x2.is_cuda:
+            y, columns = _quantized_product(x2, wq, sw, True, keep_columns=in_fp8)
+            kept = (columns,) if in_fp8 else (x2,) if needs_dw else ()
         else:
-            xq, sx = quantize_block_rows(x2)
-            kept = (x2,) if needs_dw else ()
-        y = gemm_fp8_block(xq, sx, wq, sw)
+            y = gemm_fp8_block(*quantize_block_rows(x2), wq, sw)
+            kept = quantize_block_columns(x2) if in_fp8 else (x2,) if needs_dw else ()
         ctx.save_for_backward(wq, sw, *kept)
-        ctx.wgrad_hp = wgrad_high_precision
+        ctx.in_fp8, ctx.x2_shape = in_fp8, x2.shape
         ctx.weight_ref, ctx.x_shape, ctx.x_dtype = weight, x.shape, x.dtype
-        return y.view(*x.shape[:-1], w.shape[0])
+        return y if x.dim() == 2 else y.view(*x.shape[:-1], w.shape[0])
 
     @staticmethod
     def backward(ctx, dy):  # type: ignore[override]
         wq, sw, *kept = ctx.saved_tensors
         weight = ctx.weight_ref
-        dy2 = _check_matrix(dy.reshape(-1, dy.shape[-1]), "dy")
+        (M, K), N = ctx.x2_shape, wq.shape[0]
+        dy2 = _check_matrix(dy if dy.dim() == 2 else dy.reshape(-1, N), "dy")
         main_grad = getattr(weight, "main_grad", None)
+        needs_dx = ctx.needs_input_grad[0]
         needs_dw = main_grad is not None or ctx.needs_input_grad[1]
-        wgrad_fp8 = needs_dw and not ctx.wgrad_hp
-        dx = dw = None
-        if ctx.needs_input_grad[0] and wgrad_fp8:
-            dyq, sdy, dyc, sdyc = quantize_block_rows_columns(dy2)
-        elif ctx.needs_input_grad[0]:
-            dyq, sdy = quantize_block_rows(dy2)
-        elif wgrad_fp8:
-            dyc, sdyc = quantize_block_columns(dy2)
-        if ctx.needs_input_grad[0]:
-            dx = gemm_fp8_block(dyq, sdy, wq, sw, trans_b=False).view(ctx.x_shape).to(ctx.x_dtype)
+        in_fp8 = needs_dw and ctx.in_fp8
+        dx = dw = columns = None
+        if needs_dx:
+            if dy2.is_cuda:
+                dx, columns = _quantized_product(dy2, wq, sw, False, keep_columns=in_fp8)
+            else:
+                dx = gemm_fp8_block(*quantize_block_rows(dy2), wq, sw, trans_b=False)
+            dx = dx if len(ctx.x_shape) == 2 else dx.view(ctx.x_shape)
+            dx = dx if dx.dtype == ctx.x_dtype else dx.to(ctx.x_dtype)
         if needs_dw:
-            if wgrad_fp8:
-                args, kwargs = (dyc, sdyc, *kept), dict(trans_a=True, trans_b=False, b_tiles=False)
-                product = gemm_fp8_block
+            # the kernels write bf16 or fp32, whichever the parameter has
+            out = main_grad if main_grad is not None else torch.empty(
+                (N, K), dtype=torch.bfloat16 if weight.dtype == torch.bfloat16 else torch.float32, device=dy2.device)
+            accumulate = main_grad is not None
+            if not in_fp8:
+                gemm(dy2, kept[0], trans_a=True, trans_b=False, out=out, accumulate=accumulate)
+            elif M == 0:
+                out if accumulate else out.zero_()
+            elif columns is not None:
+                _wgrad(columns, kept[0], M, N, K, out, accumulate)
             else:
-                args, kwargs, product = (dy2, kept[0]), dict(trans_a=True, trans_b=False), gemm
-            if main_grad is not None:
-                product(*args, **kwargs, out=main_grad, accumulate=True)
-                if hasattr(weight, "grad_added_to_main_grad"):
-                    weight.grad_added_to_main_grad = True
-            elif weight.dtype == torch.bfloat16:
-                dw = product(*args, **kwargs, out_dtype=torch.bfloat16)
-            else:
-                dw = product(*args, **kwargs, out_dtype=torch.float32).to(weight.dtype)
+                x_columns = _column_views(kept[0], M, K) if dy2.is_cuda else kept
+                gemm_fp8_block(*quantize_block_columns(dy2), *x_columns, trans_a=True, trans_b=False, b_tiles=False, out=out,
+                               accumulate=accumulate)
+            if main_grad is None:
+                dw = out.to(weight.dtype)
+            elif hasattr(weight, "grad_added_to_main_grad"):
+                weight.grad_added_to_main_grad = True
         return dx, dw, None, None
 
 
@@ -461,6 +536,8 @@ def fp8_block_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch
     """
     if x.shape[-1] != weight.shape[-1]:
         raise ValueError(f"x has {x.shape[-1]} features, the weight takes {weight.shape[-1]}")
+    if wgrad_high_precision and (weight.shape[-1] % 8 or weight.shape[0] % 8):
+        raise ValueError("a weight gradient in bf16 needs widths that are multiples of 8")
     y = BlockFloat8LinearFunction.apply(x, weight, wgrad_high_precision, weight_cache)
     return y if bias is None else y + bias.to(y.dtype)
 
@@ -472,8 +549,10 @@ class BlockFloat8GroupedLinearFunction(torch.autograd.Function):
         G = offsets.numel() - 1
         x2 = _check_matrix(x, "x")
         wq, sw = cached_weight_cast(cache, "block_tiles", lambda: quantize_block_tiles(w.view(G, -1, w.shape[-1])), weight._version)
-        xq, sx = quantize_block_rows(x2)
-        y = grouped_gemm_fp8_block(xq, sx, wq, sw, offsets, trans_b=trans_b)
+        if x2.is_cuda:
+            y, _ = _quantized_product(x2, wq, sw, trans_b, offsets)
+        else:
+            y = grouped_gemm_fp8_block(*quantize_block_rows(x2), wq, sw, offsets, trans_b=trans_b)
         ctx.save_for_backward(wq, sw, offsets, x2)
         ctx.trans_b, ctx.weight_ref, ctx.w_shape, ctx.x_dtype = trans_b, weight, w.shape, x.dtype
         return y
@@ -485,29 +564,32 @@ class BlockFloat8GroupedLinearFunction(torch.autograd.Function):
         dy2 = _check_matrix(dy, "dy")
         dx = dw = None
         if ctx.needs_input_grad[0]:
-            dyq, sdy = quantize_block_rows(dy2)
-            dx = grouped_gemm_fp8_block(dyq, sdy, wq, sw, offsets, trans_b=not trans_b).to(ctx.x_dtype)
+            if dy2.is_cuda:
+                dx, _ = _quantized_product(dy2, wq, sw, not trans_b, offsets)
+            else:
+                dx = grouped_gemm_fp8_block(*quantize_block_rows(dy2), wq, sw, offsets, trans_b=not trans_b)
+            dx = dx if dx.dtype == ctx.x_dtype else dx.to(ctx.x_dtype)
         main_grad = getattr(weight, "main_grad", None)
         if main_grad is not None or ctx.needs_input_grad[1]:
             a, b = (dy2, x2) if trans_b else (x2, dy2)
-            if main_grad is not None:
-                dw = main_grad.view(ctx.w_shape)
-            else:
-                dw = torch.empty(ctx.w_shape, dtype=torch.bfloat16 if weight.dtype == torch.bfloat16 else torch.float32,
-                                 device=x2.device)
+            out = main_grad.view(ctx.w_shape) if main_grad is not None else torch.empty(
+                ctx.w_shape, dtype=torch.bfloat16 if weight.dtype == torch.bfloat16 else torch.float32, device=x2.device)
             if x2.is_cuda:
-                grouped_gemm_wgrad(a.contiguous(), b.contiguous(), offsets, dw, accumulate=main_grad is not None)
+                grouped_gemm_wgrad(_rows_of_16_bytes(a), _rows_of_16_bytes(b), offsets, out, accumulate=main_grad is not None)
             else:
-                bounds, per = offsets.tolist(), dw.view(offsets.numel() - 1, -1, dw.shape[1])
+                bounds, per = offsets.tolist(), out.view(offsets.numel() - 1, -1, out.shape[1])
                 for g, (lo, hi) in enumerate(zip(bounds[:-1], bounds[1:])):
                     _store(per[g], a[lo:hi].float().t() @ b[lo:hi].float(), main_grad is not None)
-            if main_grad is not None:
-                if hasattr(weight, "grad_added_to_main_grad"):
-                    weight.grad_added_to_main_grad = True
-                dw = None
-            else:
-                dw = dw.to(weight.dtype)
+            if main_grad is None:
+                dw = out.to(weight.dtype)
+            elif hasattr(weight, "grad_added_to_main_grad"):
+                weight.grad_added_to_main_grad = True
         return dx, dw, None, None, None
+
+
+def _rows_of_16_bytes(t: torch.Tensor) -> torch.Tensor:
+    """``t`` (bf16), copied where its rows do not start on 16-byte boundaries."""
+    return t if t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
 def fp8_block_grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor, *, trans_b: bool = True,
@@ -515,11 +597,13 @@ def fp8_block_grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: tor
     """
     The experts' linear layer with block-scaled e4m3 operands in the forward product and in the input gradient; the weight
     gradient is taken in bf16, because the 128-row blocks of a column scale would run across the experts' boundaries.
-    ``x [R, K]`` sorted by expert, ``offsets`` int32 ``[G + 1]``, ``weight`` the experts' matrices stacked: ``[G * N, K]`` with
-    ``trans_b`` (``y = x W_g^T``) else ``[G * K, N]`` (``y = x W_g``). Widths must be multiples of 8.
+    ``x [R, K]`` sorted by expert, ``offsets`` int32 ``[G + 1]`` (row boundaries, see :func:`grouped_gemm_fp8_block`), ``weight``
+    the experts' matrices stacked: ``[G * N, K]`` with ``trans_b`` (``y = x W_g^T``) else ``[G * K, N]`` (``y = x W_g``). Widths
+    must be multiples of 8. Rows outside every group are undefined.
     """
     G = offsets.numel() - 1
-    w = compute_weight(weight, torch.bfloat16)
+    w = getattr(weight, "_lowp", None)
+    w = weight if w is None else w  # only its shape is needed here
     if G < 1 or w.dim() != 2 or w.shape[0] % G:
         raise ValueError(f"a weight of shape {tuple(w.shape)} does not stack {G} equal matrices")
     K = w.shape[1] if trans_b else w.shape[0] // G
@@ -527,4 +611,5 @@ def fp8_block_grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: tor
         raise ValueError(f"x of shape {tuple(x.shape)} does not fit experts that take {K} features")
     if w.shape[1] % 8 or (w.shape[0] // G) % 8:
         raise ValueError("the widths of the experts' matrices must be multiples of 8")
+    _check_offsets(offsets, G, x.device)
     return BlockFloat8GroupedLinearFunction.apply(x, weight, offsets, trans_b, weight_cache)

@@ -94,11 +94,10 @@ def _route_kernel(logits, top_k, gating, score_bias, n_groups, top_k_groups, nor
     weights = torch.empty((n, top_k), dtype=torch.float32, device=device)
     experts = torch.empty((n, top_k), dtype=torch.int64, device=device)
     counts = torch.empty(e, dtype=torch.int32, device=device)
-    with torch.cuda.device(device):
-        rc = _lib.lib().ocb_moe_route(
-            logits.data_ptr(), scores.data_ptr(), weights.data_ptr(), experts.data_ptr(), counts.data_ptr(),
-            _lib.ptr(score_bias), n, e, top_k, int(gating == "sigmoid"), normalize, n_groups, top_k_groups,
-            logits.stride(0), _lib.dt(logits), _lib.stream_ptr())
+    rc = _lib.on_device(
+        device, _lib.lib().ocb_moe_route, logits.data_ptr(), scores.data_ptr(), weights.data_ptr(), experts.data_ptr(),
+        counts.data_ptr(), _lib.ptr(score_bias), n, e, top_k, int(gating == "sigmoid"), normalize, n_groups, top_k_groups,
+        logits.stride(0), _lib.dt(logits))
     _lib.check(rc, "ocb_moe_route")
     return weights, experts, scores, counts
 
@@ -127,11 +126,10 @@ class _Route(torch.autograd.Function):
         d_weights = None if d_weights is None else d_weights.float().contiguous()
         d_scores = None if d_scores is None else d_scores.float().contiguous()
         d_logits = torch.empty((n, e), dtype=ctx.logits_dtype, device=kept.device)
-        with torch.cuda.device(kept.device):
-            rc = _lib.lib().ocb_moe_route_grad(
-                None if ctx.sigmoid else kept.data_ptr(), kept.data_ptr() if ctx.sigmoid else None, experts.data_ptr(),
-                _lib.ptr(d_weights), _lib.ptr(d_scores), d_logits.data_ptr(), n, e, experts.shape[1], int(ctx.sigmoid),
-                ctx.normalize, kept.stride(0), _lib.dt(d_logits), _lib.stream_ptr())
+        rc = _lib.on_device(
+            kept.device, _lib.lib().ocb_moe_route_grad, None if ctx.sigmoid else kept.data_ptr(),
+            kept.data_ptr() if ctx.sigmoid else None, experts.data_ptr(), _lib.ptr(d_weights), _lib.ptr(d_scores),
+            d_logits.data_ptr(), n, e, experts.shape[1], int(ctx.sigmoid), ctx.normalize, kept.stride(0), _lib.dt(d_logits))
         _lib.check(rc, "ocb_moe_route_grad")
         return (d_logits,) + (None,) * 6
 
