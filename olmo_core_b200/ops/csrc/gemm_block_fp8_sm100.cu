@@ -19,6 +19,8 @@
 // fetch those of four blocks at a time, run up to twelve blocks ahead, and lay the exponents out as the tensor core wants them), warps 4..11 = epilogue (four lane quadrants x two column halves; through shared memory, so that global accesses are
 // whole 128-byte lines). All waits are bounded (common.cuh).
 
+#include <atomic>
+
 #include "common.cuh"
 #include "ocb_api.h"
 #include "tmap.h"
@@ -944,18 +946,37 @@ gemm_block_fp8_small_kernel(const __grid_constant__ CUtensorMap tma_a, const __g
   if (p.parts > 1) cluster_sync_all();  // the other CTAs have read this one's part
 }
 
-static int num_sms() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+// Properties of a device and settings of a kernel on it are looked up once per device.
+static int current_device() {
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess ? dev : -1;
+}
+static int num_sms(int dev) {
+  static std::atomic<int> known[64];
+  if (dev < 0) return 0;
+  int n = dev < 64 ? known[dev].load(std::memory_order_relaxed) : 0;
+  if (n == 0) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+    if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
+  }
   return n;
+}
+template <class Kernel>
+static bool allow_smem(Kernel kernel, int bytes, std::atomic<uint64_t>& done, int dev) {
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0ull;
+  if ((done.load(std::memory_order_relaxed) & bit) != 0) return true;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return true;
 }
 
 template <int BN, int CTAS, int EPI>
-static int launch(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, long long max_tiles, cudaStream_t stream) {
+static int launch(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, long long max_tiles, int dev, cudaStream_t stream) {
   constexpr int bytes = Tile<BN, CTAS>::SMEM_BYTES;
   auto kernel = gemm_block_fp8_kernel<BN, CTAS, EPI>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return -3;
-  const int units = num_sms() / CTAS;
+  static std::atomic<uint64_t> done;
+  if (!allow_smem(kernel, bytes, done, dev)) return -3;
+  const int units = num_sms(dev) / CTAS;
   if (units <= 0) return -3;
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(static_cast<unsigned>(max_tiles < units ? max_tiles : units) * CTAS);
@@ -972,11 +993,11 @@ static int launch(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p,
 }
 
 template <int BN, int CTAS>
-static int launch_epi(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, long long max_tiles, int epi, cudaStream_t s) {
+static int launch_epi(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, long long max_tiles, int epi, int dev, cudaStream_t s) {
   switch (epi) {
-    case EPI_BF16: return launch<BN, CTAS, EPI_BF16>(ta, tb, p, max_tiles, s);
-    case EPI_F32_ACC: return launch<BN, CTAS, EPI_F32_ACC>(ta, tb, p, max_tiles, s);
-    case EPI_F32: return launch<BN, CTAS, EPI_F32>(ta, tb, p, max_tiles, s);
+    case EPI_BF16: return launch<BN, CTAS, EPI_BF16>(ta, tb, p, max_tiles, dev, s);
+    case EPI_F32_ACC: return launch<BN, CTAS, EPI_F32_ACC>(ta, tb, p, max_tiles, dev, s);
+    case EPI_F32: return launch<BN, CTAS, EPI_F32>(ta, tb, p, max_tiles, dev, s);
     default: return -1;
   }
 }
@@ -998,10 +1019,11 @@ namespace ocb {
 namespace blk {
 
 template <int BN, bool SWAP>
-static int launch_small(const CUtensorMap& ta, const CUtensorMap& tb, const SmallParams& p, long long tiles, cudaStream_t stream) {
+static int launch_small(const CUtensorMap& ta, const CUtensorMap& tb, const SmallParams& p, long long tiles, int dev, cudaStream_t stream) {
   constexpr int bytes = SmallTile<BN>::SMEM_BYTES;
   auto kernel = gemm_block_fp8_small_kernel<BN, SWAP>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return -3;
+  static std::atomic<uint64_t> done;
+  if (!allow_smem(kernel, bytes, done, dev)) return -3;
   if (tiles * p.parts > 0x7fffffffll) return -1;
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(static_cast<unsigned>(tiles * p.parts));
@@ -1028,7 +1050,7 @@ struct Product {
   int* status;
 };
 
-static int run_pair(const Product& x, cudaStream_t stream) {
+static int run_pair(const Product& x, int dev, cudaStream_t stream) {
   Params p;
   p.C = x.C;
   p.ldc = x.ldc;
@@ -1049,11 +1071,11 @@ static int run_pair(const Product& x, cudaStream_t stream) {
   if (!make_map(&ta, x.A, x.a_mn != 0, x.M, x.K, 1, x.lda, 0, BM, 2)) return -1001;
   if (!make_map(&tb, x.B, x.b_mn != 0, x.N, x.K, x.groups, x.ldb, x.groups > 1 ? x.b_group_bytes : x.ldb, BN / CTAS, 3)) return -2001;
   const long long tiles_m = (x.M + BM * CTAS - 1) / (BM * CTAS) + (x.offsets != nullptr ? x.groups : 0);
-  return launch_epi<BN, CTAS>(ta, tb, p, tiles_m * ((x.N + BN - 1) / BN), x.epi, stream);
+  return launch_epi<BN, CTAS>(ta, tb, p, tiles_m * ((x.N + BN - 1) / BN), x.epi, dev, stream);
 }
 
 // swap: the rows of B take the 128-row side and the rows of A the side of bn.
-static int run_small(const Product& x, bool swap, int bn, int parts, cudaStream_t stream) {
+static int run_small(const Product& x, bool swap, int bn, int parts, int dev, cudaStream_t stream) {
   SmallParams p;
   p.C = x.C;
   p.ldc = x.ldc;
@@ -1083,19 +1105,19 @@ static int run_small(const Product& x, bool swap, int bn, int parts, cudaStream_
   const long long tiles = b_tiles * ((p.M + BM - 1) / BM);
   if (swap) {
     switch (bn) {
-      case 16: return launch_small<16, true>(ta, tb, p, tiles, stream);
-      case 32: return launch_small<32, true>(ta, tb, p, tiles, stream);
-      case 64: return launch_small<64, true>(ta, tb, p, tiles, stream);
-      default: return launch_small<128, true>(ta, tb, p, tiles, stream);
+      case 16: return launch_small<16, true>(ta, tb, p, tiles, dev, stream);
+      case 32: return launch_small<32, true>(ta, tb, p, tiles, dev, stream);
+      case 64: return launch_small<64, true>(ta, tb, p, tiles, dev, stream);
+      default: return launch_small<128, true>(ta, tb, p, tiles, dev, stream);
     }
   }
-  return launch_small<128, false>(ta, tb, p, tiles, stream);
+  return launch_small<128, false>(ta, tb, p, tiles, dev, stream);
 }
 
 // Which kernel. The pair kernel moves the fewest bytes per operation but works in 256 x 256 tiles on 74 pairs; with few tiles
 // the 128-row kernel fills the SMs, if need be by splitting the reduction.
 static int run(const Product& x, cudaStream_t stream) {
-  const int sms = num_sms();
+  const int dev = current_device(), sms = num_sms(dev);
   if (sms <= 0) return -3;
   const long long kb = (x.K + BKE - 1) / BKE;
   const long long tiles_n = (x.N + 127) / 128;
@@ -1106,19 +1128,19 @@ static int run(const Product& x, cudaStream_t stream) {
   };
   if (x.offsets != nullptr) {
     const long long mean = x.M / x.groups;  // rows of a group
-    if (mean > 128) return run_pair(x, stream);
+    if (mean > 128) return run_pair(x, dev, stream);
     const int bn = mean <= 8 ? 16 : mean <= 16 ? 32 : mean <= 48 ? 64 : 128;
     const long long used = x.groups < x.M ? x.groups : x.M;
-    return run_small(x, true, bn, split(used * tiles_n), stream);
+    return run_small(x, true, bn, split(used * tiles_n), dev, stream);
   }
   if (x.M <= 128 && !x.a_mn) {
     const int bn = x.M <= 16 ? 16 : x.M <= 32 ? 32 : x.M <= 64 ? 64 : 128;
-    return run_small(x, true, bn, split(tiles_n), stream);
+    return run_small(x, true, bn, split(tiles_n), dev, stream);
   }
   const long long pair_tiles = static_cast<long long>((x.M + 255) / 256) * ((x.N + 255) / 256);
   const long long small_tiles = static_cast<long long>((x.M + 127) / 128) * tiles_n;
-  if (pair_tiles * 2 >= sms) return run_pair(x, stream);
-  return run_small(x, false, 128, split(small_tiles), stream);
+  if (pair_tiles * 2 >= sms) return run_pair(x, dev, stream);
+  return run_small(x, false, 128, split(small_tiles), dev, stream);
 }
 
 }  // namespace blk

@@ -26,7 +26,7 @@ On CPU the functions emulate the same arithmetic in PyTorch: the numerical oracl
 
 from __future__ import annotations
 
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -373,30 +373,68 @@ def _check_offsets(offsets: torch.Tensor, groups: int, device: torch.device) -> 
 # ------------------------------------------------------------------------------------------------------
 
 
-def _quantized_product(x: torch.Tensor, w_q: torch.Tensor, w_s: torch.Tensor, trans_b: bool,
-                       offsets: Optional[torch.Tensor] = None, keep_columns: bool = False):
+def _tile_buffer(w: torch.Tensor) -> torch.Tensor:
+    """:func:`quantize_block_tiles` of ``w [N, K]`` on a GPU as one buffer: codes ``[N, K rounded up to 16]``, then scales."""
+    N, K = w.shape
+    pitch = (K + 15) & -16
+    buffer = torch.empty(N * pitch + 4 * _blocks(N) * _blocks(K), dtype=torch.uint8, device=w.device)
+    if N and K:
+        at = buffer.data_ptr()
+        rc = _lib.on_device(w.device, _lib_block().ocb_quantize_block_fp8, w.data_ptr(), None, None, None, None, at,
+                            at + N * pitch, 1, N, K, w.stride(0), pitch, 0, 0)
+        _lib.check(rc, "ocb_quantize_block_fp8")
+    return buffer
+
+
+class _Weight(NamedTuple):
+    """Where the tile-quantised matrices of a product are: ``groups`` of ``rows x cols``, as a kernel takes them."""
+
+    codes: int
+    scales: int
+    rows: int
+    cols: int
+    pitch: int
+    group_bytes: int
+    scale_strides: Tuple[int, int, int]  # between groups, rows, columns of tiles
+    groups: int
+
+    @classmethod
+    def of(cls, q: torch.Tensor, s: torch.Tensor) -> "_Weight":
+        grouped = q.dim() == 3
+        groups = q.shape[0] if grouped else 1
+        pitch = _pitch(q)
+        return cls(q.data_ptr(), s.data_ptr(), q.shape[-2], q.shape[-1], pitch,
+                   q.stride(0) if groups > 1 else q.shape[-2] * pitch, s.stride() if grouped else (0, *s.stride()), groups)
+
+    @classmethod
+    def of_buffer(cls, buffer: torch.Tensor, rows: int, cols: int) -> "_Weight":
+        pitch, at = (cols + 15) & -16, buffer.data_ptr()
+        return cls(at, at + rows * pitch, rows, cols, pitch, 0, (0, _blocks(cols), 1), 1)
+
+
+def _quantized_product(x: torch.Tensor, w: _Weight, trans_b: bool, offsets: Optional[torch.Tensor] = None,
+                       keep_columns: bool = False):
     """
     ``q_rows(x) @ op(W)`` (bf16) for checked operands on a GPU, quantiser and product in one call. With ``keep_columns`` also
-    the column-scaled form of ``x``, as ``(buffer of codes and scales,)``.
+    the column-scaled form of ``x`` (see :func:`_column_buffer`).
     """
     M, K = x.shape
-    N = w_q.shape[-2] if trans_b else w_q.shape[-1]
-    out = torch.empty((M, N), dtype=torch.bfloat16, device=x.device)
+    device = x.device
+    N = w.rows if trans_b else w.cols
+    out = torch.empty((M, N), dtype=torch.bfloat16, device=device)
+    columns = _column_buffer(M, K, device) if keep_columns else None
     if M == 0 or N == 0 or K == 0:
-        return (out.zero_() if M and N else out), (_column_buffer(M, K, x.device) if keep_columns else None)
+        return (out.zero_() if M and N else out), columns
     pitch = (K + 15) & -16
     codes = M * pitch
-    rows = torch.empty(codes + 4 * _blocks(K) * M, dtype=torch.uint8, device=x.device)
-    columns = _column_buffer(M, K, x.device) if keep_columns else None
-    sw_k, sw_i = (w_s.stride(-1), w_s.stride(-2)) if trans_b else (w_s.stride(-2), w_s.stride(-1))
-    grouped = w_q.dim() == 3
-    groups = w_q.shape[0] if grouped else 1
+    rows = torch.empty(codes + 4 * _blocks(K) * M, dtype=torch.uint8, device=device)
+    sw_g, sw_n, sw_c = w.scale_strides
     at, at_c = rows.data_ptr(), None if columns is None else columns.data_ptr()
     rc = _lib.on_device(
-        x.device, _lib_block().ocb_linear_block_fp8, x.data_ptr(), x.stride(0), at, at + codes, at_c,
-        None if at_c is None else at_c + codes, pitch, w_q.data_ptr(), w_s.data_ptr(), _lib.ptr(offsets), groups,
-        out.data_ptr(), M, N, K, _pitch(w_q), w_q.stride(0) if groups > 1 else w_q.shape[-2] * _pitch(w_q), sw_k, sw_i,
-        w_s.stride(0) if grouped else 0, int(not trans_b), N, _lib.EPI_BF16, _lib.status_buffer(x.device).data_ptr())
+        device, _lib_block().ocb_linear_block_fp8, x.data_ptr(), x.stride(0), at, at + codes, at_c,
+        None if at_c is None else at_c + codes, pitch, w.codes, w.scales, None if offsets is None else offsets.data_ptr(),
+        w.groups, out.data_ptr(), M, N, K, w.pitch, w.group_bytes, sw_c if trans_b else sw_n, sw_n if trans_b else sw_c, sw_g,
+        int(not trans_b), N, _lib.EPI_BF16, _lib.status_buffer(device).data_ptr())
     _lib.check(rc, "ocb_linear_block_fp8")
     return out, columns
 
@@ -438,7 +476,7 @@ def fp8_block_matmul(x: torch.Tensor, w_q: torch.Tensor, w_s: torch.Tensor, bias
     with torch.no_grad():
         x2 = _check_matrix(x if x.dim() == 2 else x.reshape(-1, K), "x")
         if x2.is_cuda:
-            y, _ = _quantized_product(x2, w_q, w_s, True)
+            y, _ = _quantized_product(x2, _Weight.of(w_q, w_s), True)
         else:
             y = gemm_fp8_block(*quantize_block_rows(x2), w_q, w_s)
         y = y if x.dim() == 2 else y.view(*x.shape[:-1], N)
@@ -463,7 +501,7 @@ def fp8_block_grouped_matmul(x: torch.Tensor, w_q: torch.Tensor, w_s: torch.Tens
     with torch.no_grad():
         x2 = _check_matrix(x, "x")
         if x2.is_cuda and G:
-            return _quantized_product(x2, w_q, w_s, trans_b, offsets)[0]
+            return _quantized_product(x2, _Weight.of(w_q, w_s), trans_b, offsets)[0]
         return grouped_gemm_fp8_block(*quantize_block_rows(x2), w_q, w_s, offsets, trans_b=trans_b)
 
 
@@ -472,26 +510,30 @@ class BlockFloat8LinearFunction(torch.autograd.Function):
     def forward(ctx, x, weight, wgrad_high_precision: bool, cache: Optional[dict] = None):  # type: ignore[override]
         w = compute_weight(weight, torch.bfloat16)
         x2 = _check_matrix(x if x.dim() == 2 else x.reshape(-1, x.shape[-1]), "x")
-        wq, sw = cached_weight_cast(cache, "block_tiles", lambda: quantize_block_tiles(w), weight._version)
         needs_dw = ctx.needs_input_grad[1] or getattr(weight, "main_grad", None) is not None
         in_fp8 = needs_dw and not wgrad_high_precision
         # what the backward pass keeps of x is its column-scaled form: one byte per element
         if x2.is_cuda:
-            y, columns = _quantized_product(x2, wq, sw, True, keep_columns=in_fp8)
+            w = _check_matrix(w, "weight")
+            wq = (cached_weight_cast(cache, "block_tiles", lambda: _tile_buffer(w), weight._version),)
+            y, columns = _quantized_product(x2, _Weight.of_buffer(wq[0], *w.shape), True, keep_columns=in_fp8)
             kept = (columns,) if in_fp8 else (x2,) if needs_dw else ()
         else:
-            y = gemm_fp8_block(*quantize_block_rows(x2), wq, sw)
+            wq = cached_weight_cast(cache, "block_tiles", lambda: quantize_block_tiles(w), weight._version)
+            y = gemm_fp8_block(*quantize_block_rows(x2), *wq)
             kept = quantize_block_columns(x2) if in_fp8 else (x2,) if needs_dw else ()
-        ctx.save_for_backward(wq, sw, *kept)
+        ctx.save_for_backward(*wq, *kept)
+        ctx.n_weight, ctx.w_shape = len(wq), w.shape
         ctx.in_fp8, ctx.x2_shape = in_fp8, x2.shape
         ctx.weight_ref, ctx.x_shape, ctx.x_dtype = weight, x.shape, x.dtype
         return y if x.dim() == 2 else y.view(*x.shape[:-1], w.shape[0])
 
     @staticmethod
     def backward(ctx, dy):  # type: ignore[override]
-        wq, sw, *kept = ctx.saved_tensors
+        saved = ctx.saved_tensors
+        wq, kept = saved[: ctx.n_weight], saved[ctx.n_weight:]
         weight = ctx.weight_ref
-        (M, K), N = ctx.x2_shape, wq.shape[0]
+        (M, K), N = ctx.x2_shape, ctx.w_shape[0]
         dy2 = _check_matrix(dy if dy.dim() == 2 else dy.reshape(-1, N), "dy")
         main_grad = getattr(weight, "main_grad", None)
         needs_dx = ctx.needs_input_grad[0]
@@ -500,9 +542,9 @@ class BlockFloat8LinearFunction(torch.autograd.Function):
         dx = dw = columns = None
         if needs_dx:
             if dy2.is_cuda:
-                dx, columns = _quantized_product(dy2, wq, sw, False, keep_columns=in_fp8)
+                dx, columns = _quantized_product(dy2, _Weight.of_buffer(wq[0], *ctx.w_shape), False, keep_columns=in_fp8)
             else:
-                dx = gemm_fp8_block(*quantize_block_rows(dy2), wq, sw, trans_b=False)
+                dx = gemm_fp8_block(*quantize_block_rows(dy2), *wq, trans_b=False)
             dx = dx if len(ctx.x_shape) == 2 else dx.view(ctx.x_shape)
             dx = dx if dx.dtype == ctx.x_dtype else dx.to(ctx.x_dtype)
         if needs_dw:
@@ -550,7 +592,7 @@ class BlockFloat8GroupedLinearFunction(torch.autograd.Function):
         x2 = _check_matrix(x, "x")
         wq, sw = cached_weight_cast(cache, "block_tiles", lambda: quantize_block_tiles(w.view(G, -1, w.shape[-1])), weight._version)
         if x2.is_cuda:
-            y, _ = _quantized_product(x2, wq, sw, trans_b, offsets)
+            y, _ = _quantized_product(x2, _Weight.of(wq, sw), trans_b, offsets)
         else:
             y = grouped_gemm_fp8_block(*quantize_block_rows(x2), wq, sw, offsets, trans_b=trans_b)
         ctx.save_for_backward(wq, sw, offsets, x2)
@@ -565,7 +607,7 @@ class BlockFloat8GroupedLinearFunction(torch.autograd.Function):
         dx = dw = None
         if ctx.needs_input_grad[0]:
             if dy2.is_cuda:
-                dx, _ = _quantized_product(dy2, wq, sw, not trans_b, offsets)
+                dx, _ = _quantized_product(dy2, _Weight.of(wq, sw), not trans_b, offsets)
             else:
                 dx = grouped_gemm_fp8_block(*quantize_block_rows(dy2), wq, sw, offsets, trans_b=not trans_b)
             dx = dx if dx.dtype == ctx.x_dtype else dx.to(ctx.x_dtype)

@@ -115,7 +115,6 @@ class _Route(torch.autograd.Function):
         return weights, experts, scores, counts
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, d_weights, _experts, d_scores, _counts):  # type: ignore[override]
         from . import _lib
 
