@@ -27,8 +27,11 @@ namespace route {
 
 constexpr unsigned FULL = 0xffffffffu;
 constexpr float SIGMOID_FLOOR = 1e-7f;
-// Error bound of an fp32 score (all are <= 1): the fast exponential, the reciprocal and a sum of up to 1024 terms.
-constexpr float SCORE_ERROR = 3.8e-6f;  // 2^-18
+// Error bounds of an fp32 score (all are <= 1). Softmax: a sum of up to 1024 terms (37 roundings on the longest path), the fast
+// exponential and the reciprocal. Sigmoid: s (1 - s) times the exponential's relative error of (2 + 1.2 |x|) 2^-23, and three
+// roundings.
+constexpr float SOFTMAX_ERROR = 3.8e-6f;  // 2^-18
+constexpr float SIGMOID_ERROR = 4.8e-7f;  // 2^-21
 
 struct Params {
   const void* logits;
@@ -83,7 +86,7 @@ __device__ __forceinline__ bool too_close(float hi, float lo, float error) {
 // The k largest keys in falling order, lower expert first among equal ones: lane j gets the j-th. With `check`, also says
 // whether neighbours in that order (the first one left out included) are too close to be told apart.
 template <int PL, class Key>
-__device__ __forceinline__ bool pick(Key (&key)[PL], int top_k, int lane, bool check, int& mine) {
+__device__ __forceinline__ bool pick(Key (&key)[PL], int top_k, int lane, bool check, float error, int& mine) {
   bool close = false;
   float before = 0.f;
   const int rounds = top_k + (check ? 1 : 0);
@@ -98,7 +101,7 @@ __device__ __forceinline__ bool pick(Key (&key)[PL], int top_k, int lane, bool c
     const uint32_t e = __reduce_min_sync(FULL, best == top ? static_cast<uint32_t>(at * 32 + lane) : 0xffffffffu);
     if (check) {
       const float v = value_of(static_cast<uint32_t>(top));
-      if (j > 0) close |= too_close(before, v, SCORE_ERROR);
+      if (j > 0) close |= too_close(before, v, error);
       before = v;
     }
     if (j < top_k && lane == j) mine = static_cast<int>(e);
@@ -111,7 +114,7 @@ __device__ __forceinline__ bool pick(Key (&key)[PL], int top_k, int lane, bool c
 // Bit (first lane of a group) of the open groups. row: the ranked values of the token in shared memory. `close` as in pick().
 template <class Real>
 __device__ __forceinline__ uint32_t open_groups(const Real* row, const Params& p, int lane, int lanes_per_group, bool check,
-                                                bool& close) {
+                                                float error, bool& close) {
   const int size = p.n_experts / p.n_groups;
   const int g = lane / lanes_per_group, sub = lane % lanes_per_group;
   const bool valid = g < p.n_groups;
@@ -144,7 +147,7 @@ __device__ __forceinline__ uint32_t open_groups(const Real* row, const Params& p
     const uint32_t k32 = key_of(static_cast<float>(value));
     const uint32_t least_open = __reduce_min_sync(FULL, open ? k32 : 0xffffffffu);
     const uint32_t best_shut = __reduce_max_sync(FULL, valid && !open ? k32 : 0u);
-    close |= too_close(value_of(least_open), value_of(best_shut), 2.f * SCORE_ERROR);
+    close |= too_close(value_of(least_open), value_of(best_shut), 2.f * error);
   }
   return __ballot_sync(FULL, open && sub == 0);
 }
@@ -166,15 +169,31 @@ __global__ void route_kernel(const Params p, int lanes_per_group, int alone) {
   }
   const bool by_logits = p.bias == nullptr;  // the ranking of the logits is the ranking of the scores
 
-  for (long long t = static_cast<long long>(blockIdx.x) * warps + warp; t < p.n_tokens; t += static_cast<long long>(gridDim.x) * warps) {
+  const float error = p.sigmoid ? SIGMOID_ERROR : SOFTMAX_ERROR;
+  float bias[PL];
+#pragma unroll
+  for (int i = 0; i < PL; ++i) bias[i] = p.bias != nullptr && i * 32 + lane < p.n_experts ? p.bias[i * 32 + lane] : 0.f;
+
+  const long long stride = static_cast<long long>(gridDim.x) * warps;
+  float next[PL];  // the next token's logits are on their way while this one is ranked
+  auto fetch = [&](long long t) {
+#pragma unroll
+    for (int i = 0; i < PL; ++i) {
+      const int e = i * 32 + lane;
+      next[i] = t < p.n_tokens && e < p.n_experts ? load(p.logits, t * p.ld + e, p.bf16) : -INFINITY;
+    }
+  };
+  long long t = static_cast<long long>(blockIdx.x) * warps + warp;
+  fetch(t);
+  for (; t < p.n_tokens; t += stride) {
     float x[PL], s[PL];
     float top = -INFINITY;
 #pragma unroll
     for (int i = 0; i < PL; ++i) {
-      const int e = i * 32 + lane;
-      x[i] = e < p.n_experts ? load(p.logits, t * p.ld + e, p.bf16) : -INFINITY;
+      x[i] = next[i];
       top = fmaxf(top, x[i]);
     }
+    fetch(t + stride);
     if (p.sigmoid) {
 #pragma unroll
       for (int i = 0; i < PL; ++i) s[i] = 1.f / (1.f + __expf(-x[i])) + SIGMOID_FLOOR;
@@ -211,8 +230,7 @@ __global__ void route_kernel(const Params p, int lanes_per_group, int alone) {
       float r[PL];
 #pragma unroll
       for (int i = 0; i < PL; ++i) {
-        const int e = i * 32 + lane;
-        r[i] = p.bias != nullptr && e < p.n_experts ? s[i] + p.bias[e] : s[i];
+        r[i] = s[i] + bias[i];
       }
       if (GROUPS) {
         float* row32 = reinterpret_cast<float*>(row);
@@ -220,7 +238,7 @@ __global__ void route_kernel(const Params p, int lanes_per_group, int alone) {
         for (int i = 0; i < PL; ++i)
           if (i * 32 + lane < p.n_experts) row32[i * 32 + lane] = r[i];
         __syncwarp();
-        open = open_groups(row32, p, lane, lanes_per_group, true, close);
+        open = open_groups(row32, p, lane, lanes_per_group, true, error, close);
         __syncwarp();
       }
 #pragma unroll
@@ -230,7 +248,7 @@ __global__ void route_kernel(const Params p, int lanes_per_group, int alone) {
       }
     }
     int mine = 0;
-    close |= pick(key, p.top_k, lane, !by_logits, mine);
+    close |= pick(key, p.top_k, lane, !by_logits, error, mine);
     if (close) {
       double d[PL];
       if (p.sigmoid) {
@@ -249,8 +267,7 @@ __global__ void route_kernel(const Params p, int lanes_per_group, int alone) {
       }
       if (p.bias != nullptr) {
 #pragma unroll
-        for (int i = 0; i < PL; ++i)
-          if (i * 32 + lane < p.n_experts) d[i] += static_cast<double>(p.bias[i * 32 + lane]);
+        for (int i = 0; i < PL; ++i) d[i] += static_cast<double>(bias[i]);
       }
       if (GROUPS) {
 #pragma unroll
@@ -258,7 +275,7 @@ __global__ void route_kernel(const Params p, int lanes_per_group, int alone) {
           if (i * 32 + lane < p.n_experts) row[i * 32 + lane] = d[i];
         __syncwarp();
         bool unused = false;
-        open = open_groups(row, p, lane, lanes_per_group, false, unused);
+        open = open_groups(row, p, lane, lanes_per_group, false, 0.f, unused);
         __syncwarp();
       }
       unsigned long long key64[PL];
@@ -267,7 +284,7 @@ __global__ void route_kernel(const Params p, int lanes_per_group, int alone) {
         const bool in = i * 32 + lane < p.n_experts && (!GROUPS || (open >> first_lane[i]) & 1u);
         key64[i] = in ? key_of(by_logits ? static_cast<double>(x[i]) : d[i]) : 0ull;
       }
-      pick(key64, p.top_k, lane, false, mine);
+      pick(key64, p.top_k, lane, false, 0.f, mine);
     }
 
     // lane j holds the j-th expert; its score sits in another lane's registers
@@ -410,9 +427,11 @@ extern "C" int ocb_moe_route(const void* logits, float* scores, float* weights, 
   int lanes_per_group = 32;
   while (lanes_per_group * n_groups > 32) lanes_per_group >>= 1;
   const bool groups = n_groups > 1;
-  const int warps = n_experts > 512 ? 4 : 8;
+  // Large CTAs, as many as are resident together: a CTA adds its counts to the global ones once. Few tokens: a token per warp
+  // of smaller CTAs.
+  const int warps = n_experts > 512 ? 4 : n_experts > 256 || n_tokens <= 8 ? 8 : 16;
   const long long wanted = (static_cast<long long>(n_tokens) + warps - 1) / warps;
-  const long long most = static_cast<long long>(sms) * (n_experts > 256 ? 4 : 6);
+  const long long most = static_cast<long long>(sms) * (n_experts > 128 ? 2 : 3);
   const int grid = static_cast<int>(wanted < most ? wanted : most);
   const size_t bytes = (groups ? sizeof(double) * warps * n_experts : 0) + sizeof(int) * n_experts;
   if (grid > 1 && cudaMemsetAsync(counts, 0, sizeof(int) * n_experts, stream) != cudaSuccess) return -4;
