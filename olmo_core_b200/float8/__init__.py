@@ -6,7 +6,9 @@ the in-tree 8-bit linear ops: ``ao`` / ``ao_recipe`` the row-wise scaled e4m3 GE
 per-token activation scale, per-output-channel weight scale, power-of-two rounding optional, fp32 accumulation), and
 ``ao_mx`` the block-scaled MX GEMM (``olmo_core_b200.ops.mx``: one E8M0 scale per 32 reduction elements, applied by
 ``tcgen05.mma.kind::mxf8f6f4.block_scale``). Forward, dgrad and wgrad all run in 8 bits unless the recipe keeps the
-weight gradient in bf16.
+weight gradient in bf16. ``block`` selects the GEMM with one power-of-two scale per block of 128
+(``olmo_core_b200.ops.fp8_block``): weights in 128 x 128 tiles whose codes serve forward and dgrad, activations and
+gradients in blocks of 128 along the reduction, any layer sizes, and the experts of dropless mixtures too.
 """
 
 from __future__ import annotations
@@ -22,7 +24,18 @@ from ..config import Config
 from ..exceptions import OLMoConfigurationError
 from .ao import AOFloat8LinearConfig, AOFloat8LinearRecipe, AOMXLinearConfig
 
-__all__ = ["Float8Config", "AOFloat8LinearConfig", "AOFloat8LinearRecipe", "AOMXLinearConfig", "refresh_float8_scales"]
+__all__ = ["Float8Config", "AOFloat8LinearConfig", "AOFloat8LinearRecipe", "AOMXLinearConfig", "BlockFloat8LinearConfig",
+           "refresh_float8_scales"]
+
+
+@dataclass
+class BlockFloat8LinearConfig(Config):
+    """Options of the linear layers with one power-of-two scale per block of 128 (:mod:`olmo_core_b200.ops.fp8_block`)."""
+
+    wgrad_high_precision: bool = False
+    """Keep the weight gradient of dense layers in bf16 (widths that are multiples of 8). Experts always do."""
+    experts: bool = True
+    """Also run the experts of dropless mixtures in 8 bits (forward and input gradient)."""
 
 
 @dataclass
@@ -30,6 +43,7 @@ class Float8Config(Config):
     ao: Optional[AOFloat8LinearConfig] = None
     ao_recipe: Optional[AOFloat8LinearRecipe] = None
     ao_mx: Optional[AOMXLinearConfig] = None
+    block: Optional[BlockFloat8LinearConfig] = None
     modules_to_ignore: Optional[List[str]] = None
     enabled: bool = True
     cache_weight_casts: bool = False
@@ -37,13 +51,13 @@ class Float8Config(Config):
     implied by ``ao.enable_fsdp_float8_all_gather``."""
 
     def __post_init__(self):
-        if sum(x is not None for x in (self.ao, self.ao_recipe, self.ao_mx)) > 1:
-            raise OLMoConfigurationError("specify at most one of 'ao', 'ao_recipe' and 'ao_mx'")
+        if sum(x is not None for x in (self.ao, self.ao_recipe, self.ao_mx, self.block)) > 1:
+            raise OLMoConfigurationError("specify at most one of 'ao', 'ao_recipe', 'ao_mx' and 'block'")
 
     @property
     def should_precompute_float8_dynamic_scale_for_fsdp(self) -> bool:
         """Whether quantised weights are prepared once per optimizer step (src/olmo_core/float8/__init__.py:54-62)."""
-        if self.ao_recipe is not None or self.ao_mx is not None:
+        if self.ao_recipe is not None or self.ao_mx is not None or self.block is not None:
             return False
         return bool(self.ao is not None and self.ao.enable_fsdp_float8_all_gather)
 
@@ -58,17 +72,25 @@ class Float8Config(Config):
         return AOFloat8LinearRecipe.tensorwise if self.ao is not None else AOFloat8LinearRecipe.rowwise
 
     def apply_float8_linear(self, model: nn.Module, modules_to_ignore: Optional[List[str]] = None) -> None:
-        """Mark every eligible projection (all dims multiples of 16, not the LM head) to run in fp8."""
+        """Mark every eligible projection (all dims multiples of 16, any with ``block``; not the LM head) to run in fp8."""
         if not self.enabled:
             return
         from ..nn.feed_forward import Linear
+        from ..nn.moe.mlp import DroplessMoEMLP
 
         ignore = set(self.modules_to_ignore or []) | set(modules_to_ignore or []) | {"lm_head.w_out"}
         pow2 = bool(self.ao is not None and self.ao.round_scales_to_power_of_2)
         for name, module in model.named_modules():
-            if not isinstance(module, Linear):
+            is_experts = self.block is not None and self.block.experts and isinstance(module, DroplessMoEMLP)
+            if not isinstance(module, Linear) and not is_experts:
                 continue
             if any(name == pat or fnmatch(name, pat) for pat in ignore):
+                continue
+            if self.block is not None:
+                sizes = (module.d_model, module.hidden_size) if is_experts else (module.in_features, module.out_features)
+                if (is_experts or self.block.wgrad_high_precision) and any(n % 8 != 0 for n in sizes):
+                    continue
+                module.float8 = dict(block=self.block, weight_cache={} if self.cache_weight_casts else None)  # type: ignore[attr-defined]
                 continue
             if module.in_features % 16 != 0 or module.out_features % 16 != 0:
                 continue

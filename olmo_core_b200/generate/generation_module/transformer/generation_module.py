@@ -13,6 +13,7 @@ import json
 import logging
 import tempfile
 import time
+from dataclasses import replace
 from pathlib import Path
 from typing import Any, Dict, List, Optional, Tuple
 
@@ -44,7 +45,7 @@ class TransformerGenerationModule(GenerationModule):
                  float8_config=None, dp_config=None, device: Optional[torch.device] = None,
                  state_dict_load_opts: Optional[Dict[str, Any]] = None, state_dict_save_opts: Optional[Dict[str, Any]] = None,
                  load_key_mapping: Optional[Dict[str, str]] = None):
-        del compile_model, float8_config, dp_config  # generation runs every rank on its own replica
+        del compile_model, dp_config  # generation runs every rank on its own replica
         self.device = device or get_default_device()
         self.model = model
         if any(p.device.type == "meta" for p in model.parameters()):
@@ -52,6 +53,9 @@ class TransformerGenerationModule(GenerationModule):
         else:
             self.model.to(self.device)
         self.model.eval()
+        if float8_config is not None and float8_config.block is not None:
+            # linear layers with weights in 8-bit tiles, quantised at their first use (the other recipes are for training)
+            self.model.apply_fp8(replace(float8_config, cache_weight_casts=True))
         self._generation_config = generation_config
         self.state_dict_load_opts = state_dict_load_opts or {}
         self.state_dict_save_opts = state_dict_save_opts or {}

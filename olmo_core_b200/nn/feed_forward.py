@@ -104,6 +104,11 @@ class _Proj(nn.Module):
 
             return mx_linear(x, self.weight, self.bias, scale_rounding=str(getattr(f8["mx"], "scale_rounding", "rceil")),
                              weight_cache=f8.get("weight_cache"))
+        if f8 is not None and f8.get("block") is not None:
+            from ..ops.fp8_block import fp8_block_linear
+
+            return fp8_block_linear(x, self.weight, self.bias, wgrad_high_precision=f8["block"].wgrad_high_precision,
+                                    weight_cache=f8.get("weight_cache"))
         if f8 is not None and x.is_cuda and x.numel() // x.shape[-1] % 16 == 0:
             from ..ops.fp8 import fp8_linear
 

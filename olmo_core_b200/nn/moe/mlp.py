@@ -157,12 +157,19 @@ class DroplessMoEMLP(MoEMLPBase):
     def extra_repr(self) -> str:
         return f"num_experts={self.num_experts}, in_features={self.d_model}, hidden_size={self.hidden_size}"
 
-    def gmm(self, x: torch.Tensor, w: torch.Tensor, batch_sizes, trans_b: bool = False) -> torch.Tensor:
+    def gmm(self, x: torch.Tensor, w: torch.Tensor, batch_sizes, trans_b: bool = False, name: str = "") -> torch.Tensor:
         """
         Grouped matmul over expert-sorted rows. ``w``: ``[E_local * hidden, d_model]``. ``batch_sizes``: rows per expert,
-        a list or a tensor; on the kernel path a device tensor is consumed as is (no host synchronisation).
+        a list or a tensor; on the kernel path a device tensor is consumed as is (no host synchronisation). ``name`` tells
+        the weights apart whose 8-bit copies are kept (``Float8Config.cache_weight_casts``).
         """
         E = self.num_local_experts
+        f8 = getattr(self, "float8", None)  # set by Float8Config.apply_float8_linear
+        if f8 is not None and x.is_cuda and x.dtype == torch.bfloat16:
+            from ...ops.fp8_block import fp8_block_grouped_linear
+
+            cache = f8["weight_cache"].setdefault(name, {}) if f8["weight_cache"] is not None and name else None
+            return fp8_block_grouped_linear(x, w, self._offsets(batch_sizes, x.device), trans_b=trans_b, weight_cache=cache)
         if x.is_cuda and x.dtype == torch.bfloat16:
             return _GroupedLinear.apply(x, w, self._offsets(batch_sizes, x.device), trans_b)
         if torch.is_tensor(batch_sizes):
@@ -196,6 +203,6 @@ class DroplessMoEMLP(MoEMLPBase):
         if x.is_cuda and x.dtype == torch.bfloat16:
             sizes = self._offsets(batch_size_per_expert, x.device)  # computed once, shared by the three products
         w1, w2, w3 = (get_local_tensor(w) for w in (self.w1, self.w2, self.w3))
-        a = self.gmm(x, w1, sizes, trans_b=True)
-        b = self.gmm(x, w3, sizes, trans_b=True)
-        return self.gmm(swiglu(a, b), w2, sizes, trans_b=False)
+        a = self.gmm(x, w1, sizes, trans_b=True, name="w1")
+        b = self.gmm(x, w3, sizes, trans_b=True, name="w3")
+        return self.gmm(swiglu(a, b), w2, sizes, trans_b=False, name="w2")

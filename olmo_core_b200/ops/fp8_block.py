@@ -505,6 +505,16 @@ def fp8_block_grouped_matmul(x: torch.Tensor, w_q: torch.Tensor, w_s: torch.Tens
         return grouped_gemm_fp8_block(*quantize_block_rows(x2), w_q, w_s, offsets, trans_b=trans_b)
 
 
+def _cached(cache: Optional[dict], make, weight: torch.Tensor):
+    """The 8-bit form of ``weight``, kept in ``cache`` (see :func:`olmo_core_b200.ops.fp8.cached_weight_cast`)."""
+    made = cached_weight_cast(cache, "block_tiles", make, weight._version)
+    first = made if torch.is_tensor(made) else made[0]
+    if cache is not None and first.is_inference() and not torch.is_inference_mode_enabled():
+        cache.clear()  # made under inference mode, cannot be saved for a backward pass
+        made = cached_weight_cast(cache, "block_tiles", make, weight._version)
+    return made
+
+
 class BlockFloat8LinearFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, wgrad_high_precision: bool, cache: Optional[dict] = None):  # type: ignore[override]
@@ -515,11 +525,11 @@ class BlockFloat8LinearFunction(torch.autograd.Function):
         # what the backward pass keeps of x is its column-scaled form: one byte per element
         if x2.is_cuda:
             w = _check_matrix(w, "weight")
-            wq = (cached_weight_cast(cache, "block_tiles", lambda: _tile_buffer(w), weight._version),)
+            wq = (_cached(cache, lambda: _tile_buffer(w), weight),)
             y, columns = _quantized_product(x2, _Weight.of_buffer(wq[0], *w.shape), True, keep_columns=in_fp8)
             kept = (columns,) if in_fp8 else (x2,) if needs_dw else ()
         else:
-            wq = cached_weight_cast(cache, "block_tiles", lambda: quantize_block_tiles(w), weight._version)
+            wq = _cached(cache, lambda: quantize_block_tiles(w), weight)
             y = gemm_fp8_block(*quantize_block_rows(x2), *wq)
             kept = quantize_block_columns(x2) if in_fp8 else (x2,) if needs_dw else ()
         ctx.save_for_backward(*wq, *kept)
@@ -590,7 +600,7 @@ class BlockFloat8GroupedLinearFunction(torch.autograd.Function):
         w = compute_weight(weight, torch.bfloat16)
         G = offsets.numel() - 1
         x2 = _check_matrix(x, "x")
-        wq, sw = cached_weight_cast(cache, "block_tiles", lambda: quantize_block_tiles(w.view(G, -1, w.shape[-1])), weight._version)
+        wq, sw = _cached(cache, lambda: quantize_block_tiles(w.view(G, -1, w.shape[-1])), weight)
         if x2.is_cuda:
             y, _ = _quantized_product(x2, _Weight.of(wq, sw), trans_b, offsets)
         else:
