@@ -58,8 +58,6 @@ _SIGS = {
     "ocb_quantize_e4m3_rowwise": [c_void_p, c_void_p, c_void_p, c_int, c_int, c_longlong, c_longlong, c_int, c_void_p],
     "ocb_quantize_e4m3_colwise_t": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_longlong, c_longlong, c_int,
                                     c_void_p],
-    "ocb_moe_route": [c_void_p] * 6 + [c_int] * 7 + [c_longlong, c_int, c_void_p],
-    "ocb_moe_route_grad": [c_void_p] * 6 + [c_int] * 5 + [c_longlong, c_int, c_void_p],
     "ocb_moe_sort": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p],
     "ocb_moe_gather": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_longlong, c_longlong, c_void_p],
     "ocb_moe_scatter": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_longlong, c_longlong, c_void_p],
@@ -166,6 +164,24 @@ def lib() -> "_Library":
             fn.restype = c_int
         _lib = _Library(handle)
     return _lib
+
+
+_native = None
+
+
+def native():
+    """``torch.ops.ocb_native`` with the kernel library bound: the ops that allocate, launch and differentiate in C++."""
+    global _native
+    if _native is None:
+        from .build import NATIVE_LIB_PATH
+
+        lib()  # raises with instructions where the kernel library is missing
+        if not NATIVE_LIB_PATH.exists():
+            raise KernelError(f"{NATIVE_LIB_PATH} is missing. Build it with `python -m olmo_core_b200.ops.build`.")
+        torch.ops.load_library(str(NATIVE_LIB_PATH))
+        torch.ops.ocb_native.bind_kernels(str(LIB_PATH))
+        _native = torch.ops.ocb_native
+    return _native
 
 
 def register_signature(name: str, argtypes) -> None:

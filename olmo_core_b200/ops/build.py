@@ -112,27 +112,29 @@ NATIVE_LIB_PATH = OPS_DIR.parent / "nn" / "libocb_native.so"
 def build_native(force: bool = False, verbose: bool = True) -> Path:
     """
     Compile the host-side C++ helpers that need PyTorch's headers (``nn/_csrc/*.cpp``: the storage rebinding used by
-    ``OutputDiscardCheckpoint``) into ``nn/libocb_native.so``. They register dispatcher ops (``torch.ops.ocb_native.*``)
-    and are loaded with ``torch.ops.load_library``.
+    ``OutputDiscardCheckpoint``; ``csrc/torch_ops.cpp``: allocation, launches and autograd nodes of the ops with short calls)
+    into ``nn/libocb_native.so``. They register dispatcher ops (``torch.ops.ocb_native.*``) and are loaded with
+    ``torch.ops.load_library``.
     """
     import torch
     from torch.utils.cpp_extension import include_paths, library_paths
 
     BUILD_DIR.mkdir(exist_ok=True)
-    srcs = sorted(NATIVE_SRC_DIR.glob("*.cpp"))
+    srcs = sorted(NATIVE_SRC_DIR.glob("*.cpp")) + sorted(CSRC_DIR.glob("*.cpp"))
     h = hashlib.sha256(torch.__version__.encode())
-    for src in srcs:
+    for src in [*srcs, CSRC_DIR / "ocb_api.h"]:
         h.update(src.read_bytes())
     stamp = BUILD_DIR / "native.hash"
     if not force and NATIVE_LIB_PATH.exists() and stamp.exists() and stamp.read_text() == h.hexdigest():
         return NATIVE_LIB_PATH
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *map(str, srcs), "-o", str(NATIVE_LIB_PATH)]
-    for inc in include_paths():
+    cuda_include = Path(_nvcc()).parent.parent / "include"
+    for inc in [*include_paths(), str(cuda_include)]:
         cmd += ["-isystem", inc]
     for lib_dir in library_paths():
         cmd += [f"-L{lib_dir}", f"-Wl,-rpath,{lib_dir}"]
-    cmd += ["-ltorch", "-ltorch_cpu", "-lc10"]
+    cmd += ["-I", str(CSRC_DIR), "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-ldl"]
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
         raise RuntimeError(f"native helper build failed:\n{proc.stdout}\n{proc.stderr}")

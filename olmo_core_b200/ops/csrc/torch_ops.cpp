@@ -1,0 +1,289 @@
+// Dispatcher ops (torch.ops.ocb_native.*) of the kernels whose whole call is short: routing and the block-scaled linear layer.
+// Their Python form (argument checks, allocation, an autograd function each way) costs several times the kernels' time for a few
+// hundred tokens, so allocation, launches and the autograd node live here. The kernels themselves stay behind the C interface of
+// ocb_api.h; bind_kernels() resolves them in the library that ops/_lib.py loads.
+
+#include <ATen/ATen.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <dlfcn.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/library.h>
+
+#include "ocb_api.h"
+
+namespace {
+
+using at::Tensor;
+using std::optional;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+struct Kernels {
+    decltype(&ocb_moe_route) route = nullptr;
+    decltype(&ocb_moe_route_grad) route_grad = nullptr;
+    decltype(&ocb_quantize_block_fp8) quantize = nullptr;
+    decltype(&ocb_linear_block_fp8) linear = nullptr;
+    decltype(&ocb_gemm_block_fp8) gemm_block = nullptr;
+    decltype(&ocb_gemm_bf16) gemm_bf16 = nullptr;
+} kernels;
+
+template <class F>
+void resolve(void* handle, const char* name, F& fn) {
+    fn = reinterpret_cast<F>(dlsym(handle, name));
+    TORCH_CHECK(fn != nullptr, "the kernel library has no entry point ", name);
+}
+
+void bind_kernels(c10::string_view path) {
+    void* handle = dlopen(std::string(path).c_str(), RTLD_NOW | RTLD_LOCAL);
+    TORCH_CHECK(handle != nullptr, "cannot load the kernel library: ", dlerror());
+    resolve(handle, "ocb_moe_route", kernels.route);
+    resolve(handle, "ocb_moe_route_grad", kernels.route_grad);
+    resolve(handle, "ocb_quantize_block_fp8", kernels.quantize);
+    resolve(handle, "ocb_linear_block_fp8", kernels.linear);
+    resolve(handle, "ocb_gemm_block_fp8", kernels.gemm_block);
+    resolve(handle, "ocb_gemm_bf16", kernels.gemm_bf16);
+}
+
+void check(int rc, const char* what) { TORCH_CHECK(rc == 0, what, " failed with code ", rc); }
+
+int dtype_code(const Tensor& t) { return t.scalar_type() == at::kBFloat16 ? OCB_BF16 : OCB_F32; }
+
+cudaStream_t stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
+
+const float* floats(const optional<Tensor>& t) { return t.has_value() && t->defined() ? t->const_data_ptr<float>() : nullptr; }
+
+// ---- routing -----------------------------------------------------------------------------------------------------------
+
+struct RouteOptions {
+    int top_k, sigmoid, n_groups, top_groups, normalize;
+};
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> run_route(const Tensor& logits, const optional<Tensor>& bias, const RouteOptions& o) {
+    const c10::cuda::OptionalCUDAGuard guard(logits.device());
+    const int64_t n = logits.size(0), e = logits.size(1);
+    const auto opt = logits.options();
+    Tensor weights = at::empty({n, o.top_k}, opt.dtype(at::kFloat)), experts = at::empty({n, o.top_k}, opt.dtype(at::kLong));
+    Tensor scores = at::empty({n, e}, opt.dtype(at::kFloat)), counts = at::empty({e}, opt.dtype(at::kInt));
+    check(kernels.route(logits.const_data_ptr(), scores.mutable_data_ptr<float>(), weights.mutable_data_ptr<float>(),
+                        reinterpret_cast<long long*>(experts.mutable_data_ptr<int64_t>()), counts.mutable_data_ptr<int>(), floats(bias),
+                        static_cast<int>(n), static_cast<int>(e), o.top_k, o.sigmoid, o.normalize, o.n_groups, o.top_groups,
+                        logits.stride(0), dtype_code(logits), stream_of(logits)),
+          "ocb_moe_route");
+    return {weights, experts, scores, counts};
+}
+
+struct Route : torch::autograd::Function<Route> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& logits, const optional<Tensor>& bias, const RouteOptions& o) {
+        auto [weights, experts, scores, counts] = run_route(logits, bias, o);
+        ctx->save_for_backward({o.sigmoid ? logits : scores, experts});
+        ctx->saved_data["sigmoid"] = static_cast<int64_t>(o.sigmoid);
+        ctx->saved_data["normalize"] = static_cast<int64_t>(o.normalize);
+        ctx->saved_data["bf16"] = logits.scalar_type() == at::kBFloat16;
+        ctx->mark_non_differentiable({experts, counts});
+        ctx->set_materialize_grads(false);
+        return {weights, experts, scores, counts};
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const Tensor &d_weights = grads[0], &d_scores = grads[2];
+        if (!d_weights.defined() && !d_scores.defined()) return {Tensor(), Tensor(), Tensor()};
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &kept = saved[0], &experts = saved[1];
+        const c10::cuda::OptionalCUDAGuard guard(kept.device());
+        const int sigmoid = static_cast<int>(ctx->saved_data["sigmoid"].toInt());
+        const Tensor dw = d_weights.defined() ? d_weights.to(at::kFloat).contiguous() : d_weights;
+        const Tensor ds = d_scores.defined() ? d_scores.to(at::kFloat).contiguous() : d_scores;
+        Tensor d_logits = at::empty({kept.size(0), kept.size(1)}, kept.options().dtype(ctx->saved_data["bf16"].toBool() ? at::kBFloat16 : at::kFloat));
+        check(kernels.route_grad(sigmoid ? nullptr : kept.const_data_ptr<float>(), sigmoid ? kept.const_data_ptr() : nullptr,
+                                 reinterpret_cast<const long long*>(experts.const_data_ptr<int64_t>()),
+                                 dw.defined() ? dw.const_data_ptr<float>() : nullptr, ds.defined() ? ds.const_data_ptr<float>() : nullptr,
+                                 d_logits.mutable_data_ptr(), static_cast<int>(kept.size(0)), static_cast<int>(kept.size(1)),
+                                 static_cast<int>(experts.size(1)), sigmoid, static_cast<int>(ctx->saved_data["normalize"].toInt()),
+                                 kept.stride(0), dtype_code(d_logits), stream_of(kept)),
+              "ocb_moe_route_grad");
+        return {d_logits, Tensor(), Tensor()};
+    }
+};
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> route(const Tensor& logits, int64_t top_k, bool sigmoid, const optional<Tensor>& bias,
+                                                 int64_t n_groups, int64_t top_groups, int64_t normalize) {
+    const RouteOptions o{static_cast<int>(top_k), sigmoid, static_cast<int>(n_groups), static_cast<int>(top_groups),
+                         static_cast<int>(normalize)};
+    if (!logits.requires_grad() || !at::GradMode::is_enabled()) return run_route(logits, bias, o);
+    const variable_list out = Route::apply(logits, bias, o);
+    return {out[0], out[1], out[2], out[3]};
+}
+
+// ---- block-scaled linear layer -------------------------------------------------------------------------------------------
+
+int64_t blocks(int64_t n) { return (n + 127) / 128; }
+int64_t pitch_of(int64_t cols) { return (cols + 15) & -16; }
+
+Tensor bytes(int64_t n, const Tensor& like) { return at::empty({n}, like.options().dtype(at::kByte)); }
+
+// A [rows, cols] matrix in bf16 with contiguous rows.
+Tensor matrix(const Tensor& t, int64_t cols) {
+    Tensor m = t.dim() == 2 ? t : t.reshape({cols == 0 ? t.numel() : t.numel() / cols, cols});
+    if (m.scalar_type() != at::kBFloat16) m = m.to(at::kBFloat16);
+    return m.stride(1) == 1 || m.size(1) == 1 ? m : m.contiguous();
+}
+
+// The same where its rows start on 16-byte boundaries, else a copy (rows broadcast from one have stride 0).
+Tensor aligned(const Tensor& m) {
+    const bool fits = m.stride(0) >= m.size(1) && m.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(m.const_data_ptr()) % 16 == 0;
+    return fits ? m : m.clone(at::MemoryFormat::Contiguous);
+}
+
+// Codes [rows, cols rounded up to 16] and behind them the scales of 128 x 128 tiles.
+Tensor tile_buffer(const Tensor& weight) {
+    const c10::cuda::OptionalCUDAGuard guard(weight.device());
+    const Tensor w = matrix(weight, weight.size(1));
+    const int64_t rows = w.size(0), cols = w.size(1), codes = rows * pitch_of(cols);
+    Tensor buffer = bytes(codes + 4 * blocks(rows) * blocks(cols), w);
+    if (rows == 0 || cols == 0) return buffer;
+    uint8_t* at = buffer.mutable_data_ptr<uint8_t>();
+    check(kernels.quantize(w.const_data_ptr(), nullptr, nullptr, nullptr, nullptr, at, reinterpret_cast<float*>(at + codes), 1,
+                           static_cast<int>(rows), static_cast<int>(cols), w.stride(0), pitch_of(cols), 0, 0, stream_of(w)),
+          "ocb_quantize_block_fp8");
+    return buffer;
+}
+
+// Where the tile-quantised matrices [rows, cols] of a product are.
+struct Weight {
+    const void* codes;
+    const float* scales;
+    int64_t rows, cols, pitch, group_bytes;
+    int64_t s_group, s_row, s_col;  // strides of the scales between groups, rows and columns of tiles
+    int64_t groups;
+};
+
+Weight in_buffer(const Tensor& tiles, int64_t rows, int64_t cols) {
+    const uint8_t* at = tiles.const_data_ptr<uint8_t>();
+    return {at, reinterpret_cast<const float*>(at + rows * pitch_of(cols)), rows, cols, pitch_of(cols), 0, 0, blocks(cols), 1, 1};
+}
+
+// x by rows times W (transposed or not); `columns`: also x by columns.
+Tensor product(const Tensor& x, const Weight& w, bool trans, const int* offsets, Tensor* columns, int64_t status) {
+    const int64_t m = x.size(0), k = x.size(1), n = trans ? w.rows : w.cols;
+    Tensor out = at::empty({m, n}, x.options());
+    const int64_t pitch = pitch_of(k), codes = m * pitch;
+    if (columns != nullptr) *columns = bytes(codes + 4 * blocks(m) * k, x);
+    if (m == 0 || n == 0) return out;
+    if (k == 0) return out.zero_();
+    Tensor rows = bytes(codes + 4 * blocks(k) * m, x);
+    uint8_t* at = rows.mutable_data_ptr<uint8_t>();
+    uint8_t* at_c = columns != nullptr ? columns->mutable_data_ptr<uint8_t>() : nullptr;
+    check(kernels.linear(x.const_data_ptr(), x.stride(0), at, reinterpret_cast<float*>(at + codes), at_c,
+                         at_c != nullptr ? reinterpret_cast<float*>(at_c + codes) : nullptr, pitch, w.codes, w.scales, offsets,
+                         static_cast<int>(w.groups), out.mutable_data_ptr(), static_cast<int>(m), static_cast<int>(n),
+                         static_cast<int>(k), w.pitch, w.group_bytes, trans ? w.s_col : w.s_row, trans ? w.s_row : w.s_col, w.s_group,
+                         trans ? 0 : 1, n, 0, reinterpret_cast<int*>(status), stream_of(x)),
+          "ocb_linear_block_fp8");
+    return out;
+}
+
+// x [M, K] by rows times checked codes [(G,) N, K] (trans) or [(G,) K, N] with their tile scales.
+Tensor block_product(const Tensor& x, const Tensor& codes, const Tensor& scales, const optional<Tensor>& offsets, bool trans, int64_t status) {
+    const c10::cuda::OptionalCUDAGuard guard(x.device());
+    const bool grouped = codes.dim() == 3;
+    const int64_t groups = grouped ? codes.size(0) : 1, rows = codes.size(-2), cols = codes.size(-1);
+    const int64_t pitch = rows > 1 ? codes.stride(-2) : pitch_of(cols);
+    const Weight w{codes.const_data_ptr(), scales.const_data_ptr<float>(), rows, cols, pitch, groups > 1 ? codes.stride(0) : rows * pitch,
+                   grouped ? scales.stride(0) : 0, scales.stride(-2), scales.stride(-1), groups};
+    return product(matrix(x, trans ? cols : rows), w, trans, offsets.has_value() ? offsets->const_data_ptr<int>() : nullptr, nullptr, status);
+}
+
+struct BlockLinear : torch::autograd::Function<BlockLinear> {
+    // weight: what the gradient belongs to; w: its bf16 values [N, K]
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Tensor& w, const optional<Tensor>& cached,
+                          const optional<Tensor>& main_grad, bool needs_dw, bool high_precision, int64_t status) {
+        const c10::cuda::OptionalCUDAGuard guard(x.device());
+        const int64_t n = w.size(0), k = w.size(1);
+        const Tensor x2 = matrix(x, k), tiles = cached.has_value() ? *cached : tile_buffer(w);
+        const bool in_fp8 = needs_dw && !high_precision;
+        Tensor columns;  // what the backward pass keeps of x: its column-scaled form, one byte per element
+        Tensor y = product(x2, in_buffer(tiles, n, k), true, nullptr, in_fp8 ? &columns : nullptr, status);
+        ctx->save_for_backward({tiles, in_fp8 ? columns : needs_dw ? x2 : Tensor()});
+        if (main_grad.has_value()) ctx->saved_data["main_grad"] = *main_grad;  // written to by design: no version check
+        ctx->saved_data["m"] = x2.size(0);
+        ctx->saved_data["n"] = n;
+        ctx->saved_data["k"] = k;
+        ctx->saved_data["x_shape"] = x.sizes().vec();
+        ctx->saved_data["x_dtype"] = x.scalar_type();
+        ctx->saved_data["w_dtype"] = weight.scalar_type();
+        ctx->saved_data["needs_dx"] = x.requires_grad();
+        ctx->saved_data["needs_dw"] = needs_dw;
+        ctx->saved_data["in_fp8"] = in_fp8;
+        ctx->saved_data["status"] = status;
+        auto shape = x.sizes().vec();
+        shape.back() = n;
+        return y.view(shape);
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &tiles = saved[0], &kept = saved[1];
+        const bool accumulate = ctx->saved_data.count("main_grad") != 0;
+        const int64_t m = ctx->saved_data["m"].toInt(), n = ctx->saved_data["n"].toInt(), k = ctx->saved_data["k"].toInt();
+        const int64_t status = ctx->saved_data["status"].toInt();
+        const bool needs_dw = ctx->saved_data["needs_dw"].toBool(), in_fp8 = ctx->saved_data["in_fp8"].toBool();
+        const c10::cuda::OptionalCUDAGuard guard(tiles.device());
+        const Tensor dy = matrix(grads[0], n);
+        Tensor dx, dw, columns;
+        if (ctx->saved_data["needs_dx"].toBool()) {
+            dx = product(dy, in_buffer(tiles, n, k), false, nullptr, in_fp8 ? &columns : nullptr, status);
+            dx = dx.view(ctx->saved_data["x_shape"].toIntVector()).to(ctx->saved_data["x_dtype"].toScalarType());
+        }
+        if (needs_dw) {
+            const auto w_dtype = ctx->saved_data["w_dtype"].toScalarType();
+            // the kernels write bf16 or fp32, whichever the parameter has
+            Tensor out = accumulate ? ctx->saved_data["main_grad"].toTensor() : at::empty({n, k}, dy.options().dtype(w_dtype == at::kBFloat16 ? at::kBFloat16 : at::kFloat));
+            const int epilogue = out.scalar_type() == at::kBFloat16 ? 0 : accumulate ? 1 : 2;
+            TORCH_CHECK(!accumulate || out.scalar_type() == at::kFloat, "main_grad must be float32");
+            if (m == 0 || n == 0 || k == 0) {
+                if (!accumulate) out.zero_();
+            } else if (!in_fp8) {
+                const Tensor a = aligned(dy), b = aligned(kept);
+                check(kernels.gemm_bf16(a.const_data_ptr(), b.const_data_ptr(), out.mutable_data_ptr(), static_cast<int>(n),
+                                        static_cast<int>(k), static_cast<int>(m), a.stride(0), b.stride(0), out.stride(0), 1, 1, epilogue, reinterpret_cast<int*>(status), stream_of(dy)),
+                      "ocb_gemm_bf16");
+            } else {
+                const int64_t pitch_y = pitch_of(n), pitch_x = pitch_of(k);
+                if (!columns.defined()) {
+                    columns = bytes(m * pitch_y + 4 * blocks(m) * n, dy);
+                    uint8_t* at = columns.mutable_data_ptr<uint8_t>();
+                    check(kernels.quantize(dy.const_data_ptr(), nullptr, nullptr, at, reinterpret_cast<float*>(at + m * pitch_y), nullptr,
+                                           nullptr, 1, static_cast<int>(m), static_cast<int>(n), dy.stride(0), pitch_y, 0, 0, stream_of(dy)),
+                          "ocb_quantize_block_fp8");
+                }
+                const uint8_t *a = columns.const_data_ptr<uint8_t>(), *b = kept.const_data_ptr<uint8_t>();
+                check(kernels.gemm_block(a, b, out.mutable_data_ptr(), reinterpret_cast<const float*>(a + m * pitch_y),
+                                         reinterpret_cast<const float*>(b + m * pitch_x), nullptr, 1, static_cast<int>(n),
+                                         static_cast<int>(k), static_cast<int>(m), pitch_y, pitch_x, out.stride(0), 0, n, 1, 0, k, 1, 0, 0,
+                                         1, 1, epilogue, reinterpret_cast<int*>(status), stream_of(dy)),
+                      "ocb_gemm_block_fp8");
+            }
+            if (!accumulate) dw = out.scalar_type() == w_dtype ? out : out.to(w_dtype);
+        }
+        return {dx, dw, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
+
+Tensor block_linear(const Tensor& x, const Tensor& weight, const Tensor& w, const optional<Tensor>& cached,
+                    const optional<Tensor>& main_grad, bool high_precision, int64_t status) {
+    const bool needs_dw = at::GradMode::is_enabled() && (weight.requires_grad() || main_grad.has_value());
+    return BlockLinear::apply(x, weight, w, cached, main_grad, needs_dw, high_precision, status);
+}
+
+}  // namespace
+
+TORCH_LIBRARY_FRAGMENT(ocb_native, m) {
+    m.def("bind_kernels(str path) -> ()", &bind_kernels);
+    m.def("route(Tensor logits, int top_k, bool sigmoid, Tensor? bias, int n_groups, int top_groups, int normalize) -> (Tensor, Tensor, Tensor, Tensor)",
+          &route);
+    m.def("block_tile_buffer(Tensor w) -> Tensor", &tile_buffer);
+    m.def("block_product(Tensor x, Tensor codes, Tensor scales, Tensor? offsets, bool trans, int status) -> Tensor", &block_product);
+    m.def("block_linear(Tensor x, Tensor weight, Tensor w, Tensor? cached, Tensor? main_grad, bool high_precision, int status) -> Tensor",
+          &block_linear);
+}

@@ -26,7 +26,7 @@ On CPU the functions emulate the same arithmetic in PyTorch: the numerical oracl
 
 from __future__ import annotations
 
-from typing import NamedTuple, Optional, Tuple
+from typing import Optional, Tuple
 
 import torch
 
@@ -53,8 +53,6 @@ def _lib_block():
         _lib.register_signature("ocb_quantize_block_fp8", [c_void_p] * 7 + [c_int] * 3 + [c_longlong] * 4 + [c_void_p])
         _lib.register_signature("ocb_gemm_block_fp8", [c_void_p] * 6 + [c_int] * 4 + [c_longlong] * 6 + [c_int]
                                 + [c_longlong] * 3 + [c_int] * 4 + [c_void_p] * 2)
-        _lib.register_signature("ocb_linear_block_fp8", [c_void_p, c_longlong] + [c_void_p] * 4 + [c_longlong] + [c_void_p] * 3
-                                + [c_int, c_void_p] + [c_int] * 3 + [c_longlong] * 5 + [c_int, c_longlong, c_int] + [c_void_p] * 2)
         _lib_sigs_done = True
     return lib
 
@@ -373,92 +371,11 @@ def _check_offsets(offsets: torch.Tensor, groups: int, device: torch.device) -> 
 # ------------------------------------------------------------------------------------------------------
 
 
-def _tile_buffer(w: torch.Tensor) -> torch.Tensor:
-    """:func:`quantize_block_tiles` of ``w [N, K]`` on a GPU as one buffer: codes ``[N, K rounded up to 16]``, then scales."""
-    N, K = w.shape
-    pitch = (K + 15) & -16
-    buffer = torch.empty(N * pitch + 4 * _blocks(N) * _blocks(K), dtype=torch.uint8, device=w.device)
-    if N and K:
-        at = buffer.data_ptr()
-        rc = _lib.on_device(w.device, _lib_block().ocb_quantize_block_fp8, w.data_ptr(), None, None, None, None, at,
-                            at + N * pitch, 1, N, K, w.stride(0), pitch, 0, 0)
-        _lib.check(rc, "ocb_quantize_block_fp8")
-    return buffer
-
-
-class _Weight(NamedTuple):
-    """Where the tile-quantised matrices of a product are: ``groups`` of ``rows x cols``, as a kernel takes them."""
-
-    codes: int
-    scales: int
-    rows: int
-    cols: int
-    pitch: int
-    group_bytes: int
-    scale_strides: Tuple[int, int, int]  # between groups, rows, columns of tiles
-    groups: int
-
-    @classmethod
-    def of(cls, q: torch.Tensor, s: torch.Tensor) -> "_Weight":
-        grouped = q.dim() == 3
-        groups = q.shape[0] if grouped else 1
-        pitch = _pitch(q)
-        return cls(q.data_ptr(), s.data_ptr(), q.shape[-2], q.shape[-1], pitch,
-                   q.stride(0) if groups > 1 else q.shape[-2] * pitch, s.stride() if grouped else (0, *s.stride()), groups)
-
-    @classmethod
-    def of_buffer(cls, buffer: torch.Tensor, rows: int, cols: int) -> "_Weight":
-        pitch, at = (cols + 15) & -16, buffer.data_ptr()
-        return cls(at, at + rows * pitch, rows, cols, pitch, 0, (0, _blocks(cols), 1), 1)
-
-
-def _quantized_product(x: torch.Tensor, w: _Weight, trans_b: bool, offsets: Optional[torch.Tensor] = None,
-                       keep_columns: bool = False):
-    """
-    ``q_rows(x) @ op(W)`` (bf16) for checked operands on a GPU, quantiser and product in one call. With ``keep_columns`` also
-    the column-scaled form of ``x`` (see :func:`_column_buffer`).
-    """
-    M, K = x.shape
-    device = x.device
-    N = w.rows if trans_b else w.cols
-    out = torch.empty((M, N), dtype=torch.bfloat16, device=device)
-    columns = _column_buffer(M, K, device) if keep_columns else None
-    if M == 0 or N == 0 or K == 0:
-        return (out.zero_() if M and N else out), columns
-    pitch = (K + 15) & -16
-    codes = M * pitch
-    rows = torch.empty(codes + 4 * _blocks(K) * M, dtype=torch.uint8, device=device)
-    sw_g, sw_n, sw_c = w.scale_strides
-    at, at_c = rows.data_ptr(), None if columns is None else columns.data_ptr()
-    rc = _lib.on_device(
-        device, _lib_block().ocb_linear_block_fp8, x.data_ptr(), x.stride(0), at, at + codes, at_c,
-        None if at_c is None else at_c + codes, pitch, w.codes, w.scales, None if offsets is None else offsets.data_ptr(),
-        w.groups, out.data_ptr(), M, N, K, w.pitch, w.group_bytes, sw_c if trans_b else sw_n, sw_n if trans_b else sw_c, sw_g,
-        int(not trans_b), N, _lib.EPI_BF16, _lib.status_buffer(device).data_ptr())
-    _lib.check(rc, "ocb_linear_block_fp8")
-    return out, columns
-
-
-def _column_buffer(M: int, K: int, device) -> torch.Tensor:
-    """Codes ``[M, K rounded up to 16]`` and behind them scales ``[ceil(M / 128), K]`` of a column-scaled matrix, in one buffer."""
-    return torch.empty(M * ((K + 15) & -16) + 4 * _blocks(M) * K, dtype=torch.uint8, device=device)
-
-
-def _column_views(buffer: torch.Tensor, M: int, K: int) -> Tuple[torch.Tensor, torch.Tensor]:
-    pitch = (K + 15) & -16
-    return (buffer[: M * pitch].view(M, pitch)[:, :K],
-            buffer[M * pitch:].view(torch.float32).view(_blocks(M), K))
-
-
-def _wgrad(dy_columns: torch.Tensor, x_columns: torch.Tensor, M: int, N: int, K: int, out: torch.Tensor, accumulate: bool) -> None:
-    """``out [N, K] (=|+=) q_columns(dy)^T q_columns(x)`` from two column buffers."""
-    a, b = dy_columns.data_ptr(), x_columns.data_ptr()
-    pitch_a, pitch_b = (N + 15) & -16, (K + 15) & -16
-    rc = _lib.on_device(
-        out.device, _lib_block().ocb_gemm_block_fp8, a, b, out.data_ptr(), a + M * pitch_a, b + M * pitch_b, None, 1, N, K, M,
-        pitch_a, pitch_b, out.stride(0), 0, N, 1, 0, K, 1, 0, 0, 1, 1, _epilogue(out, accumulate),
-        _lib.status_buffer(out.device).data_ptr())
-    _lib.check(rc, "ocb_gemm_block_fp8")
+def _native_product(x: torch.Tensor, w_q: torch.Tensor, w_s: torch.Tensor, offsets: Optional[torch.Tensor], trans_b: bool) -> torch.Tensor:
+    """``q_rows(x) @ op(W)`` (bf16) for checked operands on a GPU: quantiser and product in one call."""
+    y = _lib.native().block_product.default(x, w_q, w_s, offsets, trans_b, _lib.status_buffer(x.device).data_ptr())
+    _lib.check(0, "ocb_linear_block_fp8")  # counted; a failed launch has raised
+    return y
 
 
 def fp8_block_matmul(x: torch.Tensor, w_q: torch.Tensor, w_s: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -474,11 +391,8 @@ def fp8_block_matmul(x: torch.Tensor, w_q: torch.Tensor, w_s: torch.Tensor, bias
         raise ValueError(f"x is on {x.device}, the weight on {w_q.device}")
     _check_scales(w_s, "w_s", (_blocks(N), _blocks(K)), w_q.device)
     with torch.no_grad():
-        x2 = _check_matrix(x if x.dim() == 2 else x.reshape(-1, K), "x")
-        if x2.is_cuda:
-            y, _ = _quantized_product(x2, _Weight.of(w_q, w_s), True)
-        else:
-            y = gemm_fp8_block(*quantize_block_rows(x2), w_q, w_s)
+        x2 = x if x.dim() == 2 else x.reshape(-1, K)
+        y = _native_product(x2, w_q, w_s, None, True) if x2.is_cuda else gemm_fp8_block(*quantize_block_rows(x2), w_q, w_s)
         y = y if x.dim() == 2 else y.view(*x.shape[:-1], N)
         return y if bias is None else y + bias.to(y.dtype)
 
@@ -499,10 +413,9 @@ def fp8_block_grouped_matmul(x: torch.Tensor, w_q: torch.Tensor, w_s: torch.Tens
     _check_offsets(offsets, G, w_q.device)
     _check_scales(w_s, "w_s", (G, _blocks(n), _blocks(k)), w_q.device)
     with torch.no_grad():
-        x2 = _check_matrix(x, "x")
-        if x2.is_cuda and G:
-            return _quantized_product(x2, _Weight.of(w_q, w_s), trans_b, offsets)[0]
-        return grouped_gemm_fp8_block(*quantize_block_rows(x2), w_q, w_s, offsets, trans_b=trans_b)
+        if x.is_cuda and G:
+            return _native_product(x, w_q, w_s, offsets, trans_b)
+        return grouped_gemm_fp8_block(*quantize_block_rows(x), w_q, w_s, offsets, trans_b=trans_b)
 
 
 def _cached(cache: Optional[dict], make, weight: torch.Tensor):
@@ -516,66 +429,36 @@ def _cached(cache: Optional[dict], make, weight: torch.Tensor):
 
 
 class BlockFloat8LinearFunction(torch.autograd.Function):
+    """The layer on CPU tensors, through the emulated operations (on a GPU: ``csrc/torch_ops.cpp``)."""
+
     @staticmethod
     def forward(ctx, x, weight, wgrad_high_precision: bool, cache: Optional[dict] = None):  # type: ignore[override]
         w = compute_weight(weight, torch.bfloat16)
-        x2 = _check_matrix(x if x.dim() == 2 else x.reshape(-1, x.shape[-1]), "x")
-        needs_dw = ctx.needs_input_grad[1] or getattr(weight, "main_grad", None) is not None
-        in_fp8 = needs_dw and not wgrad_high_precision
-        # what the backward pass keeps of x is its column-scaled form: one byte per element
-        if x2.is_cuda:
-            w = _check_matrix(w, "weight")
-            wq = (_cached(cache, lambda: _tile_buffer(w), weight),)
-            y, columns = _quantized_product(x2, _Weight.of_buffer(wq[0], *w.shape), True, keep_columns=in_fp8)
-            kept = (columns,) if in_fp8 else (x2,) if needs_dw else ()
-        else:
-            wq = _cached(cache, lambda: quantize_block_tiles(w), weight)
-            y = gemm_fp8_block(*quantize_block_rows(x2), *wq)
-            kept = quantize_block_columns(x2) if in_fp8 else (x2,) if needs_dw else ()
-        ctx.save_for_backward(*wq, *kept)
-        ctx.n_weight, ctx.w_shape = len(wq), w.shape
-        ctx.in_fp8, ctx.x2_shape = in_fp8, x2.shape
+        x2 = _check_matrix(x.reshape(-1, x.shape[-1]), "x")
+        wq, sw = _cached(cache, lambda: quantize_block_tiles(w), weight)
+        ctx.save_for_backward(wq, sw, x2)
+        ctx.wgrad_hp = wgrad_high_precision
         ctx.weight_ref, ctx.x_shape, ctx.x_dtype = weight, x.shape, x.dtype
-        return y if x.dim() == 2 else y.view(*x.shape[:-1], w.shape[0])
+        return gemm_fp8_block(*quantize_block_rows(x2), wq, sw).view(*x.shape[:-1], w.shape[0])
 
     @staticmethod
     def backward(ctx, dy):  # type: ignore[override]
-        saved = ctx.saved_tensors
-        wq, kept = saved[: ctx.n_weight], saved[ctx.n_weight:]
+        wq, sw, x2 = ctx.saved_tensors
         weight = ctx.weight_ref
-        (M, K), N = ctx.x2_shape, ctx.w_shape[0]
-        dy2 = _check_matrix(dy if dy.dim() == 2 else dy.reshape(-1, N), "dy")
+        dy2 = _check_matrix(dy.reshape(-1, wq.shape[0]), "dy")
         main_grad = getattr(weight, "main_grad", None)
-        needs_dx = ctx.needs_input_grad[0]
-        needs_dw = main_grad is not None or ctx.needs_input_grad[1]
-        in_fp8 = needs_dw and ctx.in_fp8
-        dx = dw = columns = None
-        if needs_dx:
-            if dy2.is_cuda:
-                dx, columns = _quantized_product(dy2, _Weight.of_buffer(wq[0], *ctx.w_shape), False, keep_columns=in_fp8)
-            else:
-                dx = gemm_fp8_block(*quantize_block_rows(dy2), *wq, trans_b=False)
-            dx = dx if len(ctx.x_shape) == 2 else dx.view(ctx.x_shape)
-            dx = dx if dx.dtype == ctx.x_dtype else dx.to(ctx.x_dtype)
-        if needs_dw:
-            # the kernels write bf16 or fp32, whichever the parameter has
+        dx = dw = None
+        if ctx.needs_input_grad[0]:
+            dx = gemm_fp8_block(*quantize_block_rows(dy2), wq, sw, trans_b=False).view(ctx.x_shape).to(ctx.x_dtype)
+        if main_grad is not None or ctx.needs_input_grad[1]:
             out = main_grad if main_grad is not None else torch.empty(
-                (N, K), dtype=torch.bfloat16 if weight.dtype == torch.bfloat16 else torch.float32, device=dy2.device)
-            accumulate = main_grad is not None
-            if not in_fp8:
-                gemm(dy2, kept[0], trans_a=True, trans_b=False, out=out, accumulate=accumulate)
-            elif M == 0:
-                out if accumulate else out.zero_()
-            elif columns is not None:
-                _wgrad(columns, kept[0], M, N, K, out, accumulate)
+                wq.shape, dtype=torch.bfloat16 if weight.dtype == torch.bfloat16 else torch.float32)
+            if ctx.wgrad_hp:
+                gemm(dy2, x2, trans_a=True, trans_b=False, out=out, accumulate=main_grad is not None)
             else:
-                x_columns = _column_views(kept[0], M, K) if dy2.is_cuda else kept
-                gemm_fp8_block(*quantize_block_columns(dy2), *x_columns, trans_a=True, trans_b=False, b_tiles=False, out=out,
-                               accumulate=accumulate)
-            if main_grad is None:
-                dw = out.to(weight.dtype)
-            elif hasattr(weight, "grad_added_to_main_grad"):
-                weight.grad_added_to_main_grad = True
+                gemm_fp8_block(*quantize_block_columns(dy2), *quantize_block_columns(x2), trans_a=True, trans_b=False,
+                               b_tiles=False, out=out, accumulate=main_grad is not None)
+            dw = None if main_grad is not None else out.to(weight.dtype)
         return dx, dw, None, None
 
 
@@ -588,9 +471,23 @@ def fp8_block_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch
     """
     if x.shape[-1] != weight.shape[-1]:
         raise ValueError(f"x has {x.shape[-1]} features, the weight takes {weight.shape[-1]}")
+    if x.device != weight.device:
+        raise ValueError(f"x is on {x.device}, the weight on {weight.device}")
     if wgrad_high_precision and (weight.shape[-1] % 8 or weight.shape[0] % 8):
         raise ValueError("a weight gradient in bf16 needs widths that are multiples of 8")
-    y = BlockFloat8LinearFunction.apply(x, weight, wgrad_high_precision, weight_cache)
+    main_grad = getattr(weight, "main_grad", None)
+    if x.is_cuda:
+        lowp = getattr(weight, "_lowp", None)
+        w = lowp if lowp is not None and lowp.dtype == torch.bfloat16 else weight.detach()
+        native = _lib.native()
+        tiles = None if weight_cache is None else _cached(weight_cache, lambda: native.block_tile_buffer.default(w), weight)
+        y = native.block_linear.default(x, weight, w, tiles, main_grad, wgrad_high_precision,
+                                        _lib.status_buffer(x.device).data_ptr())
+        _lib.check(0, "ocb_linear_block_fp8")  # counted; a failed launch has raised
+    else:
+        y = BlockFloat8LinearFunction.apply(x, weight, wgrad_high_precision, weight_cache)
+    if main_grad is not None and hasattr(weight, "grad_added_to_main_grad") and torch.is_grad_enabled():
+        weight.grad_added_to_main_grad = True  # by the backward pass
     return y if bias is None else y + bias.to(y.dtype)
 
 
@@ -602,7 +499,7 @@ class BlockFloat8GroupedLinearFunction(torch.autograd.Function):
         x2 = _check_matrix(x, "x")
         wq, sw = _cached(cache, lambda: quantize_block_tiles(w.view(G, -1, w.shape[-1])), weight)
         if x2.is_cuda:
-            y, _ = _quantized_product(x2, _Weight.of(wq, sw), trans_b, offsets)
+            y = _native_product(x2, wq, sw, offsets, trans_b)
         else:
             y = grouped_gemm_fp8_block(*quantize_block_rows(x2), wq, sw, offsets, trans_b=trans_b)
         ctx.save_for_backward(wq, sw, offsets, x2)
@@ -617,7 +514,7 @@ class BlockFloat8GroupedLinearFunction(torch.autograd.Function):
         dx = dw = None
         if ctx.needs_input_grad[0]:
             if dy2.is_cuda:
-                dx, _ = _quantized_product(dy2, _Weight.of(wq, sw), not trans_b, offsets)
+                dx = _native_product(dy2, wq, sw, offsets, not trans_b)
             else:
                 dx = grouped_gemm_fp8_block(*quantize_block_rows(dy2), wq, sw, offsets, trans_b=not trans_b)
             dx = dx if dx.dtype == ctx.x_dtype else dx.to(ctx.x_dtype)
@@ -640,8 +537,9 @@ class BlockFloat8GroupedLinearFunction(torch.autograd.Function):
 
 
 def _rows_of_16_bytes(t: torch.Tensor) -> torch.Tensor:
-    """``t`` (bf16), copied where its rows do not start on 16-byte boundaries."""
-    return t if t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+    """``t`` (bf16), copied where its rows do not start on 16-byte boundaries (rows broadcast from one have stride 0)."""
+    fits = t.stride(0) >= t.shape[1] and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0
+    return t if fits else t.clone(memory_format=torch.contiguous_format)
 
 
 def fp8_block_grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor, *, trans_b: bool = True,

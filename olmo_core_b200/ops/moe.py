@@ -85,54 +85,6 @@ def _route_reference(logits, top_k, gating, score_bias, n_groups, top_k_groups, 
     return weights, experts, scores, counts
 
 
-def _route_kernel(logits, top_k, gating, score_bias, n_groups, top_k_groups, normalize):
-    from . import _lib
-
-    n, e = logits.shape
-    device = logits.device
-    scores = torch.empty((n, e), dtype=torch.float32, device=device)
-    weights = torch.empty((n, top_k), dtype=torch.float32, device=device)
-    experts = torch.empty((n, top_k), dtype=torch.int64, device=device)
-    counts = torch.empty(e, dtype=torch.int32, device=device)
-    rc = _lib.on_device(
-        device, _lib.lib().ocb_moe_route, logits.data_ptr(), scores.data_ptr(), weights.data_ptr(), experts.data_ptr(),
-        counts.data_ptr(), _lib.ptr(score_bias), n, e, top_k, int(gating == "sigmoid"), normalize, n_groups, top_k_groups,
-        logits.stride(0), _lib.dt(logits))
-    _lib.check(rc, "ocb_moe_route")
-    return weights, experts, scores, counts
-
-
-class _Route(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, *options):  # type: ignore[override]
-        weights, experts, scores, counts = _route_kernel(logits, *options)
-        _, gating, _, _, _, normalize = options
-        ctx.sigmoid, ctx.normalize = gating == "sigmoid", normalize
-        ctx.save_for_backward(logits if ctx.sigmoid else scores, experts)
-        ctx.logits_dtype = logits.dtype
-        ctx.mark_non_differentiable(experts, counts)
-        ctx.set_materialize_grads(False)
-        return weights, experts, scores, counts
-
-    @staticmethod
-    def backward(ctx, d_weights, _experts, d_scores, _counts):  # type: ignore[override]
-        from . import _lib
-
-        if d_weights is None and d_scores is None:
-            return (None,) * 7
-        kept, experts = ctx.saved_tensors
-        n, e = kept.shape
-        d_weights = None if d_weights is None else d_weights.float().contiguous()
-        d_scores = None if d_scores is None else d_scores.float().contiguous()
-        d_logits = torch.empty((n, e), dtype=ctx.logits_dtype, device=kept.device)
-        rc = _lib.on_device(
-            kept.device, _lib.lib().ocb_moe_route_grad, None if ctx.sigmoid else kept.data_ptr(),
-            kept.data_ptr() if ctx.sigmoid else None, experts.data_ptr(), _lib.ptr(d_weights), _lib.ptr(d_scores),
-            d_logits.data_ptr(), n, e, experts.shape[1], int(ctx.sigmoid), ctx.normalize, kept.stride(0), _lib.dt(d_logits))
-        _lib.check(rc, "ocb_moe_route_grad")
-        return (d_logits,) + (None,) * 6
-
-
 def route(
     logits: torch.Tensor,
     top_k: int,
@@ -183,9 +135,11 @@ def route(
         raise ValueError(f"the routing kernels take at most 1024 experts, 32 chosen and 32 groups, got {e}, {top_k} and {n_groups}")
     if logits.stride(1) != 1 and e > 1:
         logits = logits.contiguous()
-    if logits.requires_grad and torch.is_grad_enabled():
-        return _Route.apply(logits, *options)
-    return _route_kernel(logits, *options)
+    from . import _lib
+
+    out = _lib.native().route.default(logits, top_k, gating == "sigmoid", score_bias, n_groups, top_k_groups, options[-1])
+    _lib.check(0, "ocb_moe_route")  # counted; a failed launch has raised
+    return out
 
 
 def histc(x: torch.Tensor, num_classes: int) -> torch.Tensor:

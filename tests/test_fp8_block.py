@@ -265,6 +265,20 @@ def test_linear_main_grad_cache_and_frozen_operands(device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("hp", [False, True])
+def test_linear_takes_broadcast_gradients_and_strided_input(hp, device):
+    wide = _rand((40, 150), 30, device)
+    w = _rand((72, 136), 31, device, 0.1).requires_grad_(True)
+    for g in (torch.ones((), dtype=torch.bfloat16, device=device).expand(40, 72), _rand((1, 72), 32, device).expand(40, 72)):
+        x = wide[:, 5:141].detach().requires_grad_(True)
+        y = fb.fp8_block_linear(x, w, wgrad_high_precision=hp)
+        dx, dw = torch.autograd.grad(y, (x, w), g)
+        want = torch.autograd.grad(fb.fp8_block_linear(x.detach().clone().requires_grad_(True), w, wgrad_high_precision=hp), w, g.contiguous())
+        assert torch.equal(dw, want[0])
+        _assert_layer(x.detach(), w.detach(), g.contiguous(), y.detach(), dx, dw, hp)
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_linear_gradient_against_differences(device):
     """Inputs that e4m3 holds exactly leave only the products, which are linear: differences of the output equal the gradient."""
     g = torch.Generator().manual_seed(17)
