@@ -263,31 +263,33 @@ __device__ __forceinline__ void tmem_ld_wait_for(uint32_t (&r)[16]) {
                : "memory");
 }
 
-// 32 consecutive columns of one row, for outputs whose rows are not 16-byte aligned.
-template <int EPI>
-__device__ __forceinline__ void store_chunk(const Params& p, long long row, int col, const uint32_t* v) {
-#pragma unroll
-  for (int j = 0; j < 32; ++j) {
-    if (col + j >= p.N) continue;
-    const float f = __uint_as_float(v[j]);
-    if (EPI == EPI_BF16) {
-      reinterpret_cast<__nv_bfloat16*>(p.C)[row * p.ldc + col + j] = __float2bfloat16_rn(f);
-    } else {
-      float* dst = reinterpret_cast<float*>(p.C) + row * p.ldc + col + j;
-      *dst = EPI == EPI_F32_ACC ? *dst + f : f;
-    }
-  }
-}
-
 // ---- epilogue staging ------------------------------------------------------------------------------------------------
 // 16-byte slot `chunk` (0..7) of staged row `row` (0..15); the XOR keeps both the row-per-thread and the 8-lanes-per-row
 // access patterns free of bank conflicts.
 __device__ __forceinline__ uint4* stg_slot(uint8_t* stg, int row, int chunk) {
   return reinterpret_cast<uint4*>(stg + row * 128 + ((chunk ^ (row & 7)) << 4));
 }
-// Moves a staged block to global memory, 8 lanes per 128-byte row; `bytes` of every row are inside the matrix.
+// Moves a staged block to global memory, 8 lanes per 128-byte row; `bytes` of every row are inside the matrix. Rows that do not
+// start on 16-byte boundaries go element by element, a row at a time.
 template <int EPI>
-__device__ __forceinline__ void stg_store(uint8_t* stg, uint8_t* dst0, long long ld_bytes, int rows, int bytes, int lane) {
+__device__ __forceinline__ void stg_store(uint8_t* stg, uint8_t* dst0, long long ld_bytes, int rows, int bytes, bool aligned, int lane) {
+  if (!aligned) {
+    constexpr int ES = EPI == EPI_BF16 ? 2 : 4;
+#pragma unroll 4
+    for (int rr = 0; rr < min(rows, 16); ++rr) {
+#pragma unroll
+      for (int j = 0; j < 4 / ES; ++j) {
+        const int at = (lane + 32 * j) * ES;
+        const uint8_t* src = reinterpret_cast<const uint8_t*>(stg_slot(stg, rr, at >> 4)) + (at & 15);
+        uint8_t* dst = dst0 + rr * ld_bytes + at;
+        if (at >= bytes) continue;
+        if (EPI == EPI_BF16) *reinterpret_cast<uint16_t*>(dst) = *reinterpret_cast<const uint16_t*>(src);
+        else if (EPI == EPI_F32) *reinterpret_cast<float*>(dst) = *reinterpret_cast<const float*>(src);
+        else *reinterpret_cast<float*>(dst) += *reinterpret_cast<const float*>(src);
+      }
+    }
+    return;
+  }
   const int cc = (lane & 7) * 16;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -570,12 +572,6 @@ gemm_block_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
       const int row0 = t.m0 + static_cast<int>(cta) * BM + quad * 32, col0 = t.n0 + half * COLS;
       const int rows = min(32, t.m_end - row0);
       if (rows <= 0) continue;
-      if (!p.aligned) {
-#pragma unroll
-        for (int c = 0; c < COLS / 32; ++c)
-          if (lane < rows) store_chunk<EPI>(p, row0 + lane, col0 + c * 32, r[c]);
-        continue;
-      }
       constexpr int ES = EPI == EPI_BF16 ? 2 : 4, CHUNK = 128 / ES;  // columns of a staged block
 #pragma unroll
       for (int c = 0; c < COLS / CHUNK; ++c) {
@@ -604,7 +600,7 @@ gemm_block_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
             for (int q = 0; q < 8; ++q) *stg_slot(stg, lane & 15, q) = o[q];
           }
           __syncwarp();
-          stg_store<EPI>(stg, dst + h * 16 * p.ldc * ES, p.ldc * ES, rows - 16 * h, bytes, lane);
+          stg_store<EPI>(stg, dst + h * 16 * p.ldc * ES, p.ldc * ES, rows - 16 * h, bytes, p.aligned != 0, lane);
         }
       }
     }
@@ -631,7 +627,7 @@ constexpr int SMALL_THREADS = 256;  // warps as above, with one epilogue warpgro
 template <int BN>
 struct SmallTile {
   static constexpr int KB_BYTES = A_BYTES + BN * BKE;
-  static constexpr int STAGES = BN >= 128 ? 5 : 6;
+  static constexpr int STAGES = BN >= 128 ? 3 : BN >= 64 ? 4 : BN >= 32 ? 5 : 6;  // about 100 KB: two CTAs per SM
   static constexpr uint32_t TMEM = BN >= 128 ? 256 : BN >= 64 ? 128 : BN >= 32 ? 64 : 32;  // BN + 16 scale columns
   static constexpr int SF_BYTES = 2 * SF_BLOCK;
   static constexpr int SMEM_BYTES = STAGES * KB_BYTES + SCALE_SLOTS * SF_BYTES + 1024 + 256;
@@ -1114,33 +1110,49 @@ static int run_small(const Product& x, bool swap, int bn, int parts, int dev, cu
   return launch_small<128, false>(ta, tb, p, tiles, dev, stream);
 }
 
-// Which kernel. The pair kernel moves the fewest bytes per operation but works in 256 x 256 tiles on 74 pairs; with few tiles
-// the 128-row kernel fills the SMs, if need be by splitting the reduction.
+// How many parts the reduction of `tiles` small tiles is cut into: the fewest that leave the busiest SM the fewest blocks to
+// work through, while all CTAs are resident (two per SM) and a part is two blocks at least.
+static int split(long long tiles, long long kb, int sms) {
+  int best = 1;
+  long long least = 0;
+  for (int parts = 1; parts <= 8; ++parts) {
+    if (parts > 1 && (tiles * parts > 2 * sms || kb < 2 * parts)) break;
+    const long long load = ((tiles * parts + sms - 1) / sms) * ((kb + parts - 1) / parts);
+    if (parts == 1 || load < least) {
+      best = parts;
+      least = load;
+    }
+  }
+  return best;
+}
+
+// Which kernel. The pair kernel does four times the work of a 128 x 128 tile per block on two SMs and is as fast per block, so it
+// takes whatever fills a fair part of the 74 pairs; the 128-row kernel takes few tokens (weights on the wide side), and products
+// of so few tiles that cutting the reduction gains more. Microseconds, measured back to back on random operands:
+//   pair:             5 + 0.43 per block and wave of 256 x 256 tiles   (1024 x 4096 x 4096: 18.8, 2048 x 2048 x 2048: 13.2)
+//   128-row, 128 wide 5.5 + 0.5 per block and wave of 128 x 128 tiles  (38.1 and 25.3), 0.7 more for a cut reduction
 static int run(const Product& x, cudaStream_t stream) {
   const int dev = current_device(), sms = num_sms(dev);
   if (sms <= 0) return -3;
   const long long kb = (x.K + BKE - 1) / BKE;
   const long long tiles_n = (x.N + 127) / 128;
-  auto split = [&](long long tiles) {  // parts that bring the CTAs to about two per SM, with two blocks each at least
-    int parts = 1;
-    while (parts < 8 && tiles * parts * 2 <= 2 * sms && kb >= 4 * parts) parts *= 2;
-    return parts;
-  };
   if (x.offsets != nullptr) {
     const long long mean = x.M / x.groups;  // rows of a group
     if (mean > 128) return run_pair(x, dev, stream);
     const int bn = mean <= 8 ? 16 : mean <= 16 ? 32 : mean <= 48 ? 64 : 128;
     const long long used = x.groups < x.M ? x.groups : x.M;
-    return run_small(x, true, bn, split(used * tiles_n), dev, stream);
+    return run_small(x, true, bn, split(used * tiles_n, kb, sms), dev, stream);
   }
   if (x.M <= 128 && !x.a_mn) {
     const int bn = x.M <= 16 ? 16 : x.M <= 32 ? 32 : x.M <= 64 ? 64 : 128;
-    return run_small(x, true, bn, split(tiles_n), dev, stream);
+    return run_small(x, true, bn, split(tiles_n, kb, sms), dev, stream);
   }
   const long long pair_tiles = static_cast<long long>((x.M + 255) / 256) * ((x.N + 255) / 256);
   const long long small_tiles = static_cast<long long>((x.M + 127) / 128) * tiles_n;
-  if (pair_tiles * 2 >= sms) return run_pair(x, dev, stream);
-  return run_small(x, false, 128, split(small_tiles), dev, stream);
+  const int parts = split(small_tiles, kb, sms), pairs = sms / 2;
+  const double pair_us = 5.0 + 0.43 * static_cast<double>(kb * ((pair_tiles + pairs - 1) / pairs));
+  const double small_us = 5.5 + 0.5 * static_cast<double>(((kb + parts - 1) / parts) * ((small_tiles * parts + sms - 1) / sms)) + (parts > 1 ? 0.7 : 0.0);
+  return small_us < pair_us ? run_small(x, false, 128, parts, dev, stream) : run_pair(x, dev, stream);
 }
 
 }  // namespace blk
