@@ -21,6 +21,7 @@
 
 #include <atomic>
 
+#include "block_quant.cuh"
 #include "common.cuh"
 #include "ocb_api.h"
 #include "tmap.h"
@@ -622,6 +623,10 @@ gemm_block_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
 // reduction is split over the CTAs of a cluster; each leaves its fp32 part in its own shared memory, and the CTAs then add the
 // parts in rank order, each for its share of the rows of C (distributed shared memory: no workspace, no atomics, the same bits
 // every time). Groups (SWAP only): a CTA finds its group and its tokens from the device-side boundaries.
+//
+// FUSED (SWAP, up to 16 tokens a tile): the tokens arrive in bf16, and the warps of the epilogue, which have nothing else to do
+// before the end, quantise them straight into the stages beside the weight's codes. Every CTA does that for its part of the reduction, out of L2; in exchange there is no quantiser
+// launch in front, which for one token costs as much as a quarter of the product (4096 x 11008: 2.4 + 12.2 us).
 constexpr int SMALL_THREADS = 256;  // warps as above, with one epilogue warpgroup
 
 template <int BN>
@@ -642,10 +647,24 @@ struct SmallParams {
   int a_mn, b_mn, epi, vector;  // vector: C rows start on 16-byte boundaries and have a multiple of 4 columns
   int parts, kb_per_part;
   Scales sa, sb;
+  const __nv_bfloat16* x;  // FUSED: the BN side [N][K]
+  long long ldx;
+  int x_vector;  // its rows start on 16-byte boundaries
   const int* offsets;
   int num_groups;
   int* status;
 };
+
+// Eight elements of a row of x, zeros outside.
+__device__ __forceinline__ uint4 load_x8(const SmallParams& p, const __nv_bfloat16* row, int k) {
+  if (row == nullptr || k >= p.K) return make_uint4(0u, 0u, 0u, 0u);
+  if (p.x_vector && k + 8 <= p.K) return __ldg(reinterpret_cast<const uint4*>(row + k));
+  uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (k + j < p.K) w[j >> 1] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(row)[k + j]) << (16 * (j & 1));
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
 
 __device__ __forceinline__ float4 load_cluster_f4(uint32_t cluster_addr) {
   float4 v;
@@ -653,11 +672,12 @@ __device__ __forceinline__ float4 load_cluster_f4(uint32_t cluster_addr) {
   return v;
 }
 
-template <int BN, bool SWAP>
-__global__ void __launch_bounds__(SMALL_THREADS)
+template <int BN, bool SWAP, bool FUSED>
+__global__ void __launch_bounds__(SMALL_THREADS, 2)
 gemm_block_fp8_small_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b, const SmallParams p) {
   using T = SmallTile<BN>;
   constexpr int STAGES = T::STAGES;
+  static_assert(!FUSED || (SWAP && BN == 16), "eight threads per token cover sixteen tokens");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sf_smem = smem + STAGES * T::KB_BYTES;
@@ -677,11 +697,11 @@ gemm_block_fp8_small_kernel(const __grid_constant__ CUtensorMap tma_a, const __g
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&full_bar[s], 1);
+      mbar_init(&full_bar[s], FUSED ? 5 : 1);  // the weight's bytes, and the four warps that write the tokens' codes
       mbar_init(&empty_bar[s], 1);
     }
     for (int i = 0; i < SCALE_SLOTS; ++i) {
-      mbar_init(&sfull_bar[i], 2);
+      mbar_init(&sfull_bar[i], FUSED ? 6 : 2);
       mbar_init(&sempty_bar[i], 1);
     }
     mbar_init(done_bar, 1);
@@ -752,12 +772,12 @@ gemm_block_fp8_small_kernel(const __grid_constant__ CUtensorMap tma_a, const __g
         uint8_t* sb = sa + A_BYTES;
         const int k0 = (kb_first + kb) * BKE;
         const int ga = SWAP ? g : 0, gb = SWAP ? 0 : g;
-        mbar_arrive_expect_tx(&full_bar[stage], T::KB_BYTES);
+        mbar_arrive_expect_tx(&full_bar[stage], FUSED ? A_BYTES : T::KB_BYTES);
         // innermost coordinates: k0 (K-major) or a0 / b0 of an ungrouped operand (MN-major), multiples of 128 bytes
         if (p.a_mn) tma_load_3d(sa, &tma_a, &full_bar[stage], a0, k0, ga);
         else tma_load_3d(sa, &tma_a, &full_bar[stage], k0, a0, ga);
-        if (p.b_mn) tma_load_3d(sb, &tma_b, &full_bar[stage], b0, k0, gb);
-        else tma_load_3d(sb, &tma_b, &full_bar[stage], k0, b0, gb);
+        if (!FUSED && p.b_mn) tma_load_3d(sb, &tma_b, &full_bar[stage], b0, k0, gb);
+        else if (!FUSED) tma_load_3d(sb, &tma_b, &full_bar[stage], k0, b0, gb);
         if (++stage == STAGES) { stage = 0; phase ^= 1u; }
       }
       if (!ok) {
@@ -809,7 +829,7 @@ gemm_block_fp8_small_kernel(const __grid_constant__ CUtensorMap tma_a, const __g
   } else if (warp < 4) {
     // ------------------------------------------------------------------ scales
     const int t64 = threadIdx.x - 64;
-    constexpr int PER = 2 + (BN + 63) / 64;
+    constexpr int PER = 2 + (FUSED ? 0 : (BN + 63) / 64);
     const float* src[PER];
     long long step[PER];
 #pragma unroll
@@ -858,7 +878,68 @@ gemm_block_fp8_small_kernel(const __grid_constant__ CUtensorMap tma_a, const __g
   } else {
     // ------------------------------------------------------------------ this CTA's part into shared memory
     const int quad = warp & 3;
-    if (kbs > 0) {
+    if (FUSED) {
+      // First the tokens: eight threads share one, sixteen elements of a block each.
+      const int token = (threadIdx.x - 128) >> 3, piece = threadIdx.x & 7;
+      const __nv_bfloat16* x_row = b0 + token < b_end ? p.x + (b0 + token) * p.ldx : nullptr;
+      const bool any = __any_sync(0xffffffffu, x_row != nullptr);  // a warp without tokens only keeps the barriers going
+      uint4 next[SCALE_BATCH][2];
+      auto fetch = [&](int kb0) {
+#pragma unroll
+        for (int b = 0; b < SCALE_BATCH; ++b)
+#pragma unroll
+          for (int q = 0; q < 2; ++q)
+            next[b][q] = load_x8(p, kb0 + b < kbs ? x_row : nullptr, (kb_first + kb0 + b) * BKE + piece * 16 + q * 8);
+      };
+      int slot = 0, stage = 0;
+      uint32_t phase = 0, stage_phase = 0;
+      fetch(0);
+      for (int kb0 = 0; kb0 < kbs && ok; kb0 += SCALE_BATCH) {
+        uint4 codes[SCALE_BATCH];
+        uint32_t word = 0u;
+        if (any) {
+#pragma unroll
+          for (int b = 0; b < SCALE_BATCH; ++b) {
+            const uint4 lo = next[b][0], hi = next[b][1];
+            uint32_t m2 = blkq::max_abs2(blkq::max_abs2(blkq::max_abs2(blkq::max_abs2(0u, lo.x), lo.y), lo.z), lo.w);
+            m2 = blkq::max_abs2(blkq::max_abs2(blkq::max_abs2(blkq::max_abs2(m2, hi.x), hi.y), hi.z), hi.w);
+#pragma unroll
+            for (int o = 4; o; o >>= 1) m2 = blkq::max_abs2(m2, __shfl_xor_sync(0xffffffffu, m2, o));
+            const float amax = fmaxf(blkq::lo(m2), blkq::hi(m2));
+            const int e = blkq::scale_exponent(amax);
+            const float inv = blkq::pow2_biased(254 - e);
+            const bool inf = amax == INFINITY;
+            const uint2 c0 = inf ? blkq::e4m3x8<true>(lo, inv) : blkq::e4m3x8<false>(lo, inv);
+            const uint2 c1 = inf ? blkq::e4m3x8<true>(hi, inv) : blkq::e4m3x8<false>(hi, inv);
+            codes[b] = make_uint4(c0.x, c0.y, c1.x, c1.y);
+            word |= static_cast<uint32_t>(e) << (8 * b);
+          }
+          fetch(kb0 + SCALE_BATCH);
+        }
+        ok = wait_for(&sempty_bar[slot], phase ^ 1u, abort_flag, p.status, kStatusTimeoutProducer);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (any && piece == 0) reinterpret_cast<uint32_t*>(sf_smem + slot * T::SF_BYTES + SF_BLOCK)[token * 4] = word;
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sfull_bar[slot]);
+        if (++slot == SCALE_SLOTS) { slot = 0; phase ^= 1u; }
+#pragma unroll
+        for (int b = 0; b < SCALE_BATCH; ++b) {
+          if (kb0 + b >= kbs) break;
+          ok = wait_for(&empty_bar[stage], stage_phase ^ 1u, abort_flag, p.status, kStatusTimeoutProducer);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          if (any)  // the 128-byte swizzle: 16-byte piece c of row r sits at c ^ (r % 8)
+            *reinterpret_cast<uint4*>(smem + stage * T::KB_BYTES + A_BYTES + token * 128 + ((piece ^ (token & 7)) << 4)) = codes[b];
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&full_bar[stage]);
+          if (++stage == STAGES) { stage = 0; stage_phase ^= 1u; }
+        }
+      }
+    }
+    if (kbs > 0 && ok) {
       ok = wait_for(done_bar, 0, abort_flag, p.status, kStatusTimeoutEpilogue);
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
@@ -1014,10 +1095,10 @@ using namespace ocb;
 namespace ocb {
 namespace blk {
 
-template <int BN, bool SWAP>
+template <int BN, bool SWAP, bool FUSED = false>
 static int launch_small(const CUtensorMap& ta, const CUtensorMap& tb, const SmallParams& p, long long tiles, int dev, cudaStream_t stream) {
   constexpr int bytes = SmallTile<BN>::SMEM_BYTES;
-  auto kernel = gemm_block_fp8_small_kernel<BN, SWAP>;
+  auto kernel = gemm_block_fp8_small_kernel<BN, SWAP, FUSED>;
   static std::atomic<uint64_t> done;
   if (!allow_smem(kernel, bytes, done, dev)) return -3;
   if (tiles * p.parts > 0x7fffffffll) return -1;
@@ -1036,7 +1117,9 @@ static int launch_small(const CUtensorMap& ta, const CUtensorMap& tb, const Smal
 }
 
 struct Product {
-  const void *A, *B;
+  const void *A, *B;  // A null: its rows are x (bf16), quantised on the way
+  const __nv_bfloat16* x;
+  long long ldx;
   void* C;
   int M, N, K, groups;
   long long lda, ldb, ldc, b_group_bytes;
@@ -1091,14 +1174,19 @@ static int run_small(const Product& x, bool swap, int bn, int parts, int dev, cu
   p.status = x.status;
   const long long group_bytes = x.groups > 1 ? x.b_group_bytes : x.ldb;
   const int rows_a = swap ? bn : BM, rows_b = swap ? BM : bn;
+  p.x = x.x;
+  p.ldx = x.ldx;
+  p.x_vector = x.ldx % 8 == 0 && (reinterpret_cast<uintptr_t>(x.x) & 15) == 0;
   CUtensorMap ma, mb;
-  if (!make_map(&ma, x.A, x.a_mn != 0, x.M, x.K, 1, x.lda, x.lda, rows_a, 3)) return -1001;
+  if (x.A != nullptr && !make_map(&ma, x.A, x.a_mn != 0, x.M, x.K, 1, x.lda, x.lda, rows_a, 3)) return -1001;
   if (!make_map(&mb, x.B, x.b_mn != 0, x.N, x.K, x.groups, x.ldb, group_bytes, rows_b, 3)) return -2001;
+  if (x.A == nullptr) ma = mb;  // not used
   const CUtensorMap &ta = swap ? mb : ma, &tb = swap ? ma : mb;
   long long b_tiles = (p.N + bn - 1) / bn;
   // every group can end inside a tile; a group without rows has none
   if (x.offsets != nullptr) b_tiles = p.N / bn + (x.groups < p.N ? x.groups : p.N);
   const long long tiles = b_tiles * ((p.M + BM - 1) / BM);
+  if (x.A == nullptr) return launch_small<16, true, true>(ta, tb, p, tiles, dev, stream);
   if (swap) {
     switch (bn) {
       case 16: return launch_small<16, true>(ta, tb, p, tiles, dev, stream);
@@ -1131,6 +1219,14 @@ static int split(long long tiles, long long kb, int sms) {
 // of so few tiles that cutting the reduction gains more. Microseconds, measured back to back on random operands:
 //   pair:             5 + 0.43 per block and wave of 256 x 256 tiles   (1024 x 4096 x 4096: 18.8, 2048 x 2048 x 2048: 13.2)
 //   128-row, 128 wide 5.5 + 0.5 per block and wave of 128 x 128 tiles  (38.1 and 25.3), 0.7 more for a cut reduction
+// The BN side of the small kernel for groups of `mean` rows (or so many rows without groups).
+static int small_width(long long mean, bool grouped) {
+  if (grouped) return mean <= 8 ? 16 : mean <= 16 ? 32 : mean <= 48 ? 64 : 128;
+  return mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 64 ? 64 : 128;
+}
+// Whether the rows of A (M of them in `groups` groups) are quantised inside the product.
+static bool fused(int M, int groups, bool grouped) { return small_width(grouped ? M / groups : M, grouped) == 16; }
+
 static int run(const Product& x, cudaStream_t stream) {
   const int dev = current_device(), sms = num_sms(dev);
   if (sms <= 0) return -3;
@@ -1139,12 +1235,12 @@ static int run(const Product& x, cudaStream_t stream) {
   if (x.offsets != nullptr) {
     const long long mean = x.M / x.groups;  // rows of a group
     if (mean > 128) return run_pair(x, dev, stream);
-    const int bn = mean <= 8 ? 16 : mean <= 16 ? 32 : mean <= 48 ? 64 : 128;
+    const int bn = small_width(mean, true);
     const long long used = x.groups < x.M ? x.groups : x.M;
     return run_small(x, true, bn, split(used * tiles_n, kb, sms), dev, stream);
   }
   if (x.M <= 128 && !x.a_mn) {
-    const int bn = x.M <= 16 ? 16 : x.M <= 32 ? 32 : x.M <= 64 ? 64 : 128;
+    const int bn = small_width(x.M, false);
     return run_small(x, true, bn, split(tiles_n, kb, sms), dev, stream);
   }
   const long long pair_tiles = static_cast<long long>((x.M + 255) / 256) * ((x.N + 255) / 256);
@@ -1158,47 +1254,64 @@ static int run(const Product& x, cudaStream_t stream) {
 }  // namespace blk
 }  // namespace ocb
 
+static int gemm_block_fp8(const void* A, const void* x, long long ldx, const void* B, void* C, const float* sa, const float* sb,
+                          const int* offsets, int num_groups, int M, int N, int K, long long lda, long long ldb, long long ldc,
+                          long long b_group_bytes, long long sa_k, long long sa_i, int sa_shift, long long sb_k, long long sb_i,
+                          long long sb_g, int sb_shift, int a_mn, int b_mn, int epilogue, int* status, cudaStream_t stream) {
+  if (M <= 0 || N <= 0 || K <= 0 || num_groups <= 0) return 0;
+  if ((lda % 16) != 0 || (ldb % 16) != 0 || (b_group_bytes % 16) != 0 || (reinterpret_cast<uintptr_t>(A) & 15) ||
+      (reinterpret_cast<uintptr_t>(B) & 15) || (A != nullptr && sa == nullptr) || sb == nullptr)
+    return -1;
+  if ((sa_shift != 0 && sa_shift != 7) || (sb_shift != 0 && sb_shift != 7) || (offsets != nullptr && a_mn)) return -1;
+  if (epilogue < blk::EPI_BF16 || epilogue > blk::EPI_F32) return -1;
+  blk::Product p;
+  p.A = A;
+  p.B = B;
+  p.x = reinterpret_cast<const __nv_bfloat16*>(x);
+  p.ldx = ldx;
+  p.C = C;
+  p.M = M;
+  p.N = N;
+  p.K = K;
+  p.groups = num_groups;
+  p.lda = lda;
+  p.ldb = ldb;
+  p.ldc = ldc;
+  p.b_group_bytes = b_group_bytes;
+  p.sa = {sa, sa_k, sa_i, 0, sa_shift};
+  p.sb = {sb, sb_k, sb_i, sb_g, sb_shift};
+  p.a_mn = a_mn;
+  p.b_mn = b_mn;
+  p.epi = epilogue;
+  p.offsets = offsets;
+  p.status = status;
+  return blk::run(p, stream);
+}
+
 // See ocb_api.h.
 extern "C" int ocb_gemm_block_fp8(const void* A, const void* B, void* C, const float* sa, const float* sb, const int* offsets,
                                   int num_groups, int M, int N, int K, long long lda, long long ldb, long long ldc,
                                   long long b_group_bytes, long long sa_k, long long sa_i, int sa_shift, long long sb_k,
                                   long long sb_i, long long sb_g, int sb_shift, int a_mn, int b_mn, int epilogue, int* status,
                                   cudaStream_t stream) {
-  if (M <= 0 || N <= 0 || K <= 0 || num_groups <= 0) return 0;
-  if ((lda % 16) != 0 || (ldb % 16) != 0 || (b_group_bytes % 16) != 0 || (reinterpret_cast<uintptr_t>(A) & 15) ||
-      (reinterpret_cast<uintptr_t>(B) & 15) || sa == nullptr || sb == nullptr)
-    return -1;
-  if ((sa_shift != 0 && sa_shift != 7) || (sb_shift != 0 && sb_shift != 7) || (offsets != nullptr && a_mn)) return -1;
-  blk::Product x;
-  x.A = A;
-  x.B = B;
-  x.C = C;
-  x.M = M;
-  x.N = N;
-  x.K = K;
-  x.groups = num_groups;
-  x.lda = lda;
-  x.ldb = ldb;
-  x.ldc = ldc;
-  x.b_group_bytes = b_group_bytes;
-  x.sa = {sa, sa_k, sa_i, 0, sa_shift};
-  x.sb = {sb, sb_k, sb_i, sb_g, sb_shift};
-  x.a_mn = a_mn;
-  x.b_mn = b_mn;
-  x.epi = epilogue;
-  x.offsets = offsets;
-  x.status = status;
-  if (epilogue < blk::EPI_BF16 || epilogue > blk::EPI_F32) return -1;
-  return blk::run(x, stream);
+  if (A == nullptr) return -1;
+  return gemm_block_fp8(A, nullptr, 0, B, C, sa, sb, offsets, num_groups, M, N, K, lda, ldb, ldc, b_group_bytes, sa_k, sa_i,
+                        sa_shift, sb_k, sb_i, sb_g, sb_shift, a_mn, b_mn, epilogue, status, stream);
 }
+
+extern "C" int ocb_linear_block_fp8_fused(int M, int num_groups, int grouped) { return blk::fused(M, num_groups < 1 ? 1 : num_groups, grouped != 0); }
 
 // See ocb_api.h.
 extern "C" int ocb_linear_block_fp8(const void* x, long long ldx, void* q_row, float* s_row, void* q_col, float* s_col,
                                     long long ldq, const void* W, const float* sw, const int* offsets, int num_groups, void* C,
                                     int M, int N, int K, long long ldw, long long w_group_bytes, long long sw_k, long long sw_i,
                                     long long sw_g, int w_mn, long long ldc, int epilogue, int* status, cudaStream_t stream) {
-  const int rc = ocb_quantize_block_fp8(x, q_row, s_row, q_col, s_col, nullptr, nullptr, 1, M, K, ldx, ldq, 0, 0, stream);
-  if (rc != 0) return rc;
-  return ocb_gemm_block_fp8(q_row, W, C, s_row, sw, offsets, num_groups, M, N, K, ldq, ldw, ldc, w_group_bytes, M, 1, 0, sw_k,
-                            sw_i, sw_g, 7, 0, w_mn, epilogue, status, stream);
+  const bool inside = q_row == nullptr;
+  if (inside && !blk::fused(M, num_groups < 1 ? 1 : num_groups, offsets != nullptr)) return -1;
+  if (!inside || q_col != nullptr) {
+    const int rc = ocb_quantize_block_fp8(x, q_row, s_row, q_col, s_col, nullptr, nullptr, 1, M, K, ldx, ldq, 0, 0, stream);
+    if (rc != 0) return rc;
+  }
+  return gemm_block_fp8(q_row, x, ldx, W, C, s_row, sw, offsets, num_groups, M, N, K, inside ? 0 : ldq, ldw, ldc, w_group_bytes,
+                        M, 1, 0, sw_k, sw_i, sw_g, 7, 0, w_mn, epilogue, status, stream);
 }

@@ -62,7 +62,9 @@ int ocb_gemm_block_fp8(const void* A, const void* B, void* C, const float* sa, c
                        long long b_group_bytes, long long sa_k, long long sa_i, int sa_shift, long long sb_k, long long sb_i,
                        long long sb_g, int sb_shift, int a_mn, int b_mn, int epilogue, int* status, cudaStream_t stream);
 // The two together: x [M, K] (bf16) by rows into q_row / s_row (and by columns into q_col / s_col where those are not null), then
-// C = q_row * W^T with the tile scales of W.
+// C = q_row * W^T with the tile scales of W. Where ocb_linear_block_fp8_fused() says 1 (few rows), q_row and s_row may be null:
+// the rows are quantised inside the product.
+int ocb_linear_block_fp8_fused(int M, int num_groups, int grouped);
 int ocb_linear_block_fp8(const void* x, long long ldx, void* q_row, float* s_row, void* q_col, float* s_col, long long ldq,
                          const void* W, const float* sw, const int* offsets, int num_groups, void* C, int M, int N, int K,
                          long long ldw, long long w_group_bytes, long long sw_k, long long sw_i, long long sw_g, int w_mn,

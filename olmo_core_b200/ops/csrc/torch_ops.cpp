@@ -24,6 +24,7 @@ struct Kernels {
     decltype(&ocb_moe_route_grad) route_grad = nullptr;
     decltype(&ocb_quantize_block_fp8) quantize = nullptr;
     decltype(&ocb_linear_block_fp8) linear = nullptr;
+    decltype(&ocb_linear_block_fp8_fused) linear_fused = nullptr;
     decltype(&ocb_gemm_block_fp8) gemm_block = nullptr;
     decltype(&ocb_gemm_bf16) gemm_bf16 = nullptr;
 } kernels;
@@ -41,6 +42,7 @@ void bind_kernels(c10::string_view path) {
     resolve(handle, "ocb_moe_route_grad", kernels.route_grad);
     resolve(handle, "ocb_quantize_block_fp8", kernels.quantize);
     resolve(handle, "ocb_linear_block_fp8", kernels.linear);
+    resolve(handle, "ocb_linear_block_fp8_fused", kernels.linear_fused);
     resolve(handle, "ocb_gemm_block_fp8", kernels.gemm_block);
     resolve(handle, "ocb_gemm_bf16", kernels.gemm_bf16);
 }
@@ -171,10 +173,11 @@ Tensor product(const Tensor& x, const Weight& w, bool trans, const int* offsets,
     if (columns != nullptr) *columns = bytes(codes + 4 * blocks(m) * k, x);
     if (m == 0 || n == 0) return out;
     if (k == 0) return out.zero_();
-    Tensor rows = bytes(codes + 4 * blocks(k) * m, x);
-    uint8_t* at = rows.mutable_data_ptr<uint8_t>();
+    Tensor rows;  // few rows are quantised inside the product
+    if (kernels.linear_fused(static_cast<int>(m), static_cast<int>(w.groups), offsets != nullptr) == 0) rows = bytes(codes + 4 * blocks(k) * m, x);
+    uint8_t* at = rows.defined() ? rows.mutable_data_ptr<uint8_t>() : nullptr;
     uint8_t* at_c = columns != nullptr ? columns->mutable_data_ptr<uint8_t>() : nullptr;
-    check(kernels.linear(x.const_data_ptr(), x.stride(0), at, reinterpret_cast<float*>(at + codes), at_c,
+    check(kernels.linear(x.const_data_ptr(), x.stride(0), at, at != nullptr ? reinterpret_cast<float*>(at + codes) : nullptr, at_c,
                          at_c != nullptr ? reinterpret_cast<float*>(at_c + codes) : nullptr, pitch, w.codes, w.scales, offsets,
                          static_cast<int>(w.groups), out.mutable_data_ptr(), static_cast<int>(m), static_cast<int>(n),
                          static_cast<int>(k), w.pitch, w.group_bytes, trans ? w.s_col : w.s_row, trans ? w.s_row : w.s_col, w.s_group,

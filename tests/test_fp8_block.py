@@ -187,6 +187,24 @@ def test_scales_that_are_no_powers_of_two_show_as_nan(bad, device):
     _assert_product(out[keep, :128], a[keep], b[:128])
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("M,N,K", [(1, 1, 1), (1, 300, 520), (2, 700, 1536), (16, 129, 2050), (15, 2000, 130), (17, 64, 300), (0, 40, 256)])
+def test_kept_weight_product_of_few_tokens(M, N, K, device):
+    """Few rows are quantised inside the product: the same bits as quantising them first."""
+    wide = _rand((M, K + 9), 33, device)
+    wq, sw, w = _operand((N, K), 34, "tiles", device)
+    for x in (wide[:, :K], wide[:, 3:K + 3], wide[:, 8:K + 8].contiguous()):
+        y = fb.fp8_block_matmul(x, wq, sw)
+        q, s = fb.quantize_block_rows(x)
+        assert torch.equal(y, fb.gemm_fp8_block(q, s, wq, sw))
+    bias = torch.ones(N, device=device)
+    assert torch.equal(fb.fp8_block_matmul(x.view(M, 1, K), wq, sw, bias)[:, 0], y + 1)
+    if M:
+        x = x.clone()
+        x[0, K // 2], x[-1, 0] = float("inf"), float("nan")
+        assert fb.fp8_block_matmul(x, wq, sw)[[0, -1]].isnan().all()
+
+
 GROUPS = [[128, 256, 128], [100, 0, 333, 7, 1], [0, 0, 5], [1, 1, 2, 0, 1, 3, 1, 1], [20, 0, 17, 3] * 10, [0] * 40 + [50, 33] + [0] * 3, [1000, 37, 0, 0, 513, 64, 65, 2]]
 
 
@@ -300,7 +318,7 @@ def test_linear_gradient_against_differences(device):
 
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("trans_b", [True, False])
-@pytest.mark.parametrize("sizes", [[100, 0, 133, 7, 1], [1, 2, 0, 1]])
+@pytest.mark.parametrize("sizes", [[100, 0, 133, 7, 1], [1, 2, 0, 1], [0, 21, 3, 0, 1, 1, 0, 9]])
 def test_grouped_linear_gradients(sizes, trans_b, device):
     G, K, N = len(sizes), 136, 72
     R = sum(sizes)
@@ -321,6 +339,8 @@ def test_grouped_linear_gradients(sizes, trans_b, device):
         _assert_layer(x.detach()[lo:hi], wi, g[lo:hi], y.detach()[lo:hi], x.grad[lo:hi], dwi, True)
     q, s = fb.quantize_block_tiles(w)
     assert torch.equal(fb.fp8_block_grouped_matmul(x.detach(), q, s, offsets, trans_b=trans_b), y.detach())
+    xq, xs = fb.quantize_block_rows(x.detach())  # few rows per group are quantised inside the product: the same bits
+    assert torch.equal(fb.grouped_gemm_fp8_block(xq, xs, q, s, offsets, trans_b=trans_b), y.detach())
 
 
 @pytest.mark.parametrize("device", DEVICES)
