@@ -50,6 +50,8 @@ __global__ void __launch_bounds__(THREADS, MODE == (ROWS | COLUMNS) ? 3 : 4) qua
   const int n_col = min(8, p.cols - col);  // columns of this thread inside the matrix (may be <= 0)
   const long long row0 = static_cast<long long>(blockIdx.y) * B;
   const __nv_bfloat16* x = p.x + static_cast<long long>(blockIdx.z) * p.x_group;
+  next_kernel_may_start();
+  previous_kernel_done();
   uint4 v[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -161,6 +163,18 @@ __global__ void __launch_bounds__(THREADS, MODE == (ROWS | COLUMNS) ? 3 : 4) qua
   }
 }
 
+template <int MODE>
+static int launch(const Params& p, int vec, dim3 grid, cudaStream_t stream) {
+  cudaLaunchConfig_t config = {};
+  config.gridDim = grid;
+  config.blockDim = dim3(THREADS);
+  config.stream = stream;
+  cudaLaunchAttribute attribute = dependent_launch();
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, quantize_block_kernel<MODE>, p, vec) == cudaSuccess ? 0 : -4;
+}
+
 }  // namespace blkq
 }  // namespace ocb
 
@@ -195,13 +209,11 @@ extern "C" int ocb_quantize_block_fp8(const void* x, void* q_row, float* s_row, 
   const dim3 grid((cols + blkq::B - 1) / blkq::B, static_cast<unsigned>(row_tiles), groups);
   if (q_tile != nullptr) {
     if (s_tile == nullptr || q_row != nullptr || q_col != nullptr) return -1;
-    blkq::quantize_block_kernel<blkq::TILES><<<grid, blkq::THREADS, 0, stream>>>(p, vec);
-  } else {
-    if (groups != 1 || (q_row != nullptr && s_row == nullptr) || (q_col != nullptr && s_col == nullptr)) return -1;
-    if (q_row != nullptr && q_col != nullptr) blkq::quantize_block_kernel<blkq::ROWS | blkq::COLUMNS><<<grid, blkq::THREADS, 0, stream>>>(p, vec);
-    else if (q_row != nullptr) blkq::quantize_block_kernel<blkq::ROWS><<<grid, blkq::THREADS, 0, stream>>>(p, vec);
-    else if (q_col != nullptr) blkq::quantize_block_kernel<blkq::COLUMNS><<<grid, blkq::THREADS, 0, stream>>>(p, vec);
-    else return -1;
+    return blkq::launch<blkq::TILES>(p, vec, grid, stream);
   }
-  return cudaGetLastError() == cudaSuccess ? 0 : -4;
+  if (groups != 1 || (q_row != nullptr && s_row == nullptr) || (q_col != nullptr && s_col == nullptr)) return -1;
+  if (q_row != nullptr && q_col != nullptr) return blkq::launch<blkq::ROWS | blkq::COLUMNS>(p, vec, grid, stream);
+  if (q_row != nullptr) return blkq::launch<blkq::ROWS>(p, vec, grid, stream);
+  if (q_col != nullptr) return blkq::launch<blkq::COLUMNS>(p, vec, grid, stream);
+  return -1;
 }
