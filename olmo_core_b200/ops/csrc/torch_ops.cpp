@@ -27,6 +27,7 @@ struct Kernels {
     decltype(&ocb_linear_block_fp8_fused) linear_fused = nullptr;
     decltype(&ocb_gemm_block_fp8) gemm_block = nullptr;
     decltype(&ocb_gemm_bf16) gemm_bf16 = nullptr;
+    decltype(&ocb_grouped_gemm_bf16) grouped_gemm_bf16 = nullptr;
 } kernels;
 
 template <class F>
@@ -45,6 +46,7 @@ void bind_kernels(c10::string_view path) {
     resolve(handle, "ocb_linear_block_fp8_fused", kernels.linear_fused);
     resolve(handle, "ocb_gemm_block_fp8", kernels.gemm_block);
     resolve(handle, "ocb_gemm_bf16", kernels.gemm_bf16);
+    resolve(handle, "ocb_grouped_gemm_bf16", kernels.grouped_gemm_bf16);
 }
 
 void check(int rc, const char* what) { TORCH_CHECK(rc == 0, what, " failed with code ", rc); }
@@ -137,16 +139,17 @@ Tensor aligned(const Tensor& m) {
     return fits ? m : m.clone(at::MemoryFormat::Contiguous);
 }
 
-// Codes [rows, cols rounded up to 16] and behind them the scales of 128 x 128 tiles.
-Tensor tile_buffer(const Tensor& weight) {
+// `groups` stacked matrices [rows, cols]: their codes [rows, cols rounded up to 16] and behind them the scales of their tiles.
+Tensor tile_buffer(const Tensor& weight, int64_t groups) {
     const c10::cuda::OptionalCUDAGuard guard(weight.device());
     const Tensor w = matrix(weight, weight.size(1));
-    const int64_t rows = w.size(0), cols = w.size(1), codes = rows * pitch_of(cols);
-    Tensor buffer = bytes(codes + 4 * blocks(rows) * blocks(cols), w);
+    const int64_t rows = w.size(0) / groups, cols = w.size(1), pitch = pitch_of(cols), codes = groups * rows * pitch;
+    Tensor buffer = bytes(codes + 4 * groups * blocks(rows) * blocks(cols), w);
     if (rows == 0 || cols == 0) return buffer;
     uint8_t* at = buffer.mutable_data_ptr<uint8_t>();
-    check(kernels.quantize(w.const_data_ptr(), nullptr, nullptr, nullptr, nullptr, at, reinterpret_cast<float*>(at + codes), 1,
-                           static_cast<int>(rows), static_cast<int>(cols), w.stride(0), pitch_of(cols), 0, 0, stream_of(w)),
+    check(kernels.quantize(w.const_data_ptr(), nullptr, nullptr, nullptr, nullptr, at, reinterpret_cast<float*>(at + codes),
+                           static_cast<int>(groups), static_cast<int>(rows), static_cast<int>(cols), w.stride(0), pitch,
+                           rows * w.stride(0), rows * pitch, stream_of(w)),
           "ocb_quantize_block_fp8");
     return buffer;
 }
@@ -160,9 +163,11 @@ struct Weight {
     int64_t groups;
 };
 
-Weight in_buffer(const Tensor& tiles, int64_t rows, int64_t cols) {
+Weight in_buffer(const Tensor& tiles, int64_t groups, int64_t rows, int64_t cols) {
     const uint8_t* at = tiles.const_data_ptr<uint8_t>();
-    return {at, reinterpret_cast<const float*>(at + rows * pitch_of(cols)), rows, cols, pitch_of(cols), 0, 0, blocks(cols), 1, 1};
+    const int64_t pitch = pitch_of(cols);
+    return {at, reinterpret_cast<const float*>(at + groups * rows * pitch), rows, cols, pitch, rows * pitch,
+            blocks(rows) * blocks(cols), blocks(cols), 1, groups};
 }
 
 // x by rows times W (transposed or not); `columns`: also x by columns.
@@ -203,10 +208,10 @@ struct BlockLinear : torch::autograd::Function<BlockLinear> {
                           const optional<Tensor>& main_grad, bool needs_dw, bool high_precision, int64_t status) {
         const c10::cuda::OptionalCUDAGuard guard(x.device());
         const int64_t n = w.size(0), k = w.size(1);
-        const Tensor x2 = matrix(x, k), tiles = cached.has_value() ? *cached : tile_buffer(w);
+        const Tensor x2 = matrix(x, k), tiles = cached.has_value() ? *cached : tile_buffer(w, 1);
         const bool in_fp8 = needs_dw && !high_precision;
         Tensor columns;  // what the backward pass keeps of x: its column-scaled form, one byte per element
-        Tensor y = product(x2, in_buffer(tiles, n, k), true, nullptr, in_fp8 ? &columns : nullptr, status);
+        Tensor y = product(x2, in_buffer(tiles, 1, n, k), true, nullptr, in_fp8 ? &columns : nullptr, status);
         ctx->save_for_backward({tiles, in_fp8 ? columns : needs_dw ? x2 : Tensor()});
         if (main_grad.has_value()) ctx->saved_data["main_grad"] = *main_grad;  // written to by design: no version check
         ctx->saved_data["m"] = x2.size(0);
@@ -235,7 +240,7 @@ struct BlockLinear : torch::autograd::Function<BlockLinear> {
         const Tensor dy = matrix(grads[0], n);
         Tensor dx, dw, columns;
         if (ctx->saved_data["needs_dx"].toBool()) {
-            dx = product(dy, in_buffer(tiles, n, k), false, nullptr, in_fp8 ? &columns : nullptr, status);
+            dx = product(dy, in_buffer(tiles, 1, n, k), false, nullptr, in_fp8 ? &columns : nullptr, status);
             dx = dx.view(ctx->saved_data["x_shape"].toIntVector()).to(ctx->saved_data["x_dtype"].toScalarType());
         }
         if (needs_dw) {
@@ -273,6 +278,67 @@ struct BlockLinear : torch::autograd::Function<BlockLinear> {
     }
 };
 
+// The experts' layer: rows sorted by group, weights stacked [G * N, K] (trans) or [G * K, N]; weight gradient in bf16.
+struct BlockGroupedLinear : torch::autograd::Function<BlockGroupedLinear> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Tensor& w, const Tensor& offsets,
+                          const optional<Tensor>& cached, const optional<Tensor>& main_grad, bool trans, bool needs_dw, int64_t status) {
+        const c10::cuda::OptionalCUDAGuard guard(x.device());
+        const int64_t groups = offsets.size(0) - 1, rows = w.size(0) / groups, cols = w.size(1);
+        const Tensor x2 = matrix(x, x.size(1)), tiles = cached.has_value() ? *cached : tile_buffer(w, groups);
+        Tensor y = product(x2, in_buffer(tiles, groups, rows, cols), trans, offsets.const_data_ptr<int>(), nullptr, status);
+        ctx->save_for_backward({tiles, offsets, needs_dw ? x2 : Tensor()});
+        if (main_grad.has_value()) ctx->saved_data["main_grad"] = *main_grad;  // written to by design: no version check
+        ctx->saved_data["rows"] = rows;
+        ctx->saved_data["cols"] = cols;
+        ctx->saved_data["trans"] = trans;
+        ctx->saved_data["x_dtype"] = x.scalar_type();
+        ctx->saved_data["w_dtype"] = weight.scalar_type();
+        ctx->saved_data["needs_dx"] = x.requires_grad();
+        ctx->saved_data["needs_dw"] = needs_dw;
+        ctx->saved_data["status"] = status;
+        return y;
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &tiles = saved[0], &offsets = saved[1], &x = saved[2];
+        const int64_t groups = offsets.size(0) - 1, rows = ctx->saved_data["rows"].toInt(), cols = ctx->saved_data["cols"].toInt();
+        const int64_t status = ctx->saved_data["status"].toInt();
+        const bool trans = ctx->saved_data["trans"].toBool(), accumulate = ctx->saved_data.count("main_grad") != 0;
+        const c10::cuda::OptionalCUDAGuard guard(tiles.device());
+        const Tensor dy = matrix(grads[0], trans ? rows : cols);
+        Tensor dx, dw;
+        if (ctx->saved_data["needs_dx"].toBool())
+            dx = product(dy, in_buffer(tiles, groups, rows, cols), !trans, offsets.const_data_ptr<int>(), nullptr, status)
+                     .to(ctx->saved_data["x_dtype"].toScalarType());
+        if (ctx->saved_data["needs_dw"].toBool()) {
+            const auto w_dtype = ctx->saved_data["w_dtype"].toScalarType();
+            Tensor out = accumulate ? ctx->saved_data["main_grad"].toTensor()
+                                    : at::empty({groups * rows, cols}, dy.options().dtype(w_dtype == at::kBFloat16 ? at::kBFloat16 : at::kFloat));
+            TORCH_CHECK(!accumulate || (out.scalar_type() == at::kFloat && out.is_contiguous()), "main_grad must be contiguous float32");
+            if (dy.size(0) == 0) {
+                if (!accumulate) out.zero_();
+            } else {
+                const Tensor a = aligned(trans ? dy : x), b = aligned(trans ? x : dy);
+                check(kernels.grouped_gemm_bf16(a.const_data_ptr(), b.const_data_ptr(), out.mutable_data_ptr(), offsets.const_data_ptr<int>(),
+                                                static_cast<int>(groups), 2, static_cast<int>(dy.size(0)), static_cast<int>(rows),
+                                                static_cast<int>(cols), 0, a.stride(0), b.stride(0), cols, 1,
+                                                out.scalar_type() == at::kBFloat16 ? 0 : accumulate ? 1 : 2,
+                                                reinterpret_cast<int*>(status), stream_of(dy)),
+                      "ocb_grouped_gemm_bf16");
+            }
+            if (!accumulate) dw = out.scalar_type() == w_dtype ? out : out.to(w_dtype);
+        }
+        return {dx, dw, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
+
+Tensor block_grouped_linear(const Tensor& x, const Tensor& weight, const Tensor& w, const Tensor& offsets, const optional<Tensor>& cached,
+                            const optional<Tensor>& main_grad, bool trans, int64_t status) {
+    const bool needs_dw = at::GradMode::is_enabled() && (weight.requires_grad() || main_grad.has_value());
+    return BlockGroupedLinear::apply(x, weight, w, offsets, cached, main_grad, trans, needs_dw, status);
+}
+
 Tensor block_linear(const Tensor& x, const Tensor& weight, const Tensor& w, const optional<Tensor>& cached,
                     const optional<Tensor>& main_grad, bool high_precision, int64_t status) {
     const bool needs_dw = at::GradMode::is_enabled() && (weight.requires_grad() || main_grad.has_value());
@@ -285,7 +351,9 @@ TORCH_LIBRARY_FRAGMENT(ocb_native, m) {
     m.def("bind_kernels(str path) -> ()", &bind_kernels);
     m.def("route(Tensor logits, int top_k, bool sigmoid, Tensor? bias, int n_groups, int top_groups, int normalize) -> (Tensor, Tensor, Tensor, Tensor)",
           &route);
-    m.def("block_tile_buffer(Tensor w) -> Tensor", &tile_buffer);
+    m.def("block_tile_buffer(Tensor w, int groups) -> Tensor", &tile_buffer);
+    m.def("block_grouped_linear(Tensor x, Tensor weight, Tensor w, Tensor offsets, Tensor? cached, Tensor? main_grad, bool trans, int status) -> Tensor",
+          &block_grouped_linear);
     m.def("block_product(Tensor x, Tensor codes, Tensor scales, Tensor? offsets, bool trans, int status) -> Tensor", &block_product);
     m.def("block_linear(Tensor x, Tensor weight, Tensor w, Tensor? cached, Tensor? main_grad, bool high_precision, int status) -> Tensor",
           &block_linear);

@@ -32,7 +32,7 @@ import torch
 
 from . import _lib
 from .fp8 import cached_weight_cast
-from .gemm import compute_weight, gemm, grouped_gemm_wgrad
+from .gemm import compute_weight, gemm
 
 __all__ = ["BLOCK", "quantize_block_rows", "quantize_block_columns", "quantize_block_tiles", "dequantize_block_rows",
            "dequantize_block_columns", "dequantize_block_tiles", "gemm_fp8_block", "grouped_gemm_fp8_block",
@@ -480,7 +480,7 @@ def fp8_block_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch
         lowp = getattr(weight, "_lowp", None)
         w = lowp if lowp is not None and lowp.dtype == torch.bfloat16 else weight.detach()
         native = _lib.native()
-        tiles = None if weight_cache is None else _cached(weight_cache, lambda: native.block_tile_buffer.default(w), weight)
+        tiles = None if weight_cache is None else _cached(weight_cache, lambda: native.block_tile_buffer.default(w, 1), weight)
         y = native.block_linear.default(x, weight, w, tiles, main_grad, wgrad_high_precision,
                                         _lib.status_buffer(x.device).data_ptr())
         _lib.check(0, "ocb_linear_block_fp8")  # counted; a failed launch has raised
@@ -492,19 +492,16 @@ def fp8_block_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch
 
 
 class BlockFloat8GroupedLinearFunction(torch.autograd.Function):
+    """The experts' layer on CPU tensors (on a GPU: ``csrc/torch_ops.cpp``)."""
+
     @staticmethod
     def forward(ctx, x, weight, offsets, trans_b: bool, cache: Optional[dict] = None):  # type: ignore[override]
         w = compute_weight(weight, torch.bfloat16)
-        G = offsets.numel() - 1
         x2 = _check_matrix(x, "x")
-        wq, sw = _cached(cache, lambda: quantize_block_tiles(w.view(G, -1, w.shape[-1])), weight)
-        if x2.is_cuda:
-            y = _native_product(x2, wq, sw, offsets, trans_b)
-        else:
-            y = grouped_gemm_fp8_block(*quantize_block_rows(x2), wq, sw, offsets, trans_b=trans_b)
+        wq, sw = _cached(cache, lambda: quantize_block_tiles(w.view(offsets.numel() - 1, -1, w.shape[-1])), weight)
         ctx.save_for_backward(wq, sw, offsets, x2)
         ctx.trans_b, ctx.weight_ref, ctx.w_shape, ctx.x_dtype = trans_b, weight, w.shape, x.dtype
-        return y
+        return grouped_gemm_fp8_block(*quantize_block_rows(x2), wq, sw, offsets, trans_b=trans_b)
 
     @staticmethod
     def backward(ctx, dy):  # type: ignore[override]
@@ -513,33 +510,16 @@ class BlockFloat8GroupedLinearFunction(torch.autograd.Function):
         dy2 = _check_matrix(dy, "dy")
         dx = dw = None
         if ctx.needs_input_grad[0]:
-            if dy2.is_cuda:
-                dx = _native_product(dy2, wq, sw, offsets, not trans_b)
-            else:
-                dx = grouped_gemm_fp8_block(*quantize_block_rows(dy2), wq, sw, offsets, trans_b=not trans_b)
-            dx = dx if dx.dtype == ctx.x_dtype else dx.to(ctx.x_dtype)
+            dx = grouped_gemm_fp8_block(*quantize_block_rows(dy2), wq, sw, offsets, trans_b=not trans_b).to(ctx.x_dtype)
         main_grad = getattr(weight, "main_grad", None)
         if main_grad is not None or ctx.needs_input_grad[1]:
             a, b = (dy2, x2) if trans_b else (x2, dy2)
-            out = main_grad.view(ctx.w_shape) if main_grad is not None else torch.empty(
-                ctx.w_shape, dtype=torch.bfloat16 if weight.dtype == torch.bfloat16 else torch.float32, device=x2.device)
-            if x2.is_cuda:
-                grouped_gemm_wgrad(_rows_of_16_bytes(a), _rows_of_16_bytes(b), offsets, out, accumulate=main_grad is not None)
-            else:
-                bounds, per = offsets.tolist(), out.view(offsets.numel() - 1, -1, out.shape[1])
-                for g, (lo, hi) in enumerate(zip(bounds[:-1], bounds[1:])):
-                    _store(per[g], a[lo:hi].float().t() @ b[lo:hi].float(), main_grad is not None)
-            if main_grad is None:
-                dw = out.to(weight.dtype)
-            elif hasattr(weight, "grad_added_to_main_grad"):
-                weight.grad_added_to_main_grad = True
+            out = main_grad.view(ctx.w_shape) if main_grad is not None else torch.empty(ctx.w_shape, dtype=weight.dtype)
+            bounds, per = offsets.tolist(), out.view(offsets.numel() - 1, -1, out.shape[1])
+            for g, (lo, hi) in enumerate(zip(bounds[:-1], bounds[1:])):
+                _store(per[g], a[lo:hi].float().t() @ b[lo:hi].float(), main_grad is not None)
+            dw = None if main_grad is not None else out
         return dx, dw, None, None, None
-
-
-def _rows_of_16_bytes(t: torch.Tensor) -> torch.Tensor:
-    """``t`` (bf16), copied where its rows do not start on 16-byte boundaries (rows broadcast from one have stride 0)."""
-    fits = t.stride(0) >= t.shape[1] and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0
-    return t if fits else t.clone(memory_format=torch.contiguous_format)
 
 
 def fp8_block_grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor, *, trans_b: bool = True,
@@ -562,4 +542,19 @@ def fp8_block_grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: tor
     if w.shape[1] % 8 or (w.shape[0] // G) % 8:
         raise ValueError("the widths of the experts' matrices must be multiples of 8")
     _check_offsets(offsets, G, x.device)
-    return BlockFloat8GroupedLinearFunction.apply(x, weight, offsets, trans_b, weight_cache)
+    main_grad = getattr(weight, "main_grad", None)
+    if x.is_cuda:
+        if x.device != weight.device:
+            raise ValueError(f"x is on {x.device}, the weights on {weight.device}")
+        lowp = getattr(weight, "_lowp", None)
+        w = lowp if lowp is not None and lowp.dtype == torch.bfloat16 else weight.detach()
+        native = _lib.native()
+        tiles = None if weight_cache is None else _cached(weight_cache, lambda: native.block_tile_buffer.default(w, G), weight)
+        y = native.block_grouped_linear.default(x, weight, w, offsets, tiles, main_grad, trans_b,
+                                                _lib.status_buffer(x.device).data_ptr())
+        _lib.check(0, "ocb_linear_block_fp8")  # counted; a failed launch has raised
+    else:
+        y = BlockFloat8GroupedLinearFunction.apply(x, weight, offsets, trans_b, weight_cache)
+    if main_grad is not None and hasattr(weight, "grad_added_to_main_grad") and torch.is_grad_enabled():
+        weight.grad_added_to_main_grad = True  # by the backward pass
+    return y

@@ -150,3 +150,29 @@ def test_training_steps_with_block_layers():
         assert grads and all(torch.isfinite(t).all() for t in grads)
         module.optim_step()
         assert torch.isfinite(module.latest_ce_loss)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_experts_main_grad_and_cache(device):
+    G, K, N, sizes = 5, 72, 136, [20, 0, 33, 1, 140]
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(sum(sizes), K, generator=g).bfloat16().to(device).requires_grad_(True)
+    w = torch.nn.Parameter((torch.randn(G * N, K, generator=g) * 0.1).to(device))
+    offsets = torch.tensor([0] + sizes, dtype=torch.int32).cumsum(0).to(torch.int32).to(device)
+    dy = torch.randn(sum(sizes), N, generator=g).bfloat16().to(device)
+    y = fb.fp8_block_grouped_linear(x, w, offsets)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    assert dw.dtype == torch.float32 and dw.shape == w.shape
+    w.main_grad, w.grad_added_to_main_grad = torch.ones(G * N, K, device=device), False
+    cache = {}
+    for n in (1, 2):
+        again = fb.fp8_block_grouped_linear(x, w, offsets, weight_cache=cache)
+        assert torch.equal(again, y) and set(cache) == {"block_tiles"}
+        x.grad = None
+        again.backward(dy)
+        assert w.grad is None and w.grad_added_to_main_grad and torch.equal(x.grad, dx)
+        # one more fp32 addition per pass
+        torch.testing.assert_close(w.main_grad, n * dw + 1, rtol=4 * 2.0 ** -24 * n, atol=4 * 2.0 ** -24 * n)
+    with torch.no_grad():
+        none = fb.fp8_block_grouped_linear(x[:0], w, torch.zeros(G + 1, dtype=torch.int32, device=device))
+    assert none.shape == (0, N)
