@@ -372,10 +372,10 @@ gemm_block_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
   }
-  next_kernel_may_start();
   previous_kernel_done();
   tc_fence_before();
   __syncthreads();
+  next_kernel_may_start();  // after this CTA has its tensor memory: one of the next kernel never waits for it with that in hand
   if (CTAS == 2) cluster_sync_all();  // the other CTA's barriers are initialised before anything is signalled across
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
@@ -716,7 +716,6 @@ gemm_block_fp8_small_kernel(const __grid_constant__ CUtensorMap tma_a, const __g
     tmem_alloc(tmem_slot, T::TMEM);
     tmem_relinquish();
   }
-  next_kernel_may_start();
   previous_kernel_done();
   if (warp == 2) {
     int g = 0, b0 = b_tile * BN, b_end = p.N;
@@ -755,6 +754,7 @@ gemm_block_fp8_small_kernel(const __grid_constant__ CUtensorMap tma_a, const __g
   }
   tc_fence_before();
   __syncthreads();
+  next_kernel_may_start();  // after this CTA has its tensor memory
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   const int g = tile_info[0], b0 = tile_info[1], b_end = tile_info[2];

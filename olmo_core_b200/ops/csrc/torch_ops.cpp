@@ -66,6 +66,7 @@ struct RouteOptions {
 std::tuple<Tensor, Tensor, Tensor, Tensor> run_route(const Tensor& logits, const optional<Tensor>& bias, const RouteOptions& o) {
     const c10::cuda::OptionalCUDAGuard guard(logits.device());
     const int64_t n = logits.size(0), e = logits.size(1);
+    TORCH_CHECK_VALUE(n <= INT32_MAX, "routing takes fewer than 2^31 tokens");
     const auto opt = logits.options();
     Tensor weights = at::empty({n, o.top_k}, opt.dtype(at::kFloat)), experts = at::empty({n, o.top_k}, opt.dtype(at::kLong));
     Tensor scores = at::empty({n, e}, opt.dtype(at::kFloat)), counts = at::empty({e}, opt.dtype(at::kInt));
@@ -173,6 +174,7 @@ Weight in_buffer(const Tensor& tiles, int64_t groups, int64_t rows, int64_t cols
 // x by rows times W (transposed or not); `columns`: also x by columns.
 Tensor product(const Tensor& x, const Weight& w, bool trans, const int* offsets, Tensor* columns, int64_t status) {
     const int64_t m = x.size(0), k = x.size(1), n = trans ? w.rows : w.cols;
+    TORCH_CHECK_VALUE(m <= INT32_MAX && k <= INT32_MAX && n <= INT32_MAX, "the block-scaled product takes sizes below 2^31");
     Tensor out = at::empty({m, n}, x.options());
     const int64_t pitch = pitch_of(k), codes = m * pitch;
     if (columns != nullptr) *columns = bytes(codes + 4 * blocks(m) * k, x);

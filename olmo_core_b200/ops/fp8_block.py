@@ -473,11 +473,10 @@ def fp8_block_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch
         raise ValueError(f"x has {x.shape[-1]} features, the weight takes {weight.shape[-1]}")
     if x.device != weight.device:
         raise ValueError(f"x is on {x.device}, the weight on {weight.device}")
-    if wgrad_high_precision and (weight.shape[-1] % 8 or weight.shape[0] % 8):
+    lowp, main_grad = getattr(weight, "_lowp", None), getattr(weight, "main_grad", None)
+    if wgrad_high_precision and any(n % 8 for n in (weight if lowp is None else lowp).shape):
         raise ValueError("a weight gradient in bf16 needs widths that are multiples of 8")
-    main_grad = getattr(weight, "main_grad", None)
     if x.is_cuda:
-        lowp = getattr(weight, "_lowp", None)
         w = lowp if lowp is not None and lowp.dtype == torch.bfloat16 else weight.detach()
         native = _lib.native()
         tiles = None if weight_cache is None else _cached(weight_cache, lambda: native.block_tile_buffer.default(w, 1), weight)

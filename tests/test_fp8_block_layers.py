@@ -176,3 +176,55 @@ def test_experts_main_grad_and_cache(device):
     with torch.no_grad():
         none = fb.fp8_block_grouped_linear(x[:0], w, torch.zeros(G + 1, dtype=torch.int32, device=device))
     assert none.shape == (0, N)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [5, 300])
+def test_training_step_in_a_graph_and_on_other_streams(tokens):
+    """Linear layer, experts and routing forward and backward: captured and replayed, and on two streams at once."""
+    from olmo_core_b200.ops.moe import route
+
+    g = torch.Generator().manual_seed(4)
+
+    def make(seed):
+        g.manual_seed(seed)
+        x = torch.randn(tokens, 264, generator=g).bfloat16().cuda().requires_grad_(True)
+        w = (torch.randn(136, 264, generator=g) * 0.1).bfloat16().cuda().requires_grad_(True)
+        we = (torch.randn(4 * 136, 264, generator=g) * 0.1).bfloat16().cuda().requires_grad_(True)
+        logits = torch.randn(tokens, 32, generator=g).cuda().requires_grad_(True)
+        dy = torch.randn(tokens, 136, generator=g).bfloat16().cuda()
+        offsets = torch.tensor([0, tokens // 3, tokens // 2, tokens // 2, tokens], dtype=torch.int32, device="cuda")
+        return x, w, we, logits, dy, offsets
+
+    def step(x, w, we, logits, dy, offsets):
+        y = fb.fp8_block_linear(x, w)
+        ye = fb.fp8_block_grouped_linear(x, we, offsets)
+        weights, experts, scores, counts = route(logits, 4, gating="sigmoid", n_groups=4, top_k_groups=2, normalize=1)
+        grads = torch.autograd.grad((y, ye, weights, scores), (x, w, we, logits), (dy, dy, weights.detach(), scores.detach()))
+        return [t.detach() for t in (y, ye, weights, experts, scores, counts, *grads)]
+
+    states = [make(1), make(2)]
+    want = [step(*s) for s in states]
+    streams = [torch.cuda.Stream() for _ in states]
+    torch.cuda.synchronize()
+    got = []
+    for stream, s in zip(streams, states):  # nothing waits between the two
+        with torch.cuda.stream(stream):
+            for _ in range(3):
+                out = step(*s)
+            got.append(out)
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
+    graphs = []
+    for stream, s in zip(streams, states):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            out = step(*s)
+        graphs.append((graph, out))
+    for _ in range(2):
+        for graph, _ in graphs:
+            graph.replay()
+    torch.cuda.synchronize()
+    for a, (_, b) in zip(want, graphs):
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
