@@ -37,6 +37,8 @@ CONFIGS = {
     # the headline model with 8-bit linear layers: row-wise scaled e4m3, and block-scaled MX (32-element E8M0 scales)
     "olmo2_7B_fsdp_fp8": dict(model="olmo2_7B", seq_len=4096, micro_batch=2, seqs_per_gpu=128, vocab_size=100352, fp8="rowwise"),
     "olmo2_7B_fsdp_mxfp8": dict(model="olmo2_7B", seq_len=4096, micro_batch=2, seqs_per_gpu=128, vocab_size=100352, fp8="mx"),
+    # the same with one power-of-two scale per block of 128
+    "olmo2_7B_fsdp_blockfp8": dict(model="olmo2_7B", seq_len=4096, micro_batch=2, seqs_per_gpu=128, vocab_size=100352, fp8="block"),
     # OLMoE-1B-7B, experts spread over all N GPUs, the rest sharded data parallel
     "olmoe_1B_7B_ep8": dict(model="olmoe_1B_7B", seq_len=4096, micro_batch=4, seqs_per_gpu=32, vocab_size=50304, ep=0),
     # OLMo-3 7B long context: ONE 65536-token sequence per context-parallel group of all N GPUs
@@ -172,13 +174,16 @@ def run_ours(args):
         extra["cp_config"] = TransformerContextParallelConfig.llama3(degree=args.cp)
         parallelism = f"cp{args.cp} (llama3 layout) x dp{world // args.cp}"
     if args.fp8:
-        from olmo_core_b200.float8 import AOFloat8LinearConfig, AOMXLinearConfig, Float8Config
+        from olmo_core_b200.float8 import AOFloat8LinearConfig, AOMXLinearConfig, BlockFloat8LinearConfig, Float8Config
 
         # quantised weights are kept for all micro-batches of a step (dropped after the parameter update)
         ao = AOFloat8LinearConfig(enable_fsdp_float8_all_gather=True)
         if args.fp8 == "mx":
             f8 = Float8Config(enabled=True, ao_mx=AOMXLinearConfig.mxfp8_cublas_rceil(), cache_weight_casts=True)
             parallelism += ", MX fp8 (e4m3, E8M0 scale per 32) linear layers"
+        elif args.fp8 == "block":
+            f8 = Float8Config(enabled=True, block=BlockFloat8LinearConfig(), cache_weight_casts=True)
+            parallelism += ", block fp8 (e4m3, one scale per 128) linear layers"
         else:
             f8 = Float8Config(enabled=True, ao=ao)
             parallelism += ", fp8 row-wise linear layers"

@@ -2,7 +2,7 @@
 Micro-benchmarks of the sm_100a kernels against their library counterparts.
 
 ``python -m olmo_core_b200.ops.bench_kernels <case> [--iters N] [--profile]`` with ``case`` one of ``gemm``, ``mlp`` (gated
-MLP with the activation in the GEMM epilogues), ``fp8``, ``mx``, ``grouped``, ``attention``, ``norm``, ``norm_rope``,
+MLP with the activation in the GEMM epilogues), ``fp8``, ``mx``, ``fp8_block``, ``grouped``, ``attention``, ``norm``, ``norm_rope``,
 ``swiglu``, ``ce``, ``adamw``, ``router``.
 
 Each case is timed with CUDA events on the launching stream after warm-up, with a buffer larger than L2 rewritten
@@ -295,6 +295,58 @@ def bench_mx(args, peaks) -> None:
                "speedup": round(t_bf / t_mx, 3)}, None)
 
 
+def bench_fp8_block(args, peaks) -> None:
+    """e4m3 products with one scale per block of 128: the three products of a layer, its quantisers, few tokens, experts."""
+    from . import fp8_block as fb
+    from .gemm import linear
+
+    M, K, N = 8192, 4096, 11008
+    x = torch.randn(M, K, device="cuda", dtype=torch.bfloat16)
+    w = torch.randn(N, K, device="cuda", dtype=torch.bfloat16) * K ** -0.5
+    dy = torch.randn(M, N, device="cuda", dtype=torch.bfloat16)
+    wq = fb.quantize_block_tiles(w)
+    if args.profile:
+        fb.gemm_fp8_block(*fb.quantize_block_rows(x), *wq)
+        fb.fp8_block_matmul(x[:1], *wq)
+        torch.cuda.synchronize()
+        return
+    xq, dyq = fb.quantize_block_rows(x), fb.quantize_block_rows(dy)
+    xc, dyc = fb.quantize_block_columns(x), fb.quantize_block_columns(dy)
+    tl = time_ms(lambda: torch.matmul(x, w.t()), args.iters)
+    for name, fn in (("forward", lambda: fb.gemm_fp8_block(*xq, *wq)),
+                     ("dgrad", lambda: fb.gemm_fp8_block(*dyq, *wq, trans_b=False)),
+                     ("wgrad", lambda: fb.gemm_fp8_block(*dyc, *xc, trans_a=True, trans_b=False, b_tiles=False))):
+        t = time_ms(fn, args.iters)
+        _emit({"kernel": f"gemm_fp8_block_{name}", "M": M, "N": N, "K": K, "ms": round(t, 4),
+               "tflops": round(2.0 * M * N * K / t / 1e9, 1), "cublas_bf16_ms": round(tl, 4)}, peaks)
+    for name, fn, size in (("rows", lambda: fb.quantize_block_rows(dy), 3.0), ("columns", lambda: fb.quantize_block_columns(dy), 3.0),
+                           ("rows_columns", lambda: fb.quantize_block_rows_columns(dy), 4.0),
+                           ("tiles", lambda: fb.quantize_block_tiles(dy), 3.0)):
+        t = time_ms(fn, args.iters)
+        _emit({"kernel": f"quantize_block_{name}", "rows": M, "cols": N, "ms": round(t, 4),
+               "gbs": round(M * N * size / t / 1e6, 1)}, peaks)
+    for tokens in (1, 16, 64, 128, 256, 1024):
+        t = time_ms(lambda: fb.fp8_block_matmul(x[:tokens], *wq), args.iters)
+        _emit({"kernel": "fp8_block_matmul", "tokens": tokens, "N": N, "K": K, "ms": round(t, 4),
+               "gbs": round((N * K + 2 * tokens * (N + K)) / t / 1e6, 1)}, peaks)
+    E, R = 64, 128
+    we = fb.quantize_block_tiles(torch.randn(E, 1024, 2048, device="cuda", dtype=torch.bfloat16))
+    xe = torch.randn(R, 2048, device="cuda", dtype=torch.bfloat16)
+    offsets = torch.arange(0, R + 1, R // E, device="cuda", dtype=torch.int32)
+    t = time_ms(lambda: fb.fp8_block_grouped_matmul(xe, *we, offsets), args.iters)
+    _emit({"kernel": "fp8_block_grouped_matmul", "experts": E, "rows": R, "ms": round(t, 4),
+           "gbs": round(E * 1024 * 2048 / t / 1e6, 1)}, peaks)
+    xg, wg = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+
+    def run(fn):
+        xg.grad = wg.grad = None
+        fn(xg, wg).backward(dy)
+
+    t8, t16 = time_ms(lambda: run(fb.fp8_block_linear), args.iters), time_ms(lambda: run(linear), args.iters)
+    _emit({"kernel": "linear_fwd_bwd", "M": M, "N": N, "K": K, "fp8_block_ms": round(t8, 4), "bf16_ms": round(t16, 4),
+           "speedup": round(t16 / t8, 3)}, None)
+
+
 def bench_grouped(args, peaks) -> None:
     """Expert MLP shapes of OLMoE-1B-7B: 64 experts, d_model 2048, hidden 1024, 32768 x 8 routed rows."""
     from .gemm import grouped_gemm, grouped_gemm_wgrad
@@ -437,7 +489,7 @@ def bench_adamw(args, peaks) -> None:
 
 def bench_router(args, peaks) -> None:
     from ..nn.moe.router import _FusedSoftmaxTopK
-    from .moe import indices_and_bins
+    from .moe import indices_and_bins, route
 
     N, E, k = 32768, 64, 8
     logits = torch.randn(N, E, device="cuda", dtype=torch.bfloat16)
@@ -450,6 +502,11 @@ def bench_router(args, peaks) -> None:
         t = time_ms(lambda: _FusedSoftmaxTopK.apply(logits, k), args.iters)
         _emit({"kernel": "router_softmax_topk", "tokens": N, "experts": E, "top_k": k, "ms": round(t, 4),
                "gbs": round((N * E * 6.0 + N * k * 8.0) / t / 1e6, 1)}, peaks)
+        big = torch.randn(N, 256, device="cuda")
+        bias = torch.zeros(256, device="cuda")
+        t = time_ms(lambda: route(big, k, gating="sigmoid", score_bias=bias, n_groups=8, top_k_groups=4, normalize=1), args.iters)
+        _emit({"kernel": "router_sigmoid_bias_groups", "tokens": N, "experts": 256, "top_k": k, "ms": round(t, 4),
+               "gbs": round((N * 256 * 8.0 + N * k * 12.0) / t / 1e6, 1)}, peaks)
         ids = _FusedSoftmaxTopK.apply(logits, k)[2]
         t = time_ms(lambda: indices_and_bins(ids, E), args.iters)
         _emit({"kernel": "routing_counting_sort", "copies": N * k, "ms": round(t, 4)}, None)
@@ -457,7 +514,7 @@ def bench_router(args, peaks) -> None:
         _emit({"kernel": "routing_torch_sort_library", "copies": N * k, "ms": round(t, 4)}, None)
 
 
-CASES = {"gemm": bench_gemm, "mlp": bench_mlp, "fp8": bench_fp8, "mx": bench_mx, "grouped": bench_grouped, "attention": bench_attention,
+CASES = {"gemm": bench_gemm, "mlp": bench_mlp, "fp8": bench_fp8, "mx": bench_mx, "fp8_block": bench_fp8_block, "grouped": bench_grouped, "attention": bench_attention,
          "norm": bench_norm, "norm_rope": bench_norm_rope, "swiglu": bench_swiglu, "ce": bench_ce, "adamw": bench_adamw,
          "router": bench_router}
 
