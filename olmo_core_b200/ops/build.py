@@ -122,7 +122,7 @@ def build_native(force: bool = False, verbose: bool = True) -> Path:
     BUILD_DIR.mkdir(exist_ok=True)
     srcs = sorted(NATIVE_SRC_DIR.glob("*.cpp")) + sorted(CSRC_DIR.glob("*.cpp"))
     h = hashlib.sha256(torch.__version__.encode())
-    for src in [*srcs, CSRC_DIR / "ocb_api.h"]:
+    for src in [*srcs, CSRC_DIR / "ocb_api.h", Path(__file__)]:
         h.update(src.read_bytes())
     stamp = BUILD_DIR / "native.hash"
     if not force and NATIVE_LIB_PATH.exists() and stamp.exists() and stamp.read_text() == h.hexdigest():
@@ -134,7 +134,9 @@ def build_native(force: bool = False, verbose: bool = True) -> Path:
         cmd += ["-isystem", inc]
     for lib_dir in library_paths():
         cmd += [f"-L{lib_dir}", f"-Wl,-rpath,{lib_dir}"]
-    cmd += ["-I", str(CSRC_DIR), "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-ldl"]
+    # the process's C++ runtime by name: a toolchain that has only the static one would put a second copy into the library, and
+    # a number streamed into an error message would then look up its facet with the wrong copy's ids
+    cmd += ["-I", str(CSRC_DIR), "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-ldl", "-l:libstdc++.so.6"]
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
         raise RuntimeError(f"native helper build failed:\n{proc.stdout}\n{proc.stderr}")
