@@ -7,8 +7,12 @@
 //   w = s[chosen], divided by its sum (normalize 1) or 2-norm (normalize 2); counts = tokens per expert
 //
 // One warp per token, expert e in register e / 32 of lane e % 32: a row is read and its scores are written once, everything
-// between stays in registers (and, for the groups, one row of shared memory). Memory bound for many tokens, latency bound for
-// few. Tokens per expert are counted in shared memory, so that global atomics number one per expert and CTA.
+// between stays in registers (and, for the groups, one row of shared memory). Tokens per expert are counted in shared memory, so
+// that global atomics number one per expert and CTA.
+//
+// What bounds it: latency for few tokens (one: 4 us, 11 with the host), the issue of instructions for many, about 500 a token with 64
+// experts and 1700 with bias and groups of 256: each of the k choices is a reduction over the warp. 32768 tokens of 64 experts: 33 us
+// (448 GB/s), of 256 in 8 groups: 88 us (800 GB/s). Two tokens a warp would halve the reductions' lanes but not their number.
 //
 // Which experts are chosen is what exact arithmetic says, although scores are fp32: without bias and groups the ranking of the
 // logits themselves decides; otherwise a token whose ranking hangs on a difference within the fp32 error (about one in a
@@ -48,16 +52,17 @@ __device__ __forceinline__ float load(const void* p, long long i, int bf16) {
   return bf16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]) : reinterpret_cast<const float*>(p)[i];
 }
 
-// Order-preserving integer keys. 0 is below every number (even -inf) and means "not to be chosen"; NaN is the largest.
+// Order-preserving integer keys. 0 is below every number (even -inf) and means "not to be chosen"; NaN is the largest. The addition
+// makes a positive zero of a negative one: the two are equal.
 __device__ __forceinline__ uint32_t key_of(float v) {
-  const uint32_t b = __float_as_uint(v);
+  const uint32_t b = __float_as_uint(__fadd_rn(v, 0.f));
   return v != v ? 0xffffffffu : (b & 0x80000000u) ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float value_of(uint32_t k) {
   return __uint_as_float((k & 0x80000000u) ? k & 0x7fffffffu : ~k);
 }
 __device__ __forceinline__ unsigned long long key_of(double v) {
-  const unsigned long long b = __double_as_longlong(v);
+  const unsigned long long b = __double_as_longlong(__dadd_rn(v, 0.0));
   return v != v ? ~0ull : (b >> 63) ? ~b : b | (1ull << 63);
 }
 __device__ __forceinline__ uint32_t warp_max(uint32_t v) { return __reduce_max_sync(FULL, v); }

@@ -115,6 +115,18 @@ def test_route_ties_masks_and_extremes(gating, groups, top_groups, biased, devic
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("gating", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("groups", [1, 4])
+@pytest.mark.parametrize("biased", [False, True])
+def test_route_takes_zeros_of_both_signs_for_equal(gating, groups, biased, device):
+    x = torch.zeros(3, 32)
+    x[0, ::2] = -0.0
+    x[1, :16] = -0.0
+    x[2, 5] = -0.0
+    _check(x, 6, gating, torch.full((32,), -0.0) if biased else None, groups, 2 if groups > 1 else 1, 1, device)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("gating", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("groups", [1, 4])
 def test_route_with_nan_and_infinity_stays_in_range(gating, groups, device):
     x = _logits(5, 32, 7)
     x[0] = float("nan")
@@ -237,6 +249,14 @@ def test_route_refusals(device):
             route(torch.zeros(2, 1025, device=device), 2)
         with pytest.raises(ValueError, match="score_bias"):
             route(x, 2, score_bias=torch.zeros(32))
+
+
+@pytest.mark.gpu
+def test_what_the_kernels_entry_refuses_is_an_exception():
+    from olmo_core_b200.ops import _lib
+
+    with pytest.raises(RuntimeError, match="ocb_moe_route failed with code -1"):
+        _lib.native().route.default(torch.zeros(2, 4, device="cuda"), 9, False, None, 1, 1, 0)
 
 
 @pytest.mark.parametrize("device", DEVICES)
