@@ -140,11 +140,18 @@ Tensor aligned(const Tensor& m) {
     return fits ? m : m.clone(at::MemoryFormat::Contiguous);
 }
 
+// The kernels round 32-bit sizes up to tiles.
+void check_sizes(int64_t m, int64_t n, int64_t k) {
+    constexpr int64_t most = INT32_MAX - 512;
+    TORCH_CHECK_VALUE(m <= most && n <= most && k <= most, "the block-scaled product takes no dimension above ", most);
+}
+
 // `groups` stacked matrices [rows, cols]: their codes [rows, cols rounded up to 16] and behind them the scales of their tiles.
 Tensor tile_buffer(const Tensor& weight, int64_t groups) {
     const c10::cuda::OptionalCUDAGuard guard(weight.device());
     const Tensor w = matrix(weight, weight.size(1));
     const int64_t rows = w.size(0) / groups, cols = w.size(1), pitch = pitch_of(cols), codes = groups * rows * pitch;
+    check_sizes(rows, cols, groups);
     Tensor buffer = bytes(codes + 4 * groups * blocks(rows) * blocks(cols), w);
     if (rows == 0 || cols == 0) return buffer;
     uint8_t* at = buffer.mutable_data_ptr<uint8_t>();
@@ -174,7 +181,7 @@ Weight in_buffer(const Tensor& tiles, int64_t groups, int64_t rows, int64_t cols
 // x by rows times W (transposed or not); `columns`: also x by columns.
 Tensor product(const Tensor& x, const Weight& w, bool trans, const int* offsets, Tensor* columns, int64_t status) {
     const int64_t m = x.size(0), k = x.size(1), n = trans ? w.rows : w.cols;
-    TORCH_CHECK_VALUE(m <= INT32_MAX && k <= INT32_MAX && n <= INT32_MAX, "the block-scaled product takes sizes below 2^31");
+    check_sizes(m, n, k);
     Tensor out = at::empty({m, n}, x.options());
     const int64_t pitch = pitch_of(k), codes = m * pitch;
     if (columns != nullptr) *columns = bytes(codes + 4 * blocks(m) * k, x);

@@ -40,6 +40,7 @@ __all__ = ["BLOCK", "quantize_block_rows", "quantize_block_columns", "quantize_b
            "BlockFloat8LinearFunction", "BlockFloat8GroupedLinearFunction"]
 
 BLOCK = 128
+MAX_SIZE = 2 ** 31 - 513  # of any dimension: the kernels round 32-bit sizes up to tiles
 
 _lib_sigs_done = False
 
@@ -97,9 +98,15 @@ def _pitch(q: torch.Tensor) -> int:
     return q.stride(-2) if q.shape[-2] > 1 else (q.shape[-1] + 15) // 16 * 16
 
 
+def _check_sizes(t: torch.Tensor, what: str) -> None:
+    if any(n > MAX_SIZE for n in t.shape):
+        raise ValueError(f"{what} of shape {tuple(t.shape)} is too large: no dimension may exceed {MAX_SIZE}")
+
+
 def _check_matrix(x: torch.Tensor, what: str, dims: Tuple[int, ...] = (2,)) -> torch.Tensor:
     if x.dim() not in dims:
         raise ValueError(f"{what} must have {' or '.join(map(str, dims))} dimensions, got shape {tuple(x.shape)}")
+    _check_sizes(x, what)
     if x.dtype != torch.bfloat16:
         x = x.to(torch.bfloat16)
     return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
@@ -208,6 +215,7 @@ def _check_codes(q: torch.Tensor, what: str, dims: int) -> None:
         raise ValueError(f"{what} must have {dims} dimensions, got shape {tuple(q.shape)}")
     if q.dtype not in (torch.uint8, torch.float8_e4m3fn):
         raise ValueError(f"{what} must hold e4m3 bytes (uint8 or float8_e4m3fn), got {q.dtype}")
+    _check_sizes(q, what)
     if q.is_cuda and q.numel() and (
             (q.stride(-1) != 1 and q.shape[-1] > 1) or q.data_ptr() % 16
             or any(st % 16 for st, n in zip(q.stride()[:-1], q.shape[:-1]) if n > 1)):

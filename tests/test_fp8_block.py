@@ -379,3 +379,15 @@ def test_refusals(device):
         fb.fp8_block_grouped_linear(_rand((10, 100), 24, device), _rand((20, 100), 25, device), off)
     with pytest.raises(ValueError, match="dimensions"):
         fb.quantize_block_rows(_rand((2, 3, 4), 26, device))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_dimensions_beyond_32_bits_are_refused(device):
+    long = torch.zeros(1, 1, dtype=torch.bfloat16, device=device).expand(2 ** 31 - 100, 1)  # no memory behind it
+    w, codes = torch.ones(8, 1, dtype=torch.bfloat16, device=device), torch.zeros(1, 16, dtype=torch.uint8, device=device)
+    q, s = fb.quantize_block_tiles(w)
+    for call in (lambda: fb.quantize_block_rows(long), lambda: fb.quantize_block_columns(long), lambda: fb.quantize_block_tiles(long),
+                 lambda: fb.gemm_fp8_block(codes.expand(2 ** 31 - 100, 16), s, q, s), lambda: fb.fp8_block_matmul(long, q, s),
+                 lambda: fb.fp8_block_linear(long, w), lambda: fb.fp8_block_linear(w, long)):
+        with pytest.raises(ValueError, match="too large|no dimension above"):
+            call()
