@@ -9,19 +9,6 @@
 
 namespace ocb {
 
-// Programmatic dependent launch: a kernel launched with this attribute may start, as far as its own set-up, while the kernel in
-// front of it in the stream runs out. It calls previous_kernel_done() before its first access to global memory, and lets the
-// kernel behind it start the same way with next_kernel_may_start() (which takes effect once every CTA has called it).
-__device__ __forceinline__ void previous_kernel_done() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void next_kernel_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-
-inline cudaLaunchAttribute dependent_launch() {
-  cudaLaunchAttribute a;
-  a.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  a.val.programmaticStreamSerializationAllowed = 1;
-  return a;
-}
-
 namespace blkq {
 
 // Biased exponent of the scale of a block with the largest magnitude `amax`.

@@ -11,9 +11,11 @@
 // One CTA holds a 128 x 128 tile in registers (16 threads across, 16 down, each 8 rows of 8 columns): the maxima over a row
 // are shuffles within half a warp, those over a column go through shared memory. Rows and columns can come out of one launch,
 // which reads the tensor once where a layer needs both (the activations of a training step and the output gradient).
-// Memory bound: 2 bytes in, 1 byte out per orientation.
+// Memory bound: 2 bytes in, 1 byte out per orientation. 8192 x 11008: rows 55 us (4.9 TB/s), columns 51 (5.3), tiles 51 (5.3), rows
+// and columns together 86 (4.2, against 106 in two passes); the measured copy rate is 6.6 TB/s.
 
 #include "block_quant.cuh"
+#include "common.cuh"
 #include "ocb_api.h"
 
 namespace ocb {

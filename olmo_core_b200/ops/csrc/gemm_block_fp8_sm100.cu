@@ -6,8 +6,10 @@
 // through the whole reduction in fp32. The instruction takes one E8M0 exponent per row and K = 32 step, a byte of a 32-bit word
 // per row in tensor memory that it selects; all four steps of a block select the same byte here, so one word, and one set of
 // copies into tensor memory, serves four blocks. Adding scaled partial sums in registers instead, which would allow scales of any value, was measured
-// first: every block has to be read back from tensor memory, and 8192 x 11008 x 4096 took 403 us (and 625 us with a scale per
-// column of B) against 2 x 8192 x 11008 x 4096 operations in the tensor pipe.
+// first: every block has to be read back from tensor memory, and 8192 x 11008 x 4096 took 403 us (625 us with a scale per
+// column of B). This form takes 254 us, 2900 TFLOP/s and 1.76 of what cuBLAS measures in bf16; the input gradient takes 252 us, the
+// weight gradient 264 us. What bounds it is the tensor pipe (617 cycles per block and pair of 256 x 256 against 512 of the
+// instructions alone) and, in longer runs, the power limit: 280 us at the 1.39 GHz that it leaves.
 //
 // Both operands are addressed in place, whatever their orientation: a K-major operand (reduction contiguous) arrives as
 // [rows x 128 bytes] boxes, an MN-major one (rows of the product contiguous) as [128 k x 128 bytes] boxes, so the input
@@ -15,9 +17,11 @@
 // Scales are fp32 and read through strides, per row of an operand (index shift 0) or per 128 rows (shift 7); one that is no
 // positive power of two becomes NaN.
 //
-// CTA layout (384 threads): warp 0 = TMA producer, warp 1 = MMA issuer and tensor-memory owner, warps 2 and 3 = scales (they
-// fetch those of four blocks at a time, run up to twelve blocks ahead, and lay the exponents out as the tensor core wants them), warps 4..11 = epilogue (four lane quadrants x two column halves; through shared memory, so that global accesses are
-// whole 128-byte lines). All waits are bounded (common.cuh).
+// Two kernels: pairs of CTAs on 256 x 256 tiles for whatever fills the machine, and one CTA per 128-row tile (further down) for few
+// tokens and for products of few tiles. Roles of the pair kernel's 384 threads: warp 0 = TMA producer, warp 1 = MMA issuer and
+// tensor-memory owner, warps 2 and 3 = scales (they fetch those of four blocks at a time, run up to twelve blocks ahead, and lay
+// the exponents out as the tensor core wants them), warps 4..11 = epilogue (four lane quadrants x two column halves; through
+// shared memory, so that global accesses are whole 128-byte lines). All waits are bounded (common.cuh).
 
 #include <atomic>
 
@@ -42,21 +46,21 @@ constexpr int SF_BLOCK = 512;  // exponents of 128 rows for one batch
 
 enum : int { EPI_BF16 = 0, EPI_F32_ACC = 1, EPI_F32 = 2 };
 
-// CTAS = 2: a pair of CTAs (cta_group::2) computes 2 x 128 rows together; each stages its own rows of A and half of B.
-template <int BN, int CTAS>
-struct Tile {
-  static constexpr int B_ROWS = BN / CTAS;  // rows of B that one CTA stages
-  static constexpr int KB_BYTES = A_BYTES + B_ROWS * BKE;
-  static constexpr int STAGE_BYTES = KBS * KB_BYTES;  // [block][A rows, B rows]
-  static constexpr int STAGES = 3;
-  static constexpr int SF_BYTES = SF_BLOCK * (1 + (BN + 127) / 128);
-  static constexpr int ACCS = BN == 256 ? 1 : 2;     // accumulators in tensor memory
-  static constexpr uint32_t SF_COL = ACCS * BN;      // two alternating sets of scale columns: 4 of A, 4 per 128 columns of B
-  static constexpr uint32_t SF_COLS = SF_BYTES / SF_BLOCK * 4;
-  static constexpr int COLS = BN / 2;                // columns per epilogue thread
-  static constexpr int STG_BYTES = 16 * 128;         // staging of one epilogue warp: 16 rows x 128 bytes
-  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + SCALE_SLOTS * SF_BYTES + EPI_WARPS * STG_BYTES + 1024 /*alignment slack*/ + 256;
-};
+// A pair of CTAs (cta_group::2) computes a 256 x 256 tile; each stages its own 128 rows of A and half of B, so a block of the
+// reduction costs an SM 32 KB of loads for four times the work of a 128 x 128 tile. The accumulator takes 256 columns; a second one
+// would leave no room for the scales.
+constexpr int CTAS = 2;
+constexpr int BN = 256;
+constexpr int B_ROWS = BN / CTAS;  // rows of B that one CTA stages
+constexpr int KB_BYTES = A_BYTES + B_ROWS * BKE;
+constexpr int STAGE_BYTES = KBS * KB_BYTES;  // [block][A rows, B rows]
+constexpr int STAGES = 3;
+constexpr int SF_BYTES = SF_BLOCK * (1 + BN / 128);
+constexpr uint32_t SF_COL = BN;    // two alternating sets of scale columns: 4 of A, 4 per 128 columns of B
+constexpr uint32_t SF_COLS = SF_BYTES / SF_BLOCK * 4;
+constexpr int COLS = BN / 2;       // columns per epilogue thread
+constexpr int STG_BYTES = 16 * 128;  // staging of one epilogue warp: 16 rows x 128 bytes
+constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + SCALE_SLOTS * SF_BYTES + EPI_WARPS * STG_BYTES + 1024 /*alignment slack*/ + 256;
 
 struct Scales {
   const float* p;
@@ -87,9 +91,9 @@ struct TileInfo {
   int m0, m_end, n0, g;
 };
 
-// Walks the tiles (bm x bn) of one CTA or one pair.
-template <int bm, int bn, int CTAS>
+// Walks the tiles of one pair.
 struct Walker {
+  static constexpr int bm = BM * CTAS, bn = BN;
   const Params& p;
   int tiles_m, tiles_n, tile, g, base;
   __device__ Walker(const Params& params) : p(params), g(0), base(0) {
@@ -165,37 +169,26 @@ __device__ __forceinline__ void cluster_sync_all() {
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
-// Tiled loads of a CTA: into its own shared memory; of a pair, the bytes count on a barrier that may be the other CTA's.
-template <int CTAS>
-__device__ __forceinline__ void load_2d(void* smem_dst, const CUtensorMap* desc, uint64_t* bar, uint32_t pair_bar, int32_t c0,
-                                        int32_t c1) {
-  if (CTAS == 1) {
-    tma_load_2d(smem_dst, desc, bar, c0, c1);
-  } else {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-        ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(desc)), "r"(pair_bar), "r"(c0), "r"(c1)
-        : "memory");
-  }
+// Tiled loads of one CTA of a pair into its own shared memory; the bytes count on a barrier that may be the other CTA's.
+__device__ __forceinline__ void pair_load_2d(void* smem_dst, const CUtensorMap* desc, uint32_t pair_bar, int32_t c0, int32_t c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+      ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(desc)), "r"(pair_bar), "r"(c0), "r"(c1)
+      : "memory");
 }
-template <int CTAS>
-__device__ __forceinline__ void load_3d(void* smem_dst, const CUtensorMap* desc, uint64_t* bar, uint32_t pair_bar, int32_t c0,
-                                        int32_t c1, int32_t c2) {
-  if (CTAS == 1) {
-    tma_load_3d(smem_dst, desc, bar, c0, c1, c2);
-  } else {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-        ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(desc)), "r"(pair_bar), "r"(c0), "r"(c1), "r"(c2)
-        : "memory");
-  }
+__device__ __forceinline__ void pair_load_3d(void* smem_dst, const CUtensorMap* desc, uint32_t pair_bar, int32_t c0, int32_t c1,
+                                             int32_t c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+      ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(desc)), "r"(pair_bar), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
 }
-// D (+)= (A * SFA) (B * SFB)^T for K = 32 with E8M0 scales in tensor memory; issued by the one thread (of a pair: of the leader)
+// D (+)= (A * SFA) (B * SFB)^T for K = 32 with E8M0 scales in tensor memory, by one CTA or a pair (GROUP); issued by the one thread (of a pair: of the leader)
 // whose `issue` is set.
-template <int CTAS>
+template <int GROUP>
 __device__ __forceinline__ void umma(uint32_t tmem_d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t tsfa,
                                      uint32_t tsfb, uint32_t accumulate, uint32_t issue) {
-  if (CTAS == 1) {
+  if (GROUP == 1) {
     asm volatile(
         "{\n\t"
         ".reg .pred p, q;\n\t"
@@ -225,17 +218,17 @@ __device__ __forceinline__ void umma(uint32_t tmem_d, uint32_t a_lo, uint32_t b_
 }
 // 32 rows x 16 bytes of scales from shared memory into 4 columns, replicated to the four lane quadrants; of a pair, each CTA
 // copies from its own shared memory into its own tensor memory.
-template <int CTAS>
+template <int GROUP>
 __device__ __forceinline__ void sf_copy(uint32_t tmem_dst, uint32_t smem_src) {
   // no swizzle, 8-row x 16-byte core matrices every 128 bytes
   const uint64_t desc = static_cast<uint64_t>((smem_src >> 4) & 0x3FFFu) | (static_cast<uint64_t>(128u >> 4) << 32) | (1ull << 46);
-  if (CTAS == 1) asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem_dst), "l"(desc) : "memory");
+  if (GROUP == 1) asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem_dst), "l"(desc) : "memory");
   else asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem_dst), "l"(desc) : "memory");
 }
 // `bar` (and the other CTA's at the same offset) observes the completion of the MMAs issued so far.
-template <int CTAS>
+template <int GROUP>
 __device__ __forceinline__ void commit(uint64_t* bar) {
-  if (CTAS == 1) {
+  if (GROUP == 1) {
     umma_commit(bar);
   } else {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
@@ -319,21 +312,18 @@ __device__ __forceinline__ void stg_store(uint8_t* stg, uint8_t* dst0, long long
   }
 }
 
-template <int BN, int CTAS, int EPI>
+template <int EPI>
 __global__ void __launch_bounds__(THREADS, 1)
 gemm_block_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b, const Params p) {
-  using T = Tile<BN, CTAS>;
-  using Walk = Walker<BM * CTAS, BN, CTAS>;
-  constexpr int STAGES = T::STAGES, ACCS = T::ACCS, COLS = T::COLS, STAGE_BYTES = T::STAGE_BYTES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sf_smem = smem + STAGES * STAGE_BYTES;
-  uint8_t* stg_smem = sf_smem + SCALE_SLOTS * T::SF_BYTES;
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(stg_smem + EPI_WARPS * T::STG_BYTES);
+  uint8_t* stg_smem = sf_smem + SCALE_SLOTS * SF_BYTES;
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(stg_smem + EPI_WARPS * STG_BYTES);
   uint64_t* empty_bar = full_bar + STAGES;
   uint64_t* tfull_bar = empty_bar + STAGES;
-  uint64_t* tempty_bar = tfull_bar + ACCS;
-  uint64_t* sfull_bar = tempty_bar + ACCS;
+  uint64_t* tempty_bar = tfull_bar + 1;
+  uint64_t* sfull_bar = tempty_bar + 1;
   uint64_t* sempty_bar = sfull_bar + SCALE_SLOTS;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sempty_bar + SCALE_SLOTS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -341,7 +331,7 @@ gemm_block_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const int num_kb = (p.K + BKE - 1) / BKE;
-  const uint32_t cta = CTAS == 2 ? cluster_ctarank() : 0u;  // 0 = leader of the pair
+  const uint32_t cta = cluster_ctarank();  // 0 = leader of the pair
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -349,13 +339,11 @@ gemm_block_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
       mbar_init(&empty_bar[s], 1);
     }
     for (int i = 0; i < SCALE_SLOTS; ++i) {
-      mbar_init(&sfull_bar[i], 2 * CTAS);  // the scale warps (of both CTAs)
+      mbar_init(&sfull_bar[i], 2 * CTAS);  // the scale warps of both CTAs
       mbar_init(&sempty_bar[i], 1);
     }
-    for (int a = 0; a < ACCS; ++a) {
-      mbar_init(&tfull_bar[a], 1);
-      mbar_init(&tempty_bar[a], EPI_WARPS * CTAS);
-    }
+    mbar_init(tfull_bar, 1);
+    mbar_init(tempty_bar, EPI_WARPS * CTAS);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -364,19 +352,14 @@ gemm_block_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
     tma_prefetch_desc(&tma_b);
   }
   if (warp == 1) {
-    if (CTAS == 1) {
-      tmem_alloc(tmem_slot, TMEM_COLS);
-      tmem_relinquish();
-    } else {
-      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(TMEM_COLS) : "memory");
-      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-    }
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(TMEM_COLS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
   previous_kernel_done();
   tc_fence_before();
   __syncthreads();
   next_kernel_may_start();  // after this CTA has its tensor memory: one of the next kernel never waits for it with that in hand
-  if (CTAS == 2) cluster_sync_all();  // the other CTA's barriers are initialised before anything is signalled across
+  cluster_sync_all();  // the other CTA's barriers are initialised before anything is signalled across
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
@@ -386,26 +369,26 @@ gemm_block_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
-      Walk walker(p);
+      Walker walker(p);
       TileInfo t;
       while (ok && walker.next(t)) {
-        const int m0 = t.m0 + static_cast<int>(cta) * BM, n0 = t.n0 + static_cast<int>(cta) * T::B_ROWS;
+        const int m0 = t.m0 + static_cast<int>(cta) * BM, n0 = t.n0 + static_cast<int>(cta) * B_ROWS;
         for (int kb = 0; kb < num_kb; kb += KBS) {
           ok = wait_for(&empty_bar[stage], phase ^ 1u, abort_flag, p.status, kStatusTimeoutProducer);
           if (!ok) break;
           const int blocks = min(KBS, num_kb - kb);
-          if (cta == 0) mbar_arrive_expect_tx(&full_bar[stage], CTAS * T::KB_BYTES * blocks);
-          const uint32_t pair_bar = CTAS == 2 ? map_to_cta(smem_u32(&full_bar[stage]), 0) : 0u;
+          if (cta == 0) mbar_arrive_expect_tx(&full_bar[stage], CTAS * KB_BYTES * blocks);
+          const uint32_t pair_bar = map_to_cta(smem_u32(&full_bar[stage]), 0);
           for (int j = 0; j < blocks; ++j) {
-            uint8_t* sa = smem + stage * STAGE_BYTES + j * T::KB_BYTES;
+            uint8_t* sa = smem + stage * STAGE_BYTES + j * KB_BYTES;
             uint8_t* sb = sa + A_BYTES;
             const int k0 = (kb + j) * BKE;
             // innermost coordinates are k0 (K-major) or tile origins (MN-major): multiples of 128 bytes either way; group
             // boundaries only enter the outer coordinate of a K-major A
-            if (p.a_mn) load_2d<CTAS>(sa, &tma_a, &full_bar[stage], pair_bar, m0, k0);
-            else load_2d<CTAS>(sa, &tma_a, &full_bar[stage], pair_bar, k0, m0);
-            if (p.b_mn) load_3d<CTAS>(sb, &tma_b, &full_bar[stage], pair_bar, n0, k0, t.g);
-            else load_3d<CTAS>(sb, &tma_b, &full_bar[stage], pair_bar, k0, n0, t.g);
+            if (p.a_mn) pair_load_2d(sa, &tma_a, pair_bar, m0, k0);
+            else pair_load_2d(sa, &tma_a, pair_bar, k0, m0);
+            if (p.b_mn) pair_load_3d(sb, &tma_b, pair_bar, n0, k0, t.g);
+            else pair_load_3d(sb, &tma_b, pair_bar, k0, n0, t.g);
           }
           if (++stage == STAGES) { stage = 0; phase ^= 1u; }
         }
@@ -415,7 +398,7 @@ gemm_block_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
       }
     }
   } else if (warp == 1) {
-    // ------------------------------------------------------------------ issuer (of a pair: the leader's)
+    // ------------------------------------------------------------------ issuer (the leader's)
     // The whole warp walks the loop, so that descriptors can live in uniform registers; one lane issues.
     if (cta == 0) {
       const uint32_t issue = lane == 0;
@@ -430,30 +413,29 @@ gemm_block_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
       const uint32_t a_lo0 = desc_lo_sw128(smem_u32(smem), 16);
       const uint32_t b_lo0 = desc_lo_sw128(smem_u32(smem) + A_BYTES, 16);
       const uint32_t sf0 = smem_u32(sf_smem);
-      int stage = 0, acc = 0, slot = 0;
+      int stage = 0, slot = 0;
       uint32_t phase = 0, acc_phase = 0, slot_phase = 0;
       // the two sets of scale columns take turns
-      uint32_t tsfa = tmem_base + T::SF_COL;
-      const uint32_t sf_flip = tsfa ^ (tsfa + T::SF_COLS);
+      uint32_t tsfa = tmem_base + SF_COL;
+      const uint32_t sf_flip = tsfa ^ (tsfa + SF_COLS);
       bool ok = true;
-      Walk walker(p);
+      Walker walker(p);
       TileInfo t;
       while (ok && walker.next(t)) {
-        ok = wait_for(&tempty_bar[acc], acc_phase ^ 1u, abort_flag, p.status, kStatusTimeoutMma);
+        ok = wait_for(tempty_bar, acc_phase ^ 1u, abort_flag, p.status, kStatusTimeoutMma);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t d_tmem = tmem_base + acc * BN;
         for (int kb = 0; kb < num_kb; kb += KBS) {
           const bool first_of_batch = (kb & (SCALE_BATCH - 1)) == 0;
           if (first_of_batch) {  // copies and MMAs of one thread execute in issue order
             ok = wait_for(&sfull_bar[slot], slot_phase, abort_flag, p.status, kStatusTimeoutMma);
             if (!ok) break;
             tc_fence_after();
-            const uint32_t ss = sf0 + slot * T::SF_BYTES;
+            const uint32_t ss = sf0 + slot * SF_BYTES;
             if (issue) {
               sf_copy<CTAS>(tsfa, ss);
 #pragma unroll
-              for (uint32_t b = 0; b < (BN + 127) / 128; ++b) sf_copy<CTAS>(tsfa + 4 + 4 * b, ss + SF_BLOCK * (1 + b));
+              for (uint32_t b = 0; b < BN / 128; ++b) sf_copy<CTAS>(tsfa + 4 + 4 * b, ss + SF_BLOCK * (1 + b));
             }
           }
           ok = wait_for(&full_bar[stage], phase, abort_flag, p.status, kStatusTimeoutMma);
@@ -464,14 +446,14 @@ gemm_block_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
           uint32_t id = idesc + byte0 * ((1u << 29) | (1u << 4)), ta = tsfa + (byte0 << 30), tb = ta + 4;
 #pragma unroll
           for (uint32_t k = 0; k < BKE / 32; ++k)
-            umma<CTAS>(d_tmem, a_lo + k * a_step, b_lo + k * b_step, kDescHi, id, ta, tb, (kb | static_cast<int>(k)) != 0, issue);
+            umma<CTAS>(tmem_base, a_lo + k * a_step, b_lo + k * b_step, kDescHi, id, ta, tb, (kb | static_cast<int>(k)) != 0, issue);
           if (kb + 1 < num_kb) {
             id += (1u << 29) | (1u << 4);
             ta += 1u << 30;
             tb += 1u << 30;
 #pragma unroll
             for (uint32_t k = 0; k < BKE / 32; ++k)
-              umma<CTAS>(d_tmem, a_lo + (T::KB_BYTES >> 4) + k * a_step, b_lo + (T::KB_BYTES >> 4) + k * b_step, kDescHi, id, ta, tb, 1u, issue);
+              umma<CTAS>(tmem_base, a_lo + (KB_BYTES >> 4) + k * a_step, b_lo + (KB_BYTES >> 4) + k * b_step, kDescHi, id, ta, tb, 1u, issue);
           }
           if (issue) commit<CTAS>(&empty_bar[stage]);
           if (++stage == STAGES) { stage = 0; phase ^= 1u; }
@@ -481,19 +463,19 @@ gemm_block_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
             if (++slot == SCALE_SLOTS) { slot = 0; slot_phase ^= 1u; }
           }
         }
-        if (ok && issue) commit<CTAS>(&tfull_bar[acc]);
-        if (++acc == ACCS) { acc = 0; acc_phase ^= 1u; }
+        if (ok && issue) commit<CTAS>(tfull_bar);
+        acc_phase ^= 1u;
       }
     }
   } else if (warp < 4) {
     // ------------------------------------------------------------------ scales (warps 2 and 3)
     const int t64 = threadIdx.x - 64;
     constexpr int PER = (BM + BN) / 64;  // rows whose scales a thread carries: t64 + 64 i of A, then of B
-    const uint32_t sfull_leader = CTAS == 2 ? map_to_cta(smem_u32(sfull_bar), 0) : 0u;
+    const uint32_t sfull_leader = map_to_cta(smem_u32(sfull_bar), 0);
     int slot = 0;
     uint32_t phase = 0;
     bool ok = true;
-    Walk walker(p);
+    Walker walker(p);
     TileInfo t;
     while (ok && walker.next(t)) {
       const float* src[PER];
@@ -530,7 +512,7 @@ gemm_block_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
         ok = wait_for(&sempty_bar[slot], phase ^ 1u, abort_flag, p.status, kStatusTimeoutProducer);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        uint32_t* dst = reinterpret_cast<uint32_t*>(sf_smem + slot * T::SF_BYTES);
+        uint32_t* dst = reinterpret_cast<uint32_t*>(sf_smem + slot * SF_BYTES);
 #pragma unroll
         for (int i = 0; i < PER; ++i) {  // row r of a 128-row block: 32-bit word 4 (r % 32) + r / 32 of its 512 bytes
           const int f = t64 + 64 * i;
@@ -538,40 +520,33 @@ gemm_block_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
         }
         fence_proxy_async_smem();  // the tensor core's copy reads what the threads wrote
         __syncwarp();
-        if (lane == 0) {
-          if (CTAS == 1) mbar_arrive(&sfull_bar[slot]);
-          else mbar_arrive_cluster(sfull_leader + slot * 8);
-        }
+        if (lane == 0) mbar_arrive_cluster(sfull_leader + slot * 8);
         if (++slot == SCALE_SLOTS) { slot = 0; phase ^= 1u; }
       }
     }
   } else {
     // ------------------------------------------------------------------ epilogue
     const int quad = warp & 3, half = (warp - 4) >> 2;
-    uint8_t* stg = stg_smem + (warp - 4) * T::STG_BYTES;
+    uint8_t* stg = stg_smem + (warp - 4) * STG_BYTES;
     const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + half * COLS;
-    const uint32_t tempty_leader = CTAS == 2 ? map_to_cta(smem_u32(tempty_bar), 0) : 0u;
-    int acc = 0;
+    const uint32_t tempty_leader = map_to_cta(smem_u32(tempty_bar), 0);
     uint32_t acc_phase = 0;
     bool ok = true;
-    Walk walker(p);
+    Walker walker(p);
     TileInfo t;
     while (ok && walker.next(t)) {
-      ok = wait_for(&tfull_bar[acc], acc_phase, abort_flag, p.status, kStatusTimeoutEpilogue);
+      ok = wait_for(tfull_bar, acc_phase, abort_flag, p.status, kStatusTimeoutEpilogue);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
       uint32_t r[COLS / 32][32];
 #pragma unroll
-      for (int c = 0; c < COLS / 32; ++c) tmem_ld_32x32(t_row + acc * BN + c * 32, r[c]);
+      for (int c = 0; c < COLS / 32; ++c) tmem_ld_32x32(t_row + c * 32, r[c]);
 #pragma unroll
       for (int c = 0; c < COLS / 32; ++c) tmem_ld_wait_for(r[c]);
       tc_fence_before();  // the accumulator is in registers: the issuer may start the next tile
-      if (lane == 0) {
-        if (CTAS == 1) mbar_arrive(&tempty_bar[acc]);
-        else mbar_arrive_cluster(tempty_leader + acc * 8);
-      }
-      if (++acc == ACCS) { acc = 0; acc_phase ^= 1u; }
+      if (lane == 0) mbar_arrive_cluster(tempty_leader);
+      acc_phase ^= 1u;
       const int row0 = t.m0 + static_cast<int>(cta) * BM + quad * 32, col0 = t.n0 + half * COLS;
       const int rows = min(32, t.m_end - row0);
       if (rows <= 0) continue;
@@ -611,11 +586,10 @@ gemm_block_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
 
   tc_fence_before();
   __syncthreads();
-  if (CTAS == 2) cluster_sync_all();  // nothing of the other CTA signals into this one's shared memory any more
+  cluster_sync_all();  // nothing of the other CTA signals into this one's shared memory any more
   if (warp == 1) {
     __syncwarp();
-    if (CTAS == 1) tmem_dealloc(tmem_base, TMEM_COLS);
-    else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
   }
 }
 
@@ -627,8 +601,13 @@ gemm_block_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
 // every time). Groups (SWAP only): a CTA finds its group and its tokens from the device-side boundaries.
 //
 // FUSED (SWAP, up to 16 tokens a tile): the tokens arrive in bf16, and the warps of the epilogue, which have nothing else to do
-// before the end, quantise them straight into the stages beside the weight's codes. Every CTA does that for its part of the reduction, out of L2; in exchange there is no quantiser
-// launch in front, which for one token costs as much as a quarter of the product (4096 x 11008: 2.4 + 12.2 us).
+// before the end, quantise them straight into the stages beside the weight's codes. Every CTA does that for its part of the
+// reduction, out of L2; in exchange there is no quantiser launch in front (one token against 4096 x 11008, with the host: 18.4 us
+// with the launch, 14.4 without; two scale warps in place of the epilogue's took 16.8).
+//
+// What bounds it: the weight's bytes (one token against 4096 x 11008: 12.8 us, 3.5 TB/s, against 6.9 us at the measured copy
+// rate), and about 4.4 us in which barriers, tensor memory and tensor maps are set up, the first loads arrive, and the parts are
+// added. 64 experts of 1024 x 2048 for 128 rows: 28.5 us, 4.7 TB/s.
 constexpr int SMALL_THREADS = 256;  // warps as above, with one epilogue warpgroup
 
 template <int BN>
@@ -1051,10 +1030,10 @@ static bool allow_smem(Kernel kernel, int bytes, std::atomic<uint64_t>& done, in
   return true;
 }
 
-template <int BN, int CTAS, int EPI>
+template <int EPI>
 static int launch(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, long long max_tiles, int dev, cudaStream_t stream) {
-  constexpr int bytes = Tile<BN, CTAS>::SMEM_BYTES;
-  auto kernel = gemm_block_fp8_kernel<BN, CTAS, EPI>;
+  constexpr int bytes = SMEM_BYTES;
+  auto kernel = gemm_block_fp8_kernel<EPI>;
   static std::atomic<uint64_t> done;
   if (!allow_smem(kernel, bytes, done, dev)) return -3;
   const int units = num_sms(dev) / CTAS;
@@ -1069,16 +1048,15 @@ static int launch(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p,
   attributes[1].val.clusterDim.x = CTAS;
   attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
   config.attrs = attributes;
-  config.numAttrs = CTAS == 2 ? 2 : 1;
+  config.numAttrs = 2;
   return cudaLaunchKernelEx(&config, kernel, ta, tb, p) == cudaSuccess ? 0 : -4;
 }
 
-template <int BN, int CTAS>
 static int launch_epi(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, long long max_tiles, int epi, int dev, cudaStream_t s) {
   switch (epi) {
-    case EPI_BF16: return launch<BN, CTAS, EPI_BF16>(ta, tb, p, max_tiles, dev, s);
-    case EPI_F32_ACC: return launch<BN, CTAS, EPI_F32_ACC>(ta, tb, p, max_tiles, dev, s);
-    case EPI_F32: return launch<BN, CTAS, EPI_F32>(ta, tb, p, max_tiles, dev, s);
+    case EPI_BF16: return launch<EPI_BF16>(ta, tb, p, max_tiles, dev, s);
+    case EPI_F32_ACC: return launch<EPI_F32_ACC>(ta, tb, p, max_tiles, dev, s);
+    case EPI_F32: return launch<EPI_F32>(ta, tb, p, max_tiles, dev, s);
     default: return -1;
   }
 }
@@ -1090,14 +1068,6 @@ static bool make_map(CUtensorMap* out, const void* ptr, bool mn, uint64_t rows, 
   const uint32_t box[3] = {128, static_cast<uint32_t>(mn ? BKE : box_rows), 1};
   return encode_tensor_map(out, ptr, rank, dims, str, box, 1);
 }
-
-}  // namespace blk
-}  // namespace ocb
-
-using namespace ocb;
-
-namespace ocb {
-namespace blk {
 
 template <int BN, bool SWAP, bool FUSED = false>
 static int launch_small(const CUtensorMap& ta, const CUtensorMap& tb, const SmallParams& p, long long tiles, int dev, cudaStream_t stream) {
@@ -1149,12 +1119,11 @@ static int run_pair(const Product& x, int dev, cudaStream_t stream) {
   p.offsets = x.offsets;
   p.num_groups = x.groups;
   p.status = x.status;
-  constexpr int BN = 256, CTAS = 2;
   CUtensorMap ta, tb;
   if (!make_map(&ta, x.A, x.a_mn != 0, x.M, x.K, 1, x.lda, 0, BM, 2)) return -1001;
-  if (!make_map(&tb, x.B, x.b_mn != 0, x.N, x.K, x.groups, x.ldb, x.groups > 1 ? x.b_group_bytes : x.ldb, BN / CTAS, 3)) return -2001;
+  if (!make_map(&tb, x.B, x.b_mn != 0, x.N, x.K, x.groups, x.ldb, x.groups > 1 ? x.b_group_bytes : x.ldb, B_ROWS, 3)) return -2001;
   const long long tiles_m = (x.M + BM * CTAS - 1) / (BM * CTAS) + (x.offsets != nullptr ? x.groups : 0);
-  return launch_epi<BN, CTAS>(ta, tb, p, tiles_m * ((x.N + BN - 1) / BN), x.epi, dev, stream);
+  return launch_epi(ta, tb, p, tiles_m * ((x.N + BN - 1) / BN), x.epi, dev, stream);
 }
 
 // swap: the rows of B take the 128-row side and the rows of A the side of bn.
@@ -1260,6 +1229,8 @@ static int run(const Product& x, cudaStream_t stream) {
 }  // namespace blk
 }  // namespace ocb
 
+using namespace ocb;
+
 static int gemm_block_fp8(const void* A, const void* x, long long ldx, const void* B, void* C, const float* sa, const float* sb,
                           const int* offsets, int num_groups, int M, int N, int K, long long lda, long long ldb, long long ldc,
                           long long b_group_bytes, long long sa_k, long long sa_i, int sa_shift, long long sb_k, long long sb_i,
@@ -1268,6 +1239,8 @@ static int gemm_block_fp8(const void* A, const void* x, long long ldx, const voi
   if ((lda % 16) != 0 || (ldb % 16) != 0 || (b_group_bytes % 16) != 0 || (reinterpret_cast<uintptr_t>(A) & 15) ||
       (reinterpret_cast<uintptr_t>(B) & 15) || (A != nullptr && sa == nullptr) || sb == nullptr)
     return -1;
+  // sizes are rounded up to tiles in 32 bits
+  if (M > 0x7fffffff - 512 || N > 0x7fffffff - 512 || K > 0x7fffffff - 512) return -1;
   if ((sa_shift != 0 && sa_shift != 7) || (sb_shift != 0 && sb_shift != 7) || (offsets != nullptr && a_mn)) return -1;
   if (epilogue < blk::EPI_BF16 || epilogue > blk::EPI_F32) return -1;
   blk::Product p;

@@ -54,7 +54,8 @@ int ocb_quantize_block_fp8(const void* x, void* q_row, float* s_row, void* q_col
                            int groups, int rows, int cols, long long ldx, long long ldq, long long x_group,
                            long long q_group, cudaStream_t stream);
 // C[M, N] (=|+=) sum over blocks kb of 128: sa * sb * A_kb B_kb^T. A: [M, K], or stored [K, M] (a_mn); B: [N, K], or stored
-// [K, N] (b_mn). Scale of (kb, row i): s[kb * s_k + (i >> shift) * s_i], shift 0 or 7. With `offsets` (int32 [num_groups + 1])
+// [K, N] (b_mn). Scale of (kb, row i): s[kb * s_k + (i >> shift) * s_i], shift 0 or 7, a positive power of two (any other value
+// makes the products NaN). With `offsets` (int32 [num_groups + 1])
 // the rows of A and C belong to groups, group g uses the B at b_group_bytes * g and the scales at sb + sb_g * g; rows outside
 // every group stay as they are. epilogue: 0 = bf16 store, 1 = fp32 accumulate, 2 = fp32 store.
 int ocb_gemm_block_fp8(const void* A, const void* B, void* C, const float* sa, const float* sb, const int* offsets,
