@@ -228,3 +228,28 @@ def test_training_step_in_a_graph_and_on_other_streams(tokens):
     torch.cuda.synchronize()
     for a, (_, b) in zip(want, graphs):
         assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_layers_and_routing_under_activation_checkpointing(device):
+    from torch.utils.checkpoint import checkpoint
+
+    from olmo_core_b200.ops import fp8_block as fb
+    from olmo_core_b200.ops.moe import route
+
+    gen = torch.Generator().manual_seed(3)
+    x, w, wr = (torch.randn(*shape, generator=gen).to(device, torch.bfloat16) for shape in ((200, 64), (64, 64), (8, 64)))
+
+    def block(x, w, wr):
+        h = fb.fp8_block_linear(x, w)
+        weights, experts, _, _ = route((h @ wr.t()).float(), 2, normalize=1)
+        return (h.float() * weights.gather(1, experts.argsort(1)).sum(1, keepdim=True)).sum()
+
+    grads = []
+    for wrapped in (False, True):
+        leaves = [t.clone().requires_grad_(True) for t in (x, w, wr)]
+        loss = checkpoint(block, *leaves, use_reentrant=False) if wrapped else block(*leaves)
+        loss.backward()
+        grads.append([loss.detach()] + [t.grad for t in leaves])
+    for a, b in zip(*grads):
+        assert torch.equal(a, b)
