@@ -25,6 +25,14 @@
 //   EPI_SWIGLU_BWD  the GEMM computes dh = dy W2 ([M, H]); the epilogue reads a and b from AB [M, 2H] and stores
 //                   da = dh * b * silu'(a), db = dh * silu(a) into C [M, 2H] and the recomputed h into C2 [M, H]
 //                   (when C2 is given), so dh never reaches memory.
+//
+// Grouped over the reduction (GROUPED; the experts' weight gradients dW_g = dy_g^T x_g): a tile's reduction is the rows of its
+// group, whose boundaries are read on the device. Groups differ in length, so their tiles are dealt out in falling order of
+// length, to the pairs forwards and backwards in turn (with loads spread as exp(1.2 N(0, 1)) over 64 groups the busiest pair has
+// 1.08 to 1.3 times the mean; 1.3 to 1.6 times in the groups' own order). The last block of a group
+// reaches into the next one's rows; a warp of its own in each CTA blanks those lines in shared memory. For that the loads
+// of such a block count on a barrier of the CTA itself, and "stage full" in the leader counts one arrival per CTA: by the
+// producer when it has issued its loads, or, for a last block, by the blanking warp when it is done.
 
 #include <mutex>
 
@@ -49,6 +57,9 @@ constexpr int STAGE_BYTES = A_STAGE_BYTES + B_STAGE_BYTES;
 constexpr int EPI_STAGING_BYTES = 4 * 2 * 32 * 128;  // four epilogue warps, two 32-row x 128-byte buffers each
 constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_STAGING_BYTES + 1024 /*alignment slack*/ + 256 /*barriers*/;
 constexpr int THREADS = 192;
+constexpr int GROUPED_THREADS = THREADS + 32;  // and the blanking warp
+constexpr int SORTED_GROUPS = 256;              // up to this many groups are sorted by length
+constexpr int GROUPED_SMEM_BYTES = SMEM_BYTES + SORTED_GROUPS * 4;
 constexpr int TMEM_COLS = 512;
 
 enum : int { EPI_BF16 = 0, EPI_F32_ACC = 1, EPI_F32 = 2, EPI_BF16_ACC = 3, EPI_SWIGLU_FWD = 5, EPI_SWIGLU_BWD = 6 };
@@ -64,6 +75,8 @@ struct Params {
   int H;        // fused epilogues: row offset of w3 inside B and column offset of b / db inside C
   int group_m;
   int* status;
+  const int* offsets;  // GROUPED: [num_groups + 1] reduction boundaries of the groups; C holds num_groups matrices [M, N]
+  int num_groups;
 };
 
 // ---- cluster helpers ---------------------------------------------------------------------------------------------
@@ -84,6 +97,10 @@ __device__ __forceinline__ void cluster_sync_all() {
 // Arrive on an mbarrier of any CTA of the cluster (address from map_to_cta).
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// The same where nothing this thread wrote has to be seen by the one that waits.
+__device__ __forceinline__ void mbar_arrive_issued(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 // Tiled TMA load of a CTA pair: the destination is this CTA's shared memory, the completion bytes are counted on
 // `bar_cluster_addr`, which may belong to the other CTA of the pair.
@@ -136,6 +153,45 @@ __device__ __forceinline__ void tile_coords(int tile, int tiles_m, int tiles_n, 
   tn = r / gm;
 }
 
+// Where a tile lies.
+struct TilePos {
+  int tm, tn;
+  int k0, num_kb;    // first reduction row and number of BK-deep blocks (GROUPED: 0 for a group without rows)
+  int k_tail;        // reduction rows of the last block
+  long long c_row0;  // first row of the matrix it belongs to
+};
+__device__ __forceinline__ int group_rows(const Params& p, int g) {
+  const int lo = min(max(p.offsets[g], 0), p.K);
+  return max(min(p.offsets[g + 1], p.K) - lo, 0);
+}
+template <bool GROUPED>
+__device__ __forceinline__ TilePos tile_pos(const Params& p, int tile, int tiles_m, int tiles_n, const int16_t* order) {
+  TilePos t;
+  if (GROUPED) {
+    const int per_group = tiles_m * tiles_n, at = tile / per_group, local = tile - at * per_group;
+    const int g = p.num_groups <= SORTED_GROUPS ? order[at] : at;
+    const int lo = min(max(p.offsets[g], 0), p.K), rows = group_rows(p, g);
+    t.tm = local % tiles_m;
+    t.tn = local / tiles_m;
+    t.k0 = lo;
+    t.num_kb = (rows + BK - 1) / BK;
+    t.k_tail = rows - (t.num_kb - 1) * BK;
+    t.c_row0 = static_cast<long long>(g) * p.M;
+  } else {
+    tile_coords(tile, tiles_m, tiles_n, p.group_m, t.tm, t.tn);
+    t.k0 = 0;
+    t.num_kb = (p.K + BK - 1) / BK;
+    t.k_tail = BK;
+    t.c_row0 = 0;
+  }
+  return t;
+}
+
+// The tile of a pair in a round of tiles: GROUPED goes back and forth, so that no pair always gets the longest of a round.
+template <bool GROUPED>
+__device__ __forceinline__ int tile_of(int round, int pair, int num_pairs) {
+  return round * num_pairs + (GROUPED && (round & 1) ? num_pairs - 1 - pair : pair);
+}
 
 // ---- epilogue staging ------------------------------------------------------------------------------------------------
 constexpr int STG_BYTES = 32 * 128;  // one warp's 32 rows x 128 bytes
@@ -237,8 +293,8 @@ __device__ __forceinline__ void ab_stash(const uint4 (&va)[8], const uint4 (&vb)
 
 __device__ __forceinline__ float silu_f(float a) { return __fdividef(a, 1.f + __expf(-a)); }
 
-template <int A_MN, int B_MN, int EPI>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+template <int A_MN, int B_MN, int EPI, bool GROUPED = false>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GROUPED ? GROUPED_THREADS : THREADS, 1)
 gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b, const Params p) {
   constexpr int TILE_N = EPI == EPI_SWIGLU_FWD ? BNH : BN;  // columns of p.N one pair tile covers
   extern __shared__ uint8_t smem_raw[];
@@ -247,8 +303,11 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
   uint64_t* empty_bar = full_bar + STAGES;
   uint64_t* tfull_bar = empty_bar + STAGES;
   uint64_t* tempty_bar = tfull_bar + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty_bar + 2);
+  uint64_t* tail_bar = tempty_bar + 2;  // GROUPED: this CTA's loads of a group's last block
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tail_bar + STAGES);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int16_t* order = reinterpret_cast<int16_t*>(full_bar + 32);  // GROUPED: groups in falling order of their lengths
+  uint16_t* length = reinterpret_cast<uint16_t*>(order + SORTED_GROUPS);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -257,8 +316,9 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&full_bar[s], 1);
+      mbar_init(&full_bar[s], GROUPED ? 2 : 1);
       mbar_init(&empty_bar[s], 1);
+      if (GROUPED) mbar_init(&tail_bar[s], 1);
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&tfull_bar[a], 1);
@@ -275,6 +335,16 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
     tmem_alloc_pair(tmem_slot, TMEM_COLS);
     tmem_relinquish_pair();
   }
+  if (GROUPED && p.num_groups <= SORTED_GROUPS) {
+    for (int g = threadIdx.x; g < p.num_groups; g += GROUPED_THREADS)
+      length[g] = static_cast<uint16_t>(min((group_rows(p, g) + BK - 1) / BK, 65535));
+    __syncthreads();
+    for (int g = threadIdx.x; g < p.num_groups; g += GROUPED_THREADS) {
+      int ahead = 0;
+      for (int h = 0; h < p.num_groups; ++h) ahead += length[h] > length[g] || (length[h] == length[g] && h < g);
+      order[ahead] = static_cast<int16_t>(g);
+    }
+  }
   tc_fence_before();
   __syncthreads();
   cluster_sync_all();  // the other CTA's barriers are initialised before anything is signalled across
@@ -283,8 +353,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
 
   const int tiles_m = (p.M + 2 * BM - 1) / (2 * BM);
   const int tiles_n = (p.N + TILE_N - 1) / TILE_N;
-  const int num_tiles = tiles_m * tiles_n;
-  const int num_kb = (p.K + BK - 1) / BK;
+  const int num_tiles = tiles_m * tiles_n * (GROUPED ? p.num_groups : 1);
 
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer (both CTAs)
@@ -292,10 +361,12 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int tile = pair; ok && tile < num_tiles; tile += num_pairs) {
-        int tm, tn;
-        tile_coords(tile, tiles_m, tiles_n, p.group_m, tm, tn);
-        const int m0 = tm * (2 * BM) + static_cast<int>(cta) * BM;
+      for (int round = 0; ok && round * num_pairs < num_tiles; ++round) {
+        const int tile = tile_of<GROUPED>(round, pair, num_pairs);
+        if (tile >= num_tiles) continue;
+        const TilePos t = tile_pos<GROUPED>(p, tile, tiles_m, tiles_n, order);
+        const int tn = t.tn, num_kb = t.num_kb;
+        const int m0 = t.tm * (2 * BM) + static_cast<int>(cta) * BM;
         // B rows of this CTA: its half of the 256 columns, or (fused forward) the same 128 columns of w1 / w3
         const int n0 = EPI == EPI_SWIGLU_FWD ? tn * BNH + static_cast<int>(cta) * p.H : tn * BN + static_cast<int>(cta) * BNH;
         for (int kb = 0; kb < num_kb; ++kb) {
@@ -303,9 +374,16 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
           if (!ok) break;
           uint8_t* sa = smem + stage * STAGE_BYTES;
           uint8_t* sb = sa + A_STAGE_BYTES;
-          const uint32_t bar = map_to_cta(smem_u32(&full_bar[stage]), 0);
-          if (cta == 0) mbar_arrive_expect_tx(&full_bar[stage], 2 * STAGE_BYTES);
-          const int k0 = kb * BK;
+          uint32_t bar = map_to_cta(smem_u32(&full_bar[stage]), 0);
+          if (GROUPED && kb == num_kb - 1 && t.k_tail < BK) {
+            bar = map_to_cta(smem_u32(&tail_bar[stage]), cta);
+            mbar_arrive_expect_tx(&tail_bar[stage], STAGE_BYTES);
+          } else if (cta == 0) {
+            mbar_arrive_expect_tx(&full_bar[stage], 2 * STAGE_BYTES);
+          } else if (GROUPED) {
+            mbar_arrive_issued(bar);
+          }
+          const int k0 = t.k0 + kb * BK;
           if (A_MN == 0) {
             tma_load_2d_pair(sa, &tma_a, bar, k0, m0);
           } else {
@@ -341,9 +419,14 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
       uint32_t phase = 0;
       bool ok = true;
       int it = 0;
-      for (int tile = pair; ok && tile < num_tiles; tile += num_pairs, ++it) {
+      for (int round = 0; ok && round * num_pairs < num_tiles; ++round) {
+        const int tile = tile_of<GROUPED>(round, pair, num_pairs);
+        if (tile >= num_tiles) continue;
+        const int num_kb = tile_pos<GROUPED>(p, tile, tiles_m, tiles_n, order).num_kb;
+        if (GROUPED && num_kb == 0) continue;  // nothing to add up: the epilogue needs no accumulator
         const int acc = it & 1;
         const uint32_t acc_phase = (it >> 1) & 1;
+        ++it;
         ok = mbar_wait_bounded(&tempty_bar[acc], acc_phase ^ 1u, abort_flag, p.status, kStatusTimeoutMma);
         if (!ok) break;
         tc_fence_after();
@@ -368,6 +451,34 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
         }
       }
     }
+  } else if (GROUPED && warp == THREADS / 32) {
+    // ------------------------------------------------------------------ ragged ends of the groups (both CTAs)
+    int stage = 0;
+    uint32_t phases = 0;  // bit s: of tail_bar[s]
+    for (int round = 0; round * num_pairs < num_tiles; ++round) {
+      const int tile = tile_of<GROUPED>(round, pair, num_pairs);
+      if (tile >= num_tiles) continue;
+      const TilePos t = tile_pos<GROUPED>(p, tile, tiles_m, tiles_n, order);
+      if (t.num_kb == 0) continue;
+      const int last = (stage + t.num_kb - 1) % STAGES;
+      stage = (stage + t.num_kb) % STAGES;
+      if (t.k_tail == BK) continue;
+      bool ok = mbar_wait_bounded(&tail_bar[last], (phases >> last) & 1u, abort_flag, p.status, kStatusTimeoutMma);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      phases ^= 1u << last;
+      // A reduction row is one 128-byte line of each [BK x 64] box (the swizzle only permutes within a line). Both operands
+      // are blanked: a zero on one side alone would let a NaN on the other through.
+      const int first = t.k_tail * 8, count = (BK - t.k_tail) * 8;  // in 16-byte units
+#pragma unroll
+      for (int j = 0; j < (BM + BNH) / 64; ++j) {
+        uint4* box = reinterpret_cast<uint4*>(smem + last * STAGE_BYTES + j * (64 * BK * 2)) + first;
+        for (int i = lane; i < count; i += 32) box[i] = make_uint4(0u, 0u, 0u, 0u);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&full_bar[last]), 0));
+    }
   } else {
     // ------------------------------------------------------------------ epilogue (warps 2..5, both CTAs)
     // A thread owns one accumulator row (tcgen05.ld 32x32b). Writing rows straight to memory would make every warp
@@ -387,15 +498,23 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
       const uint8_t* src = reinterpret_cast<const uint8_t*>(p.AB) + (static_cast<long long>(frow0) * p.ldab + fh0) * 2;
       ab_fetch(va, vb, src, src + static_cast<long long>(p.H) * 2, p.ldab * 2, min(32, p.M - frow0), min(64, p.N - fh0) * 2, lane);
     }
-    for (int tile = pair; ok && tile < num_tiles; tile += num_pairs, ++it) {
+    for (int round = 0; ok && round * num_pairs < num_tiles; ++round) {
+      const int tile = tile_of<GROUPED>(round, pair, num_pairs);
+      if (tile >= num_tiles) continue;
+      const TilePos pos = tile_pos<GROUPED>(p, tile, tiles_m, tiles_n, order);
+      const int tm = pos.tm, tn = pos.tn;
       const int acc = it & 1;
       const uint32_t acc_phase = (it >> 1) & 1;
-      ok = mbar_wait_bounded(&tfull_bar[acc], acc_phase, abort_flag, p.status, kStatusTimeoutEpilogue);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      tc_fence_after();
-      int tm, tn;
-      tile_coords(tile, tiles_m, tiles_n, p.group_m, tm, tn);
+      const bool empty = GROUPED && pos.num_kb == 0;  // a group without rows: zeros, no accumulator
+      if (empty) {
+        if (EPI == EPI_F32_ACC) continue;
+      } else {
+        ++it;
+        ok = mbar_wait_bounded(&tfull_bar[acc], acc_phase, abort_flag, p.status, kStatusTimeoutEpilogue);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+      }
       const int row0 = tm * (2 * BM) + static_cast<int>(cta) * BM + quad * 32;  // first row of this warp
       const int rows_valid = min(32, p.M - row0);                               // <= 0: nothing to store
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + acc * BN;
@@ -407,14 +526,19 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
       };
       if (EPI == EPI_BF16 || EPI == EPI_BF16_ACC) {
         const int n0 = tn * BN;
-        uint8_t* c_base = reinterpret_cast<uint8_t*>(p.C) + (static_cast<long long>(row0) * p.ldc + n0) * 2;
+        uint8_t* c_base = reinterpret_cast<uint8_t*>(p.C) + ((pos.c_row0 + row0) * p.ldc + n0) * 2;
 #pragma unroll 1
         for (int c = 0; c < BN / 64; ++c) {
           uint32_t r0[32], r1[32];
-          tmem_ld_32x32(t_row + c * 64, r0);
-          tmem_ld_32x32(t_row + c * 64 + 32, r1);
-          tmem_ld_wait();
-          if (c == BN / 64 - 1) release_acc();
+          if (GROUPED && empty) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) r0[j] = r1[j] = 0u;
+          } else {
+            tmem_ld_32x32(t_row + c * 64, r0);
+            tmem_ld_32x32(t_row + c * 64 + 32, r1);
+            tmem_ld_wait();
+            if (c == BN / 64 - 1) release_acc();
+          }
           const int cols_valid = min(64, p.N - (n0 + c * 64));
           if (rows_valid <= 0 || cols_valid <= 0) continue;
           uint8_t* stg = (c & 1) ? stg1 : stg0;
@@ -436,13 +560,18 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
         __syncwarp();
       } else if (EPI == EPI_F32 || EPI == EPI_F32_ACC) {
         const int n0 = tn * BN;
-        uint8_t* c_base = reinterpret_cast<uint8_t*>(p.C) + (static_cast<long long>(row0) * p.ldc + n0) * 4;
+        uint8_t* c_base = reinterpret_cast<uint8_t*>(p.C) + ((pos.c_row0 + row0) * p.ldc + n0) * 4;
 #pragma unroll 1
         for (int c = 0; c < BN / 32; ++c) {
           uint32_t r[32];
-          tmem_ld_32x32(t_row + c * 32, r);
-          tmem_ld_wait();
-          if (c == BN / 32 - 1) release_acc();
+          if (GROUPED && empty) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) r[j] = 0u;
+          } else {
+            tmem_ld_32x32(t_row + c * 32, r);
+            tmem_ld_wait();
+            if (c == BN / 32 - 1) release_acc();
+          }
           const int cols_valid = min(32, p.N - (n0 + c * 32));
           if (rows_valid <= 0 || cols_valid <= 0) continue;
           uint8_t* stg = (c & 1) ? stg1 : stg0;
@@ -616,19 +745,21 @@ static int max_pairs(const void* kern) {
   return cached;
 }
 
-template <int A_MN, int B_MN, int EPI>
+template <int A_MN, int B_MN, int EPI, bool GROUPED = false>
 static int launch(const CUtensorMap& ta, const CUtensorMap& tb, const Params& p, cudaStream_t stream) {
-  auto kern = gemm_pair_kernel<A_MN, B_MN, EPI>;
+  auto kern = gemm_pair_kernel<A_MN, B_MN, EPI, GROUPED>;
+  constexpr int bytes = GROUPED ? GROUPED_SMEM_BYTES : SMEM_BYTES;
   static bool configured = false;
   if (!configured) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess) return -3;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return -3;
     configured = true;
   }
   constexpr int TILE_N = EPI == EPI_SWIGLU_FWD ? BNH : BN;
-  const long long tiles = static_cast<long long>((p.M + 2 * BM - 1) / (2 * BM)) * ((p.N + TILE_N - 1) / TILE_N);
+  const long long tiles = static_cast<long long>((p.M + 2 * BM - 1) / (2 * BM)) * ((p.N + TILE_N - 1) / TILE_N) *
+                          (GROUPED ? p.num_groups : 1);
   const int pairs_max = max_pairs(reinterpret_cast<const void*>(kern));
   const int pairs = tiles < pairs_max ? static_cast<int>(tiles) : pairs_max;
-  kern<<<2 * pairs, THREADS, SMEM_BYTES, stream>>>(ta, tb, p);
+  kern<<<2 * pairs, GROUPED ? GROUPED_THREADS : THREADS, bytes, stream>>>(ta, tb, p);
   return cudaGetLastError() == cudaSuccess ? 0 : -4;
 }
 
@@ -685,6 +816,31 @@ extern "C" int ocb_gemm_bf16_pair(const void* A, const void* B, void* C, int M, 
   if (a_mn_major && b_mn_major) { OCB_PAIR_EPI(1, 1) }
   OCB_PAIR_EPI(1, 0)
 #undef OCB_PAIR_EPI
+}
+
+// Mode 2 of ocb_grouped_gemm_bf16 (gemm_sm100.cu), whose checks it relies on, computed by CTA pairs; C rows start on 16-byte
+// boundaries.
+extern "C" int ocb_grouped_wgrad_bf16_pair(const void* A, const void* B, void* C, const int* offsets, int num_groups, int total_rows,
+                                           int M, int N, long long lda, long long ldb, long long ldc, int epilogue, int* status,
+                                           cudaStream_t stream) {
+  CUtensorMap ta, tb;
+  if (!operand_maps(&ta, &tb, A, B, M, N, total_rows, lda, ldb, 1, 1)) return -1000;
+  Params p = {};
+  p.C = C;
+  p.ldc = ldc;
+  p.M = M;
+  p.N = N;
+  p.K = total_rows;
+  p.group_m = 8;
+  p.status = status;
+  p.offsets = offsets;
+  p.num_groups = num_groups;
+  switch (epilogue) {
+    case EPI_BF16: return launch<1, 1, EPI_BF16, true>(ta, tb, p, stream);
+    case EPI_F32_ACC: return launch<1, 1, EPI_F32_ACC, true>(ta, tb, p, stream);
+    case EPI_F32: return launch<1, 1, EPI_F32, true>(ta, tb, p, stream);
+    default: return -1;
+  }
 }
 
 // Gated-MLP up-projection with the activation in the epilogue: W13 = [w1; w3] ([2H, K], K-major, row stride ldw).
