@@ -10,7 +10,7 @@ def _offsets(sizes):
     return torch.tensor([0] + sizes, dtype=torch.int32).cumsum(0).to(torch.int32).cuda()
 
 
-@pytest.mark.parametrize("sizes", [[64], [1], [0, 0, 5], [128, 256, 64], [100, 0, 333, 7, 1, 63, 65], [3000, 0, 17, 450, 129] + [40] * 40])
+@pytest.mark.parametrize("sizes", [[320], [257], [0, 0, 1030, 5], [640, 128, 64], [1900, 0, 333, 7, 1, 63, 65], [9000, 0, 17, 4500, 129] + [40] * 40, [11] * 299 + [90000]])
 @pytest.mark.parametrize("M,N", [(136, 264), (256, 256), (520, 768)])
 @pytest.mark.parametrize("form", ["bf16", "fp32", "accumulate"])
 def test_against_fp64_and_the_single_cta_kernel(sizes, M, N, form):
@@ -54,7 +54,7 @@ def test_against_fp64_and_the_single_cta_kernel(sizes, M, N, form):
 def test_poisoned_neighbours_stay_out():
     from olmo_core_b200.ops.gemm import grouped_gemm_wgrad
 
-    sizes = [30, 70, 64, 1, 200]
+    sizes = [30, 1100, 64, 1, 200]
     offsets = _offsets(sizes)
     a = torch.randn(sum(sizes), 256, device="cuda", dtype=torch.bfloat16)
     b = torch.randn(sum(sizes), 320, device="cuda", dtype=torch.bfloat16)
