@@ -11,8 +11,10 @@
 // One CTA holds a 128 x 128 tile in registers (16 threads across, 16 down, each 8 rows of 8 columns): the maxima over a row
 // are shuffles within half a warp, those over a column go through shared memory. Rows and columns can come out of one launch,
 // which reads the tensor once where a layer needs both (the activations of a training step and the output gradient).
-// Memory bound: 2 bytes in, 1 byte out per orientation. 8192 x 11008: rows 55 us (4.9 TB/s), columns 51 (5.3), tiles 51 (5.3), rows
-// and columns together 86 (4.2, against 106 in two passes); the measured copy rate is 6.6 TB/s.
+// Memory bound: 2 bytes in, 1 byte out per orientation. 8192 x 11008: rows 47 us (5.7 TB/s), columns 47, tiles 46, rows and columns
+// together 61 (5.9, against 94 in two passes); the measured copy rate is 6.6 TB/s. Three things got it there from 55, 51, 51 and 86 us,
+// when the issue of instructions was the bound (13 per element and orientation): scaling in packed pairs, infinities patched in afterwards
+// instead of inside the cast, and a copy of the code for whole tiles that checks no edges.
 
 #include "block_quant.cuh"
 #include "common.cuh"
@@ -34,135 +36,136 @@ struct Params {
   long long x_group, q_group;  // elements between the matrices of a stack (tiles only)
 };
 
-__device__ __forceinline__ void store8(uint8_t* dst, uint2 v, int n) {
-  if (n >= 8) {
-    *reinterpret_cast<uint2*>(dst) = v;
-  } else {
-    for (int j = 0; j < n; ++j) dst[j] = static_cast<uint8_t>((j < 4 ? v.x >> (8 * j) : v.y >> (8 * (j - 4))) & 0xffu);
-  }
-}
+// What a tile needs besides its registers.
+struct Shared {
+  uint32_t top[8][B / 2];  // column maxima (pairs) of each warp; the tile form uses top[0][0..7]
+  uint32_t factor[B / 2];  // reciprocals of the columns' scales, in pairs; a sign says that the column holds an infinity
+  float row_scale[B];
+};
 
-template <int MODE>
-__global__ void __launch_bounds__(THREADS, MODE == (ROWS | COLUMNS) ? 3 : 4) quantize_block_kernel(const Params p, int vec) {
-  __shared__ uint32_t red[8][B / 2];  // column maxima (pairs) of each warp; the tile form uses red[0][0..7]
-  __shared__ float factor[B], row_scale[B];
-  const int across = threadIdx.x & 15, down = threadIdx.x >> 4;
-  const int warp = threadIdx.x >> 5;
+// FULL: the tile lies inside the matrix and its rows start on 16-byte boundaries.
+template <int MODE, bool FULL>
+__device__ __forceinline__ void quantize_tile(const Params& p, int vec, Shared& sh) {
+  const int across = threadIdx.x & 15, down = threadIdx.x >> 4, warp = threadIdx.x >> 5;
   const int col = blockIdx.x * B + across * 8;
-  const int n_col = min(8, p.cols - col);  // columns of this thread inside the matrix (may be <= 0)
-  const long long row0 = static_cast<long long>(blockIdx.y) * B;
-  const __nv_bfloat16* x = p.x + static_cast<long long>(blockIdx.z) * p.x_group;
-  next_kernel_may_start();
-  previous_kernel_done();
+  const int n_col = FULL ? 8 : min(8, p.cols - col);  // columns of this thread inside the matrix (may be <= 0)
+  const long long row0 = static_cast<long long>(blockIdx.y) * B + down;
+  const int n_row = FULL ? 8 : n_col <= 0 ? 0 : static_cast<int>(min(8ll, (p.rows - row0 + 15) / 16));  // rows row0 + 16 i
+
   uint4 v[8];
+  {
+    const __nv_bfloat16* src = p.x + static_cast<long long>(blockIdx.z) * p.x_group + row0 * p.ldx + col;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const long long row = row0 + down + 16 * i;
-    v[i] = make_uint4(0u, 0u, 0u, 0u);
-    if (row < p.rows && n_col > 0) {
-      const __nv_bfloat16* src = x + row * p.ldx + col;
-      if (vec && n_col == 8) {
+    for (int i = 0; i < 8; ++i, src += 16 * p.ldx) {
+      v[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (!FULL && i >= n_row) continue;
+      if (FULL || (vec && n_col == 8)) {
         v[i] = *reinterpret_cast<const uint4*>(src);
       } else {
-        const uint16_t* h = reinterpret_cast<const uint16_t*>(src);
         uint32_t w[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          if (j < n_col) w[j >> 1] |= static_cast<uint32_t>(h[j]) << (16 * (j & 1));
+          if (j < n_col) w[j >> 1] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(src)[j]) << (16 * (j & 1));
         v[i] = make_uint4(w[0], w[1], w[2], w[3]);
       }
     }
   }
+  auto store = [&](uint8_t* dst, uint2 c) {
+    if (FULL || n_col == 8) {
+      *reinterpret_cast<uint2*>(dst) = c;
+    } else {
+      for (int j = 0; j < n_col; ++j) dst[j] = static_cast<uint8_t>((j < 4 ? c.x >> (8 * j) : c.y >> (8 * (j - 4))) & 0xffu);
+    }
+  };
 
   if (MODE & ROWS) {
+    uint8_t* dst = p.q_row + row0 * p.ldq + col;
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {  // two rows share a register on their way through the half-warp
-      const uint32_t a = max_abs2(max_abs2(max_abs2(max_abs2(0u, v[i].x), v[i].y), v[i].z), v[i].w);
-      const uint32_t b = max_abs2(max_abs2(max_abs2(max_abs2(0u, v[i + 1].x), v[i + 1].y), v[i + 1].z), v[i + 1].w);
-      uint32_t m2 = max_abs2(__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632));
+      const uint32_t a = max_mag2(v[i]), b = max_mag2(v[i + 1]);
+      uint32_t m2 = max_mag2(__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632));
 #pragma unroll
-      for (int o = 8; o; o >>= 1) m2 = max_abs2(m2, __shfl_xor_sync(0xffffffffu, m2, o));
+      for (int o = 8; o; o >>= 1) m2 = max_mag2(m2, __shfl_xor_sync(0xffffffffu, m2, o));
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float amax = h ? hi(m2) : lo(m2);
+      for (int h = 0; h < 2; ++h, dst += 16 * p.ldq) {
+        const uint32_t amax = (h ? m2 >> 16 : m2) & 0x7fffu;
         const int e = scale_exponent(amax);
-        const float inv = pow2_biased(254 - e);
-        const int local = down + 16 * (i + h);
-        const long long row = row0 + local;
-        if (across == 0) row_scale[local] = pow2_biased(e);
-        if (row < p.rows && n_col > 0)
-          store8(p.q_row + row * p.ldq + col, amax == INFINITY ? e4m3x8<true>(v[i + h], inv) : e4m3x8<false>(v[i + h], inv), n_col);
+        if (across == 0) sh.row_scale[down + 16 * (i + h)] = pow2_biased(e);
+        uint2 c = e4m3x8(v[i + h], inverse_bf16(e) * 0x10001u);
+        if (amax == BF16_INF) c = infinities_to_nan(v[i + h], c);
+        if (FULL || i + h < n_row) store(dst, c);
       }
     }
   }
 
   if (MODE & (COLUMNS | TILES)) {
-    uint32_t m2[4] = {0u, 0u, 0u, 0u};
+    uint4 m = make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      m2[0] = max_abs2(m2[0], v[i].x);
-      m2[1] = max_abs2(m2[1], v[i].y);
-      m2[2] = max_abs2(m2[2], v[i].z);
-      m2[3] = max_abs2(m2[3], v[i].w);
-    }
-    float inv[8];
-    bool has_inf = false;
+    for (int i = 0; i < 8; ++i) m = make_uint4(max_mag2(m.x, v[i].x), max_mag2(m.y, v[i].y), max_mag2(m.z, v[i].z), max_mag2(m.w, v[i].w));
+    uint4 inv;
+    bool has_inf;
     if (MODE & COLUMNS) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) m2[j] = max_abs2(m2[j], __shfl_xor_sync(0xffffffffu, m2[j], 16));
-      if ((threadIdx.x & 16) == 0) *reinterpret_cast<uint4*>(&red[warp][across * 4]) = make_uint4(m2[0], m2[1], m2[2], m2[3]);
+      m = make_uint4(max_mag2(m.x, __shfl_xor_sync(0xffffffffu, m.x, 16)), max_mag2(m.y, __shfl_xor_sync(0xffffffffu, m.y, 16)),
+                     max_mag2(m.z, __shfl_xor_sync(0xffffffffu, m.z, 16)), max_mag2(m.w, __shfl_xor_sync(0xffffffffu, m.w, 16)));
+      if ((threadIdx.x & 16) == 0) *reinterpret_cast<uint4*>(&sh.top[warp][across * 4]) = m;
       __syncthreads();
       if (threadIdx.x < B / 2) {
-        uint32_t top = red[0][threadIdx.x];
+        uint32_t top = sh.top[0][threadIdx.x];
 #pragma unroll
-        for (int w = 1; w < 8; ++w) top = max_abs2(top, red[w][threadIdx.x]);
-        const float amax[2] = {lo(top), hi(top)};
+        for (int w = 1; w < 8; ++w) top = max_mag2(top, sh.top[w][threadIdx.x]);
+        uint32_t pair = 0u;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int e = scale_exponent(amax[h]);
-          // the reciprocal; its sign says that the column holds an infinity
-          factor[2 * threadIdx.x + h] = amax[h] == INFINITY ? -pow2_biased(254 - e) : pow2_biased(254 - e);
+          const uint32_t amax = (h ? top >> 16 : top) & 0x7fffu;
+          const int e = scale_exponent(amax);
+          pair |= (inverse_bf16(e) | (amax == BF16_INF ? 0x8000u : 0u)) << (16 * h);
           const int c = blockIdx.x * B + 2 * threadIdx.x + h;
-          if (c < p.cols) p.s_col[static_cast<long long>(blockIdx.y) * p.cols + c] = pow2_biased(e);
+          if (FULL || c < p.cols) p.s_col[static_cast<long long>(blockIdx.y) * p.cols + c] = pow2_biased(e);
         }
+        sh.factor[threadIdx.x] = pair;
       }
       __syncthreads();
-#pragma unroll
-      for (int j = 0; j < 8; j += 4) {
-        const float4 f = *reinterpret_cast<const float4*>(&factor[across * 8 + j]);
-        inv[j] = fabsf(f.x); inv[j + 1] = fabsf(f.y); inv[j + 2] = fabsf(f.z); inv[j + 3] = fabsf(f.w);
-        has_inf |= fminf(fminf(f.x, f.y), fminf(f.z, f.w)) < 0.f;
-      }
+      inv = *reinterpret_cast<const uint4*>(&sh.factor[across * 4]);
+      has_inf = ((inv.x | inv.y | inv.z | inv.w) & 0x80008000u) != 0u;
+      inv = make_uint4(inv.x & 0x7fff7fffu, inv.y & 0x7fff7fffu, inv.z & 0x7fff7fffu, inv.w & 0x7fff7fffu);
     } else {
-      uint32_t top2 = max_abs2(max_abs2(m2[0], m2[1]), max_abs2(m2[2], m2[3]));
+      uint32_t top = max_mag2(m);
 #pragma unroll
-      for (int o = 16; o; o >>= 1) top2 = max_abs2(top2, __shfl_xor_sync(0xffffffffu, top2, o));
-      if ((threadIdx.x & 31) == 0) red[0][warp] = top2;
+      for (int o = 16; o; o >>= 1) top = max_mag2(top, __shfl_xor_sync(0xffffffffu, top, o));
+      if ((threadIdx.x & 31) == 0) sh.top[0][warp] = top;
       __syncthreads();
 #pragma unroll
-      for (int w = 0; w < 8; ++w) top2 = max_abs2(top2, red[0][w]);
-      const float top = fmaxf(lo(top2), hi(top2));
-      has_inf = top == INFINITY;
-      const int e = scale_exponent(top);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) inv[j] = pow2_biased(254 - e);
+      for (int w = 0; w < 8; ++w) top = max_mag2(top, sh.top[0][w]);
+      const uint32_t amax = max(top & 0x7fffu, (top >> 16) & 0x7fffu);  // magnitudes order as their bits
+      has_inf = amax == BF16_INF;
+      const int e = scale_exponent(amax);
+      inv.x = inv.y = inv.z = inv.w = inverse_bf16(e) * 0x10001u;
       if (threadIdx.x == 0)
         p.s_tile[(static_cast<long long>(blockIdx.z) * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x] = pow2_biased(e);
     }
-    uint8_t* q = (MODE & COLUMNS) ? p.q_col : p.q_tile + static_cast<long long>(blockIdx.z) * p.q_group;
-    if (n_col > 0) {
+    uint8_t* dst = ((MODE & COLUMNS) ? p.q_col : p.q_tile + static_cast<long long>(blockIdx.z) * p.q_group) + row0 * p.ldq + col;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const long long row = row0 + down + 16 * i;
-        if (row < p.rows) store8(q + row * p.ldq + col, has_inf ? e4m3x8<true>(v[i], inv) : e4m3x8<false>(v[i], inv), n_col);
-      }
+    for (int i = 0; i < 8; ++i, dst += 16 * p.ldq) {
+      uint2 c = e4m3x8(v[i], inv);
+      if (has_inf) c = infinities_to_nan(v[i], c);
+      if (FULL || i < n_row) store(dst, c);
     }
   }
   if (MODE & ROWS) {
     __syncthreads();
-    if (threadIdx.x < B && row0 + threadIdx.x < p.rows)
-      p.s_row[static_cast<long long>(blockIdx.x) * p.rows + row0 + threadIdx.x] = row_scale[threadIdx.x];
+    const long long row = static_cast<long long>(blockIdx.y) * B + threadIdx.x;
+    if (threadIdx.x < B && (FULL || row < p.rows)) p.s_row[static_cast<long long>(blockIdx.x) * p.rows + row] = sh.row_scale[threadIdx.x];
   }
+}
+
+template <int MODE>
+__global__ void __launch_bounds__(THREADS, MODE == (ROWS | COLUMNS) ? 3 : 4) quantize_block_kernel(const Params p, int vec) {
+  __shared__ Shared sh;
+  next_kernel_may_start();
+  previous_kernel_done();
+  const bool full = vec && (blockIdx.x + 1ll) * B <= p.cols && (blockIdx.y + 1ll) * B <= p.rows;
+  if (full) quantize_tile<MODE, true>(p, vec, sh);
+  else quantize_tile<MODE, false>(p, vec, sh);
 }
 
 template <int MODE>

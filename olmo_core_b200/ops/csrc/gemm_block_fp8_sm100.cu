@@ -884,16 +884,17 @@ gemm_block_fp8_small_kernel(const __grid_constant__ CUtensorMap tma_a, const __g
 #pragma unroll
           for (int b = 0; b < SCALE_BATCH; ++b) {
             const uint4 lo = next[b][0], hi = next[b][1];
-            uint32_t m2 = blkq::max_abs2(blkq::max_abs2(blkq::max_abs2(blkq::max_abs2(0u, lo.x), lo.y), lo.z), lo.w);
-            m2 = blkq::max_abs2(blkq::max_abs2(blkq::max_abs2(blkq::max_abs2(m2, hi.x), hi.y), hi.z), hi.w);
+            uint32_t m2 = blkq::max_mag2(blkq::max_mag2(lo), blkq::max_mag2(hi));
 #pragma unroll
-            for (int o = 4; o; o >>= 1) m2 = blkq::max_abs2(m2, __shfl_xor_sync(0xffffffffu, m2, o));
-            const float amax = fmaxf(blkq::lo(m2), blkq::hi(m2));
+            for (int o = 4; o; o >>= 1) m2 = blkq::max_mag2(m2, __shfl_xor_sync(0xffffffffu, m2, o));
+            const uint32_t amax = max(m2 & 0x7fffu, (m2 >> 16) & 0x7fffu);
             const int e = blkq::scale_exponent(amax);
-            const float inv = blkq::pow2_biased(254 - e);
-            const bool inf = amax == INFINITY;
-            const uint2 c0 = inf ? blkq::e4m3x8<true>(lo, inv) : blkq::e4m3x8<false>(lo, inv);
-            const uint2 c1 = inf ? blkq::e4m3x8<true>(hi, inv) : blkq::e4m3x8<false>(hi, inv);
+            const uint32_t inv = blkq::inverse_bf16(e) * 0x10001u;
+            uint2 c0 = blkq::e4m3x8(lo, inv), c1 = blkq::e4m3x8(hi, inv);
+            if (amax == blkq::BF16_INF) {
+              c0 = blkq::infinities_to_nan(lo, c0);
+              c1 = blkq::infinities_to_nan(hi, c1);
+            }
             codes[b] = make_uint4(c0.x, c0.y, c1.x, c1.y);
             word |= static_cast<uint32_t>(e) << (8 * b);
           }
