@@ -24,6 +24,7 @@
 // shared memory, so that global accesses are whole 128-byte lines). All waits are bounded (common.cuh).
 
 #include <atomic>
+#include <cmath>
 
 #include "block_quant.cuh"
 #include "common.cuh"
@@ -607,18 +608,21 @@ gemm_block_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
 //
 // What bounds it: the weight's bytes (one token against 4096 x 11008: 12.8 us, 3.5 TB/s, against 6.9 us at the measured copy
 // rate), and about 4.4 us in which barriers, tensor memory and tensor maps are set up, the first loads arrive, and the parts are
-// added. 64 experts of 1024 x 2048 for 128 rows: 28.5 us, 4.7 TB/s.
+// added. 64 experts of 1024 x 2048 for 128 rows that reach 53 of them: 22.1 us, 4.9 TB/s.
 constexpr int SMALL_THREADS = 256;  // warps as above, with one epilogue warpgroup
 
-template <int BN>
+// MANY: three CTAs per SM with a short ring each, instead of two with a deeper one (see fuller_with_three()).
+template <int BN, bool MANY>
 struct SmallTile {
+  static constexpr int CTAS = MANY ? 3 : 2;
   static constexpr int KB_BYTES = A_BYTES + BN * BKE;
-  static constexpr int STAGES = BN >= 128 ? 3 : BN >= 64 ? 4 : BN >= 32 ? 5 : 6;  // about 100 KB: two CTAs per SM
+  static constexpr int STAGES = MANY || BN >= 128 ? 3 : BN >= 64 ? 4 : BN >= 32 ? 5 : 6;
   static constexpr uint32_t TMEM = BN >= 128 ? 256 : BN >= 64 ? 128 : BN >= 32 ? 64 : 32;  // BN + 16 scale columns
   static constexpr int SF_BYTES = 2 * SF_BLOCK;
   static constexpr int SMEM_BYTES = STAGES * KB_BYTES + SCALE_SLOTS * SF_BYTES + 1024 + 256;
   // the fp32 part reuses the stages: [BN][128] (SWAP) or [128][BN + 4]
   static_assert(STAGES * KB_BYTES >= 128 * (BN + 4) * 4, "the parts do not fit");
+  static_assert(CTAS * (SMEM_BYTES + 1024) <= 228 * 1024, "the CTAs of an SM do not fit");
 };
 
 struct SmallParams {
@@ -653,10 +657,10 @@ __device__ __forceinline__ float4 load_cluster_f4(uint32_t cluster_addr) {
   return v;
 }
 
-template <int BN, bool SWAP, bool FUSED>
-__global__ void __launch_bounds__(SMALL_THREADS, 2)
+template <int BN, bool SWAP, bool FUSED, bool MANY>
+__global__ void __launch_bounds__(SMALL_THREADS, (SmallTile<BN, MANY>::CTAS))
 gemm_block_fp8_small_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b, const SmallParams p) {
-  using T = SmallTile<BN>;
+  using T = SmallTile<BN, MANY>;
   constexpr int STAGES = T::STAGES;
   static_assert(!FUSED || (SWAP && BN == 16), "eight threads per token cover sixteen tokens");
   extern __shared__ uint8_t smem_raw[];
@@ -1070,10 +1074,10 @@ static bool make_map(CUtensorMap* out, const void* ptr, bool mn, uint64_t rows, 
   return encode_tensor_map(out, ptr, rank, dims, str, box, 1);
 }
 
-template <int BN, bool SWAP, bool FUSED = false>
+template <int BN, bool SWAP, bool FUSED = false, bool MANY = false>
 static int launch_small(const CUtensorMap& ta, const CUtensorMap& tb, const SmallParams& p, long long tiles, int dev, cudaStream_t stream) {
-  constexpr int bytes = SmallTile<BN>::SMEM_BYTES;
-  auto kernel = gemm_block_fp8_small_kernel<BN, SWAP, FUSED>;
+  constexpr int bytes = SmallTile<BN, MANY>::SMEM_BYTES;
+  auto kernel = gemm_block_fp8_small_kernel<BN, SWAP, FUSED, MANY>;
   static std::atomic<uint64_t> done;
   if (!allow_smem(kernel, bytes, done, dev)) return -3;
   if (tiles * p.parts > 0x7fffffffll) return -1;
@@ -1127,8 +1131,13 @@ static int run_pair(const Product& x, int dev, cudaStream_t stream) {
   return launch_epi(ta, tb, p, tiles_m * ((x.N + BN - 1) / BN), x.epi, dev, stream);
 }
 
-// swap: the rows of B take the 128-row side and the rows of A the side of bn.
-static int run_small(const Product& x, bool swap, int bn, int parts, int dev, cudaStream_t stream) {
+// Whether `tiles` CTAs fill the SMs in fewer rounds at three per SM than at two. Up to 16 rows against weights of 64 experts, two and
+// three per SM: 424 tiles of 16 blocks 28.5 and 22.1 us, of 8 blocks 31.0 and 24.8 (848 tiles), 384 of 32 blocks 47.3 and 36.5; but 504 of 16
+// blocks 31.2 and 32.9, 512 of 32 blocks 49.7 and 58.3 (two rounds either way, and the second is emptier with three).
+static bool fuller_with_three(double tiles, int sms) { return std::ceil(tiles / (3 * sms)) < std::ceil(tiles / (2 * sms)); }
+
+// swap: the rows of B take the 128-row side and the rows of A the side of bn. many: see SmallTile, for bn = 16.
+static int run_small(const Product& x, bool swap, int bn, int parts, bool many, int dev, cudaStream_t stream) {
   SmallParams p;
   p.C = x.C;
   p.ldc = x.ldc;
@@ -1160,10 +1169,12 @@ static int run_small(const Product& x, bool swap, int bn, int parts, int dev, cu
   // every group can end inside a tile; a group without rows has none
   if (x.offsets != nullptr) b_tiles = p.N / bn + (x.groups < p.N ? x.groups : p.N);
   const long long tiles = b_tiles * ((p.M + BM - 1) / BM);
-  if (x.A == nullptr) return launch_small<16, true, true>(ta, tb, p, tiles, dev, stream);
+  if (x.A == nullptr)
+    return many ? launch_small<16, true, true, true>(ta, tb, p, tiles, dev, stream) : launch_small<16, true, true>(ta, tb, p, tiles, dev, stream);
   if (swap) {
     switch (bn) {
-      case 16: return launch_small<16, true>(ta, tb, p, tiles, dev, stream);
+      case 16: if (many) return launch_small<16, true, false, true>(ta, tb, p, tiles, dev, stream);
+               return launch_small<16, true>(ta, tb, p, tiles, dev, stream);
       case 32: return launch_small<32, true>(ta, tb, p, tiles, dev, stream);
       case 64: return launch_small<64, true>(ta, tb, p, tiles, dev, stream);
       default: return launch_small<128, true>(ta, tb, p, tiles, dev, stream);
@@ -1213,18 +1224,22 @@ static int run(const Product& x, cudaStream_t stream) {
     if (mean > 128) return run_pair(x, dev, stream);
     const int bn = small_width(mean, true);
     const long long used = x.groups < x.M ? x.groups : x.M;
-    return run_small(x, true, bn, split(used * tiles_n, kb, sms, true), dev, stream);
+    const int parts = split(used * tiles_n, kb, sms, true);
+    // rows that fall on the groups evenly at random leave some without any
+    const double some = x.groups * (1.0 - std::exp(-static_cast<double>(x.M) / x.groups));
+    return run_small(x, true, bn, parts, parts == 1 && bn == 16 && fuller_with_three(some * tiles_n, sms), dev, stream);
   }
   if (x.M <= 128 && !x.a_mn) {
     const int bn = small_width(x.M, false);
-    return run_small(x, true, bn, split(tiles_n, kb, sms, true), dev, stream);
+    const int parts = split(tiles_n, kb, sms, true);
+    return run_small(x, true, bn, parts, parts == 1 && bn == 16 && fuller_with_three(static_cast<double>(tiles_n), sms), dev, stream);
   }
   const long long pair_tiles = static_cast<long long>((x.M + 255) / 256) * ((x.N + 255) / 256);
   const long long small_tiles = static_cast<long long>((x.M + 127) / 128) * tiles_n;
   const int parts = split(small_tiles, kb, sms, false), pairs = sms / 2;
   const double pair_us = 5.0 + 0.43 * static_cast<double>(kb * ((pair_tiles + pairs - 1) / pairs));
   const double small_us = 5.5 + 0.5 * static_cast<double>(((kb + parts - 1) / parts) * ((small_tiles * parts + sms - 1) / sms)) + (parts > 1 ? 0.7 : 0.0);
-  return small_us < pair_us ? run_small(x, false, 128, parts, dev, stream) : run_pair(x, dev, stream);
+  return small_us < pair_us ? run_small(x, false, 128, parts, false, dev, stream) : run_pair(x, dev, stream);
 }
 
 }  // namespace blk
