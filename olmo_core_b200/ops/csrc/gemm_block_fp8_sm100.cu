@@ -7,9 +7,10 @@
 // per row in tensor memory that it selects; all four steps of a block select the same byte here, so one word, and one set of
 // copies into tensor memory, serves four blocks. Adding scaled partial sums in registers instead, which would allow scales of any value, was measured
 // first: every block has to be read back from tensor memory, and 8192 x 11008 x 4096 took 403 us (625 us with a scale per
-// column of B). This form takes 254 us, 2900 TFLOP/s and 1.76 of what cuBLAS measures in bf16; the input gradient takes 252 us, the
-// weight gradient 264 us. What bounds it is the tensor pipe (617 cycles per block and pair of 256 x 256 against 512 of the
-// instructions alone) and, in longer runs, the power limit: 280 us at the 1.39 GHz that it leaves.
+// column of B). This form takes 250 us, 2950 TFLOP/s and 1.79 of what cuBLAS measures in bf16, so does the input gradient, and the
+// weight gradient takes 260 us. A block of a 256 x 256 tile takes 617 cycles; the instructions alone need 512, and so does shared memory (32 KB in
+// and 32 KB out per SM at 128 B a cycle), which the result's way through it, 0.6 us a tile, delays further. In longer runs the power limit
+// binds: 280 us at the 1.39 GHz that it leaves. Storing the result by TMA gained 3 % at K = 1024 and nothing at 4096.
 //
 // Both operands are addressed in place, whatever their orientation: a K-major operand (reduction contiguous) arrives as
 // [rows x 128 bytes] boxes, an MN-major one (rows of the product contiguous) as [128 k x 128 bytes] boxes, so the input
@@ -606,7 +607,7 @@ gemm_block_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
 // reduction, out of L2; in exchange there is no quantiser launch in front (one token against 4096 x 11008, with the host: 18.4 us
 // with the launch, 14.4 without; two scale warps in place of the epilogue's took 16.8).
 //
-// What bounds it: the weight's bytes (one token against 4096 x 11008: 12.8 us, 3.5 TB/s, against 6.9 us at the measured copy
+// What bounds it: the weight's bytes (one token against 4096 x 11008: 12.2 us, 3.7 TB/s, against 6.9 us at the measured copy
 // rate), and about 4.4 us in which barriers, tensor memory and tensor maps are set up, the first loads arrive, and the parts are
 // added. 64 experts of 1024 x 2048 for 128 rows that reach 53 of them: 22.1 us, 4.9 TB/s.
 constexpr int SMALL_THREADS = 256;  // warps as above, with one epilogue warpgroup
