@@ -250,7 +250,10 @@ class MoERouter(nn.Module):
         """
         x = self.jitter(x)
         logits = self.get_expert_logits(x).float()
-        fused = (logits.is_cuda and not self.uniform_expert_assignment
+        # a subclass may choose from biased or sigmoid scores in its own way
+        own_choice = type(self).get_top_k is not MoERouter.get_top_k and (
+            self.bias_gamma is not None or self.gating_function != MoERouterGatingFunction.softmax)
+        fused = (logits.is_cuda and not self.uniform_expert_assignment and not own_choice
                  and moe_ops.route_supported(self.num_experts, self.top_k, self.n_groups))
         normalized = False
         if fused or self.n_groups > 1:

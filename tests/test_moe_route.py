@@ -251,6 +251,20 @@ def test_route_refusals(device):
             route(x, 2, score_bias=torch.zeros(32))
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_router_with_its_own_choice_is_asked(device):
+    from olmo_core_b200.nn.moe.router import MoELinearRouter, MoERouterGatingFunction
+
+    class Last(MoELinearRouter):
+        def get_top_k(self, scores):
+            indices = torch.arange(6, 8, device=scores.device).expand(*scores.shape[:-1], 2)
+            return scores.gather(-1, indices), indices
+
+    router = Last(d_model=16, num_experts=8, top_k=2, gating_function=MoERouterGatingFunction.sigmoid).to(device)
+    _, experts, counts, _ = router(_logits(6, 16, 5).view(2, 3, 16).to(device))
+    assert experts.flatten().tolist() == [6, 7] * 6 and counts.flatten().tolist() == [0] * 6 + [6, 6]
+
+
 @pytest.mark.gpu
 def test_what_the_kernels_entry_refuses_is_an_exception():
     from olmo_core_b200.ops import _lib
