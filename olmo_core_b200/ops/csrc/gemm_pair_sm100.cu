@@ -32,7 +32,9 @@
 // 1.08 to 1.3 times the mean; 1.3 to 1.6 times in the groups' own order). The last block of a group
 // reaches into the next one's rows; a warp of its own in each CTA blanks those lines in shared memory. For that the loads
 // of such a block count on a barrier of the CTA itself, and "stage full" in the leader counts one arrival per CTA: by the
-// producer when it has issued its loads, or, for a last block, by the blanking warp when it is done.
+// producer when it has issued its loads, or, for a last block, by the blanking warp when it is done. Eight warps carry the results
+// out (four: 172 instead of 157 us for 64 matrices of 2048 x 1024 in bf16 from 32768 rows spread as above); writing those 268 MB
+// alone takes 70 to 90 us, the products 75.
 
 #include <mutex>
 
@@ -57,7 +59,7 @@ constexpr int STAGE_BYTES = A_STAGE_BYTES + B_STAGE_BYTES;
 constexpr int EPI_STAGING_BYTES = 4 * 2 * 32 * 128;  // four epilogue warps, two 32-row x 128-byte buffers each
 constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_STAGING_BYTES + 1024 /*alignment slack*/ + 256 /*barriers*/;
 constexpr int THREADS = 192;
-constexpr int GROUPED_THREADS = THREADS + 32;  // and the blanking warp
+constexpr int GROUPED_THREADS = THREADS + 4 * 32 + 32;  // four more epilogue warps, and the blanking warp
 constexpr int SORTED_GROUPS = 256;              // up to this many groups are sorted by length
 constexpr int GROUPED_SMEM_BYTES = SMEM_BYTES + SORTED_GROUPS * 4;
 constexpr int TMEM_COLS = 512;
@@ -322,7 +324,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&tfull_bar[a], 1);
-      mbar_init(&tempty_bar[a], 8);  // four epilogue warps in each CTA of the pair
+      mbar_init(&tempty_bar[a], GROUPED ? 16 : 8);  // the epilogue warps of both CTAs of the pair
     }
     *abort_flag = 0;
     fence_mbar_init();
@@ -451,7 +453,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
         }
       }
     }
-  } else if (GROUPED && warp == THREADS / 32) {
+  } else if (GROUPED && warp == GROUPED_THREADS / 32 - 1) {
     // ------------------------------------------------------------------ ragged ends of the groups (both CTAs)
     int stage = 0;
     uint32_t phases = 0;  // bit s: of tail_bar[s]
@@ -485,8 +487,12 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
     // store touch 32 different lines, so each warp turns its 32 x 128-byte block through two staging buffers in shared
     // memory (16-byte slots, XOR-swizzled by row) and moves it to / from global memory with 8 lanes per 128-byte line.
     const int quad = warp & 3;
-    uint8_t* stg0 = smem + STAGES * STAGE_BYTES + (warp - 2) * (2 * STG_BYTES);
-    uint8_t* stg1 = stg0 + STG_BYTES;
+    // GROUPED: short reductions, so the results' way out counts as much as the products: eight warps, each with half of the
+    // columns of its rows and one buffer
+    constexpr int PARTS = GROUPED ? 2 : 1;
+    const int part = GROUPED ? (warp - 2) >> 2 : 0;
+    uint8_t* stg0 = smem + STAGES * STAGE_BYTES + (warp - 2) * (2 / PARTS * STG_BYTES);
+    uint8_t* stg1 = GROUPED ? stg0 : stg0 + STG_BYTES;
     const uint32_t tempty_leader0 = map_to_cta(smem_u32(&tempty_bar[0]), 0);
     bool ok = true;
     int it = 0;
@@ -528,7 +534,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
         const int n0 = tn * BN;
         uint8_t* c_base = reinterpret_cast<uint8_t*>(p.C) + ((pos.c_row0 + row0) * p.ldc + n0) * 2;
 #pragma unroll 1
-        for (int c = 0; c < BN / 64; ++c) {
+        for (int c = part * (BN / 64 / PARTS); c < (part + 1) * (BN / 64 / PARTS); ++c) {
           uint32_t r0[32], r1[32];
           if (GROUPED && empty) {
 #pragma unroll
@@ -537,11 +543,12 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
             tmem_ld_32x32(t_row + c * 64, r0);
             tmem_ld_32x32(t_row + c * 64 + 32, r1);
             tmem_ld_wait();
-            if (c == BN / 64 - 1) release_acc();
+            if (c == (part + 1) * (BN / 64 / PARTS) - 1) release_acc();
           }
           const int cols_valid = min(64, p.N - (n0 + c * 64));
           if (rows_valid <= 0 || cols_valid <= 0) continue;
           uint8_t* stg = (c & 1) ? stg1 : stg0;
+          if (GROUPED) __syncwarp();  // one buffer: the last chunk has left it
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
             *stg_slot(stg, lane, v) = make_uint4(pack_bf16x2(__uint_as_float(r0[8 * v + 0]), __uint_as_float(r0[8 * v + 1])),
@@ -562,7 +569,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
         const int n0 = tn * BN;
         uint8_t* c_base = reinterpret_cast<uint8_t*>(p.C) + ((pos.c_row0 + row0) * p.ldc + n0) * 4;
 #pragma unroll 1
-        for (int c = 0; c < BN / 32; ++c) {
+        for (int c = part * (BN / 32 / PARTS); c < (part + 1) * (BN / 32 / PARTS); ++c) {
           uint32_t r[32];
           if (GROUPED && empty) {
 #pragma unroll
@@ -570,11 +577,12 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
           } else {
             tmem_ld_32x32(t_row + c * 32, r);
             tmem_ld_wait();
-            if (c == BN / 32 - 1) release_acc();
+            if (c == (part + 1) * (BN / 32 / PARTS) - 1) release_acc();
           }
           const int cols_valid = min(32, p.N - (n0 + c * 32));
           if (rows_valid <= 0 || cols_valid <= 0) continue;
           uint8_t* stg = (c & 1) ? stg1 : stg0;
+          if (GROUPED) __syncwarp();
 #pragma unroll
           for (int v = 0; v < 8; ++v) *stg_slot(stg, lane, v) = make_uint4(r[4 * v], r[4 * v + 1], r[4 * v + 2], r[4 * v + 3]);
           __syncwarp();

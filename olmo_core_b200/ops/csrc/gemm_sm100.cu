@@ -818,7 +818,7 @@ extern "C" int ocb_grouped_gemm_bf16(const void* A, const void* B, void* C, cons
   if (M <= 0) return 0;
   // Pairs draw two thirds through L2 of what single CTAs draw, and fill from 129 rows and columns on; below that half of a pair's
   // tile is empty. 64 matrices of 2048 x 1024 in bf16, microseconds, pairs and single CTAs: 119 and 103 for 64 rows a group, 123 and
-  // 121 for 256, 150 and 164 for 512, 223 and 258 for 1024; 1024 x 2048 accumulated in fp32 from 4096 rows each: 793 and 1018. Only
+  // 121 for 256, 134 and 165 for 512, 223 and 256 for 1024; 1024 x 2048 accumulated in fp32 from 4096 rows each: 793 and 1018. Only
   // the mean of the groups' sizes is known here.
   const int c_elem = epilogue == EPI_BF16 ? 2 : 4;
   if (g_pair_mode && M > 128 && N > 128 && total_rows / num_groups > 256 && (ldc * c_elem) % 16 == 0 && (reinterpret_cast<uintptr_t>(C) & 15) == 0 &&
