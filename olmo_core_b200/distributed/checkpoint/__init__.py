@@ -175,6 +175,8 @@ def optim_state(model: nn.Module, optim: torch.optim.Optimizer, *, flatten: bool
 @torch.no_grad()
 def load_model_state(model: nn.Module, state: Dict[str, torch.Tensor], *, strict: bool = True) -> None:
     """Copy ``state`` (as produced by :func:`model_state`, possibly loaded into in place) into ``model``."""
+    from ...float8 import refresh_float8_scales
+
     params = dict(model.named_parameters())
     buffers = dict(model.named_buffers())
     for n, value in state.items():
@@ -194,6 +196,7 @@ def load_model_state(model: nn.Module, state: Dict[str, torch.Tensor], *, strict
     rt = _runtime_of(model)
     if rt is not None and rt.materialized:
         rt.sync_lowp()
+    refresh_float8_scales(model)  # 8-bit copies of the weights that were just overwritten
 
 
 @torch.no_grad()

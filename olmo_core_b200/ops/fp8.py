@@ -24,7 +24,7 @@ from . import _lib
 from .gemm import compute_weight, gemm
 
 __all__ = ["quantize_rowwise", "quantize_colwise_transposed", "gemm_fp8", "fp8_linear", "Float8LinearFunction",
-           "cached_weight_cast", "E4M3_MAX"]
+           "cached_weight_cast", "weight_state", "E4M3_MAX"]
 
 E4M3_MAX = 448.0
 
@@ -98,16 +98,28 @@ def gemm_fp8(a_q: torch.Tensor, a_scale: torch.Tensor, b_q: torch.Tensor, b_scal
     return out
 
 
-def cached_weight_cast(cache: Optional[dict], key: str, make, version: int = 0):
+def weight_state(weight: torch.Tensor):
+    """
+    What ``weight`` holds and where, as far as PyTorch tells without looking at its elements: equal values of this mean that a cast
+    made from it still stands. In-place operations on the parameter move its version counter; ``parameter.data = ...`` and
+    ``module.to(...)`` do not, but move its memory. ``None`` for tensors made under inference mode, which count no versions. What
+    writes through ``parameter.data`` shows in neither and calls :func:`olmo_core_b200.float8.refresh_float8_scales`.
+    """
+    if weight.is_inference():
+        return None
+    return weight._version, weight.device, weight.data_ptr(), weight.dtype, weight.shape, weight.stride()
+
+
+def cached_weight_cast(cache: Optional[dict], key: str, make, version=0):
     """
     ``make()`` once per optimizer step: ``cache`` is a dict owned by the layer and emptied by
     :func:`olmo_core_b200.float8.refresh_float8_scales` after every parameter update, so the quantised copies of a weight
     are shared by all micro-batches of a step and by forward and backward (the effect the reference gets from casting
     weights once before the sharded all-gather: src/olmo_core/float8/__init__.py:141-162). ``None`` disables caching.
-    ``version`` (the parameter's autograd version counter) additionally drops an entry when the weight was rewritten by
-    an ordinary in-place tensor operation, e.g. when a checkpoint is loaded.
+    ``version`` (:func:`weight_state` of the parameter) additionally drops an entry when the weight was rewritten by an ordinary
+    in-place tensor operation, replaced or moved; where it is ``None`` nothing is kept.
     """
-    if cache is None:
+    if cache is None or version is None:
         return make()
     hit = cache.get(key)
     if hit is None or hit[0] != version:
@@ -122,7 +134,7 @@ class Float8LinearFunction(torch.autograd.Function):
         x2 = x.reshape(-1, x.shape[-1])
         x2 = x2 if x2.dtype == torch.bfloat16 else x2.to(torch.bfloat16)
         xq, sx = quantize_rowwise(x2, pow2)
-        wq, sw = cached_weight_cast(cache, "row", lambda: quantize_rowwise(w, pow2), weight._version)
+        wq, sw = cached_weight_cast(cache, "row", lambda: quantize_rowwise(w, pow2), weight_state(weight))
         y = gemm_fp8(xq, sx, wq, sw)
         ctx.save_for_backward(x2, w)
         ctx.opts = (pow2, wgrad_high_precision)
@@ -140,7 +152,7 @@ class Float8LinearFunction(torch.autograd.Function):
         dx = None
         if ctx.needs_input_grad[0]:
             dyq, sdy = quantize_rowwise(dy2, pow2)
-            wtq, swt = cached_weight_cast(ctx.cache, "col_t", lambda: quantize_colwise_transposed(w, pow2), weight._version)  # [K, N]
+            wtq, swt = cached_weight_cast(ctx.cache, "col_t", lambda: quantize_colwise_transposed(w, pow2), weight_state(weight))  # [K, N]
             dx = gemm_fp8(dyq, sdy, wtq, swt).view(ctx.x_shape).to(ctx.x_dtype)
         main_grad = getattr(weight, "main_grad", None)
         dw = None

@@ -31,7 +31,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .fp8 import cached_weight_cast
+from .fp8 import cached_weight_cast, weight_state
 from .gemm import compute_weight, gemm
 
 __all__ = ["BLOCK", "quantize_block_rows", "quantize_block_columns", "quantize_block_tiles", "dequantize_block_rows",
@@ -428,11 +428,12 @@ def fp8_block_grouped_matmul(x: torch.Tensor, w_q: torch.Tensor, w_s: torch.Tens
 
 def _cached(cache: Optional[dict], make, weight: torch.Tensor):
     """The 8-bit form of ``weight``, kept in ``cache`` (see :func:`olmo_core_b200.ops.fp8.cached_weight_cast`)."""
-    made = cached_weight_cast(cache, "block_tiles", make, weight._version)
+    state = weight_state(weight)
+    made = cached_weight_cast(cache, "block_tiles", make, state)
     first = made if torch.is_tensor(made) else made[0]
     if cache is not None and first.is_inference() and not torch.is_inference_mode_enabled():
         cache.clear()  # made under inference mode, cannot be saved for a backward pass
-        made = cached_weight_cast(cache, "block_tiles", make, weight._version)
+        made = cached_weight_cast(cache, "block_tiles", make, state)
     return made
 
 

@@ -21,7 +21,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .fp8 import cached_weight_cast
+from .fp8 import cached_weight_cast, weight_state
 from .gemm import compute_weight
 
 __all__ = ["MX_BLOCK", "quantize_mx_rowwise", "quantize_mx_colwise_transposed", "scales_as_matrix", "scales_from_matrix",
@@ -185,7 +185,7 @@ class MXLinearFunction(torch.autograd.Function):
         x2 = x.reshape(-1, x.shape[-1])
         x2 = x2 if x2.dtype == torch.bfloat16 else x2.to(torch.bfloat16)
         xq, sx = quantize_mx_rowwise(x2, mode)
-        wq, sw = cached_weight_cast(cache, "mx_row", lambda: quantize_mx_rowwise(w, mode), weight._version)
+        wq, sw = cached_weight_cast(cache, "mx_row", lambda: quantize_mx_rowwise(w, mode), weight_state(weight))
         y = gemm_mx(xq, sx, wq, sw)
         ctx.save_for_backward(x2, w)
         ctx.mode = mode
@@ -203,7 +203,7 @@ class MXLinearFunction(torch.autograd.Function):
         dx = None
         if ctx.needs_input_grad[0]:
             dyq, sdy = quantize_mx_rowwise(dy2, mode)
-            wtq, swt = cached_weight_cast(ctx.cache, "mx_col_t", lambda: quantize_mx_colwise_transposed(w, mode), weight._version)  # [K, N], blocks along N
+            wtq, swt = cached_weight_cast(ctx.cache, "mx_col_t", lambda: quantize_mx_colwise_transposed(w, mode), weight_state(weight))  # [K, N], blocks along N
             dx = gemm_mx(dyq, sdy, wtq, swt).view(ctx.x_shape).to(ctx.x_dtype)
         main_grad = getattr(weight, "main_grad", None)
         dw = None

@@ -22,6 +22,7 @@ import torch
 from ...distributed.checkpoint import save_state_dict
 from ...distributed.utils import barrier, get_local_tensor, get_rank
 from ...exceptions import OLMoConfigurationError
+from ...float8 import refresh_float8_scales
 from ...io import clear_directory, dir_is_empty, is_url, join_path
 from .callback import Callback
 from .checkpointer import CheckpointerCallback
@@ -156,6 +157,7 @@ class ModelMergeCallback(Callback):
         runtime = getattr(tm, "runtime", None)
         if runtime is not None:
             runtime.sync_lowp()
+        refresh_float8_scales(tm.model)  # no 8-bit copies of the live weights in the evaluation, and none of the merged ones after
         barrier()
         try:
             save_state_dict(join_path(out, "model_and_optim"), tm.state_dict_to_save(optim=False),
@@ -168,6 +170,7 @@ class ModelMergeCallback(Callback):
                 p.copy_(live[n])
             if runtime is not None:
                 runtime.sync_lowp()
+            refresh_float8_scales(tm.model)
             barrier()
         del self._accumulators[merge_step], self._accumulator_counts[merge_step]
         self._completed_merges.add(merge_step)

@@ -247,6 +247,7 @@ class TransformerTrainModule(TrainModule):
 
     def load_state_dict(self, state_dict: Dict[str, Any]) -> None:
         from ....distributed.utils import get_local_tensor
+        from ....float8 import refresh_float8_scales
 
         if self.load_key_mapping is not None:
             from ....distributed.checkpoint import swap_param_keys
@@ -293,6 +294,7 @@ class TransformerTrainModule(TrainModule):
                                 group[field] = osd[key]
         if self.runtime is not None:
             self.runtime.sync_lowp()
+        refresh_float8_scales(self.model)  # 8-bit copies of the weights that were just overwritten
         gc_cuda()
 
     # -- training ------------------------------------------------------------------------------------------------
