@@ -211,6 +211,28 @@ Tensor block_product(const Tensor& x, const Tensor& codes, const Tensor& scales,
     return product(matrix(x, trans ? cols : rows), w, trans, offsets.has_value() ? offsets->const_data_ptr<int>() : nullptr, nullptr, status);
 }
 
+// What the kernels write to and read from by address alone: `main_grad` of a weight w (rows of a dense one may be apart), and its
+// codes and scales as tile_buffer() makes them.
+void check_main_grad(const optional<Tensor>& grad, const Tensor& w, bool stacked) {
+    if (!grad.has_value()) return;
+    TORCH_CHECK_VALUE(grad->scalar_type() == at::kFloat && grad->device() == w.device(), "main_grad must be float32 on ", w.device(),
+                      ", got ", grad->scalar_type(), " on ", grad->device());
+    const bool fits = stacked ? grad->numel() == w.numel() && grad->is_contiguous()
+                              : grad->sizes() == w.sizes() && (w.size(1) <= 1 || grad->stride(1) == 1) &&
+                                    (w.size(0) <= 1 || grad->stride(0) >= w.size(1));
+    TORCH_CHECK_VALUE(fits, "main_grad of shape ", grad->sizes(), " and strides ", grad->strides(), " does not fit a weight of shape ", w.sizes(),
+                      stacked ? ": it must be contiguous" : ": rows must be contiguous");
+}
+
+void check_cached(const optional<Tensor>& tiles, const Tensor& w, int64_t groups) {
+    if (!tiles.has_value()) return;
+    const int64_t rows = w.size(0) / groups, cols = w.size(1);
+    TORCH_CHECK_VALUE(tiles->scalar_type() == at::kByte && tiles->device() == w.device() && tiles->is_contiguous() &&
+                          tiles->numel() == groups * (rows * pitch_of(cols) + 4 * blocks(rows) * blocks(cols)),
+                      "the kept 8-bit form (", tiles->numel(), " x ", tiles->scalar_type(), " on ", tiles->device(),
+                      ") is not that of a weight of shape ", w.sizes(), " on ", w.device());
+}
+
 struct BlockLinear : torch::autograd::Function<BlockLinear> {
     // weight: what the gradient belongs to; w: its bf16 values [N, K]
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Tensor& w, const optional<Tensor>& cached,
@@ -257,7 +279,6 @@ struct BlockLinear : torch::autograd::Function<BlockLinear> {
             // the kernels write bf16 or fp32, whichever the parameter has
             Tensor out = accumulate ? ctx->saved_data["main_grad"].toTensor() : at::empty({n, k}, dy.options().dtype(w_dtype == at::kBFloat16 ? at::kBFloat16 : at::kFloat));
             const int epilogue = out.scalar_type() == at::kBFloat16 ? 0 : accumulate ? 1 : 2;
-            TORCH_CHECK(!accumulate || out.scalar_type() == at::kFloat, "main_grad must be float32");
             if (m == 0 || n == 0 || k == 0) {
                 if (!accumulate) out.zero_();
             } else if (!in_fp8) {
@@ -324,7 +345,6 @@ struct BlockGroupedLinear : torch::autograd::Function<BlockGroupedLinear> {
             const auto w_dtype = ctx->saved_data["w_dtype"].toScalarType();
             Tensor out = accumulate ? ctx->saved_data["main_grad"].toTensor()
                                     : at::empty({groups * rows, cols}, dy.options().dtype(w_dtype == at::kBFloat16 ? at::kBFloat16 : at::kFloat));
-            TORCH_CHECK(!accumulate || (out.scalar_type() == at::kFloat && out.is_contiguous()), "main_grad must be contiguous float32");
             if (dy.size(0) == 0) {
                 if (!accumulate) out.zero_();
             } else {
@@ -345,12 +365,16 @@ struct BlockGroupedLinear : torch::autograd::Function<BlockGroupedLinear> {
 Tensor block_grouped_linear(const Tensor& x, const Tensor& weight, const Tensor& w, const Tensor& offsets, const optional<Tensor>& cached,
                             const optional<Tensor>& main_grad, bool trans, int64_t status) {
     const bool needs_dw = at::GradMode::is_enabled() && (weight.requires_grad() || main_grad.has_value());
+    if (needs_dw) check_main_grad(main_grad, w, true);
+    check_cached(cached, w, offsets.size(0) - 1);
     return BlockGroupedLinear::apply(x, weight, w, offsets, cached, main_grad, trans, needs_dw, status);
 }
 
 Tensor block_linear(const Tensor& x, const Tensor& weight, const Tensor& w, const optional<Tensor>& cached,
                     const optional<Tensor>& main_grad, bool high_precision, int64_t status) {
     const bool needs_dw = at::GradMode::is_enabled() && (weight.requires_grad() || main_grad.has_value());
+    if (needs_dw) check_main_grad(main_grad, w, false);
+    check_cached(cached, w, 1);
     return BlockLinear::apply(x, weight, w, cached, main_grad, needs_dw, high_precision, status);
 }
 

@@ -437,6 +437,22 @@ def _cached(cache: Optional[dict], make, weight: torch.Tensor):
     return made
 
 
+def _check_main_grad(grad: Optional[torch.Tensor], w: torch.Tensor, stacked: bool) -> None:
+    """The host's check before anything is written to ``main_grad`` (on a GPU: ``csrc/torch_ops.cpp``)."""
+    if grad is None or not torch.is_grad_enabled():
+        return
+    if grad.dtype != torch.float32 or grad.device != w.device:
+        raise ValueError(f"main_grad must be float32 on {w.device}, got {grad.dtype} on {grad.device}")
+    if stacked:
+        fits = grad.numel() == w.numel() and grad.is_contiguous()
+    else:
+        N, K = w.shape
+        fits = grad.shape == w.shape and (K <= 1 or grad.stride(1) == 1) and (N <= 1 or grad.stride(0) >= K)
+    if not fits:
+        raise ValueError(f"main_grad of shape {tuple(grad.shape)} and strides {grad.stride()} does not fit a weight of shape "
+                         f"{tuple(w.shape)}: {'it' if stacked else 'rows'} must be contiguous")
+
+
 class BlockFloat8LinearFunction(torch.autograd.Function):
     """The layer on CPU tensors, through the emulated operations (on a GPU: ``csrc/torch_ops.cpp``)."""
 
@@ -493,6 +509,7 @@ def fp8_block_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch
                                         _lib.status_buffer(x.device).data_ptr())
         _lib.check(0, "ocb_linear_block_fp8")  # counted; a failed launch has raised
     else:
+        _check_main_grad(main_grad, weight if lowp is None else lowp, False)
         y = BlockFloat8LinearFunction.apply(x, weight, wgrad_high_precision, weight_cache)
     if main_grad is not None and hasattr(weight, "grad_added_to_main_grad") and torch.is_grad_enabled():
         weight.grad_added_to_main_grad = True  # by the backward pass
@@ -562,6 +579,7 @@ def fp8_block_grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: tor
                                                 _lib.status_buffer(x.device).data_ptr())
         _lib.check(0, "ocb_linear_block_fp8")  # counted; a failed launch has raised
     else:
+        _check_main_grad(main_grad, w, True)
         y = BlockFloat8GroupedLinearFunction.apply(x, weight, offsets, trans_b, weight_cache)
     if main_grad is not None and hasattr(weight, "grad_added_to_main_grad") and torch.is_grad_enabled():
         weight.grad_added_to_main_grad = True  # by the backward pass

@@ -1,0 +1,68 @@
+"""What the block-scaled layers check before they launch, and how they behave inside autograd."""
+
+import pytest
+import torch
+
+from olmo_core_b200.ops import fp8_block as fb
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+def _rand(shape, seed, device, std=1.0):
+    return (torch.randn(shape, generator=torch.Generator().manual_seed(seed)) * std).bfloat16().to(device)
+
+
+def _bad_main_grads(n, k, device):
+    """(main_grad, what the message says) that do not fit a weight of n x k."""
+    yield torch.zeros(n - 8, k, device=device), "does not fit"
+    yield torch.zeros(n, k - 8, device=device), "does not fit"
+    yield torch.zeros(k, n, device=device).t(), "does not fit"
+    yield torch.zeros(1, k, device=device).expand(n, k), "does not fit"
+    yield torch.zeros(n, k, dtype=torch.float64, device=device), "must be float32"
+    if device == "cuda":
+        yield torch.zeros(n, k), "must be float32 on"
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("hp", [False, True])
+def test_linear_refuses_a_main_grad_that_does_not_fit(hp, device):
+    x, w = _rand((16, 64), 1, device), torch.nn.Parameter(_rand((48, 64), 2, device))
+    for bad, text in _bad_main_grads(48, 64, device):
+        w.main_grad = bad
+        with pytest.raises(ValueError, match=text):
+            fb.fp8_block_linear(x, w, wgrad_high_precision=hp)
+        with torch.no_grad():  # nothing is going to be written
+            assert fb.fp8_block_linear(x, w).shape == (16, 48)
+    wide = torch.zeros(48, 72, device=device)
+    w.main_grad = wide[:, :64]  # rows apart are fine
+    fb.fp8_block_linear(x, w, wgrad_high_precision=hp).sum().backward()
+    assert wide[:, :64].abs().sum() > 0 and (wide[:, 64:] == 0).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_experts_refuse_a_main_grad_that_does_not_fit(device):
+    x, w = _rand((16, 64), 3, device), torch.nn.Parameter(_rand((2 * 48, 64), 4, device))
+    offsets = torch.tensor([0, 5, 16], dtype=torch.int32, device=device)
+    for bad, text in [*_bad_main_grads(96, 64, device), (torch.zeros(96, 72, device=device)[:, :64], "contiguous")]:
+        w.main_grad = bad
+        with pytest.raises(ValueError, match=text):
+            fb.fp8_block_grouped_linear(x, w, offsets)
+    w.main_grad = torch.zeros(2, 48, 64, device=device)
+    fb.fp8_block_grouped_linear(x, w, offsets).sum().backward()
+    assert w.main_grad.abs().sum() > 0
+
+
+@pytest.mark.gpu
+def test_kept_weights_of_another_size_are_refused():
+    from olmo_core_b200.ops import _lib
+
+    native, status = _lib.native(), _lib.status_buffer(torch.device("cuda", 0)).data_ptr()
+    x, w = _rand((16, 64), 5, "cuda"), _rand((48, 64), 6, "cuda")
+    offsets = torch.tensor([0, 5, 16], dtype=torch.int32, device="cuda")
+    tiles = native.block_tile_buffer(w, 1)
+    native.block_linear(x, w, w, tiles, None, False, status)
+    for bad in (tiles[:-4], tiles.cpu(), tiles.view(torch.int32), native.block_tile_buffer(_rand((40, 64), 7, "cuda"), 1)):
+        with pytest.raises(ValueError, match="kept 8-bit form"):
+            native.block_linear(x, w, w, bad, None, False, status)
+        with pytest.raises(ValueError, match="kept 8-bit form"):
+            native.block_grouped_linear(x, w, w, offsets, bad, None, True, status)
