@@ -401,6 +401,8 @@ __device__ __forceinline__ uint64_t bf16x2_to_f32x2(uint32_t u) {
 // ---- Programmatic dependent launch: a kernel launched with this attribute may start, as far as its own set-up, while the kernel in
 // front of it in the stream runs out. It calls previous_kernel_done() before its first access to global memory, and lets the
 // kernel behind it start the same way with next_kernel_may_start() (which takes effect once every CTA has called it).
+// Such a kernel lives while what it will read is still being written, so it reads global memory with plain loads or TMA only: the
+// read-only path (__ldg, ld.global.nc, const __restrict__ pointers) promises data that nobody writes as long as the kernel lives.
 __device__ __forceinline__ void previous_kernel_done() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void next_kernel_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

@@ -499,7 +499,7 @@ gemm_block_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
         for (int b = 0; b < SCALE_BATCH; ++b)
 #pragma unroll
           for (int i = 0; i < PER; ++i)  // rows outside the matrix: any valid scale, their products are not stored
-            next[b][i] = kb0 + b < num_kb && src[i] != nullptr ? __ldg(src[i] + (kb0 + b) * step[i]) : 1.f;
+            next[b][i] = kb0 + b < num_kb && src[i] != nullptr ? src[i][(kb0 + b) * step[i]] : 1.f;
       };
       fetch(0);
       for (int kb0 = 0; kb0 < num_kb; kb0 += SCALE_BATCH) {
@@ -644,7 +644,7 @@ struct SmallParams {
 // Eight elements of a row of x, zeros outside.
 __device__ __forceinline__ uint4 load_x8(const SmallParams& p, const __nv_bfloat16* row, int k) {
   if (row == nullptr || k >= p.K) return make_uint4(0u, 0u, 0u, 0u);
-  if (p.x_vector && k + 8 <= p.K) return __ldg(reinterpret_cast<const uint4*>(row + k));
+  if (p.x_vector && k + 8 <= p.K) return *reinterpret_cast<const uint4*>(row + k);
   uint32_t w[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
   for (int j = 0; j < 8; ++j)
@@ -837,7 +837,7 @@ gemm_block_fp8_small_kernel(const __grid_constant__ CUtensorMap tma_a, const __g
 #pragma unroll
       for (int b = 0; b < SCALE_BATCH; ++b)
 #pragma unroll
-        for (int i = 0; i < PER; ++i) next[b][i] = kb0 + b < kbs && src[i] != nullptr ? __ldg(src[i] + (kb0 + b) * step[i]) : 1.f;
+        for (int i = 0; i < PER; ++i) next[b][i] = kb0 + b < kbs && src[i] != nullptr ? src[i][(kb0 + b) * step[i]] : 1.f;
     };
     fetch(0);
     for (int kb0 = 0; kb0 < kbs; kb0 += SCALE_BATCH) {

@@ -66,3 +66,16 @@ def test_kept_weights_of_another_size_are_refused():
             native.block_linear(x, w, w, bad, None, False, status)
         with pytest.raises(ValueError, match="kept 8-bit form"):
             native.block_grouped_linear(x, w, w, offsets, bad, None, True, status)
+
+
+def test_kernels_that_start_early_use_no_read_only_loads():
+    """A kernel under programmatic dependent launch lives while its inputs are still written: the read-only path is not for it."""
+    import re
+
+    from olmo_core_b200.ops.build import CSRC_DIR
+
+    early = [f for f in sorted(CSRC_DIR.glob("*.cu")) if "previous_kernel_done()" in f.read_text()]
+    assert {f.name for f in early} == {"block_quant_sm100.cu", "gemm_block_fp8_sm100.cu"}
+    for f in [*early, CSRC_DIR / "block_quant.cuh"]:
+        code = re.sub(r"//[^\n]*", "", f.read_text())
+        assert not re.search(r"__ldg|ld\.global\.nc|__restrict__|__ldcs|__ldca", code), f.name
