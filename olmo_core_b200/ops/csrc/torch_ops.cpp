@@ -90,6 +90,25 @@ struct Route : torch::autograd::Function<Route> {
         return {weights, experts, scores, counts};
     }
 
+    // The gradient in tensor operations, for a graph that is going to be differentiated itself. kept: the logits (sigmoid) or the
+    // scores, with their own history. Same formulas as the kernel's.
+    static Tensor differentiable(const Tensor& kept, const Tensor& experts, const Tensor& d_weights, const Tensor& d_scores, bool sigmoid,
+                                 int64_t normalize) {
+        const Tensor x = kept.to(at::kFloat), p = sigmoid ? x.sigmoid() : x, s = sigmoid ? p + 1e-7 : x;
+        Tensor d = d_scores.defined() ? d_scores.to(at::kFloat) : at::zeros_like(s);
+        if (d_weights.defined()) {
+            Tensor g = d_weights.to(at::kFloat);
+            if (normalize != 0) {
+                const Tensor c = s.gather(1, experts), total = (normalize == 1 ? c : c * c).sum(1, true), none = total == 0;
+                const Tensor safe = total.masked_fill(none, 1.0), norm = normalize == 1 ? safe : safe.sqrt(), w = c / norm;
+                const Tensor along = (g * w).sum(1, true);
+                g = ((g - (normalize == 1 ? along : along * w)) / norm).masked_fill(none, 0.0);
+            }
+            d = d.scatter_add(1, experts, g);
+        }
+        return sigmoid ? d * p * (-x).sigmoid() : s * (d - (d * s).sum(1, true));
+    }
+
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const Tensor &d_weights = grads[0], &d_scores = grads[2];
         if (!d_weights.defined() && !d_scores.defined()) return {Tensor(), Tensor(), Tensor()};
@@ -97,6 +116,9 @@ struct Route : torch::autograd::Function<Route> {
         const Tensor &kept = saved[0], &experts = saved[1];
         const c10::cuda::OptionalCUDAGuard guard(kept.device());
         const int sigmoid = static_cast<int>(ctx->saved_data["sigmoid"].toInt());
+        if (at::GradMode::is_enabled())
+            return {differentiable(kept, experts, d_weights, d_scores, sigmoid != 0, ctx->saved_data["normalize"].toInt())
+                        .to(ctx->saved_data["bf16"].toBool() ? at::kBFloat16 : at::kFloat), Tensor(), Tensor()};
         const Tensor dw = d_weights.defined() ? d_weights.to(at::kFloat).contiguous() : d_weights;
         const Tensor ds = d_scores.defined() ? d_scores.to(at::kFloat).contiguous() : d_scores;
         Tensor d_logits = at::empty({kept.size(0), kept.size(1)}, kept.options().dtype(ctx->saved_data["bf16"].toBool() ? at::kBFloat16 : at::kFloat));
@@ -115,6 +137,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> route(const Tensor& logits, int64_t t
                                                  int64_t n_groups, int64_t top_groups, int64_t normalize) {
     const RouteOptions o{static_cast<int>(top_k), sigmoid, static_cast<int>(n_groups), static_cast<int>(top_groups),
                          static_cast<int>(normalize)};
+    TORCH_CHECK(!logits._fw_grad(0).defined(), "the routing kernel computes no tangents: routing differentiates forwards in tensor operations");
     if (!logits.requires_grad() || !at::GradMode::is_enabled()) return run_route(logits, bias, o);
     const variable_list out = Route::apply(logits, bias, o);
     return {out[0], out[1], out[2], out[3]};

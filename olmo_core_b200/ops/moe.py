@@ -85,6 +85,12 @@ def _route_reference(logits, top_k, gating, score_bias, n_groups, top_k_groups, 
     return weights, experts, scores, counts
 
 
+def _transformed(x: torch.Tensor) -> bool:
+    """Whether ``x`` carries a tangent or stands for another tensor inside a ``torch.func`` transform."""
+    return (torch._C._functorch.is_functorch_wrapped_tensor(x)
+            or torch.autograd.forward_ad.unpack_dual(x).tangent is not None)
+
+
 def route(
     logits: torch.Tensor,
     top_k: int,
@@ -108,8 +114,9 @@ def route(
     experts stay open. The ranking is that of exact arithmetic. A token without any logit above ``-inf`` gets softmax scores
     and weights of zero.
 
-    Gradients flow from ``weights`` and ``scores`` to ``logits``. One kernel each way on CUDA (at most 1024 experts, 32 chosen,
-    32 groups).
+    Gradients flow from ``weights`` and ``scores`` to ``logits``, of any order, and tangents the other way. One kernel each way on
+    CUDA (at most 1024 experts, 32 chosen, 32 groups); gradients that are differentiated themselves (``create_graph=True``),
+    forward-mode derivatives and ``torch.func`` transforms take tensor operations.
     """
     if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16):
         raise ValueError(f"logits must be float32 or bfloat16 [N, E], got {logits.dtype} {tuple(logits.shape)}")
@@ -129,7 +136,7 @@ def route(
                              f"{tuple(score_bias.shape)} on {score_bias.device}")
         score_bias = score_bias.detach().contiguous()
     options = (top_k, gating, score_bias, n_groups, top_k_groups, int(normalize or 0))
-    if not logits.is_cuda:
+    if not logits.is_cuda or _transformed(logits):
         return _route_reference(logits, *options)
     if not route_supported(e, top_k, n_groups):
         raise ValueError(f"the routing kernels take at most 1024 experts, 32 chosen and 32 groups, got {e}, {top_k} and {n_groups}")

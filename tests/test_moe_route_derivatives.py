@@ -1,0 +1,133 @@
+"""Derivatives of the routing beyond the first gradient: second order, forward mode, and torch.func transforms."""
+
+import pytest
+import torch
+
+from olmo_core_b200.ops.moe import _route_reference, route
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+OPTIONS = [dict(gating=gating, normalize=normalize, n_groups=groups, top_k_groups=max(1, groups // 2), biased=biased)
+           for gating in ("softmax", "sigmoid") for normalize in (None, 1, 2) for groups, biased in ((1, False), (4, True))]
+# fp32 sums of 32 terms of size one, a few operations deep on either side: 2^-24 times a hundred
+TOLERANCE = dict(rtol=1e-5, atol=1e-5)
+
+
+def _case(options, device, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    options = dict(options)
+    x = torch.randn(9, 32, generator=g).to(device)
+    options["score_bias"] = (torch.randn(32, generator=g) * 0.1).to(device) if options.pop("biased") else None
+    d_weights, d_scores = torch.randn(9, 4, generator=g).to(device), torch.randn(9, 32, generator=g).to(device)
+    return x, options, d_weights, d_scores
+
+
+def _exact(x, experts, options):
+    """weights and scores of the experts that were chosen, in fp64."""
+    x = x.double()
+    scores = x.softmax(-1) if options["gating"] == "softmax" else torch.sigmoid(x) + 1e-7
+    weights = scores.gather(1, experts)
+    return weights if options["normalize"] is None else weights / weights.norm(p=options["normalize"], dim=1, keepdim=True), scores
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("options", OPTIONS)
+def test_second_order(options, device):
+    x, options, dw, ds = _case(options, device)
+    results = []
+    for exact in (False, True):
+        leaf = x.clone().requires_grad_(True)
+        a, b = dw.clone().requires_grad_(True), ds.clone().requires_grad_(True)
+        weights, experts, scores, _ = route(leaf, 4, **options)
+        if exact:
+            weights, scores = _exact(leaf, experts, options)
+            a, b = a.double().detach().requires_grad_(True), b.double().detach().requires_grad_(True)
+        (first,) = torch.autograd.grad((weights, scores), leaf, (a, b), create_graph=True)
+        assert first.requires_grad
+        loss = first.square().sum() + (first * x).sum() + weights.square().sum()
+        results.append([first.detach(), *torch.autograd.grad(loss, (leaf, a, b))])
+    for got, want in zip(*results):
+        torch.testing.assert_close(got.double(), want.double(), **TOLERANCE)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("which", [0, 2])
+def test_second_order_of_one_output_and_in_bf16(which, device):
+    x, options, _, _ = _case(OPTIONS[1], device)
+    leaf = x.bfloat16().requires_grad_(True)
+    out = route(leaf, 4, **options)
+    (first,) = torch.autograd.grad(out[which].square().sum(), leaf, create_graph=True)
+    (second,) = torch.autograd.grad(first.float().square().sum(), leaf)
+    assert first.dtype == second.dtype == torch.bfloat16
+    first_of = torch.func.grad(lambda t: _exact(t, out[1], options)[which // 2].square().sum())
+    exact = x.bfloat16().double()
+    first, hessian = first_of(exact), torch.func.jacrev(first_of)(exact)
+    want = (hessian * 2 * first).sum((2, 3))
+    # the first gradient and the gradient that reaches it are rounded to bf16 (2^-8 each), and so is the result
+    bound = (hessian.abs() * 4 * 2.0 ** -8 * first.abs()).sum((2, 3)) + 2.0 ** -8 * want.abs() + 1e-5
+    assert ((second.double() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("options", OPTIONS)
+@pytest.mark.parametrize("needs_grad", [False, True])
+def test_forward_mode(options, needs_grad, device):
+    import torch.autograd.forward_ad as fwd
+
+    x, options, _, _ = _case(options, device)
+    tangent = torch.randn(9, 32, generator=torch.Generator().manual_seed(5)).to(device)
+    with fwd.dual_level():
+        weights, experts, scores, counts = route(fwd.make_dual(x.clone().requires_grad_(needs_grad), tangent), 4, **options)
+        got = [fwd.unpack_dual(t).tangent for t in (weights, scores)]
+        want = [fwd.unpack_dual(t).tangent for t in _exact(fwd.make_dual(x.double(), tangent.double()), experts, options)]
+    assert all(t is not None for t in got)
+    for a, b in zip(got, want):
+        torch.testing.assert_close(a.double(), b, **TOLERANCE)
+    plain = route(x, 4, **options)
+    assert torch.equal(plain[1], experts) and torch.equal(plain[3], counts)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("options", OPTIONS[:2] + OPTIONS[-2:])
+def test_func_transforms(options, device):
+    x, options, dw, ds = _case(options, device)
+
+    def loss(t):
+        weights, _, scores, _ = route(t, 4, **options)
+        return (weights * dw).sum() + (scores * ds).sum()
+
+    leaf = x.clone().requires_grad_(True)
+    loss(leaf).backward()
+    torch.testing.assert_close(torch.func.grad(loss)(x), leaf.grad, **TOLERANCE)
+    _, along = torch.func.jvp(loss, (x,), (dw.sum() * ds,))
+    torch.testing.assert_close(along, (leaf.grad * dw.sum() * ds).sum(), rtol=1e-4, atol=1e-4)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("gating", ["softmax", "sigmoid"])
+def test_router_module_second_order(gating, device):
+    from olmo_core_b200.nn.moe.router import MoERouterConfig, MoERouterGatingFunction
+
+    router = MoERouterConfig(top_k=2, gating_function=MoERouterGatingFunction(gating)).build(16, 8).to(device)
+    x = torch.randn(1, 5, 16, generator=torch.Generator().manual_seed(1)).to(device).requires_grad_(True)
+    weights, _, _, _ = router(x)
+    (first,) = torch.autograd.grad(weights.square().sum(), x, create_graph=True)
+    penalty = first.square().sum() + x.sum()  # another term carries a graph of its own
+    (got,) = torch.autograd.grad(penalty, router.weight)
+    assert got.abs().sum() > 0
+    logits = router.get_expert_logits(x).view(5, 8)
+    want_weights, _, _, _ = _route_reference(logits, 2, gating, None, 1, 1, 0)
+    (first,) = torch.autograd.grad(want_weights.square().sum(), x, create_graph=True)
+    (want,) = torch.autograd.grad(first.square().sum() + x.sum(), router.weight)
+    torch.testing.assert_close(got, want, **TOLERANCE)
+
+
+@pytest.mark.gpu
+def test_the_kernels_op_itself_refuses_tangents():
+    import torch.autograd.forward_ad as fwd
+
+    from olmo_core_b200.ops import _lib
+
+    x = torch.randn(3, 8, device="cuda")
+    for needs_grad in (False, True):
+        with fwd.dual_level(), pytest.raises(RuntimeError, match="tangents"):
+            _lib.native().route.default(fwd.make_dual(x.clone().requires_grad_(needs_grad), x), 2, False, None, 1, 1, 0)
