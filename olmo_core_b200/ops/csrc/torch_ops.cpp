@@ -8,6 +8,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <dlfcn.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 
 #include "ocb_api.h"
@@ -234,6 +235,16 @@ Tensor block_product(const Tensor& x, const Tensor& codes, const Tensor& scales,
     return product(matrix(x, trans ? cols : rows), w, trans, offsets.has_value() ? offsets->const_data_ptr<int>() : nullptr, nullptr, status);
 }
 
+// The gradients of a layer whose own derivative is not built: where a graph of them is kept, differentiating it is an error.
+variable_list first_order(variable_list grads) {
+    if (!at::GradMode::is_enabled()) return grads;
+    for (Tensor& g : grads)
+        if (g.defined()) g = g.detach().requires_grad_(true);
+    const auto error = std::make_shared<torch::autograd::DelayedError>("the block-scaled layers have no second derivative",
+                                                                       static_cast<int>(grads.size()));
+    return (*error)(std::move(grads));
+}
+
 // What the kernels write to and read from by address alone: `main_grad` of a weight w (rows of a dense one may be apart), and its
 // codes and scales as tile_buffer() makes them.
 void check_main_grad(const optional<Tensor>& grad, const Tensor& w, bool stacked) {
@@ -327,7 +338,7 @@ struct BlockLinear : torch::autograd::Function<BlockLinear> {
             }
             if (!accumulate) dw = out.scalar_type() == w_dtype ? out : out.to(w_dtype);
         }
-        return {dx, dw, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+        return first_order({dx, dw, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()});
     }
 };
 
@@ -381,7 +392,7 @@ struct BlockGroupedLinear : torch::autograd::Function<BlockGroupedLinear> {
             }
             if (!accumulate) dw = out.scalar_type() == w_dtype ? out : out.to(w_dtype);
         }
-        return {dx, dw, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+        return first_order({dx, dw, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()});
     }
 };
 

@@ -26,6 +26,7 @@ On CPU the functions emulate the same arithmetic in PyTorch: the numerical oracl
 
 from __future__ import annotations
 
+import functools
 from typing import Optional, Tuple
 
 import torch
@@ -453,6 +454,21 @@ def _check_main_grad(grad: Optional[torch.Tensor], w: torch.Tensor, stacked: boo
                          f"{tuple(w.shape)}: {'it' if stacked else 'rows'} must be contiguous")
 
 
+def _first_order(backward):
+    """For a backward pass whose own derivative is not built: differentiating its result is an error."""
+
+    @functools.wraps(backward)
+    def wrapper(ctx, dy):
+        with torch.no_grad():
+            grads = backward(ctx, dy)
+        if not torch.is_grad_enabled():
+            return grads
+        error = torch._C._functions.DelayedError(b"the block-scaled layers have no second derivative", len(grads))
+        return error(*[g if g is None else g.detach().requires_grad_(True) for g in grads])
+
+    return wrapper
+
+
 class BlockFloat8LinearFunction(torch.autograd.Function):
     """The layer on CPU tensors, through the emulated operations (on a GPU: ``csrc/torch_ops.cpp``)."""
 
@@ -467,6 +483,7 @@ class BlockFloat8LinearFunction(torch.autograd.Function):
         return gemm_fp8_block(*quantize_block_rows(x2), wq, sw).view(*x.shape[:-1], w.shape[0])
 
     @staticmethod
+    @_first_order
     def backward(ctx, dy):  # type: ignore[override]
         wq, sw, x2 = ctx.saved_tensors
         weight = ctx.weight_ref
@@ -492,7 +509,7 @@ def fp8_block_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch
     """
     ``x @ weight^T (+ bias)`` with block-scaled e4m3 operands in all three products; any sizes. ``wgrad_high_precision``
     keeps the weight gradient in bf16 (widths must then be multiples of 8). ``weight_cache``: see
-    :func:`olmo_core_b200.ops.fp8.cached_weight_cast`.
+    :func:`olmo_core_b200.ops.fp8.cached_weight_cast`. First derivatives only: differentiating the gradients is an error.
     """
     if x.shape[-1] != weight.shape[-1]:
         raise ValueError(f"x has {x.shape[-1]} features, the weight takes {weight.shape[-1]}")
@@ -529,6 +546,7 @@ class BlockFloat8GroupedLinearFunction(torch.autograd.Function):
         return grouped_gemm_fp8_block(*quantize_block_rows(x2), wq, sw, offsets, trans_b=trans_b)
 
     @staticmethod
+    @_first_order
     def backward(ctx, dy):  # type: ignore[override]
         wq, sw, offsets, x2 = ctx.saved_tensors
         trans_b, weight = ctx.trans_b, ctx.weight_ref
@@ -554,7 +572,7 @@ def fp8_block_grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: tor
     gradient is taken in bf16, because the 128-row blocks of a column scale would run across the experts' boundaries.
     ``x [R, K]`` sorted by expert, ``offsets`` int32 ``[G + 1]`` (row boundaries, see :func:`grouped_gemm_fp8_block`), ``weight``
     the experts' matrices stacked: ``[G * N, K]`` with ``trans_b`` (``y = x W_g^T``) else ``[G * K, N]`` (``y = x W_g``). Widths
-    must be multiples of 8. Rows outside every group are undefined.
+    must be multiples of 8. Rows outside every group are undefined. First derivatives only, as :func:`fp8_block_linear`.
     """
     G = offsets.numel() - 1
     w = getattr(weight, "_lowp", None)

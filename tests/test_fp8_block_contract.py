@@ -79,3 +79,24 @@ def test_kernels_that_start_early_use_no_read_only_loads():
     for f in [*early, CSRC_DIR / "block_quant.cuh"]:
         code = re.sub(r"//[^\n]*", "", f.read_text())
         assert not re.search(r"__ldg|ld\.global\.nc|__restrict__|__ldcs|__ldca", code), f.name
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("grouped", [False, True])
+@pytest.mark.parametrize("constant", [False, True])
+def test_layers_refuse_a_second_derivative(constant, grouped, device):
+    x, w = _rand((16, 64), 8, device).requires_grad_(True), _rand((48, 64), 9, device).requires_grad_(True)
+    offsets = torch.tensor([0, 5, 16], dtype=torch.int32, device=device)
+    dy = _rand((16, 24 if grouped else 48), 10, device).requires_grad_(not constant)
+
+    def grads(**kwargs):
+        y = fb.fp8_block_grouped_linear(x, w, offsets) if grouped else fb.fp8_block_linear(x, w)
+        return torch.autograd.grad(y, (x, w), dy, **kwargs)
+
+    first = grads(create_graph=True)
+    for a, b in zip(first, grads()):
+        assert torch.equal(a, b)
+    for g in first:
+        with pytest.raises(RuntimeError, match="no second derivative"):
+            (g.float().square().sum() + x.float().sum()).backward(retain_graph=True)
+    x.float().square().sum().backward()  # a graph that does not pass through them is none of their business
