@@ -31,9 +31,10 @@ namespace route {
 
 constexpr unsigned FULL = 0xffffffffu;
 constexpr float SIGMOID_FLOOR = 1e-7f;
-// Error bounds of an fp32 score (all are <= 1). Softmax: a sum of up to 1024 terms (37 roundings on the longest path), the fast
-// exponential and the reciprocal. Sigmoid: s (1 - s) times the exponential's relative error of (2 + 1.2 |x|) 2^-23, and three
-// roundings.
+// Bounds on the absolute error of an fp32 score (all are <= 1), at least twice what the operations can add up to. Softmax: a sum of
+// up to 1024 terms (37 roundings on the longest path), exponentials (two steps of 2^-23) and the reciprocal: below 43 2^-24.
+// Sigmoid: s (1 - s) times the exponential's relative error, and three roundings: 2^-22. The exponential is expf, not the fast one,
+// whose relative error grows with |x|: small sigmoid scores, and weights made from them, would be off by |x| steps.
 constexpr float SOFTMAX_ERROR = 3.8e-6f;  // 2^-18
 constexpr float SIGMOID_ERROR = 4.8e-7f;  // 2^-21
 
@@ -201,14 +202,14 @@ __global__ void route_kernel(const Params p, int lanes_per_group, int alone) {
     fetch(t + stride);
     if (p.sigmoid) {
 #pragma unroll
-      for (int i = 0; i < PL; ++i) s[i] = 1.f / (1.f + __expf(-x[i])) + SIGMOID_FLOOR;
+      for (int i = 0; i < PL; ++i) s[i] = 1.f / (1.f + expf(-x[i])) + SIGMOID_FLOOR;
     } else {
 #pragma unroll
       for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, o));
       float sum = 0.f;
 #pragma unroll
       for (int i = 0; i < PL; ++i) {
-        s[i] = (i * 32 + lane) < p.n_experts ? __expf(x[i] - top) : 0.f;
+        s[i] = (i * 32 + lane) < p.n_experts ? expf(x[i] - top) : 0.f;
         sum += s[i];
       }
       const float inv = 1.f / sum_warp(sum);
@@ -354,7 +355,7 @@ __global__ void route_grad_kernel(const GradParams p) {
           const float v = __shfl_sync(FULL, s[i], mine & 31);
           w = (mine & ~31) == i * 32 ? v : w;
         }
-        if (p.sigmoid) w = 1.f / (1.f + __expf(-w)) + SIGMOID_FLOOR;
+        if (p.sigmoid) w = 1.f / (1.f + expf(-w)) + SIGMOID_FLOOR;
         if (lane >= p.top_k) w = 0.f;
         const float total = sum_warp(p.normalize == 1 ? w : w * w);
         const float norm = p.normalize == 1 ? total : sqrtf(total);
@@ -372,7 +373,7 @@ __global__ void route_grad_kernel(const GradParams p) {
     if (p.sigmoid) {
 #pragma unroll
       for (int i = 0; i < PL; ++i) {
-        const float z = __expf(-fabsf(s[i]));  // p (1 - p) = z / (1 + z)^2, without cancellation
+        const float z = expf(-fabsf(s[i]));  // p (1 - p) = z / (1 + z)^2, without cancellation
         d[i] *= z / ((1.f + z) * (1.f + z));
       }
     } else {

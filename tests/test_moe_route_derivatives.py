@@ -131,3 +131,31 @@ def test_the_kernels_op_itself_refuses_tangents():
     for needs_grad in (False, True):
         with fwd.dual_level(), pytest.raises(RuntimeError, match="tangents"):
             _lib.native().route.default(fwd.make_dual(x.clone().requires_grad_(needs_grad), x), 2, False, None, 1, 1, 0)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("biased", [False, True])
+def test_scores_weights_and_gradients_keep_their_relative_accuracy(biased, device):
+    """Sigmoid scores over many magnitudes, with U = 2^-24 per rounding: the exponential 4 U (two steps), three more operations;
+    weights: twice that, a sum of 4 and a division; gradient p (1 - p) = z / (1 + z)^2: 4 U of z, 2 (1 + 2) of 1 + z, four more."""
+    U = 2.0 ** -24
+    x = torch.linspace(-25, 25, 64 * 500).view(500, 64)[:, torch.randperm(64, generator=torch.Generator().manual_seed(2))].to(device)
+    bias = torch.zeros(64, device=device) if biased else None
+    leaf = x.clone().requires_grad_(True)
+    weights, experts, scores, _ = route(leaf, 4, gating="sigmoid", score_bias=bias, normalize=1)
+    d = torch.randn(500, 64, generator=torch.Generator().manual_seed(3)).to(device)
+    (grad,) = torch.autograd.grad(scores, leaf, d)
+    xd = x.double()
+    want = torch.sigmoid(xd) + 1e-7
+    assert ((scores.double() - want).abs() <= 8 * U * want).all()
+    chosen = want.gather(1, experts)
+    chosen = chosen / chosen.sum(1, keepdim=True)
+    assert ((weights.double() - chosen).abs() <= 24 * U * chosen).all()
+    if device == "cuda":  # the tensor form takes 1 - p as it comes
+        slope = d.double() * torch.sigmoid(xd) * torch.sigmoid(-xd)
+        assert ((grad.double() - slope).abs() <= 16 * U * slope.abs()).all()
+    soft = route(x, 4, score_bias=bias)[2].double()
+    want = xd.softmax(-1)
+    # the difference to the maximum is rounded once (half a step of numbers up to 64: 32 U of the exponential), the exponential 4 U;
+    # the same for the terms of the sum, whose own additions are 6 deep; reciprocal and product
+    assert ((soft - want).abs() <= (2 * (32 + 4) + 8 + 3) * U * want).all()
