@@ -86,9 +86,11 @@ def _route_reference(logits, top_k, gating, score_bias, n_groups, top_k_groups, 
 
 
 def _transformed(x: torch.Tensor) -> bool:
-    """Whether ``x`` carries a tangent or stands for another tensor inside a ``torch.func`` transform."""
-    return (torch._C._functorch.is_functorch_wrapped_tensor(x)
-            or torch.autograd.forward_ad.unpack_dual(x).tangent is not None)
+    """Whether ``x`` carries a tangent or stands for another tensor inside a ``torch.func`` transform. Asks first whether there is
+    any level of either, which is the cheap question."""
+    functorch, forward_ad = torch._C._functorch, torch.autograd.forward_ad
+    return ((functorch.maybe_current_level() is not None and functorch.is_functorch_wrapped_tensor(x))
+            or (forward_ad._current_level >= 0 and forward_ad.unpack_dual(x).tangent is not None))
 
 
 def route(
