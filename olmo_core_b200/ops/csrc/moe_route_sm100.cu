@@ -194,6 +194,7 @@ __global__ void route_kernel(const Params p, int lanes_per_group, int alone) {
   for (; t < p.n_tokens; t += stride) {
     float x[PL], s[PL];
     float top = -INFINITY;
+    bool any = false;  // softmax: a logit above -inf, or NaN
 #pragma unroll
     for (int i = 0; i < PL; ++i) {
       x[i] = next[i];
@@ -213,8 +214,7 @@ __global__ void route_kernel(const Params p, int lanes_per_group, int alone) {
         sum += s[i];
       }
       const float inv = 1.f / sum_warp(sum);
-      // NaN logits do not take part in the maximum, so a maximum of -inf with a sum that is not NaN cannot happen
-      bool any = false;
+      // NaN logits do not take part in the maximum: beside -inf alone they leave it at -inf, with a sum of NaN
 #pragma unroll
       for (int i = 0; i < PL; ++i) any |= (i * 32 + lane) < p.n_experts && !(x[i] == -INFINITY);
       any = __any_sync(FULL, any);
@@ -269,7 +269,7 @@ __global__ void route_kernel(const Params p, int lanes_per_group, int alone) {
         }
         sum = sum_warp(sum);
 #pragma unroll
-        for (int i = 0; i < PL; ++i) d[i] = top == -INFINITY ? 0.0 : d[i] / sum;
+        for (int i = 0; i < PL; ++i) d[i] = any ? d[i] / sum : 0.0;
       }
       if (p.bias != nullptr) {
 #pragma unroll

@@ -1,4 +1,4 @@
-"""Derivatives of the routing beyond the first gradient: second order, forward mode, and torch.func transforms."""
+"""Routing: derivatives beyond the first gradient (second order, forward mode, torch.func transforms), accuracy, and rows of NaN."""
 
 import pytest
 import torch
@@ -159,3 +159,19 @@ def test_scores_weights_and_gradients_keep_their_relative_accuracy(biased, devic
     # the difference to the maximum is rounded once (half a step of numbers up to 64: 32 U of the exponential), the exponential 4 U;
     # the same for the terms of the sum, whose own additions are 6 deep; reciprocal and product
     assert ((soft - want).abs() <= (2 * (32 + 4) + 8 + 3) * U * want).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("groups", [1, 4])
+def test_a_row_of_nan_and_masked_logits_ranks_like_nan(groups, device):
+    """Softmax scores of such a row are all NaN, so no expert is ahead of another, whatever the bias."""
+    x = torch.randn(3, 16, generator=torch.Generator().manual_seed(6))
+    x[1] = float("-inf")
+    x[1, 5] = float("nan")
+    bias = torch.linspace(-1, 1, 16)
+    options = dict(score_bias=bias.to(device), n_groups=groups, top_k_groups=max(1, groups // 2))
+    weights, experts, scores, _ = route(x.to(device), 4, **options)
+    assert scores[1].isnan().all() and weights[1].isnan().all() and experts[1].tolist() == [0, 1, 2, 3]
+    for t in (0, 2):
+        alone = route(x[t:t + 1].to(device), 4, **options)
+        assert torch.equal(alone[1][0], experts[t]) and torch.equal(alone[0][0], weights[t])
