@@ -250,13 +250,13 @@ class MoERouter(nn.Module):
         """
         x = self.jitter(x)
         logits = self.get_expert_logits(x).float()
-        # a subclass may choose from biased or sigmoid scores in its own way
+        # a subclass may choose from biased or sigmoid scores, or among groups, in its own way
         own_choice = type(self).get_top_k is not MoERouter.get_top_k and (
-            self.bias_gamma is not None or self.gating_function != MoERouterGatingFunction.softmax)
+            self.bias_gamma is not None or self.n_groups > 1 or self.gating_function != MoERouterGatingFunction.softmax)
         fused = (logits.is_cuda and not self.uniform_expert_assignment and not own_choice
                  and moe_ops.route_supported(self.num_experts, self.top_k, self.n_groups))
         normalized = False
-        if fused or self.n_groups > 1:
+        if fused or (self.n_groups > 1 and not own_choice):
             normalized = self.normalize_expert_weights in (1, 2)
             weights, indices, scores, kernel_counts = moe_ops.route(
                 logits.reshape(-1, self.num_experts), self.top_k, gating=str(self.gating_function),

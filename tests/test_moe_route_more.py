@@ -175,3 +175,21 @@ def test_a_row_of_nan_and_masked_logits_ranks_like_nan(groups, device):
     for t in (0, 2):
         alone = route(x[t:t + 1].to(device), 4, **options)
         assert torch.equal(alone[1][0], experts[t]) and torch.equal(alone[0][0], weights[t])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("gating", ["softmax", "sigmoid"])
+def test_a_router_with_its_own_choice_is_asked_with_groups_too(gating, device):
+    from olmo_core_b200.nn.moe.router import MoELinearRouter, MoERouterGatingFunction
+
+    class Last(MoELinearRouter):
+        def get_top_k(self, scores):
+            indices = torch.arange(6, 8, device=scores.device).expand(*scores.shape[:-1], 2)
+            return scores.gather(-1, indices), indices
+
+    router = Last(d_model=16, num_experts=8, top_k=2, n_groups=4, top_k_groups=2, normalize_expert_weights=1.0,
+                  gating_function=MoERouterGatingFunction(gating)).to(device)
+    x = torch.randn(2, 3, 16, generator=torch.Generator().manual_seed(5)).to(device)
+    weights, experts, counts, _ = router(x)
+    assert experts.flatten().tolist() == [6, 7] * 6 and counts.flatten().tolist() == [0] * 6 + [6, 6]
+    torch.testing.assert_close(weights.sum(-1), torch.ones(2, 3, device=device))
