@@ -134,6 +134,8 @@ def set_nvtx(enabled: bool) -> None:
     if isinstance(_lib, _Library):
         for name in [k for k in vars(_lib) if k != "_handle"]:
             object.__delattr__(_lib, name)
+    if _native is not None:
+        _set_native_ranges()
 
 
 def nvtx_enabled() -> bool:
@@ -179,9 +181,25 @@ def native():
         if not NATIVE_LIB_PATH.exists():
             raise KernelError(f"{NATIVE_LIB_PATH} is missing. Build it with `python -m olmo_core_b200.ops.build`.")
         torch.ops.load_library(str(NATIVE_LIB_PATH))
-        torch.ops.ocb_native.bind_kernels(str(LIB_PATH))
+        torch.ops.ocb_native.bind_kernels(str(LIB_PATH), id(KernelError))
         _native = torch.ops.ocb_native
+        _set_native_ranges()
     return _native
+
+
+@ctypes.CFUNCTYPE(None, ctypes.c_char_p)
+def _push_range(name: bytes) -> None:
+    torch.cuda.nvtx.range_push(name.decode())
+
+
+@ctypes.CFUNCTYPE(None)
+def _pop_range() -> None:
+    torch.cuda.nvtx.range_pop()
+
+
+def _set_native_ranges() -> None:
+    push, pop = (ctypes.cast(fn, c_void_p).value if _nvtx_enabled else 0 for fn in (_push_range, _pop_range))
+    torch.ops.ocb_native.set_ranges(push, pop)
 
 
 def register_signature(name: str, argtypes) -> None:
@@ -216,13 +234,19 @@ def dt(t: torch.Tensor) -> int:
     raise KernelError(f"unsupported dtype {t.dtype}: the sm_100a kernels take bfloat16 or float32")
 
 
-launch_count = 0
+_checked_launches = 0
+
+
+def __getattr__(name: str):
+    if name == "launch_count":  # launcher calls so far, from Python and from the native ops, backward passes included
+        return _checked_launches + (0 if _native is None else torch.ops.ocb_native.launch_count())
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 
 
 def check(rc: int, what: str) -> None:
     """Validate a launcher's return code; also counts launcher calls (see ``launch_count``)."""
-    global launch_count
-    launch_count += 1
+    global _checked_launches
+    _checked_launches += 1
     if rc != 0:
         raise KernelError(f"{what} failed with code {rc}")
 

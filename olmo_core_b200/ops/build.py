@@ -14,6 +14,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 from typing import List, Optional
@@ -130,7 +131,7 @@ def build_native(force: bool = False, verbose: bool = True) -> Path:
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *map(str, srcs), "-o", str(NATIVE_LIB_PATH)]
     cuda_include = Path(_nvcc()).parent.parent / "include"
-    for inc in [*include_paths(), str(cuda_include)]:
+    for inc in [*include_paths(), str(cuda_include), sysconfig.get_paths()["include"]]:
         cmd += ["-isystem", inc]
     for lib_dir in library_paths():
         cmd += [f"-L{lib_dir}", f"-Wl,-rpath,{lib_dir}"]

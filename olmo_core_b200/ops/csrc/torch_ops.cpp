@@ -7,9 +7,12 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <dlfcn.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
+
+#include <atomic>
 
 #include "ocb_api.h"
 
@@ -37,9 +40,17 @@ void resolve(void* handle, const char* name, F& fn) {
     TORCH_CHECK(fn != nullptr, "the kernel library has no entry point ", name);
 }
 
-void bind_kernels(c10::string_view path) {
+PyObject* kernel_error = nullptr;  // the class in ops/_lib.py, which lives as long as the process
+
+struct KernelFailure : torch::PyTorchError {
+    using PyTorchError::PyTorchError;
+    PyObject* python_type() override { return kernel_error; }
+};
+
+void bind_kernels(c10::string_view path, int64_t error_class) {
     void* handle = dlopen(std::string(path).c_str(), RTLD_NOW | RTLD_LOCAL);
     TORCH_CHECK(handle != nullptr, "cannot load the kernel library: ", dlerror());
+    kernel_error = reinterpret_cast<PyObject*>(error_class);
     resolve(handle, "ocb_moe_route", kernels.route);
     resolve(handle, "ocb_moe_route_grad", kernels.route_grad);
     resolve(handle, "ocb_quantize_block_fp8", kernels.quantize);
@@ -50,7 +61,40 @@ void bind_kernels(c10::string_view path) {
     resolve(handle, "ocb_grouped_gemm_bf16", kernels.grouped_gemm_bf16);
 }
 
-void check(int rc, const char* what) { TORCH_CHECK(rc == 0, what, " failed with code ", rc); }
+std::atomic<int64_t> launches{0};
+using RangePush = void (*)(const char*);
+using RangePop = void (*)();
+std::atomic<RangePush> range_push{nullptr};  // both or neither
+std::atomic<RangePop> range_pop{nullptr};
+
+int64_t launch_count() { return launches.load(std::memory_order_relaxed); }
+
+void set_ranges(int64_t push, int64_t pop) {
+    range_push.store(nullptr);
+    range_pop.store(reinterpret_cast<RangePop>(pop));
+    range_push.store(reinterpret_cast<RangePush>(push));
+}
+
+struct Range {
+    RangePop pop = nullptr;
+    explicit Range(const char* name) {
+        const RangePush push = range_push.load();
+        if (push == nullptr) return;
+        pop = range_pop.load();
+        push(name);
+    }
+    ~Range() {
+        if (pop != nullptr) pop();
+    }
+};
+
+template <class Launcher, class... Args>
+void launch(const char* name, Launcher launcher, Args... args) {
+    launches.fetch_add(1, std::memory_order_relaxed);
+    const Range range(name);
+    const int rc = launcher(args...);
+    if (rc != 0) throw KernelFailure(std::string(name) + " failed with code " + std::to_string(rc));
+}
 
 int dtype_code(const Tensor& t) { return t.scalar_type() == at::kBFloat16 ? OCB_BF16 : OCB_F32; }
 
@@ -71,11 +115,10 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> run_route(const Tensor& logits, const
     const auto opt = logits.options();
     Tensor weights = at::empty({n, o.top_k}, opt.dtype(at::kFloat)), experts = at::empty({n, o.top_k}, opt.dtype(at::kLong));
     Tensor scores = at::empty({n, e}, opt.dtype(at::kFloat)), counts = at::empty({e}, opt.dtype(at::kInt));
-    check(kernels.route(logits.const_data_ptr(), scores.mutable_data_ptr<float>(), weights.mutable_data_ptr<float>(),
+    launch("ocb_moe_route", kernels.route, logits.const_data_ptr(), scores.mutable_data_ptr<float>(), weights.mutable_data_ptr<float>(),
                         reinterpret_cast<long long*>(experts.mutable_data_ptr<int64_t>()), counts.mutable_data_ptr<int>(), floats(bias),
                         static_cast<int>(n), static_cast<int>(e), o.top_k, o.sigmoid, o.normalize, o.n_groups, o.top_groups,
-                        logits.stride(0), dtype_code(logits), stream_of(logits)),
-          "ocb_moe_route");
+                        logits.stride(0), dtype_code(logits), stream_of(logits));
     return {weights, experts, scores, counts};
 }
 
@@ -123,13 +166,12 @@ struct Route : torch::autograd::Function<Route> {
         const Tensor dw = d_weights.defined() ? d_weights.to(at::kFloat).contiguous() : d_weights;
         const Tensor ds = d_scores.defined() ? d_scores.to(at::kFloat).contiguous() : d_scores;
         Tensor d_logits = at::empty({kept.size(0), kept.size(1)}, kept.options().dtype(ctx->saved_data["bf16"].toBool() ? at::kBFloat16 : at::kFloat));
-        check(kernels.route_grad(sigmoid ? nullptr : kept.const_data_ptr<float>(), sigmoid ? kept.const_data_ptr() : nullptr,
+        launch("ocb_moe_route_grad", kernels.route_grad, sigmoid ? nullptr : kept.const_data_ptr<float>(), sigmoid ? kept.const_data_ptr() : nullptr,
                                  reinterpret_cast<const long long*>(experts.const_data_ptr<int64_t>()),
                                  dw.defined() ? dw.const_data_ptr<float>() : nullptr, ds.defined() ? ds.const_data_ptr<float>() : nullptr,
                                  d_logits.mutable_data_ptr(), static_cast<int>(kept.size(0)), static_cast<int>(kept.size(1)),
                                  static_cast<int>(experts.size(1)), sigmoid, static_cast<int>(ctx->saved_data["normalize"].toInt()),
-                                 kept.stride(0), dtype_code(d_logits), stream_of(kept)),
-              "ocb_moe_route_grad");
+                                 kept.stride(0), dtype_code(d_logits), stream_of(kept));
         return {d_logits, Tensor(), Tensor()};
     }
 };
@@ -179,10 +221,9 @@ Tensor tile_buffer(const Tensor& weight, int64_t groups) {
     Tensor buffer = bytes(codes + 4 * groups * blocks(rows) * blocks(cols), w);
     if (rows == 0 || cols == 0) return buffer;
     uint8_t* at = buffer.mutable_data_ptr<uint8_t>();
-    check(kernels.quantize(w.const_data_ptr(), nullptr, nullptr, nullptr, nullptr, at, reinterpret_cast<float*>(at + codes),
+    launch("ocb_quantize_block_fp8", kernels.quantize, w.const_data_ptr(), nullptr, nullptr, nullptr, nullptr, at, reinterpret_cast<float*>(at + codes),
                            static_cast<int>(groups), static_cast<int>(rows), static_cast<int>(cols), w.stride(0), pitch,
-                           rows * w.stride(0), rows * pitch, stream_of(w)),
-          "ocb_quantize_block_fp8");
+                           rows * w.stride(0), rows * pitch, stream_of(w));
     return buffer;
 }
 
@@ -215,12 +256,11 @@ Tensor product(const Tensor& x, const Weight& w, bool trans, const int* offsets,
     if (kernels.linear_fused(static_cast<int>(m), static_cast<int>(w.groups), offsets != nullptr) == 0) rows = bytes(codes + 4 * blocks(k) * m, x);
     uint8_t* at = rows.defined() ? rows.mutable_data_ptr<uint8_t>() : nullptr;
     uint8_t* at_c = columns != nullptr ? columns->mutable_data_ptr<uint8_t>() : nullptr;
-    check(kernels.linear(x.const_data_ptr(), x.stride(0), at, at != nullptr ? reinterpret_cast<float*>(at + codes) : nullptr, at_c,
+    launch("ocb_linear_block_fp8", kernels.linear, x.const_data_ptr(), x.stride(0), at, at != nullptr ? reinterpret_cast<float*>(at + codes) : nullptr, at_c,
                          at_c != nullptr ? reinterpret_cast<float*>(at_c + codes) : nullptr, pitch, w.codes, w.scales, offsets,
                          static_cast<int>(w.groups), out.mutable_data_ptr(), static_cast<int>(m), static_cast<int>(n),
                          static_cast<int>(k), w.pitch, w.group_bytes, trans ? w.s_col : w.s_row, trans ? w.s_row : w.s_col, w.s_group,
-                         trans ? 0 : 1, n, 0, reinterpret_cast<int*>(status), stream_of(x)),
-          "ocb_linear_block_fp8");
+                         trans ? 0 : 1, n, 0, reinterpret_cast<int*>(status), stream_of(x));
     return out;
 }
 
@@ -317,24 +357,21 @@ struct BlockLinear : torch::autograd::Function<BlockLinear> {
                 if (!accumulate) out.zero_();
             } else if (!in_fp8) {
                 const Tensor a = aligned(dy), b = aligned(kept);
-                check(kernels.gemm_bf16(a.const_data_ptr(), b.const_data_ptr(), out.mutable_data_ptr(), static_cast<int>(n),
-                                        static_cast<int>(k), static_cast<int>(m), a.stride(0), b.stride(0), out.stride(0), 1, 1, epilogue, reinterpret_cast<int*>(status), stream_of(dy)),
-                      "ocb_gemm_bf16");
+                launch("ocb_gemm_bf16", kernels.gemm_bf16, a.const_data_ptr(), b.const_data_ptr(), out.mutable_data_ptr(), static_cast<int>(n),
+                                        static_cast<int>(k), static_cast<int>(m), a.stride(0), b.stride(0), out.stride(0), 1, 1, epilogue, reinterpret_cast<int*>(status), stream_of(dy));
             } else {
                 const int64_t pitch_y = pitch_of(n), pitch_x = pitch_of(k);
                 if (!columns.defined()) {
                     columns = bytes(m * pitch_y + 4 * blocks(m) * n, dy);
                     uint8_t* at = columns.mutable_data_ptr<uint8_t>();
-                    check(kernels.quantize(dy.const_data_ptr(), nullptr, nullptr, at, reinterpret_cast<float*>(at + m * pitch_y), nullptr,
-                                           nullptr, 1, static_cast<int>(m), static_cast<int>(n), dy.stride(0), pitch_y, 0, 0, stream_of(dy)),
-                          "ocb_quantize_block_fp8");
+                    launch("ocb_quantize_block_fp8", kernels.quantize, dy.const_data_ptr(), nullptr, nullptr, at, reinterpret_cast<float*>(at + m * pitch_y), nullptr,
+                                           nullptr, 1, static_cast<int>(m), static_cast<int>(n), dy.stride(0), pitch_y, 0, 0, stream_of(dy));
                 }
                 const uint8_t *a = columns.const_data_ptr<uint8_t>(), *b = kept.const_data_ptr<uint8_t>();
-                check(kernels.gemm_block(a, b, out.mutable_data_ptr(), reinterpret_cast<const float*>(a + m * pitch_y),
+                launch("ocb_gemm_block_fp8", kernels.gemm_block, a, b, out.mutable_data_ptr(), reinterpret_cast<const float*>(a + m * pitch_y),
                                          reinterpret_cast<const float*>(b + m * pitch_x), nullptr, 1, static_cast<int>(n),
                                          static_cast<int>(k), static_cast<int>(m), pitch_y, pitch_x, out.stride(0), 0, n, 1, 0, k, 1, 0, 0,
-                                         1, 1, epilogue, reinterpret_cast<int*>(status), stream_of(dy)),
-                      "ocb_gemm_block_fp8");
+                                         1, 1, epilogue, reinterpret_cast<int*>(status), stream_of(dy));
             }
             if (!accumulate) dw = out.scalar_type() == w_dtype ? out : out.to(w_dtype);
         }
@@ -383,12 +420,11 @@ struct BlockGroupedLinear : torch::autograd::Function<BlockGroupedLinear> {
                 if (!accumulate) out.zero_();
             } else {
                 const Tensor a = aligned(trans ? dy : x), b = aligned(trans ? x : dy);
-                check(kernels.grouped_gemm_bf16(a.const_data_ptr(), b.const_data_ptr(), out.mutable_data_ptr(), offsets.const_data_ptr<int>(),
+                launch("ocb_grouped_gemm_bf16", kernels.grouped_gemm_bf16, a.const_data_ptr(), b.const_data_ptr(), out.mutable_data_ptr(), offsets.const_data_ptr<int>(),
                                                 static_cast<int>(groups), 2, static_cast<int>(dy.size(0)), static_cast<int>(rows),
                                                 static_cast<int>(cols), 0, a.stride(0), b.stride(0), cols, 1,
                                                 out.scalar_type() == at::kBFloat16 ? 0 : accumulate ? 1 : 2,
-                                                reinterpret_cast<int*>(status), stream_of(dy)),
-                      "ocb_grouped_gemm_bf16");
+                                                reinterpret_cast<int*>(status), stream_of(dy));
             }
             if (!accumulate) dw = out.scalar_type() == w_dtype ? out : out.to(w_dtype);
         }
@@ -415,7 +451,9 @@ Tensor block_linear(const Tensor& x, const Tensor& weight, const Tensor& w, cons
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(ocb_native, m) {
-    m.def("bind_kernels(str path) -> ()", &bind_kernels);
+    m.def("bind_kernels(str path, int error_class) -> ()", &bind_kernels);
+    m.def("launch_count() -> int", &launch_count);
+    m.def("set_ranges(int push, int pop) -> ()", &set_ranges);
     m.def("route(Tensor logits, int top_k, bool sigmoid, Tensor? bias, int n_groups, int top_groups, int normalize) -> (Tensor, Tensor, Tensor, Tensor)",
           &route);
     m.def("block_tile_buffer(Tensor w, int groups) -> Tensor", &tile_buffer);

@@ -383,7 +383,6 @@ def _check_offsets(offsets: torch.Tensor, groups: int, device: torch.device) -> 
 def _native_product(x: torch.Tensor, w_q: torch.Tensor, w_s: torch.Tensor, offsets: Optional[torch.Tensor], trans_b: bool) -> torch.Tensor:
     """``q_rows(x) @ op(W)`` (bf16) for checked operands on a GPU: quantiser and product in one call."""
     y = _lib.native().block_product.default(x, w_q, w_s, offsets, trans_b, _lib.status_buffer(x.device).data_ptr())
-    _lib.check(0, "ocb_linear_block_fp8")  # counted; a failed launch has raised
     return y
 
 
@@ -524,7 +523,6 @@ def fp8_block_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch
         tiles = None if weight_cache is None else _cached(weight_cache, lambda: native.block_tile_buffer.default(w, 1), weight)
         y = native.block_linear.default(x, weight, w, tiles, main_grad, wgrad_high_precision,
                                         _lib.status_buffer(x.device).data_ptr())
-        _lib.check(0, "ocb_linear_block_fp8")  # counted; a failed launch has raised
     else:
         _check_main_grad(main_grad, weight if lowp is None else lowp, False)
         y = BlockFloat8LinearFunction.apply(x, weight, wgrad_high_precision, weight_cache)
@@ -595,7 +593,6 @@ def fp8_block_grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: tor
         tiles = None if weight_cache is None else _cached(weight_cache, lambda: native.block_tile_buffer.default(w, G), weight)
         y = native.block_grouped_linear.default(x, weight, w, offsets, tiles, main_grad, trans_b,
                                                 _lib.status_buffer(x.device).data_ptr())
-        _lib.check(0, "ocb_linear_block_fp8")  # counted; a failed launch has raised
     else:
         _check_main_grad(main_grad, w, True)
         y = BlockFloat8GroupedLinearFunction.apply(x, weight, offsets, trans_b, weight_cache)

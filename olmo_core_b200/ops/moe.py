@@ -147,7 +147,6 @@ def route(
     from . import _lib
 
     out = _lib.native().route.default(logits, top_k, gating == "sigmoid", score_bias, n_groups, top_k_groups, options[-1])
-    _lib.check(0, "ocb_moe_route")  # counted; a failed launch has raised
     return out
 
 
