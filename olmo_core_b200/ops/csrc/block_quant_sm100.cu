@@ -34,6 +34,8 @@ struct Params {
   int rows, cols;
   long long ldx, ldq;
   long long x_group, q_group;  // elements between the matrices of a stack (tiles only)
+  int row_tiles;
+  int tile0, group0;  // what the launch's blockIdx.y and .z count from: neither can exceed 65535
 };
 
 // What a tile needs besides its registers.
@@ -47,14 +49,15 @@ struct Shared {
 template <int MODE, bool FULL>
 __device__ __forceinline__ void quantize_tile(const Params& p, int vec, Shared& sh) {
   const int across = threadIdx.x & 15, down = threadIdx.x >> 4, warp = threadIdx.x >> 5;
+  const int row_tile = p.tile0 + blockIdx.y, group = p.group0 + blockIdx.z;
   const int col = blockIdx.x * B + across * 8;
   const int n_col = FULL ? 8 : min(8, p.cols - col);  // columns of this thread inside the matrix (may be <= 0)
-  const long long row0 = static_cast<long long>(blockIdx.y) * B + down;
+  const long long row0 = static_cast<long long>(row_tile) * B + down;
   const int n_row = FULL ? 8 : n_col <= 0 ? 0 : static_cast<int>(min(8ll, (p.rows - row0 + 15) / 16));  // rows row0 + 16 i
 
   uint4 v[8];
   {
-    const __nv_bfloat16* src = p.x + static_cast<long long>(blockIdx.z) * p.x_group + row0 * p.ldx + col;
+    const __nv_bfloat16* src = p.x + static_cast<long long>(group) * p.x_group + row0 * p.ldx + col;
 #pragma unroll
     for (int i = 0; i < 8; ++i, src += 16 * p.ldx) {
       v[i] = make_uint4(0u, 0u, 0u, 0u);
@@ -120,7 +123,7 @@ __device__ __forceinline__ void quantize_tile(const Params& p, int vec, Shared& 
           const int e = scale_exponent(amax);
           pair |= (inverse_bf16(e) | (amax == BF16_INF ? 0x8000u : 0u)) << (16 * h);
           const int c = blockIdx.x * B + 2 * threadIdx.x + h;
-          if (FULL || c < p.cols) p.s_col[static_cast<long long>(blockIdx.y) * p.cols + c] = pow2_biased(e);
+          if (FULL || c < p.cols) p.s_col[static_cast<long long>(row_tile) * p.cols + c] = pow2_biased(e);
         }
         sh.factor[threadIdx.x] = pair;
       }
@@ -141,9 +144,9 @@ __device__ __forceinline__ void quantize_tile(const Params& p, int vec, Shared& 
       const int e = scale_exponent(amax);
       inv.x = inv.y = inv.z = inv.w = inverse_bf16(e) * 0x10001u;
       if (threadIdx.x == 0)
-        p.s_tile[(static_cast<long long>(blockIdx.z) * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x] = pow2_biased(e);
+        p.s_tile[(static_cast<long long>(group) * p.row_tiles + row_tile) * gridDim.x + blockIdx.x] = pow2_biased(e);
     }
-    uint8_t* dst = ((MODE & COLUMNS) ? p.q_col : p.q_tile + static_cast<long long>(blockIdx.z) * p.q_group) + row0 * p.ldq + col;
+    uint8_t* dst = ((MODE & COLUMNS) ? p.q_col : p.q_tile + static_cast<long long>(group) * p.q_group) + row0 * p.ldq + col;
 #pragma unroll
     for (int i = 0; i < 8; ++i, dst += 16 * p.ldq) {
       uint2 c = e4m3x8(v[i], inv);
@@ -153,7 +156,7 @@ __device__ __forceinline__ void quantize_tile(const Params& p, int vec, Shared& 
   }
   if (MODE & ROWS) {
     __syncthreads();
-    const long long row = static_cast<long long>(blockIdx.y) * B + threadIdx.x;
+    const long long row = static_cast<long long>(row_tile) * B + threadIdx.x;
     if (threadIdx.x < B && (FULL || row < p.rows)) p.s_row[static_cast<long long>(blockIdx.x) * p.rows + row] = sh.row_scale[threadIdx.x];
   }
 }
@@ -163,21 +166,27 @@ __global__ void __launch_bounds__(THREADS, MODE == (ROWS | COLUMNS) ? 3 : 4) qua
   __shared__ Shared sh;
   next_kernel_may_start();
   previous_kernel_done();
-  const bool full = vec && (blockIdx.x + 1ll) * B <= p.cols && (blockIdx.y + 1ll) * B <= p.rows;
+  const bool full = vec && (blockIdx.x + 1ll) * B <= p.cols && (p.tile0 + blockIdx.y + 1ll) * B <= p.rows;
   if (full) quantize_tile<MODE, true>(p, vec, sh);
   else quantize_tile<MODE, false>(p, vec, sh);
 }
 
 template <int MODE>
-static int launch(const Params& p, int vec, dim3 grid, cudaStream_t stream) {
+static int launch(Params p, int vec, int groups, cudaStream_t stream) {
+  constexpr int MOST = 65535;  // CTAs along y and z of one launch
   cudaLaunchConfig_t config = {};
-  config.gridDim = grid;
   config.blockDim = dim3(THREADS);
   config.stream = stream;
   cudaLaunchAttribute attribute = dependent_launch();
   config.attrs = &attribute;
   config.numAttrs = 1;
-  return cudaLaunchKernelEx(&config, quantize_block_kernel<MODE>, p, vec) == cudaSuccess ? 0 : -4;
+  for (p.group0 = 0; p.group0 < groups; p.group0 += MOST) {
+    for (p.tile0 = 0; p.tile0 < p.row_tiles; p.tile0 += MOST) {
+      config.gridDim = dim3((p.cols + B - 1) / B, min(p.row_tiles - p.tile0, MOST), min(groups - p.group0, MOST));
+      if (cudaLaunchKernelEx(&config, quantize_block_kernel<MODE>, p, vec) != cudaSuccess) return -4;
+    }
+  }
+  return 0;
 }
 
 }  // namespace blkq
@@ -209,16 +218,15 @@ extern "C" int ocb_quantize_block_fp8(const void* x, void* q_row, float* s_row, 
   p.x_group = x_group;
   p.q_group = q_group;
   const int vec = (ldx % 8) == 0 && (x_group % 8) == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
-  const long long row_tiles = (static_cast<long long>(rows) + blkq::B - 1) / blkq::B;
-  if (row_tiles > 65535 || groups > 65535) return -1;
-  const dim3 grid((cols + blkq::B - 1) / blkq::B, static_cast<unsigned>(row_tiles), groups);
+  if (rows > 0x7fffffff - 512 || cols > 0x7fffffff - 512 || groups > 0x7fffffff - 65536) return -1;  // rounded up in 32 bits
+  p.row_tiles = (rows + blkq::B - 1) / blkq::B;
   if (q_tile != nullptr) {
     if (s_tile == nullptr || q_row != nullptr || q_col != nullptr) return -1;
-    return blkq::launch<blkq::TILES>(p, vec, grid, stream);
+    return blkq::launch<blkq::TILES>(p, vec, groups, stream);
   }
   if (groups != 1 || (q_row != nullptr && s_row == nullptr) || (q_col != nullptr && s_col == nullptr)) return -1;
-  if (q_row != nullptr && q_col != nullptr) return blkq::launch<blkq::ROWS | blkq::COLUMNS>(p, vec, grid, stream);
-  if (q_row != nullptr) return blkq::launch<blkq::ROWS>(p, vec, grid, stream);
-  if (q_col != nullptr) return blkq::launch<blkq::COLUMNS>(p, vec, grid, stream);
+  if (q_row != nullptr && q_col != nullptr) return blkq::launch<blkq::ROWS | blkq::COLUMNS>(p, vec, groups, stream);
+  if (q_row != nullptr) return blkq::launch<blkq::ROWS>(p, vec, groups, stream);
+  if (q_col != nullptr) return blkq::launch<blkq::COLUMNS>(p, vec, groups, stream);
   return -1;
 }

@@ -100,3 +100,51 @@ def test_layers_refuse_a_second_derivative(constant, grouped, device):
         with pytest.raises(RuntimeError, match="no second derivative"):
             (g.float().square().sum() + x.float().sum()).backward(retain_graph=True)
     x.float().square().sum().backward()  # a graph that does not pass through them is none of their business
+
+
+@pytest.mark.gpu
+def test_more_rows_and_matrices_than_a_grid_has_ctas_along_an_axis():
+    rows = 65535 * 128 + 300  # 65538 tiles
+    x = torch.randn(rows, 8, generator=torch.Generator(device="cuda").manual_seed(11), device="cuda").bfloat16()
+    last = 65535 * 128 - 128  # the last tile of the first launch, and those behind it
+    q, s = fb.quantize_block_rows(x)
+    want_q, want_s = fb.quantize_block_rows(x[last:].cpu())
+    assert torch.equal(q[last:].cpu(), want_q) and torch.equal(s[:, last:].cpu(), want_s)
+    q, s = fb.quantize_block_columns(x)
+    want_q, want_s = fb.quantize_block_columns(x[last:].cpu())
+    assert torch.equal(q[last:].cpu(), want_q) and torch.equal(s[last // 128:].cpu(), want_s)
+    qr, sr, qc, sc = fb.quantize_block_rows_columns(x)
+    assert torch.equal(qc, q) and torch.equal(sc, s)
+    q, s = fb.quantize_block_tiles(x)
+    want_q, want_s = fb.quantize_block_tiles(x[last:].cpu())
+    assert torch.equal(q[last:].cpu(), want_q) and torch.equal(s[last // 128:].cpu(), want_s)
+    stack = x[:65540 * 2].view(65540, 2, 8)
+    q, s = fb.quantize_block_tiles(stack)
+    want_q, want_s = fb.quantize_block_tiles(stack.cpu())
+    assert torch.equal(q.cpu(), want_q) and torch.equal(s.cpu(), want_s)
+
+
+@pytest.mark.gpu
+def test_linear_step_over_more_rows_than_one_launch_quantises():
+    rows = 65535 * 128 + 300
+    x = torch.randn(rows, 16, generator=torch.Generator(device="cuda").manual_seed(12), device="cuda").bfloat16().requires_grad_(True)
+    w = _rand((24, 16), 13, "cuda").requires_grad_(True)
+    dy = torch.zeros(rows, 24, dtype=torch.bfloat16, device="cuda")
+    at = torch.tensor([0, 65535 * 128 - 1, 65535 * 128, rows - 1], device="cuda")
+    dy[at] = _rand((4, 24), 14, "cuda")
+    y = fb.fp8_block_linear(x, w)
+    y.backward(dy)
+    few = x.detach()[at].requires_grad_(True)
+    w2 = w.detach().clone().requires_grad_(True)
+    yf = fb.fp8_block_linear(few, w2)
+    yf.backward(dy[at])
+    assert torch.equal(y[at], yf) and torch.equal(x.grad[at], few.grad)
+    rest = torch.ones(rows, dtype=torch.bool, device="cuda")
+    rest[at] = False
+    assert (x.grad[rest] == 0).all()
+    # the column blocks of both operands differ from those of the four rows alone, so the weight gradient is compared as numbers:
+    # a product of two values off by half an e4m3 step each (2^-4)
+    want = dy[at].double().t() @ x.detach()[at].double()
+    bound = (2 * 2.0 ** -4 + 2.0 ** -8 + 2.0 ** -8) * (dy[at].double().abs().t() @ x.detach()[at].double().abs()) + 2.0 ** -8 * want.abs()
+    floor = 2.0 ** -10 * x.detach().abs().max().double() * dy.abs().max().double() * 4  # codes below 2^-6 are off by 2^-10 of the scale
+    assert ((w.grad.double() - want).abs() <= bound + 8 * floor).all()
