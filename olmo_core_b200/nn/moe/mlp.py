@@ -165,11 +165,12 @@ class DroplessMoEMLP(MoEMLPBase):
         """
         E = self.num_local_experts
         f8 = getattr(self, "float8", None)  # set by Float8Config.apply_float8_linear
-        if f8 is not None and x.is_cuda and x.dtype == torch.bfloat16:
+        if f8 is not None:
             from ...ops.fp8_block import fp8_block_grouped_linear
 
             cache = f8["weight_cache"].setdefault(name, {}) if f8["weight_cache"] is not None and name else None
-            return fp8_block_grouped_linear(x, w, self._offsets(batch_sizes, x.device), trans_b=trans_b, weight_cache=cache)
+            y = fp8_block_grouped_linear(x, w, self._offsets(batch_sizes, x.device), trans_b=trans_b, weight_cache=cache)
+            return y.to(x.dtype)  # the experts' rows keep their type through the three products
         if x.is_cuda and x.dtype == torch.bfloat16:
             return _GroupedLinear.apply(x, w, self._offsets(batch_sizes, x.device), trans_b)
         if torch.is_tensor(batch_sizes):

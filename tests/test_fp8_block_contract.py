@@ -148,3 +148,26 @@ def test_linear_step_over_more_rows_than_one_launch_quantises():
     bound = (2 * 2.0 ** -4 + 2.0 ** -8 + 2.0 ** -8) * (dy[at].double().abs().t() @ x.detach()[at].double().abs()) + 2.0 ** -8 * want.abs()
     floor = 2.0 ** -10 * x.detach().abs().max().double() * dy.abs().max().double() * 4  # codes below 2^-6 are off by 2^-10 of the scale
     assert ((w.grad.double() - want).abs() <= bound + 8 * floor).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_experts_marked_for_8_bits_run_in_8_bits(dtype, device):
+    """On the CPU and for fp32 activations too, as the dense layers do."""
+    from olmo_core_b200.float8 import BlockFloat8LinearConfig, Float8Config
+    from olmo_core_b200.nn.moe.mlp import DroplessMoEMLP
+    from olmo_core_b200.ops.elementwise import swiglu
+
+    torch.manual_seed(0)
+    mlp = DroplessMoEMLP(d_model=72, hidden_size=136, num_experts=3, dtype=dtype, init_device="cpu").to(device)
+    Float8Config(block=BlockFloat8LinearConfig(), cache_weight_casts=True).apply_float8_linear(torch.nn.Sequential(mlp))
+    x = _rand((40, 72), 15, device).to(dtype).requires_grad_(True)
+    sizes = [13, 0, 27]
+    y = mlp(x, sizes)
+    assert y.dtype == dtype and set(mlp.float8["weight_cache"]) == {"w1", "w2", "w3"}
+    offsets = torch.tensor([0, 13, 13, 40], dtype=torch.int32, device=device)
+    a, b = (fb.fp8_block_grouped_linear(x, w, offsets).to(dtype) for w in (mlp.w1, mlp.w3))
+    want = fb.fp8_block_grouped_linear(swiglu(a, b), mlp.w2, offsets, trans_b=False).to(dtype)
+    assert torch.equal(y, want)
+    y.float().square().sum().backward()
+    assert x.grad.dtype == dtype and all(p.grad is not None and torch.isfinite(p.grad).all() for p in (mlp.w1, mlp.w2, mlp.w3))
