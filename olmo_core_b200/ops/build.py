@@ -137,7 +137,7 @@ def build_native(force: bool = False, verbose: bool = True) -> Path:
         cmd += [f"-L{lib_dir}", f"-Wl,-rpath,{lib_dir}"]
     # the process's C++ runtime by name: a toolchain that has only the static one would put a second copy into the library, and
     # a number streamed into an error message would then look up its facet with the wrong copy's ids
-    cmd += ["-I", str(CSRC_DIR), "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-ldl", "-l:libstdc++.so.6"]
+    cmd += ["-I", str(CSRC_DIR), "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_cuda", "-ldl", "-l:libstdc++.so.6"]
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
         raise RuntimeError(f"native helper build failed:\n{proc.stdout}\n{proc.stderr}")

@@ -10,6 +10,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/library.h>
 
 #include <atomic>
@@ -287,15 +288,28 @@ variable_list first_order(variable_list grads) {
 
 // What the kernels write to and read from by address alone: `main_grad` of a weight w (rows of a dense one may be apart), and its
 // codes and scales as tile_buffer() makes them.
-void check_main_grad(const optional<Tensor>& grad, const Tensor& w, bool stacked) {
-    if (!grad.has_value()) return;
-    TORCH_CHECK_VALUE(grad->scalar_type() == at::kFloat && grad->device() == w.device(), "main_grad must be float32 on ", w.device(),
-                      ", got ", grad->scalar_type(), " on ", grad->device());
-    const bool fits = stacked ? grad->numel() == w.numel() && grad->is_contiguous()
-                              : grad->sizes() == w.sizes() && (w.size(1) <= 1 || grad->stride(1) == 1) &&
-                                    (w.size(0) <= 1 || grad->stride(0) >= w.size(1));
-    TORCH_CHECK_VALUE(fits, "main_grad of shape ", grad->sizes(), " and strides ", grad->strides(), " does not fit a weight of shape ", w.sizes(),
-                      stacked ? ": it must be contiguous" : ": rows must be contiguous");
+void check_main_grad(const Tensor& grad, int64_t rows, int64_t cols, at::Device device, bool stacked) {
+    TORCH_CHECK_VALUE(grad.scalar_type() == at::kFloat && grad.device() == device, "main_grad must be float32 on ", device, ", got ",
+                      grad.scalar_type(), " on ", grad.device());
+    const bool fits = stacked ? grad.numel() == rows * cols && grad.is_contiguous()
+                              : grad.dim() == 2 && grad.size(0) == rows && grad.size(1) == cols && (cols <= 1 || grad.stride(1) == 1) &&
+                                    (rows <= 1 || grad.stride(0) >= cols);
+    TORCH_CHECK_VALUE(fits, "main_grad of shape ", grad.sizes(), " and strides ", grad.strides(), " does not fit a weight of shape [", rows,
+                      ", ", cols, "]: ", stacked ? "it" : "rows", " must be contiguous");
+}
+
+// The `main_grad` that the weight's Python object has by now (undefined: none), and the note there that it has been added to. Only
+// asked for a weight that had one in the forward pass: taking the interpreter's lock costs a few microseconds.
+Tensor main_grad_of(const Tensor& weight) {
+    const pybind11::gil_scoped_acquire gil;
+    const auto object = pybind11::reinterpret_steal<pybind11::object>(THPVariable_Wrap(weight));
+    const auto grad = pybind11::getattr(object, "main_grad", pybind11::none());
+    return THPVariable_Check(grad.ptr()) ? THPVariable_Unpack(grad.ptr()) : Tensor();
+}
+void note_main_grad(const Tensor& weight) {
+    const pybind11::gil_scoped_acquire gil;
+    const auto object = pybind11::reinterpret_steal<pybind11::object>(THPVariable_Wrap(weight));
+    if (pybind11::hasattr(object, "grad_added_to_main_grad")) pybind11::setattr(object, "grad_added_to_main_grad", pybind11::bool_(true));
 }
 
 void check_cached(const optional<Tensor>& tiles, const Tensor& w, int64_t groups) {
@@ -310,7 +324,7 @@ void check_cached(const optional<Tensor>& tiles, const Tensor& w, int64_t groups
 struct BlockLinear : torch::autograd::Function<BlockLinear> {
     // weight: what the gradient belongs to; w: its bf16 values [N, K]
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Tensor& w, const optional<Tensor>& cached,
-                          const optional<Tensor>& main_grad, bool needs_dw, bool high_precision, int64_t status) {
+                          bool has_main_grad, bool needs_dw, bool high_precision, int64_t status) {
         const c10::cuda::OptionalCUDAGuard guard(x.device());
         const int64_t n = w.size(0), k = w.size(1);
         const Tensor x2 = matrix(x, k), tiles = cached.has_value() ? *cached : tile_buffer(w, 1);
@@ -318,7 +332,7 @@ struct BlockLinear : torch::autograd::Function<BlockLinear> {
         Tensor columns;  // what the backward pass keeps of x: its column-scaled form, one byte per element
         Tensor y = product(x2, in_buffer(tiles, 1, n, k), true, nullptr, in_fp8 ? &columns : nullptr, status);
         ctx->save_for_backward({tiles, in_fp8 ? columns : needs_dw ? x2 : Tensor()});
-        if (main_grad.has_value()) ctx->saved_data["main_grad"] = *main_grad;  // written to by design: no version check
+        if (has_main_grad) ctx->saved_data["weight"] = weight;
         ctx->saved_data["m"] = x2.size(0);
         ctx->saved_data["n"] = n;
         ctx->saved_data["k"] = k;
@@ -337,7 +351,6 @@ struct BlockLinear : torch::autograd::Function<BlockLinear> {
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto saved = ctx->get_saved_variables();
         const Tensor &tiles = saved[0], &kept = saved[1];
-        const bool accumulate = ctx->saved_data.count("main_grad") != 0;
         const int64_t m = ctx->saved_data["m"].toInt(), n = ctx->saved_data["n"].toInt(), k = ctx->saved_data["k"].toInt();
         const int64_t status = ctx->saved_data["status"].toInt();
         const bool needs_dw = ctx->saved_data["needs_dw"].toBool(), in_fp8 = ctx->saved_data["in_fp8"].toBool();
@@ -350,8 +363,12 @@ struct BlockLinear : torch::autograd::Function<BlockLinear> {
         }
         if (needs_dw) {
             const auto w_dtype = ctx->saved_data["w_dtype"].toScalarType();
+            const auto weight = ctx->saved_data.find("weight");
+            const Tensor main_grad = weight != ctx->saved_data.end() ? main_grad_of(weight->second.toTensor()) : Tensor();
+            const bool accumulate = main_grad.defined();
+            if (accumulate) check_main_grad(main_grad, n, k, dy.device(), false);
             // the kernels write bf16 or fp32, whichever the parameter has
-            Tensor out = accumulate ? ctx->saved_data["main_grad"].toTensor() : at::empty({n, k}, dy.options().dtype(w_dtype == at::kBFloat16 ? at::kBFloat16 : at::kFloat));
+            Tensor out = accumulate ? main_grad : at::empty({n, k}, dy.options().dtype(w_dtype == at::kBFloat16 ? at::kBFloat16 : at::kFloat));
             const int epilogue = out.scalar_type() == at::kBFloat16 ? 0 : accumulate ? 1 : 2;
             if (m == 0 || n == 0 || k == 0) {
                 if (!accumulate) out.zero_();
@@ -373,7 +390,8 @@ struct BlockLinear : torch::autograd::Function<BlockLinear> {
                                          static_cast<int>(k), static_cast<int>(m), pitch_y, pitch_x, out.stride(0), 0, n, 1, 0, k, 1, 0, 0,
                                          1, 1, epilogue, reinterpret_cast<int*>(status), stream_of(dy));
             }
-            if (!accumulate) dw = out.scalar_type() == w_dtype ? out : out.to(w_dtype);
+            if (accumulate) note_main_grad(weight->second.toTensor());
+            else dw = out.scalar_type() == w_dtype ? out : out.to(w_dtype);
         }
         return first_order({dx, dw, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()});
     }
@@ -382,13 +400,13 @@ struct BlockLinear : torch::autograd::Function<BlockLinear> {
 // The experts' layer: rows sorted by group, weights stacked [G * N, K] (trans) or [G * K, N]; weight gradient in bf16.
 struct BlockGroupedLinear : torch::autograd::Function<BlockGroupedLinear> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Tensor& w, const Tensor& offsets,
-                          const optional<Tensor>& cached, const optional<Tensor>& main_grad, bool trans, bool needs_dw, int64_t status) {
+                          const optional<Tensor>& cached, bool has_main_grad, bool trans, bool needs_dw, int64_t status) {
         const c10::cuda::OptionalCUDAGuard guard(x.device());
         const int64_t groups = offsets.size(0) - 1, rows = w.size(0) / groups, cols = w.size(1);
         const Tensor x2 = matrix(x, x.size(1)), tiles = cached.has_value() ? *cached : tile_buffer(w, groups);
         Tensor y = product(x2, in_buffer(tiles, groups, rows, cols), trans, offsets.const_data_ptr<int>(), nullptr, status);
         ctx->save_for_backward({tiles, offsets, needs_dw ? x2 : Tensor()});
-        if (main_grad.has_value()) ctx->saved_data["main_grad"] = *main_grad;  // written to by design: no version check
+        if (has_main_grad) ctx->saved_data["weight"] = weight;
         ctx->saved_data["rows"] = rows;
         ctx->saved_data["cols"] = cols;
         ctx->saved_data["trans"] = trans;
@@ -405,7 +423,7 @@ struct BlockGroupedLinear : torch::autograd::Function<BlockGroupedLinear> {
         const Tensor &tiles = saved[0], &offsets = saved[1], &x = saved[2];
         const int64_t groups = offsets.size(0) - 1, rows = ctx->saved_data["rows"].toInt(), cols = ctx->saved_data["cols"].toInt();
         const int64_t status = ctx->saved_data["status"].toInt();
-        const bool trans = ctx->saved_data["trans"].toBool(), accumulate = ctx->saved_data.count("main_grad") != 0;
+        const bool trans = ctx->saved_data["trans"].toBool();
         const c10::cuda::OptionalCUDAGuard guard(tiles.device());
         const Tensor dy = matrix(grads[0], trans ? rows : cols);
         Tensor dx, dw;
@@ -414,7 +432,11 @@ struct BlockGroupedLinear : torch::autograd::Function<BlockGroupedLinear> {
                      .to(ctx->saved_data["x_dtype"].toScalarType());
         if (ctx->saved_data["needs_dw"].toBool()) {
             const auto w_dtype = ctx->saved_data["w_dtype"].toScalarType();
-            Tensor out = accumulate ? ctx->saved_data["main_grad"].toTensor()
+            const auto weight = ctx->saved_data.find("weight");
+            const Tensor main_grad = weight != ctx->saved_data.end() ? main_grad_of(weight->second.toTensor()) : Tensor();
+            const bool accumulate = main_grad.defined();
+            if (accumulate) check_main_grad(main_grad, groups * rows, cols, dy.device(), true);
+            Tensor out = accumulate ? main_grad
                                     : at::empty({groups * rows, cols}, dy.options().dtype(w_dtype == at::kBFloat16 ? at::kBFloat16 : at::kFloat));
             if (dy.size(0) == 0) {
                 if (!accumulate) out.zero_();
@@ -426,7 +448,8 @@ struct BlockGroupedLinear : torch::autograd::Function<BlockGroupedLinear> {
                                                 out.scalar_type() == at::kBFloat16 ? 0 : accumulate ? 1 : 2,
                                                 reinterpret_cast<int*>(status), stream_of(dy));
             }
-            if (!accumulate) dw = out.scalar_type() == w_dtype ? out : out.to(w_dtype);
+            if (accumulate) note_main_grad(weight->second.toTensor());
+            else dw = out.scalar_type() == w_dtype ? out : out.to(w_dtype);
         }
         return first_order({dx, dw, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()});
     }
@@ -435,17 +458,17 @@ struct BlockGroupedLinear : torch::autograd::Function<BlockGroupedLinear> {
 Tensor block_grouped_linear(const Tensor& x, const Tensor& weight, const Tensor& w, const Tensor& offsets, const optional<Tensor>& cached,
                             const optional<Tensor>& main_grad, bool trans, int64_t status) {
     const bool needs_dw = at::GradMode::is_enabled() && (weight.requires_grad() || main_grad.has_value());
-    if (needs_dw) check_main_grad(main_grad, w, true);
+    if (needs_dw && main_grad.has_value()) check_main_grad(*main_grad, w.size(0), w.size(1), w.device(), true);
     check_cached(cached, w, offsets.size(0) - 1);
-    return BlockGroupedLinear::apply(x, weight, w, offsets, cached, main_grad, trans, needs_dw, status);
+    return BlockGroupedLinear::apply(x, weight, w, offsets, cached, main_grad.has_value(), trans, needs_dw, status);
 }
 
 Tensor block_linear(const Tensor& x, const Tensor& weight, const Tensor& w, const optional<Tensor>& cached,
                     const optional<Tensor>& main_grad, bool high_precision, int64_t status) {
     const bool needs_dw = at::GradMode::is_enabled() && (weight.requires_grad() || main_grad.has_value());
-    if (needs_dw) check_main_grad(main_grad, w, false);
+    if (needs_dw && main_grad.has_value()) check_main_grad(*main_grad, w.size(0), w.size(1), w.device(), false);
     check_cached(cached, w, 1);
-    return BlockLinear::apply(x, weight, w, cached, main_grad, needs_dw, high_precision, status);
+    return BlockLinear::apply(x, weight, w, cached, main_grad.has_value(), needs_dw, high_precision, status);
 }
 
 }  // namespace

@@ -439,7 +439,7 @@ def _cached(cache: Optional[dict], make, weight: torch.Tensor):
 
 def _check_main_grad(grad: Optional[torch.Tensor], w: torch.Tensor, stacked: bool) -> None:
     """The host's check before anything is written to ``main_grad`` (on a GPU: ``csrc/torch_ops.cpp``)."""
-    if grad is None or not torch.is_grad_enabled():
+    if grad is None:
         return
     if grad.dtype != torch.float32 or grad.device != w.device:
         raise ValueError(f"main_grad must be float32 on {w.device}, got {grad.dtype} on {grad.device}")
@@ -451,6 +451,15 @@ def _check_main_grad(grad: Optional[torch.Tensor], w: torch.Tensor, stacked: boo
     if not fits:
         raise ValueError(f"main_grad of shape {tuple(grad.shape)} and strides {grad.stride()} does not fit a weight of shape "
                          f"{tuple(w.shape)}: {'it' if stacked else 'rows'} must be contiguous")
+
+
+def _weight_gradient(weight: torch.Tensor, main_grad: Optional[torch.Tensor], out: torch.Tensor) -> Optional[torch.Tensor]:
+    """What a backward pass returns for the weight: nothing once ``main_grad`` (``out`` then) has it."""
+    if main_grad is None:
+        return out.to(weight.dtype)
+    if hasattr(weight, "grad_added_to_main_grad"):
+        weight.grad_added_to_main_grad = True
+    return None
 
 
 def _first_order(backward):
@@ -477,7 +486,7 @@ class BlockFloat8LinearFunction(torch.autograd.Function):
         x2 = _check_matrix(x.reshape(-1, x.shape[-1]), "x")
         wq, sw = _cached(cache, lambda: quantize_block_tiles(w), weight)
         ctx.save_for_backward(wq, sw, x2)
-        ctx.wgrad_hp = wgrad_high_precision
+        ctx.wgrad_hp, ctx.has_main_grad = wgrad_high_precision, getattr(weight, "main_grad", None) is not None
         ctx.weight_ref, ctx.x_shape, ctx.x_dtype = weight, x.shape, x.dtype
         return gemm_fp8_block(*quantize_block_rows(x2), wq, sw).view(*x.shape[:-1], w.shape[0])
 
@@ -487,7 +496,8 @@ class BlockFloat8LinearFunction(torch.autograd.Function):
         wq, sw, x2 = ctx.saved_tensors
         weight = ctx.weight_ref
         dy2 = _check_matrix(dy.reshape(-1, wq.shape[0]), "dy")
-        main_grad = getattr(weight, "main_grad", None)
+        main_grad = getattr(weight, "main_grad", None) if ctx.has_main_grad else None
+        _check_main_grad(main_grad, wq, False)
         dx = dw = None
         if ctx.needs_input_grad[0]:
             dx = gemm_fp8_block(*quantize_block_rows(dy2), wq, sw, trans_b=False).view(ctx.x_shape).to(ctx.x_dtype)
@@ -499,7 +509,7 @@ class BlockFloat8LinearFunction(torch.autograd.Function):
             else:
                 gemm_fp8_block(*quantize_block_columns(dy2), *quantize_block_columns(x2), trans_a=True, trans_b=False,
                                b_tiles=False, out=out, accumulate=main_grad is not None)
-            dw = None if main_grad is not None else out.to(weight.dtype)
+            dw = _weight_gradient(weight, main_grad, out)
         return dx, dw, None, None
 
 
@@ -508,7 +518,8 @@ def fp8_block_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch
     """
     ``x @ weight^T (+ bias)`` with block-scaled e4m3 operands in all three products; any sizes. ``wgrad_high_precision``
     keeps the weight gradient in bf16 (widths must then be multiples of 8). ``weight_cache``: see
-    :func:`olmo_core_b200.ops.fp8.cached_weight_cast`. First derivatives only: differentiating the gradients is an error.
+    :func:`olmo_core_b200.ops.fp8.cached_weight_cast`. The gradient of a weight that has a ``main_grad`` (fp32) in the forward pass is
+    added to the one that it has in the backward pass. First derivatives only: differentiating the gradients is an error.
     """
     if x.shape[-1] != weight.shape[-1]:
         raise ValueError(f"x has {x.shape[-1]} features, the weight takes {weight.shape[-1]}")
@@ -524,10 +535,8 @@ def fp8_block_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch
         y = native.block_linear.default(x, weight, w, tiles, main_grad, wgrad_high_precision,
                                         _lib.status_buffer(x.device).data_ptr())
     else:
-        _check_main_grad(main_grad, weight if lowp is None else lowp, False)
+        _check_main_grad(main_grad if torch.is_grad_enabled() else None, weight if lowp is None else lowp, False)
         y = BlockFloat8LinearFunction.apply(x, weight, wgrad_high_precision, weight_cache)
-    if main_grad is not None and hasattr(weight, "grad_added_to_main_grad") and torch.is_grad_enabled():
-        weight.grad_added_to_main_grad = True  # by the backward pass
     return y if bias is None else y + bias.to(y.dtype)
 
 
@@ -541,6 +550,7 @@ class BlockFloat8GroupedLinearFunction(torch.autograd.Function):
         wq, sw = _cached(cache, lambda: quantize_block_tiles(w.view(offsets.numel() - 1, -1, w.shape[-1])), weight)
         ctx.save_for_backward(wq, sw, offsets, x2)
         ctx.trans_b, ctx.weight_ref, ctx.w_shape, ctx.x_dtype = trans_b, weight, w.shape, x.dtype
+        ctx.has_main_grad = getattr(weight, "main_grad", None) is not None
         return grouped_gemm_fp8_block(*quantize_block_rows(x2), wq, sw, offsets, trans_b=trans_b)
 
     @staticmethod
@@ -552,14 +562,15 @@ class BlockFloat8GroupedLinearFunction(torch.autograd.Function):
         dx = dw = None
         if ctx.needs_input_grad[0]:
             dx = grouped_gemm_fp8_block(*quantize_block_rows(dy2), wq, sw, offsets, trans_b=not trans_b).to(ctx.x_dtype)
-        main_grad = getattr(weight, "main_grad", None)
+        main_grad = getattr(weight, "main_grad", None) if ctx.has_main_grad else None
         if main_grad is not None or ctx.needs_input_grad[1]:
+            _check_main_grad(main_grad, wq, True)
             a, b = (dy2, x2) if trans_b else (x2, dy2)
             out = main_grad.view(ctx.w_shape) if main_grad is not None else torch.empty(ctx.w_shape, dtype=weight.dtype)
             bounds, per = offsets.tolist(), out.view(offsets.numel() - 1, -1, out.shape[1])
             for g, (lo, hi) in enumerate(zip(bounds[:-1], bounds[1:])):
                 _store(per[g], a[lo:hi].float().t() @ b[lo:hi].float(), main_grad is not None)
-            dw = None if main_grad is not None else out
+            dw = _weight_gradient(weight, main_grad, out)
         return dx, dw, None, None, None
 
 
@@ -594,8 +605,6 @@ def fp8_block_grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: tor
         y = native.block_grouped_linear.default(x, weight, w, offsets, tiles, main_grad, trans_b,
                                                 _lib.status_buffer(x.device).data_ptr())
     else:
-        _check_main_grad(main_grad, w, True)
+        _check_main_grad(main_grad if torch.is_grad_enabled() else None, w, True)
         y = BlockFloat8GroupedLinearFunction.apply(x, weight, offsets, trans_b, weight_cache)
-    if main_grad is not None and hasattr(weight, "grad_added_to_main_grad") and torch.is_grad_enabled():
-        weight.grad_added_to_main_grad = True  # by the backward pass
     return y

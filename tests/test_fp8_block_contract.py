@@ -171,3 +171,40 @@ def test_experts_marked_for_8_bits_run_in_8_bits(dtype, device):
     assert torch.equal(y, want)
     y.float().square().sum().backward()
     assert x.grad.dtype == dtype and all(p.grad is not None and torch.isfinite(p.grad).all() for p in (mlp.w1, mlp.w2, mlp.w3))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("grouped", [False, True])
+def test_the_backward_pass_uses_the_main_grad_of_its_own_time(grouped, device):
+    x, w = _rand((16, 64), 16, device), torch.nn.Parameter(_rand((48, 64), 17, device).float())
+    offsets = torch.tensor([0, 5, 16], dtype=torch.int32, device=device)
+
+    def forward():
+        return (fb.fp8_block_grouped_linear(x, w, offsets) if grouped else fb.fp8_block_linear(x, w)).float().sum()
+
+    forward().backward()
+    want = w.grad
+    w.grad, w.grad_added_to_main_grad = None, False
+    y = forward()  # attached after the forward pass: an ordinary gradient
+    w.main_grad = first = torch.zeros(48, 64, device=device)
+    y.backward()
+    assert torch.equal(w.grad, want) and not w.grad_added_to_main_grad and (first == 0).all()
+    w.grad = None
+    forward().backward()
+    assert w.grad is None and w.grad_added_to_main_grad and torch.equal(first, want)
+    w.grad_added_to_main_grad = False
+    y = forward()  # replaced
+    assert not w.grad_added_to_main_grad
+    w.main_grad = second = torch.zeros(48, 64, device=device)
+    y.backward()
+    assert w.grad is None and w.grad_added_to_main_grad and torch.equal(second, want) and torch.equal(first, want)
+    y = forward()  # replaced by one that does not fit
+    w.main_grad = torch.zeros(40, 64, device=device)
+    with pytest.raises(ValueError, match="does not fit"):
+        y.backward()
+    w.main_grad = second
+    w.grad_added_to_main_grad = False
+    y = forward()  # taken away
+    del w.main_grad
+    y.backward()
+    assert torch.equal(w.grad, want) and torch.equal(second, want) and not w.grad_added_to_main_grad
