@@ -33,7 +33,7 @@ import torch
 
 from . import _lib
 from .fp8 import cached_weight_cast, weight_state
-from .gemm import compute_weight, gemm
+from .gemm import gemm
 
 __all__ = ["BLOCK", "quantize_block_rows", "quantize_block_columns", "quantize_block_tiles", "dequantize_block_rows",
            "dequantize_block_columns", "dequantize_block_tiles", "gemm_fp8_block", "grouped_gemm_fp8_block",
@@ -426,6 +426,12 @@ def fp8_block_grouped_matmul(x: torch.Tensor, w_q: torch.Tensor, w_s: torch.Tens
         return grouped_gemm_fp8_block(*quantize_block_rows(x), w_q, w_s, offsets, trans_b=trans_b)
 
 
+def _whole(weight: torch.Tensor) -> torch.Tensor:
+    """All rows of a weight: of a sharded one, which holds this rank's rows itself, the resident copy, whatever its type."""
+    lowp = getattr(weight, "_lowp", None)
+    return weight.detach() if lowp is None else lowp
+
+
 def _cached(cache: Optional[dict], make, weight: torch.Tensor):
     """The 8-bit form of ``weight``, kept in ``cache`` (see :func:`olmo_core_b200.ops.fp8.cached_weight_cast`)."""
     state = weight_state(weight)
@@ -482,7 +488,7 @@ class BlockFloat8LinearFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, wgrad_high_precision: bool, cache: Optional[dict] = None):  # type: ignore[override]
-        w = compute_weight(weight, torch.bfloat16)
+        w = _whole(weight).to(torch.bfloat16)
         x2 = _check_matrix(x.reshape(-1, x.shape[-1]), "x")
         wq, sw = _cached(cache, lambda: quantize_block_tiles(w), weight)
         ctx.save_for_backward(wq, sw, x2)
@@ -525,17 +531,16 @@ def fp8_block_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch
         raise ValueError(f"x has {x.shape[-1]} features, the weight takes {weight.shape[-1]}")
     if x.device != weight.device:
         raise ValueError(f"x is on {x.device}, the weight on {weight.device}")
-    lowp, main_grad = getattr(weight, "_lowp", None), getattr(weight, "main_grad", None)
-    if wgrad_high_precision and any(n % 8 for n in (weight if lowp is None else lowp).shape):
+    w, main_grad = _whole(weight), getattr(weight, "main_grad", None)
+    if wgrad_high_precision and any(n % 8 for n in w.shape):
         raise ValueError("a weight gradient in bf16 needs widths that are multiples of 8")
     if x.is_cuda:
-        w = lowp if lowp is not None and lowp.dtype == torch.bfloat16 else weight.detach()
         native = _lib.native()
         tiles = None if weight_cache is None else _cached(weight_cache, lambda: native.block_tile_buffer.default(w, 1), weight)
         y = native.block_linear.default(x, weight, w, tiles, main_grad, wgrad_high_precision,
                                         _lib.status_buffer(x.device).data_ptr())
     else:
-        _check_main_grad(main_grad if torch.is_grad_enabled() else None, weight if lowp is None else lowp, False)
+        _check_main_grad(main_grad if torch.is_grad_enabled() else None, w, False)
         y = BlockFloat8LinearFunction.apply(x, weight, wgrad_high_precision, weight_cache)
     return y if bias is None else y + bias.to(y.dtype)
 
@@ -545,7 +550,7 @@ class BlockFloat8GroupedLinearFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, offsets, trans_b: bool, cache: Optional[dict] = None):  # type: ignore[override]
-        w = compute_weight(weight, torch.bfloat16)
+        w = _whole(weight).to(torch.bfloat16)
         x2 = _check_matrix(x, "x")
         wq, sw = _cached(cache, lambda: quantize_block_tiles(w.view(offsets.numel() - 1, -1, w.shape[-1])), weight)
         ctx.save_for_backward(wq, sw, offsets, x2)
@@ -584,8 +589,7 @@ def fp8_block_grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: tor
     must be multiples of 8. Rows outside every group are undefined. First derivatives only, as :func:`fp8_block_linear`.
     """
     G = offsets.numel() - 1
-    w = getattr(weight, "_lowp", None)
-    w = weight if w is None else w  # only its shape is needed here
+    w = _whole(weight)
     if G < 1 or w.dim() != 2 or w.shape[0] % G:
         raise ValueError(f"a weight of shape {tuple(w.shape)} does not stack {G} equal matrices")
     K = w.shape[1] if trans_b else w.shape[0] // G
@@ -598,8 +602,6 @@ def fp8_block_grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: tor
     if x.is_cuda:
         if x.device != weight.device:
             raise ValueError(f"x is on {x.device}, the weights on {weight.device}")
-        lowp = getattr(weight, "_lowp", None)
-        w = lowp if lowp is not None and lowp.dtype == torch.bfloat16 else weight.detach()
         native = _lib.native()
         tiles = None if weight_cache is None else _cached(weight_cache, lambda: native.block_tile_buffer.default(w, G), weight)
         y = native.block_grouped_linear.default(x, weight, w, offsets, tiles, main_grad, trans_b,
