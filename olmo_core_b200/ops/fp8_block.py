@@ -393,8 +393,8 @@ def fp8_block_matmul(x: torch.Tensor, w_q: torch.Tensor, w_s: torch.Tensor, bias
     """
     _check_codes(w_q, "w_q", 2)
     N, K = w_q.shape
-    if x.shape[-1] != K:
-        raise ValueError(f"x has {x.shape[-1]} features, the weight takes {K}")
+    if x.dim() == 0 or x.shape[-1] != K:
+        raise ValueError(f"x of shape {tuple(x.shape)} does not have the {K} features that the weight takes")
     if x.device != w_q.device:
         raise ValueError(f"x is on {x.device}, the weight on {w_q.device}")
     _check_scales(w_s, "w_s", (_blocks(N), _blocks(K)), w_q.device)
@@ -527,11 +527,13 @@ def fp8_block_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch
     :func:`olmo_core_b200.ops.fp8.cached_weight_cast`. The gradient of a weight that has a ``main_grad`` (fp32) in the forward pass is
     added to the one that it has in the backward pass. First derivatives only: differentiating the gradients is an error.
     """
-    if x.shape[-1] != weight.shape[-1]:
-        raise ValueError(f"x has {x.shape[-1]} features, the weight takes {weight.shape[-1]}")
+    w, main_grad = _whole(weight), getattr(weight, "main_grad", None)
+    if w.dim() != 2 or x.dim() == 0:
+        raise ValueError(f"the layer takes x [..., K] and a weight [N, K], got shapes {tuple(x.shape)} and {tuple(w.shape)}")
+    if x.shape[-1] != w.shape[1]:
+        raise ValueError(f"x has {x.shape[-1]} features, the weight takes {w.shape[1]}")
     if x.device != weight.device:
         raise ValueError(f"x is on {x.device}, the weight on {weight.device}")
-    w, main_grad = _whole(weight), getattr(weight, "main_grad", None)
     if wgrad_high_precision and any(n % 8 for n in w.shape):
         raise ValueError("a weight gradient in bf16 needs widths that are multiples of 8")
     if x.is_cuda:

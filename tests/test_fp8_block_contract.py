@@ -208,3 +208,17 @@ def test_the_backward_pass_uses_the_main_grad_of_its_own_time(grouped, device):
     del w.main_grad
     y.backward()
     assert torch.equal(w.grad, want) and torch.equal(second, want) and not w.grad_added_to_main_grad
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_layer_refuses_shapes_that_are_no_matrix_product(device):
+    x, w = _rand((4, 64), 18, device), _rand((48, 64), 19, device)
+    for bad in ((x, w[0]), (x, w.view(2, 24, 64)), (x[0, 0], w), (x[0, 0], w[0])):
+        with pytest.raises(ValueError, match="takes x"):
+            fb.fp8_block_linear(*bad)
+    q, s = fb.quantize_block_tiles(w)
+    with pytest.raises(ValueError, match="features"):
+        fb.fp8_block_matmul(x[0, 0], q, s)
+    for shape in ((64,), (4, 64), (2, 2, 64), (0, 64), (2, 0, 64)):
+        assert fb.fp8_block_linear(_rand(shape, 20, device), w).shape == (*shape[:-1], 48)
+        assert fb.fp8_block_matmul(_rand(shape, 20, device), q, s).shape == (*shape[:-1], 48)
