@@ -98,6 +98,13 @@ def gemm_fp8(a_q: torch.Tensor, a_scale: torch.Tensor, b_q: torch.Tensor, b_scal
     return out
 
 
+_IN_GRAPHS: list = []  # kept casts that captured graphs read
+
+
+def _capturing() -> bool:
+    return torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing()
+
+
 def weight_state(weight: torch.Tensor):
     """
     What ``weight`` holds and where, as far as PyTorch tells without looking at its elements: equal values of this mean that a cast
@@ -118,13 +125,22 @@ def cached_weight_cast(cache: Optional[dict], key: str, make, version=0):
     weights once before the sharded all-gather: src/olmo_core/float8/__init__.py:141-162). ``None`` disables caching.
     ``version`` (:func:`weight_state` of the parameter) additionally drops an entry when the weight was rewritten by an ordinary
     in-place tensor operation, replaced or moved; where it is ``None`` nothing is kept.
+
+    While a CUDA graph is being captured nothing is put into ``cache``, because what the graph makes holds nothing before its first
+    replay. An entry that is there already is used, and lives as long as the process: a graph captured with it goes on with
+    these weights, and has to be captured again once they change.
     """
     if cache is None or version is None:
         return make()
     hit = cache.get(key)
-    if hit is None or hit[0] != version:
-        hit = cache[key] = (version, make())
-    return hit[1]
+    if hit is not None and hit[0] == version:
+        if _capturing() and not any(entry is hit for entry in _IN_GRAPHS):
+            _IN_GRAPHS.append(hit)
+        return hit[1]
+    made = make()
+    if not _capturing():
+        cache[key] = (version, made)
+    return made
 
 
 class Float8LinearFunction(torch.autograd.Function):

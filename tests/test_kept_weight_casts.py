@@ -138,3 +138,51 @@ def test_weights_made_under_inference_mode_are_not_kept(config, device):
         first = lin(x)
         lin.weight.mul_(2)  # counts no version
         assert torch.equal(lin(x), 2 * first)
+
+
+def _captured(fn):
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=side):
+        out = fn()
+    return graph, out
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("config", [Float8Config(block=BlockFloat8LinearConfig(), cache_weight_casts=True),
+                                    Float8Config(ao_mx=AOMXLinearConfig.mxfp8_cublas_rceil(), cache_weight_casts=True)])
+def test_what_a_graph_makes_is_not_kept(config):
+    lin = Linear(256, 128, False, torch.bfloat16, "cpu").to("cuda")
+    config.apply_float8_linear(torch.nn.Sequential(lin))
+    x = torch.randn(128, 256, device="cuda", dtype=torch.bfloat16)
+    with torch.no_grad():
+        want = lin(x).clone()
+        lin.float8["weight_cache"].clear()
+        graph, out = _captured(lambda: lin(x))
+        assert not lin.float8["weight_cache"]
+        assert torch.equal(lin(x), want)  # before the first replay
+        graph.replay()
+        assert torch.equal(out, want)
+        del graph, out  # what eager calls kept does not depend on it
+        torch.empty(1 << 26, device="cuda").fill_(float("nan"))
+        assert torch.equal(lin(x), want)
+
+
+@pytest.mark.gpu
+def test_a_kept_cast_outlives_its_place_in_the_cache_for_a_graph_that_reads_it():
+    from olmo_core_b200.float8 import refresh_float8_scales
+
+    lin = Linear(256, 128, False, torch.bfloat16, "cpu").to("cuda")
+    _kept(lin)
+    x = torch.randn(3, 256, device="cuda", dtype=torch.bfloat16)
+    with torch.no_grad():
+        want = lin(x).clone()
+        graph, out = _captured(lambda: lin(x))
+        lin.weight.mul_(2)
+        refresh_float8_scales(lin)
+        assert torch.equal(lin(x), 2 * want)
+        torch.cuda.synchronize()
+        junk = [torch.full_like(lin.float8["weight_cache"]["block_tiles"][1], 0x7F) for _ in range(64)]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and len(junk) == 64
