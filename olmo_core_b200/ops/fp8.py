@@ -134,13 +134,33 @@ def cached_weight_cast(cache: Optional[dict], key: str, make, version=0):
         return make()
     hit = cache.get(key)
     if hit is not None and hit[0] == version:
-        if _capturing() and not any(entry is hit for entry in _IN_GRAPHS):
-            _IN_GRAPHS.append(hit)
+        _join(hit)
         return hit[1]
     made = make()
     if not _capturing():
-        cache[key] = (version, made)
+        first = _tensors(made)[0]
+        stream = torch.cuda.current_stream(first.device) if first.is_cuda else None
+        cache[key] = (version, made, stream, None if stream is None else stream.record_event())
     return made
+
+
+def _tensors(made):
+    return (made,) if torch.is_tensor(made) else made
+
+
+def _join(hit) -> None:
+    """The current stream may use a kept cast: after it was made, and for as long as it takes."""
+    _, made, stream, done = hit
+    if stream is None:
+        return
+    if _capturing():  # of a graph, whose capture begins with everything before it done
+        if not any(entry is hit for entry in _IN_GRAPHS):
+            _IN_GRAPHS.append(hit)
+    elif torch._C._cuda_getCurrentRawStream(stream.device_index) != stream.cuda_stream:
+        current = torch.cuda.current_stream(stream.device)
+        current.wait_event(done)
+        for t in _tensors(made):
+            t.record_stream(current)
 
 
 class Float8LinearFunction(torch.autograd.Function):

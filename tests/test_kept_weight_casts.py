@@ -186,3 +186,28 @@ def test_a_kept_cast_outlives_its_place_in_the_cache_for_a_graph_that_reads_it()
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want) and len(junk) == 64
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("config", [Float8Config(block=BlockFloat8LinearConfig(), cache_weight_casts=True),
+                                    Float8Config(ao_mx=AOMXLinearConfig.mxfp8_cublas_rceil(), cache_weight_casts=True)])
+def test_another_stream_waits_for_the_cast_that_it_uses(config):
+    lin = Linear(1024, 512, False, torch.bfloat16, "cpu").to("cuda")
+    x = torch.randn(128, 1024, device="cuda", dtype=torch.bfloat16)
+    config.apply_float8_linear(torch.nn.Sequential(lin))
+    one, two = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.no_grad():
+        want = lin(x).clone()
+        with torch.cuda.stream(two):
+            lin(x)  # its own buffers are warm
+        lin.float8["weight_cache"].clear()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(one):
+            junk = [torch.full((n,), 0x7F, dtype=torch.uint8, device="cuda") for n in (512 * 1024 + 4 * 32, 512 * 1024, 512 * 32)]
+            del junk  # what this stream allocates next holds no weights
+            torch.cuda._sleep(20_000_000)  # about 10 ms
+            first = lin(x)
+        with torch.cuda.stream(two):
+            second = lin(x)
+        torch.cuda.synchronize()
+    assert torch.equal(first, want) and torch.equal(second, want)
