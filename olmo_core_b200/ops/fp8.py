@@ -117,6 +117,18 @@ def weight_state(weight: torch.Tensor):
     return weight._version, weight.device, weight.data_ptr(), weight.dtype, weight.shape, weight.stride()
 
 
+class _Kept:
+    """A cast in a layer's cache, with the stream that made it and an event behind that (``None`` on the CPU)."""
+
+    __slots__ = ("version", "made", "stream", "done")
+
+    def __init__(self, version=None, made=None, stream=None, done=None):
+        self.version, self.made, self.stream, self.done = version, made, stream, done
+
+    def __reduce__(self):
+        return _Kept, ()  # a copy of the layer has weights of its own and casts them itself
+
+
 def cached_weight_cast(cache: Optional[dict], key: str, make, version=0):
     """
     ``make()`` once per optimizer step: ``cache`` is a dict owned by the layer and emptied by
@@ -133,14 +145,14 @@ def cached_weight_cast(cache: Optional[dict], key: str, make, version=0):
     if cache is None or version is None:
         return make()
     hit = cache.get(key)
-    if hit is not None and hit[0] == version:
+    if hit is not None and hit.version == version:
         _join(hit)
-        return hit[1]
+        return hit.made
     made = make()
     if not _capturing():
         first = _tensors(made)[0]
         stream = torch.cuda.current_stream(first.device) if first.is_cuda else None
-        cache[key] = (version, made, stream, None if stream is None else stream.record_event())
+        cache[key] = _Kept(version, made, stream, None if stream is None else stream.record_event())
     return made
 
 
@@ -148,9 +160,9 @@ def _tensors(made):
     return (made,) if torch.is_tensor(made) else made
 
 
-def _join(hit) -> None:
+def _join(hit: _Kept) -> None:
     """The current stream may use a kept cast: after it was made, and for as long as it takes."""
-    _, made, stream, done = hit
+    stream = hit.stream
     if stream is None:
         return
     if _capturing():  # of a graph, whose capture begins with everything before it done
@@ -158,8 +170,8 @@ def _join(hit) -> None:
             _IN_GRAPHS.append(hit)
     elif torch._C._cuda_getCurrentRawStream(stream.device_index) != stream.cuda_stream:
         current = torch.cuda.current_stream(stream.device)
-        current.wait_event(done)
-        for t in _tensors(made):
+        current.wait_event(hit.done)
+        for t in _tensors(hit.made):
             t.record_stream(current)
 
 

@@ -182,7 +182,7 @@ def test_a_kept_cast_outlives_its_place_in_the_cache_for_a_graph_that_reads_it()
         refresh_float8_scales(lin)
         assert torch.equal(lin(x), 2 * want)
         torch.cuda.synchronize()
-        junk = [torch.full_like(lin.float8["weight_cache"]["block_tiles"][1], 0x7F) for _ in range(64)]
+        junk = [torch.full_like(lin.float8["weight_cache"]["block_tiles"].made, 0x7F) for _ in range(64)]
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want) and len(junk) == 64
@@ -211,3 +211,19 @@ def test_another_stream_waits_for_the_cast_that_it_uses(config):
             second = lin(x)
         torch.cuda.synchronize()
     assert torch.equal(first, want) and torch.equal(second, want)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_layers_with_kept_casts_can_be_copied_and_pickled(device):
+    import copy
+    import pickle
+
+    lin = Linear(64, 48, False, torch.bfloat16, "cpu").to(device)
+    _kept(lin)
+    x = torch.randn(7, 64, device=device, dtype=torch.bfloat16)
+    want = lin(x)
+    for other in (copy.deepcopy(lin), pickle.loads(pickle.dumps(lin))):
+        assert torch.equal(other(x), want)
+        with torch.no_grad():
+            other.weight.mul_(2)
+        assert torch.equal(other(x), 2 * want) and torch.equal(lin(x), want)
