@@ -117,16 +117,13 @@ def weight_state(weight: torch.Tensor):
     return weight._version, weight.device, weight.data_ptr(), weight.dtype, weight.shape, weight.stride()
 
 
-class _Kept:
-    """A cast in a layer's cache, with the stream that made it and an event behind that (``None`` on the CPU)."""
+class _Kept(tuple):
+    """``(version, cast)`` in a layer's cache, with the stream that made it and an event behind that (``None`` on the CPU)."""
 
-    __slots__ = ("version", "made", "stream", "done")
-
-    def __init__(self, version=None, made=None, stream=None, done=None):
-        self.version, self.made, self.stream, self.done = version, made, stream, done
+    stream = done = None
 
     def __reduce__(self):
-        return _Kept, ()  # a copy of the layer has weights of its own and casts them itself
+        return _Kept, ((None, None),)  # a copy of the layer has weights of its own and casts them itself
 
 
 def cached_weight_cast(cache: Optional[dict], key: str, make, version=0):
@@ -145,14 +142,16 @@ def cached_weight_cast(cache: Optional[dict], key: str, make, version=0):
     if cache is None or version is None:
         return make()
     hit = cache.get(key)
-    if hit is not None and hit.version == version:
+    if hit is not None and hit[0] == version:
         _join(hit)
-        return hit.made
+        return hit[1]
     made = make()
     if not _capturing():
+        kept = cache[key] = _Kept((version, made))
         first = _tensors(made)[0]
-        stream = torch.cuda.current_stream(first.device) if first.is_cuda else None
-        cache[key] = _Kept(version, made, stream, None if stream is None else stream.record_event())
+        if first.is_cuda:
+            kept.stream = torch.cuda.current_stream(first.device)
+            kept.done = kept.stream.record_event()
     return made
 
 
@@ -171,7 +170,7 @@ def _join(hit: _Kept) -> None:
     elif torch._C._cuda_getCurrentRawStream(stream.device_index) != stream.cuda_stream:
         current = torch.cuda.current_stream(stream.device)
         current.wait_event(hit.done)
-        for t in _tensors(hit.made):
+        for t in _tensors(hit[1]):
             t.record_stream(current)
 
 

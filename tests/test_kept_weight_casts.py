@@ -182,7 +182,7 @@ def test_a_kept_cast_outlives_its_place_in_the_cache_for_a_graph_that_reads_it()
         refresh_float8_scales(lin)
         assert torch.equal(lin(x), 2 * want)
         torch.cuda.synchronize()
-        junk = [torch.full_like(lin.float8["weight_cache"]["block_tiles"].made, 0x7F) for _ in range(64)]
+        junk = [torch.full_like(lin.float8["weight_cache"]["block_tiles"][1], 0x7F) for _ in range(64)]
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want) and len(junk) == 64
