@@ -97,6 +97,8 @@ def adamw_step_(
         _lib.stream_ptr(),
     )
     _lib.check(rc, "ocb_adamw_step")
+    if not p.is_inference():
+        torch.autograd.graph.increment_version(p)  # as any in-place operation does
 
 
 _scratch: dict = {}

@@ -227,3 +227,23 @@ def test_layers_with_kept_casts_can_be_copied_and_pickled(device):
         with torch.no_grad():
             other.weight.mul_(2)
         assert torch.equal(other(x), 2 * want) and torch.equal(lin(x), want)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("name", ["AdamWConfig", "SkipStepAdamWConfig", "AdamConfig", "LionConfig", "SkipStepLionConfig", "MuonConfig"])
+def test_an_optimizer_step_alone_drops_the_casts(name, device):
+    import olmo_core_b200.optim as optim
+
+    lin = Linear(64, 48, False, torch.float32, "cpu").to(device)
+    _kept(lin)
+    optimizer = getattr(optim, name)(lr=0.1).build(lin)
+    x = torch.randn(7, 64, device=device, dtype=torch.bfloat16)
+    for _ in range(2):
+        if hasattr(optimizer, "latest_loss"):
+            optimizer.latest_loss = torch.tensor(1.0, device=device)
+        y = lin(x)
+        y.float().square().sum().backward()
+        optimizer.step()
+        optimizer.zero_grad()
+        after = lin(x)
+        assert torch.equal(after, fb.fp8_block_linear(x, lin.weight)) and not torch.equal(after, y)
