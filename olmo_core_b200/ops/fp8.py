@@ -112,15 +112,16 @@ def weight_state(weight: torch.Tensor):
     ``module.to(...)`` do not, but move its memory. ``None`` for tensors made under inference mode, which count no versions. What
     writes through ``parameter.data`` shows in neither and calls :func:`olmo_core_b200.float8.refresh_float8_scales`.
     """
-    if weight.is_inference():
+    try:
+        return weight._version, weight.data_ptr(), weight.shape, weight.stride()
+    except RuntimeError:  # made under inference mode
         return None
-    return weight._version, weight.device, weight.data_ptr(), weight.dtype, weight.shape, weight.stride()
 
 
 class _Kept(tuple):
-    """``(version, cast)`` in a layer's cache, with the stream that made it and an event behind that (``None`` on the CPU)."""
+    """``(version, cast)`` in a layer's cache, with the stream that made it (``None`` on the CPU), its handle, and an event behind it."""
 
-    stream = done = None
+    stream = handle = done = None
 
     def __reduce__(self):
         return _Kept, ((None, None),)  # a copy of the layer has weights of its own and casts them itself
@@ -151,7 +152,7 @@ def cached_weight_cast(cache: Optional[dict], key: str, make, version=0):
         first = _tensors(made)[0]
         if first.is_cuda:
             kept.stream = torch.cuda.current_stream(first.device)
-            kept.done = kept.stream.record_event()
+            kept.handle, kept.done = kept.stream.cuda_stream, kept.stream.record_event()
     return made
 
 
@@ -164,10 +165,13 @@ def _join(hit: _Kept) -> None:
     stream = hit.stream
     if stream is None:
         return
+    handle = torch._C._cuda_getCurrentRawStream(stream.device_index)
+    if handle == hit.handle == 0:
+        return  # the default stream, as when it was made; that one is never captured
     if _capturing():  # of a graph, whose capture begins with everything before it done
         if not any(entry is hit for entry in _IN_GRAPHS):
             _IN_GRAPHS.append(hit)
-    elif torch._C._cuda_getCurrentRawStream(stream.device_index) != stream.cuda_stream:
+    elif handle != hit.handle:
         current = torch.cuda.current_stream(stream.device)
         current.wait_event(hit.done)
         for t in _tensors(hit[1]):

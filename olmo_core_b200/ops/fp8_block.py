@@ -528,10 +528,12 @@ def fp8_block_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch
     added to the one that it has in the backward pass. First derivatives only: differentiating the gradients is an error.
     """
     w, main_grad = _whole(weight), getattr(weight, "main_grad", None)
-    if w.dim() != 2 or x.dim() == 0:
-        raise ValueError(f"the layer takes x [..., K] and a weight [N, K], got shapes {tuple(x.shape)} and {tuple(w.shape)}")
-    if x.shape[-1] != w.shape[1]:
-        raise ValueError(f"x has {x.shape[-1]} features, the weight takes {w.shape[1]}")
+    try:
+        (_, K), features = w.shape, x.shape[-1]
+    except (ValueError, IndexError):
+        raise ValueError(f"the layer takes x [..., K] and a weight [N, K], got shapes {tuple(x.shape)} and {tuple(w.shape)}") from None
+    if features != K:
+        raise ValueError(f"x has {features} features, the weight takes {K}")
     if x.device != weight.device:
         raise ValueError(f"x is on {x.device}, the weight on {weight.device}")
     if wgrad_high_precision and any(n % 8 for n in w.shape):
