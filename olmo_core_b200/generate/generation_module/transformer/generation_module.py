@@ -54,7 +54,8 @@ class TransformerGenerationModule(GenerationModule):
             self.model.to(self.device)
         self.model.eval()
         if float8_config is not None and float8_config.block is not None:
-            # linear layers with weights in 8-bit tiles, quantised at their first use (the other recipes are for training)
+            # linear layers with weights in 8-bit tiles, quantised at their first use and kept beside the weights themselves (the other
+            # recipes are for training)
             self.model.apply_fp8(replace(float8_config, cache_weight_casts=True))
         self._generation_config = generation_config
         self.state_dict_load_opts = state_dict_load_opts or {}

@@ -488,18 +488,17 @@ def bench_adamw(args, peaks) -> None:
 
 
 def bench_router(args, peaks) -> None:
-    from ..nn.moe.router import _FusedSoftmaxTopK
     from .moe import indices_and_bins, route
 
     N, E, k = 32768, 64, 8
     logits = torch.randn(N, E, device="cuda", dtype=torch.bfloat16)
     if args.profile:
-        _, _, ids, _ = _FusedSoftmaxTopK.apply(logits, k)
+        ids = route(logits, k)[1]
         indices_and_bins(ids, E)
         torch.cuda.synchronize()
         return
     with torch.no_grad():
-        t = time_ms(lambda: _FusedSoftmaxTopK.apply(logits, k), args.iters)
+        t = time_ms(lambda: route(logits, k), args.iters)
         _emit({"kernel": "router_softmax_topk", "tokens": N, "experts": E, "top_k": k, "ms": round(t, 4),
                "gbs": round((N * E * 6.0 + N * k * 8.0) / t / 1e6, 1)}, peaks)
         big = torch.randn(N, 256, device="cuda")
@@ -507,7 +506,7 @@ def bench_router(args, peaks) -> None:
         t = time_ms(lambda: route(big, k, gating="sigmoid", score_bias=bias, n_groups=8, top_k_groups=4, normalize=1), args.iters)
         _emit({"kernel": "router_sigmoid_bias_groups", "tokens": N, "experts": 256, "top_k": k, "ms": round(t, 4),
                "gbs": round((N * 256 * 8.0 + N * k * 12.0) / t / 1e6, 1)}, peaks)
-        ids = _FusedSoftmaxTopK.apply(logits, k)[2]
+        ids = route(logits, k)[1]
         t = time_ms(lambda: indices_and_bins(ids, E), args.iters)
         _emit({"kernel": "routing_counting_sort", "copies": N * k, "ms": round(t, 4)}, None)
         t = time_ms(lambda: torch.sort(ids.reshape(-1), stable=True), args.iters)

@@ -7,8 +7,8 @@
 // per row in tensor memory that it selects; all four steps of a block select the same byte here, so one word, and one set of
 // copies into tensor memory, serves four blocks. Adding scaled partial sums in registers instead, which would allow scales of any value, was measured
 // first: every block has to be read back from tensor memory, and 8192 x 11008 x 4096 took 403 us (625 us with a scale per
-// column of B). This form takes 250 us, 2950 TFLOP/s and 1.79 of what cuBLAS measures in bf16, so does the input gradient, and the
-// weight gradient takes 260 us. A block of a 256 x 256 tile takes 617 cycles; the instructions alone need 512, and so does shared memory (32 KB in
+// column of B). This form takes 250 to 256 us, 2890 to 2960 TFLOP/s and 1.75 to 1.79 of the bf16 rate of cuBLAS, the input gradient 244 to
+// 250, and the weight gradient 258 to 260. A block of a 256 x 256 tile takes 617 cycles; the instructions alone need 512, and so does shared memory (32 KB in
 // and 32 KB out per SM at 128 B a cycle), which the result's way through it, 0.6 us a tile, delays further. In longer runs the power limit
 // binds: 280 us at the 1.39 GHz that it leaves. Storing the result by TMA gained 3 % at K = 1024 and nothing at 4096.
 //
@@ -22,7 +22,7 @@
 // tokens and for products of few tiles. Roles of the pair kernel's 384 threads: warp 0 = TMA producer, warp 1 = MMA issuer and
 // tensor-memory owner, warps 2 and 3 = scales (they fetch those of four blocks at a time, run up to twelve blocks ahead, and lay
 // the exponents out as the tensor core wants them), warps 4..11 = epilogue (four lane quadrants x two column halves; through
-// shared memory, so that global accesses are whole 128-byte lines). All waits are bounded (common.cuh).
+// shared memory, so that global accesses are whole 128-byte lines). Waits on barriers in shared memory are bounded (common.cuh).
 
 #include <atomic>
 #include <cmath>
@@ -607,9 +607,9 @@ gemm_block_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
 // reduction, out of L2; in exchange there is no quantiser launch in front (one token against 4096 x 11008, with the host: 18.4 us
 // with the launch, 14.4 without; two scale warps in place of the epilogue's took 16.8).
 //
-// What bounds it: the weight's bytes (one token against 4096 x 11008: 12.2 us, 3.7 TB/s, against 6.9 us at the measured copy
+// What bounds it: the weight's bytes (one token against 4096 x 11008: 12.5 us, 3.6 TB/s, against 6.9 us at the measured copy
 // rate), and about 4.4 us in which barriers, tensor memory and tensor maps are set up, the first loads arrive, and the parts are
-// added. 64 experts of 1024 x 2048 for 128 rows that reach 53 of them: 22.1 us, 4.9 TB/s.
+// added. 64 experts of 1024 x 2048 for 128 random rows, which reach 50 of them: 21.4 us, 4.9 TB/s.
 constexpr int SMALL_THREADS = 256;  // warps as above, with one epilogue warpgroup
 
 // MANY: three CTAs per SM with a short ring each, instead of two with a deeper one (see fuller_with_three()).
@@ -630,7 +630,7 @@ struct SmallParams {
   void* C;
   long long ldc;
   int M, N, K;   // rows of the 128-row side (of one group), rows of the BN side (all groups), reduction
-  int a_mn, b_mn, epi, vector;  // vector: C rows start on 16-byte boundaries and have a multiple of 4 columns
+  int a_mn, b_mn, epi, vector;  // vector: C rows start on 16-byte boundaries
   int parts, kb_per_part;
   Scales sa, sb;
   const __nv_bfloat16* x;  // FUSED: the BN side [N][K]
@@ -1132,7 +1132,9 @@ static int run_pair(const Product& x, int dev, cudaStream_t stream) {
   return launch_epi(ta, tb, p, tiles_m * ((x.N + BN - 1) / BN), x.epi, dev, stream);
 }
 
-// Whether `tiles` CTAs fill the SMs in fewer rounds at three per SM than at two. Up to 16 rows against weights of 64 experts, two and
+// Whether `tiles` CTAs fill the SMs in fewer rounds at three per SM than at two. For groups `tiles` is what rows that fall on them at
+// random are expected to reach; how many there are is known on the device alone. With as many as there can be three per SM cost a little:
+// 64 groups of two rows each, 512 tiles: 38.9 us against 36.9 (product alone, cold L2). Up to 16 rows against weights of 64 experts, two and
 // three per SM: 424 tiles of 16 blocks 28.5 and 22.1 us, of 8 blocks 31.0 and 24.8 (848 tiles), 384 of 32 blocks 47.3 and 36.5; but 504 of 16
 // blocks 31.2 and 32.9, 512 of 32 blocks 49.7 and 58.3 (two rounds either way, and the second is emptier with three).
 static bool fuller_with_three(double tiles, int sms) { return std::ceil(tiles / (3 * sms)) < std::ceil(tiles / (2 * sms)); }
@@ -1207,7 +1209,12 @@ static int split(long long tiles, long long kb, int sms, bool stream) {
 // of so few tiles that cutting the reduction gains more. Microseconds, measured back to back on random operands:
 //   pair:             5 + 0.43 per block and wave of 256 x 256 tiles   (1024 x 4096 x 4096: 18.8, 2048 x 2048 x 2048: 13.2)
 //   128-row, 128 wide 5.5 + 0.5 per block and wave of 128 x 128 tiles  (38.1 and 25.3), 0.7 more for a cut reduction
-// The BN side of the small kernel for groups of `mean` rows (or so many rows without groups).
+// The BN side of the small kernel for groups of `mean` rows (or so many rows without groups). 64 groups of 1024 x 2048 with rows at random,
+// microseconds (in timer steps of 2) of the product alone from cold L2, for 16, 32, 64 and 128 columns and for pairs of CTAs, which run()
+// takes above 128:
+//   mean   8:  37   37   39   41   45        mean  48:  68   51   41   43   47        mean 128:   -   88   66   55   49
+//   mean  16:  43   39   39   41   45        mean  64:   -   59   47   43   47        mean 160:   -    -   76   66   49
+//   mean  32:  55   45   41   41   45        mean  96:   -   72   55   47   49        mean 256:   -    -  100   80   59
 static int small_width(long long mean, bool grouped) {
   if (grouped) return mean <= 8 ? 16 : mean <= 16 ? 32 : mean <= 48 ? 64 : 128;
   return mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 64 ? 64 : 128;

@@ -10,9 +10,10 @@
 // between stays in registers (and, for the groups, one row of shared memory). Tokens per expert are counted in shared memory, so
 // that global atomics number one per expert and CTA.
 //
-// What bounds it: latency for few tokens (one: 4 us, 11 with the host), the issue of instructions for many, about 500 a token with 64
-// experts and 1700 with bias and groups of 256: each of the k choices is a reduction over the warp. 32768 tokens of 64 experts: 33 us
-// (448 GB/s), of 256 in 8 groups: 88 us (800 GB/s). Two tokens a warp would halve the reductions' lanes but not their number.
+// What bounds it: latency for few tokens (one: 2.6 us, 11.8 with the host), the issue of instructions for many, about 500 a token with 64
+// experts and 1700 with bias and groups of 256: each of the k choices is a reduction over the whole warp for one token. 32768 tokens of
+// 64 experts: 33 us (448 GB/s), of 256 in 8 groups: 88 us (798 GB/s). The gradient of 16384 x 64 takes 5.3 us, of 8191 x 256 9 us.
+// Several tokens a warp, with reductions over 4 to 16 lanes, would share those instructions; that form is not built.
 //
 // Which experts are chosen is what exact arithmetic says, although scores are fp32: without bias and groups the ranking of the
 // logits themselves decides; otherwise a token whose ranking hangs on a difference within the fp32 error (about one in a
@@ -433,8 +434,9 @@ extern "C" int ocb_moe_route(const void* logits, float* scores, float* weights, 
   int lanes_per_group = 32;
   while (lanes_per_group * n_groups > 32) lanes_per_group >>= 1;
   const bool groups = n_groups > 1;
-  // Large CTAs, as many as are resident together: a CTA adds its counts to the global ones once. Few tokens: a token per warp
-  // of smaller CTAs.
+  // Large CTAs and few of them, because a CTA adds its counts to the global ones once. Few tokens: a token per warp of smaller CTAs.
+  // The registers (48 a thread with 64 experts, 117 with 256 in groups) let two and one of the three and two per SM run together;
+  // the others follow.
   const int warps = n_experts > 512 ? 4 : n_experts > 256 || n_tokens <= 8 ? 8 : 16;
   const long long wanted = (static_cast<long long>(n_tokens) + warps - 1) / warps;
   const long long most = static_cast<long long>(sms) * (n_experts > 128 ? 2 : 3);
