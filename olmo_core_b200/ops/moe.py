@@ -80,8 +80,9 @@ def _route_reference(logits, top_k, gating, score_bias, n_groups, top_k_groups, 
         counts = torch.bincount(experts.reshape(-1), minlength=e).to(torch.int32)
     weights = scores.gather(1, experts)
     if normalize:
-        norm = weights.sum(-1, keepdim=True) if normalize == 1 else weights.square().sum(-1, keepdim=True).sqrt()
-        weights = torch.where(norm == 0, 0.0, weights / torch.where(norm == 0, 1.0, norm))
+        norm = (weights if normalize == 1 else weights.square()).sum(-1, keepdim=True)
+        none, norm = norm == 0, torch.where(norm == 0, 1.0, norm)  # before the root, whose slope is infinite at zero
+        weights = torch.where(none, 0.0, weights / (norm if normalize == 1 else norm.sqrt()))
     return weights, experts, scores, counts
 
 

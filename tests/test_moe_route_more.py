@@ -193,3 +193,22 @@ def test_a_router_with_its_own_choice_is_asked_with_groups_too(gating, device):
     weights, experts, counts, _ = router(x)
     assert experts.flatten().tolist() == [6, 7] * 6 and counts.flatten().tolist() == [0] * 6 + [6, 6]
     torch.testing.assert_close(weights.sum(-1), torch.ones(2, 3, device=device))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("normalize", [1, 2])
+@pytest.mark.parametrize("create_graph", [False, True])
+def test_chosen_experts_without_any_weight_have_finite_gradients(create_graph, normalize, device):
+    """The bias opens a group whose experts are all masked for the token: its weights are zero, and their gradient counts for nothing."""
+    x = torch.randn(3, 8, generator=torch.Generator().manual_seed(7))
+    x[1, 4:] = float("-inf")
+    bias = torch.tensor([0.0] * 4 + [5.0] * 4)
+    leaf = x.to(device).requires_grad_(True)
+    weights, experts, scores, _ = route(leaf, 2, score_bias=bias.to(device), n_groups=2, top_k_groups=1, normalize=normalize)
+    assert (weights[1] == 0).all() and experts[1].tolist() == [4, 5]
+    dw, ds = torch.randn(3, 2, generator=torch.Generator().manual_seed(8)).to(device), torch.randn(3, 8, generator=torch.Generator().manual_seed(9)).to(device)
+    (grad,) = torch.autograd.grad((weights, scores), leaf, (dw, ds), create_graph=create_graph)
+    assert torch.isfinite(grad).all()
+    s = x[1].to(device).double().softmax(0)
+    want = s * (ds[1].double() - (s * ds[1].double()).sum())
+    assert (grad[1].detach().double() - want).abs().max() <= 16 * 2.0 ** -24 * ds[1].abs().max()
