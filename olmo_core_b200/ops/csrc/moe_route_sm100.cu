@@ -4,7 +4,8 @@
 //   r = s + bias                              what is ranked (bias: balances the load, no part of the weights)
 //   value of a group of experts = sum of its two largest r; the `top_groups` best groups stay open
 //   chosen = the k largest r of the open groups, the lower id first where two are equal
-//   w = s[chosen], divided by its sum (normalize 1) or 2-norm (normalize 2); counts = tokens per expert
+//   w = s[chosen], divided by its sum (normalize 1) or 2-norm (normalize 2), 0 where they are all below 2^-120;
+//   counts = tokens per expert
 //
 // One warp per token, expert e in register e / 32 of lane e % 32: a row is read and its scores are written once, everything
 // between stays in registers (and, for the groups, one row of shared memory). Tokens per expert are counted in shared memory, so
@@ -83,6 +84,13 @@ __device__ __forceinline__ double sum_warp(double v) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
   return v;
+}
+
+// The power of two that brings the largest of a warp's scores into [1, 2), so that squares of small ones do not vanish; 0 where
+// all are below 2^-120: such a norm counts as zero, because its reciprocal leaves fp32.
+__device__ __forceinline__ float norm_scale(float w) {
+  const uint32_t e = __reduce_max_sync(FULL, __float_as_uint(w)) >> 23;  // scores are not negative
+  return e < 7u ? 0.f : __uint_as_float((254u - e) << 23);
 }
 
 // Whether two fp32 rankings as close as `hi` and `lo` may be the other way round in exact arithmetic. NaN counts as close.
@@ -303,9 +311,10 @@ __global__ void route_kernel(const Params p, int lanes_per_group, int alone) {
     }
     if (lane >= p.top_k) w = 0.f;
     if (p.normalize != 0) {
-      const float total = sum_warp(p.normalize == 1 ? w : w * w);
+      const float scale = norm_scale(w), c = w * scale;
+      const float total = sum_warp(p.normalize == 1 ? c : c * c);
       const float norm = p.normalize == 1 ? total : sqrtf(total);
-      w = norm == 0.f ? 0.f : w / norm;
+      w = scale == 0.f ? 0.f : c / norm;
     }
     if (lane < p.top_k) {
       p.weights[t * p.top_k + lane] = w;
@@ -358,9 +367,10 @@ __global__ void route_grad_kernel(const GradParams p) {
         }
         if (p.sigmoid) w = 1.f / (1.f + expf(-w)) + SIGMOID_FLOOR;
         if (lane >= p.top_k) w = 0.f;
-        const float total = sum_warp(p.normalize == 1 ? w : w * w);
+        const float scale = norm_scale(w), c = w * scale;
+        const float total = sum_warp(p.normalize == 1 ? c : c * c);
         const float norm = p.normalize == 1 ? total : sqrtf(total);
-        const float inv = norm == 0.f ? 0.f : 1.f / norm;
+        const float inv = scale == 0.f ? 0.f : 1.f / norm * scale;
         const float along = sum_warp(g * (w * inv));
         g = (g - along * (p.normalize == 1 ? 1.f : w * inv)) * inv;
       }

@@ -144,10 +144,11 @@ struct Route : torch::autograd::Function<Route> {
         if (d_weights.defined()) {
             Tensor g = d_weights.to(at::kFloat);
             if (normalize != 0) {
-                const Tensor c = s.gather(1, experts), total = (normalize == 1 ? c : c * c).sum(1, true), none = total == 0;
-                const Tensor safe = total.masked_fill(none, 1.0), norm = normalize == 1 ? safe : safe.sqrt(), w = c / norm;
-                const Tensor along = (g * w).sum(1, true);
-                g = ((g - (normalize == 1 ? along : along * w)) / norm).masked_fill(none, 0.0);
+                const Tensor chosen = s.gather(1, experts), top = chosen.detach().amax(1, true), none = top < 0x1p-120;
+                const Tensor scale = at::ldexp(at::ones_like(top), 1 - std::get<1>(at::frexp(top))).masked_fill(none, 0.0);
+                const Tensor c = (chosen * scale).masked_fill(none, 1.0), total = (normalize == 1 ? c : c * c).sum(1, true);
+                const Tensor norm = normalize == 1 ? total : total.sqrt(), w = c / norm, along = (g * w).sum(1, true);
+                g = (g - (normalize == 1 ? along : along * w)) / norm * scale;
             }
             d = d.scatter_add(1, experts, g);
         }

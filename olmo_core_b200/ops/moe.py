@@ -80,9 +80,15 @@ def _route_reference(logits, top_k, gating, score_bias, n_groups, top_k_groups, 
         counts = torch.bincount(experts.reshape(-1), minlength=e).to(torch.int32)
     weights = scores.gather(1, experts)
     if normalize:
-        norm = (weights if normalize == 1 else weights.square()).sum(-1, keepdim=True)
-        none, norm = norm == 0, torch.where(norm == 0, 1.0, norm)  # before the root, whose slope is infinite at zero
-        weights = torch.where(none, 0.0, weights / (norm if normalize == 1 else norm.sqrt()))
+        # squares of small scores vanish, so the largest is brought near one by a power of two; where all are below 2^-120 the norm
+        # counts as zero, because its reciprocal leaves fp32
+        with torch.no_grad():
+            top = weights.detach().amax(-1, keepdim=True)
+            none = top < 2.0 ** -120
+            scale = torch.ldexp(torch.ones_like(top), 1 - torch.frexp(top)[1])
+        c = torch.where(none, 1.0, weights * scale)  # the root's slope is infinite at zero
+        norm = (c if normalize == 1 else c.square()).sum(-1, keepdim=True)
+        weights = torch.where(none, 0.0, c / (norm if normalize == 1 else norm.sqrt()))
     return weights, experts, scores, counts
 
 
@@ -115,7 +121,7 @@ def route(
     Experts are ranked by score plus ``score_bias`` (fp32 ``[E]``; it enters no weight). With ``n_groups > 1`` the experts form
     that many equal groups of consecutive ids, of which the ``top_k_groups`` with the largest sum of their two best ranked
     experts stay open. The ranking is that of exact arithmetic. A token without any logit above ``-inf`` gets softmax scores
-    and weights of zero.
+    and weights of zero; normalised weights are zero too where every chosen score is below ``2^-120``.
 
     Gradients flow from ``weights`` and ``scores`` to ``logits``, of any order, and tangents the other way. One kernel each way on
     CUDA (at most 1024 experts, 32 chosen, 32 groups); gradients that are differentiated themselves (``create_graph=True``),

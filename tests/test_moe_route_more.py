@@ -212,3 +212,32 @@ def test_chosen_experts_without_any_weight_have_finite_gradients(create_graph, n
     s = x[1].to(device).double().softmax(0)
     want = s * (ds[1].double() - (s * ds[1].double()).sum())
     assert (grad[1].detach().double() - want).abs().max() <= 16 * 2.0 ** -24 * ds[1].abs().max()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("normalize", [1, 2])
+@pytest.mark.parametrize("create_graph", [False, True])
+def test_small_scores_are_normalised_like_large_ones(create_graph, normalize, device):
+    """Logits 30 to 82 below the best ones: the squares of their scores leave fp32 long before they do. Where all chosen scores are below
+    2^-120 = e^-83.2 (a gap of 82 and a sum of four: e^-82 / 4 = e^-83.4) weights are zero."""
+    U = 2.0 ** -24
+    gaps = torch.tensor([30.0, 45.0, 60.0, 75.0, 82.0, 85.0, 120.0])
+    x = torch.randn(7, 8, generator=torch.Generator().manual_seed(10)) * 0.25
+    x[:, 4:] -= gaps[:, None]
+    bias = torch.tensor([0.0] * 4 + [5.0] * 4)  # opens the group of the small ones
+    leaf = x.to(device).requires_grad_(True)
+    weights, experts, scores, _ = route(leaf, 3, score_bias=bias.to(device), n_groups=2, top_k_groups=1, normalize=normalize)
+    assert (experts >= 4).all()
+    dw = torch.randn(7, 3, generator=torch.Generator().manual_seed(11)).to(device)
+    (grad,) = torch.autograd.grad(weights, leaf, dw, create_graph=create_graph)
+    exact = x.to(device).double().requires_grad_(True)
+    chosen = exact.softmax(-1).gather(1, experts)
+    want = chosen / chosen.norm(p=normalize, dim=1, keepdim=True)
+    (slope,) = torch.autograd.grad(want, exact, dw.double())
+    # the exponential of a difference of up to 128, rounded to 64 U of it, twice; weights and gradients are of size one
+    tolerance = (2 * 64 + 64) * U
+    some = chosen.amax(1) >= 2.0 ** -120
+    assert some.tolist() == [True] * 4 + [False] * 3
+    assert (weights[some].double() - want[some]).abs().max() <= tolerance
+    assert (grad[some].detach().double() - slope[some]).abs().max() <= 8 * tolerance * dw.abs().max()
+    assert (weights[~some] == 0).all() and (grad[~some] == 0).all()
